@@ -602,6 +602,103 @@ int sdf_delaunay_merge_verified(const float *points, uint32_t num_points,
                                 uint64_t *result, void *scratch, size_t scratch_bytes,
                                 void *stream);
 
+/* ---- label fields (no counterpart in the reference) -------------------
+ *
+ * A foam whose cells carry learned rows: the rows of the cells that rays end
+ * in (the trace's depth_indices), the distance of the logits a head makes of
+ * them from a teacher's best few, and what such logits answer.
+ *
+ * Element types (SDF_TYPE_*) and id types (SDF_ID_*; signed ids may be read as
+ * either signedness) of the arrays below.  An id outside [0, limit) -- negative,
+ * 0xffffffff as the trace writes it, or too large -- names no cell or label.
+ * Strides are in elements; rows themselves are contiguous.  Scratch is 256-byte
+ * aligned. */
+#define SDF_TYPE_F32 0
+#define SDF_TYPE_F16 1
+#define SDF_TYPE_BF16 2
+#define SDF_ID_U32 0
+#define SDF_ID_I32 1
+#define SDF_ID_I64 2
+#define SDF_REDUCE_NONE 0
+#define SDF_REDUCE_SUM 1
+#define SDF_REDUCE_MEAN 2 /* over all rows, those that do not count included */
+
+/* rows[i, :] = scale * weight[i] * table[cells[i], :] (weight NULL: 1), zeros
+ * where cells[i] is no cell.  table [num_cells, width] with rows table_stride
+ * apart, rows [count, width] contiguous, both of `type`; fewer than 2^31 cells
+ * and ids. */
+int sdf_cell_rows(int type, const void *table, uint64_t table_stride,
+                  uint64_t num_cells, uint32_t width, int id_type,
+                  const void *cells, uint64_t count, const float *weight,
+                  float scale, void *rows, void *stream);
+
+/* Gradients of sdf_cell_rows: table_grad [num_cells, width] (of `type`, every
+ * row written: zeros for cells that no id names; NULL: not wanted) and, where
+ * weight_grad is not NULL, weight_grad[i] = scale * <table[cells[i], :], rows_grad[i, :]> (fp32, 0
+ * for no cell; table is read for it only).  Each cell's rows are summed in fp32
+ * in an order that the ids alone decide. */
+size_t sdf_cell_rows_backward_scratch_bytes(uint64_t num_cells, uint32_t width,
+                                            uint64_t count);
+int sdf_cell_rows_backward(int type, const void *rows_grad,
+                           uint64_t rows_grad_stride, const void *table,
+                           uint64_t table_stride, uint64_t num_cells,
+                           uint32_t width, int id_type, const void *cells,
+                           uint64_t count, const float *weight, float scale,
+                           void *table_grad, float *weight_grad, void *scratch,
+                           size_t scratch_bytes, void *stream);
+
+/* Distillation: logits [rows, labels] (`type`, rows `stride` apart) against a
+ * teacher's `top` (at most 1024) logits per row at teacher_labels, both
+ * [rows, top] contiguous.  Entries whose label is none or whose logit is -inf do
+ * not count.  With q and p the softmax of the counting entries' and of the row's
+ * logits over the temperature T and u = row_weight[r] (NULL: 1),
+ *   loss_r = u T^2 sum_k q_k (log q_k - log p[label_k]),
+ * 0 where u is 0 (the row's logits are not read), no entry counts or every logit
+ * is -inf.  loss: [rows] for SDF_REDUCE_NONE, else their sum or mean over all
+ * rows.  stats [rows, 2] (NULL: not kept): the rows' softmax for
+ * sdf_distill_backward.  logits_grad [rows, labels] contiguous (NULL: not
+ * wanted): the gradient, times loss_grad ([rows] for SDF_REDUCE_NONE, else one
+ * value; NULL: 1). */
+size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels);
+int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels,
+                uint64_t stride, int id_type, const void *teacher_labels,
+                int teacher_type, const void *teacher_logits, uint32_t top,
+                float temperature, const float *row_weight, int reduction,
+                const float *loss_grad, float *loss, float *stats,
+                void *logits_grad, void *scratch, size_t scratch_bytes,
+                void *stream);
+int sdf_distill_backward(int type, const void *logits, uint64_t rows,
+                         uint64_t labels, uint64_t stride, int id_type,
+                         const void *teacher_labels, int teacher_type,
+                         const void *teacher_logits, uint32_t top,
+                         float temperature, const float *row_weight,
+                         int reduction, const float *loss_grad,
+                         const float *stats, void *logits_grad, void *stream);
+
+/* Per row of logits [rows, labels] over the temperature: log_prob of label_ids
+ * (0 for no label, -inf for one masked by -inf), the entropy of the softmax (0
+ * for a row of nothing but -inf), and the `top` (at most 64) largest logits'
+ * log probabilities and labels, largest first, ties to the lowest label; -inf
+ * and -1 where fewer are above -inf.  stats [rows, 2] as above. */
+size_t sdf_label_log_probs_scratch_bytes(uint64_t rows, uint64_t labels,
+                                         uint32_t top);
+int sdf_label_log_probs(int type, const void *logits, uint64_t rows,
+                        uint64_t labels, uint64_t stride, int id_type,
+                        const void *label_ids, uint32_t top, float temperature,
+                        float *log_prob, float *entropy, float *top_log_probs,
+                        int64_t *top_labels, float *stats, void *scratch,
+                        size_t scratch_bytes, void *stream);
+
+/* The logits' gradient [rows, labels] (contiguous) from those of log_prob and
+ * entropy (either NULL: 0), with the entropy and stats of the forward. */
+int sdf_label_log_probs_backward(int type, const void *logits, uint64_t rows,
+                                 uint64_t labels, uint64_t stride, int id_type,
+                                 const void *label_ids, float temperature,
+                                 const float *entropy, const float *stats,
+                                 const float *log_prob_grad,
+                                 const float *entropy_grad, void *logits_grad,
+                                 void *stream);
+
 /* ---- measurement and test hooks (no counterpart in the reference) ----- */
 
 /* Per-ray walk statistics of the forward (backward = 0) or backward

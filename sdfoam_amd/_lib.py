@@ -18,6 +18,15 @@ SDF_ALPHA_STANDARD = 0
 SDF_ALPHA_NEUS = 1
 SDF_ATTR_F32 = 0
 SDF_ATTR_F16 = 1
+SDF_TYPE_F32 = 0
+SDF_TYPE_F16 = 1
+SDF_TYPE_BF16 = 2
+SDF_ID_U32 = 0
+SDF_ID_I32 = 1
+SDF_ID_I64 = 2
+SDF_REDUCE_NONE = 0
+SDF_REDUCE_SUM = 1
+SDF_REDUCE_MEAN = 2
 
 # every symbol include/sdfoam_hip.h declares
 EXPORTS = (
@@ -68,6 +77,15 @@ EXPORTS = (
     "sdf_nn",
     "sdf_nn_scratch_bytes",
     "sdf_nn_planned",
+    "sdf_cell_rows",
+    "sdf_cell_rows_backward_scratch_bytes",
+    "sdf_cell_rows_backward",
+    "sdf_distill_scratch_bytes",
+    "sdf_distill",
+    "sdf_distill_backward",
+    "sdf_label_log_probs_scratch_bytes",
+    "sdf_label_log_probs",
+    "sdf_label_log_probs_backward",
     "sdf_trace_walk_stats",
     "sdf_debug_fpmath",
     "sdf_set_timing",
@@ -143,6 +161,8 @@ _lib = None
 
 P = C.c_void_p
 U32 = C.c_uint32
+U64 = C.c_uint64
+F32 = C.c_float
 SZ = C.c_size_t
 
 
@@ -264,6 +284,28 @@ def lib() -> C.CDLL:
     L.sdf_nn_scratch_bytes.argtypes = [U32, U32]
     L.sdf_nn_planned.restype = C.c_int
     L.sdf_nn_planned.argtypes = [P, P, P, U32, U32, P, P, SZ, P]
+    L.sdf_cell_rows.restype = C.c_int
+    L.sdf_cell_rows.argtypes = [C.c_int, P, U64, U64, U32, C.c_int, P, U64, P, F32, P, P]
+    L.sdf_cell_rows_backward_scratch_bytes.restype = SZ
+    L.sdf_cell_rows_backward_scratch_bytes.argtypes = [U64, U32, U64]
+    L.sdf_cell_rows_backward.restype = C.c_int
+    L.sdf_cell_rows_backward.argtypes = [C.c_int, P, U64, P, U64, U64, U32, C.c_int, P, U64, P,
+                                         F32, P, P, P, SZ, P]
+    distill = [C.c_int, P, U64, U64, U64, C.c_int, P, C.c_int, P, U32, F32, P, C.c_int]
+    L.sdf_distill_scratch_bytes.restype = SZ
+    L.sdf_distill_scratch_bytes.argtypes = [U64, U64]
+    L.sdf_distill.restype = C.c_int
+    L.sdf_distill.argtypes = distill + [P, P, P, P, P, SZ, P]
+    L.sdf_distill_backward.restype = C.c_int
+    L.sdf_distill_backward.argtypes = distill + [P, P, P, P]
+    L.sdf_label_log_probs_scratch_bytes.restype = SZ
+    L.sdf_label_log_probs_scratch_bytes.argtypes = [U64, U64, U32]
+    L.sdf_label_log_probs.restype = C.c_int
+    L.sdf_label_log_probs.argtypes = [C.c_int, P, U64, U64, U64, C.c_int, P, U32, F32, P, P, P, P,
+                                      P, P, SZ, P]
+    L.sdf_label_log_probs_backward.restype = C.c_int
+    L.sdf_label_log_probs_backward.argtypes = [C.c_int, P, U64, U64, U64, C.c_int, P, F32, P, P,
+                                               P, P, P, P]
     L.sdf_trace_walk_stats.restype = C.c_int
     L.sdf_trace_walk_stats.argtypes = [
         C.c_int, C.POINTER(TraceSettings), C.c_int, U32, P, P, U32, P, P, U32, P, P, P,
