@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(const T *__restrict__ 
     if (c >= 0)
         for (uint32_t d = threadIdx.x & 63u; d < width; d += 64u)
             s = fmaf((float)grad[i * grad_stride + d], (float)table[(uint64_t)c * table_stride + d], s);
-    s = wave_sum(s);
+    s = group_sum<64>(s);
     if ((threadIdx.x & 63u) == 0) weight_grad[i] = scale * s;
 }
 

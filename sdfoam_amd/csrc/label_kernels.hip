@@ -24,40 +24,128 @@ constexpr uint32_t kMaxTeacher = 1024; // teacher's entries a row
 constexpr uint32_t kMaxTop = 64;       // best labels returned a row
 constexpr float kLog2e = 1.44269504088896341f;
 
-__device__ __forceinline__ float block_max(float x, float *shared) {
-    x = wave_max(x);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) shared[threadIdx.x >> 6] = x;
-    __syncthreads();
-    for (uint32_t k = 0; k < blockDim.x / 64u; ++k) x = fmaxf(x, shared[k]);
-    return x;
-}
-__device__ __forceinline__ float block_sum(float x, float *shared) {
-    x = wave_sum(x);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) shared[threadIdx.x >> 6] = x;
-    __syncthreads();
-    float s = 0.0f;
-    for (uint32_t k = 0; k < blockDim.x / 64u; ++k) s += shared[k];
-    return s;
-}
-
-// The largest logit of a row (0 for a row of nothing but -inf, so that
-// differences from it stay defined) and S.  NaN reaches S.
-struct RowStats {
-    float m, s;
+// Softmax statistics of the labels seen so far: the largest logit, and relative
+// to it S and W = sum d e, d = (z - m) c, e = 2^d, c = log2(e) / T (the logits
+// are scaled to base 2 once, so that an exponential is one instruction).
+// Nothing but -inf seen: m = -inf, S = 0.  A NaN reaches S, and so does +inf.
+struct Part {
+    float m, s, w;
 };
+// m >= p.m.  Where p.m is -inf, S is 0 and stays so; the bound on d keeps
+// 0 * inf out of W.
+template <bool kEntropy> __device__ __forceinline__ void rebase(Part &p, float m, float c) {
+    const float d = p.m == m ? 0.0f : (p.m - m) * c;
+    const float f = __builtin_amdgcn_exp2f(d);
+    if (kEntropy) p.w = (p.w + fmaxf(d, -200.0f) * p.s) * f;
+    p.s *= f;
+    p.m = m;
+}
+// The elements of kU chunks into p: one change of base, then a subtraction, a
+// product, an exponential and a sum each.
+template <bool kEntropy, typename T, int kU>
+__device__ __forceinline__ void absorb(Part &p, const Chunk<T> (&ch)[kU], float c) {
+    float m = p.m;
+#pragma unroll
+    for (int i = 0; i < kU; ++i)
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::kN; ++e) m = fmaxf(m, (float)ch[i].v[e]);
+    rebase<kEntropy>(p, m, c);
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < kU; ++i)
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::kN; ++e) {
+            const float d = ((float)ch[i].v[e] - base) * c;
+            const float x = __builtin_amdgcn_exp2f(d);
+            p.s += x;
+            if (kEntropy) p.w = fmaf(fmaxf(d, -200.0f), x, p.w);
+        }
+}
+// One Part of the kLanes neighbouring lanes' (in all of them).
+template <int kLanes, bool kEntropy> __device__ __forceinline__ void merge_lanes(Part &p, float c) {
+    rebase<kEntropy>(p, group_max<kLanes>(p.m), c);
+    p.s = group_sum<kLanes>(p.s);
+    if (kEntropy) p.w = group_sum<kLanes>(p.w);
+}
+// One Part of n others.
+template <bool kEntropy> __device__ __forceinline__ Part merge_parts(const Part *parts, uint32_t n, float c) {
+    Part all = {-INFINITY, 0.0f, 0.0f};
+    for (uint32_t k = 0; k < n; ++k) all.m = fmaxf(all.m, parts[k].m);
+    for (uint32_t k = 0; k < n; ++k) {
+        Part p = parts[k];
+        rebase<kEntropy>(p, all.m, c);
+        all.s += p.s;
+        if (kEntropy) all.w += p.w;
+    }
+    return all;
+}
+// One Part of the block's threads; `parts` holds one per wavefront.  Leaves a
+// barrier behind it that orders the threads' earlier writes to LDS.
+template <bool kEntropy> __device__ __forceinline__ Part merge_block(Part p, Part *parts, float c) {
+    merge_lanes<64, kEntropy>(p, c);
+    if ((threadIdx.x & 63u) == 0) parts[threadIdx.x >> 6] = p;
+    __syncthreads();
+    return merge_parts<kEntropy>(parts, blockDim.x >> 6, c);
+}
 
-template <typename T>
-__device__ RowStats row_stats(const T *z, uint32_t labels, float c, float *shared) {
-    float m = -INFINITY;
-    for (uint32_t v = threadIdx.x; v < labels; v += blockDim.x) m = fmaxf(m, (float)z[v]);
-    m = block_max(m, shared);
-    if (m == -INFINITY) m = 0.0f;
-    float s = 0.0f;
-    for (uint32_t v = threadIdx.x; v < labels; v += blockDim.x)
-        s += __builtin_amdgcn_exp2f(((float)z[v] - m) * c);
-    return {m, block_sum(s, shared)};
+// f(chunks, at) for the elements [begin, end) of a row, kU chunks of each of
+// kThreads threads at a time, chunk i at `at` + i kThreads kN; what is not a
+// chunk's own (place()) is -inf where kMask, else as it was read.
+// (for_steps: only the steps that begin in [first, last).)
+template <int kThreads, int kU, bool kMask, typename T, typename F>
+__device__ __forceinline__ void for_steps(const T *z, uint32_t first, uint32_t last, uint32_t begin,
+                                          uint32_t end, F f) {
+    constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
+    for (; first < last; first += kStep * kU) {
+        const uint32_t at = first + threadIdx.x % kThreads * Chunk<T>::kN;
+        Chunk<T> ch[kU];
+        if (first + kStep * kU <= end) {
+#pragma unroll
+            for (int i = 0; i < kU; ++i) ch[i] = load_chunk(z + at + i * kStep);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kU; ++i)
+                ch[i] = load_raw(z, at + i * kStep, begin, end, (T)-INFINITY);
+            if (kMask) {
+#pragma unroll
+                for (int i = 0; i < kU; ++i)
+                    mask_chunk(ch[i], at + i * kStep, begin, end, (T)-INFINITY);
+            }
+        }
+        f(ch, at);
+    }
+}
+template <int kThreads, int kU, bool kMask, typename T, typename F>
+__device__ __forceinline__ void for_chunks(const T *z, uint32_t begin, uint32_t end, F f) {
+    for_steps<kThreads, kU, kMask>(z, begin, end, begin, end, f);
+}
+// row[i] = f(z[i]) chunk by chunk over [begin, end)
+template <int kThreads, int kU, typename T, typename F>
+__device__ __forceinline__ void map_chunks(const T *z, T *row, uint32_t begin, uint32_t end, F f) {
+    constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
+    for_chunks<kThreads, kU, false>(z, begin, end, [&](const Chunk<T>(&ch)[kU], uint32_t at) {
+#pragma unroll
+        for (int i = 0; i < kU; ++i)
+            if (at + i * kStep < end) {
+                const uint32_t to = place<T>(at + i * kStep, begin, end);
+                const Chunk<T> o = f(ch[i], to);
+                // two threads may write one element, and then the same value
+                if (end - begin >= (uint32_t)Chunk<T>::kN) store_chunk(row + to, o);
+                else store_own(row, to, begin, end, o);
+            }
+    });
+}
+
+constexpr int kStream = 256; // threads a block where rows are streamed
+constexpr int kUnroll = 4;   // chunks in flight per thread
+
+template <bool kEntropy, typename T>
+__device__ __forceinline__ Part stream_part(const T *z, uint32_t begin, uint32_t end, float c) {
+    Part p = {-INFINITY, 0.0f, 0.0f};
+    for_chunks<kStream, kUnroll, true>(z, begin, end, [&](const Chunk<T>(&ch)[kUnroll], uint32_t) {
+        absorb<kEntropy>(p, ch, c);
+    });
+    return p;
 }
 
 struct DistillArgs {
@@ -75,7 +163,7 @@ struct DistillArgs {
     uint32_t loss_grad_stride; // 0: one for all rows
     float reduce;              // what a row's loss counts in the result
     float *loss;               // [rows]; NULL: not written
-    float2 *stats;             // [rows] {m, S}; read where `have_stats`, else written unless NULL
+    float2 *stats;             // [rows] {m, S}: the backward's input, else written unless NULL
     void *logits_grad;         // [rows, labels]; NULL: not written
 };
 
@@ -85,79 +173,294 @@ __device__ __forceinline__ float teacher_logit(const DistillArgs &a, uint64_t i)
     return static_cast<const float *>(a.teacher_logits)[i];
 }
 
-template <typename T, bool have_stats>
-__global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
-    __shared__ float shared[4];
-    __shared__ float q[kMaxTeacher];
-    __shared__ int32_t id[kMaxTeacher];
-    const uint64_t r = blockIdx.x;
-    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
-    T *dz = a.logits_grad ? static_cast<T *>(a.logits_grad) + r * a.labels : nullptr;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
-    const float u = a.row_weight ? a.row_weight[r] : 1.0f;
-
-    float tm = -INFINITY;
-    for (uint32_t k = threadIdx.x; k < a.top; k += 256u) {
-        const int32_t j = load_id(a.teacher_labels, a.id_type, r * a.top + k, a.labels);
-        const float t = j < 0 ? -INFINITY : teacher_logit(a, r * a.top + k);
-        id[k] = t == -INFINITY ? -1 : j;
-        q[k] = t;
-        tm = fmaxf(tm, t);
+// A row's teacher: which entries count, their softmax, and the row's factor.
+// Every group of kLanes lanes computes it for itself (a wavefront with the
+// whole row, or a few lanes that share one).
+struct Teacher {
+    float u, m, s; // row weight, largest counting logit (0: none), sum relative to it
+    bool counts;   // some entry counts and the weight is not 0
+};
+__device__ __forceinline__ float entry(const DistillArgs &a, uint64_t r, uint32_t k, int32_t &j) {
+    j = load_id(a.teacher_labels, a.id_type, r * a.top + k, a.labels);
+    const float t = j < 0 ? -INFINITY : teacher_logit(a, r * a.top + k);
+    if (t == -INFINITY) j = -1;
+    return t;
+}
+template <int kLanes>
+__device__ __forceinline__ Teacher teacher_of(const DistillArgs &a, uint64_t r, float c) {
+    const uint32_t l = threadIdx.x & (kLanes - 1);
+    Teacher t = {a.row_weight ? a.row_weight[r] : 1.0f, -INFINITY, 0.0f, false};
+    int32_t j;
+    for (uint32_t k = l; k < a.top; k += kLanes) t.m = fmaxf(t.m, entry(a, r, k, j));
+    t.m = group_max<kLanes>(t.m);
+    if (t.m == -INFINITY) t.m = 0.0f;
+    for (uint32_t k = l; k < a.top; k += kLanes)
+        t.s += __builtin_amdgcn_exp2f((entry(a, r, k, j) - t.m) * c);
+    t.s = group_sum<kLanes>(t.s);
+    t.counts = !(t.u == 0.0f) && !(t.s == 0.0f);
+    return t;
+}
+// The counting entries' shares q and labels into LDS (label -1: none) by the
+// kLanes lanes of a group.
+template <int kLanes>
+__device__ __forceinline__ void store_shares(const DistillArgs &a, uint64_t r, const Teacher &t,
+                                             float c, float *q, int32_t *id) {
+    for (uint32_t k = threadIdx.x & (kLanes - 1); k < a.top; k += kLanes) {
+        int32_t j;
+        const float x = entry(a, r, k, j);
+        q[k] = __builtin_amdgcn_exp2f((x - t.m) * c) / t.s;
+        id[k] = j;
     }
-    tm = block_max(tm, shared);
-    if (tm == -INFINITY) tm = 0.0f;
-    float ts = 0.0f;
-    for (uint32_t k = threadIdx.x; k < a.top; k += 256u)
-        ts += __builtin_amdgcn_exp2f((q[k] - tm) * c);
-    ts = block_sum(ts, shared);
-
-    RowStats st = {0.0f, 0.0f};
-    const bool counts = !(u == 0.0f) && !(ts == 0.0f);
-    if (counts) {
-        if (have_stats) {
-            const float2 h = a.stats[r];
-            st = {h.x, h.y};
-        } else {
-            st = row_stats(z, a.labels, c, shared);
-        }
-    }
-    const bool live = counts && !(st.s == 0.0f);
-    if (!have_stats && a.stats && threadIdx.x == 0) a.stats[r] = make_float2(st.m, st.s);
-    if (!live) {
-        if (threadIdx.x == 0 && a.loss) a.loss[r] = 0.0f;
-        if (dz)
-            for (uint32_t v = threadIdx.x; v < a.labels; v += 256u) dz[v] = (T)0.0f;
-        return;
-    }
-
+}
+// sum q (log q - log p) over the entries of the kLanes lanes of a group.
+template <int kLanes, typename T>
+__device__ __forceinline__ float row_loss(const DistillArgs &a, uint64_t r, const T *z,
+                                          const Teacher &t, const Part &st, float c, float inv_t) {
+    const float log_s = logf(st.s), log_ts = logf(t.s);
     float sum = 0.0f;
-    const float log_s = logf(st.s), log_ts = logf(ts);
-    for (uint32_t k = threadIdx.x; k < a.top; k += 256u) {
-        const float d = (q[k] - tm) * inv_t;
-        const float qk = __builtin_amdgcn_exp2f((q[k] - tm) * c) / ts;
+    for (uint32_t k = threadIdx.x & (kLanes - 1); k < a.top; k += kLanes) {
+        int32_t j;
+        const float x = entry(a, r, k, j);
+        const float q = __builtin_amdgcn_exp2f((x - t.m) * c) / t.s;
         // an entry of no mass adds nothing, whatever its label's probability
-        if (a.loss && !(qk == 0.0f))
-            sum += qk * (d - log_ts - (((float)z[id[k]] - st.m) * inv_t - log_s));
-        q[k] = qk;
+        if (j >= 0 && !(q == 0.0f))
+            sum += q * ((x - t.m) * inv_t - log_ts - (((float)z[j] - st.m) * inv_t - log_s));
     }
-    if (a.loss) {
-        sum = block_sum(sum, shared);
-        if (threadIdx.x == 0) a.loss[r] = u * a.temperature * a.temperature * sum;
-    }
-    if (!dz) return;
-    const float g = a.loss_grad ? a.loss_grad[r * a.loss_grad_stride] : 1.0f;
-    const float coef = g * a.reduce * u * a.temperature, share = coef / st.s;
-    for (uint32_t v = threadIdx.x; v < a.labels; v += 256u)
-        dz[v] = (T)(share * __builtin_amdgcn_exp2f(((float)z[v] - st.m) * c));
-    __syncthreads(); // the teacher's labels are written over what stands there
-    for (uint32_t k = threadIdx.x; k < a.top; k += 256u) {
+    return t.u * a.temperature * a.temperature * group_sum<kLanes>(sum);
+}
+// The row's gradient at the teacher's labels in [begin, end), over what stands
+// there: entries `first`, `first` + `step`, ...
+template <typename T>
+__device__ __forceinline__ void write_shares(const DistillArgs &a, const T *z, T *dz, const float *q,
+                                             const int32_t *id, const Part &st, float c, float coef,
+                                             uint32_t first, uint32_t step, uint32_t begin,
+                                             uint32_t end) {
+    for (uint32_t k = first; k < a.top; k += step) {
         const int32_t j = id[k];
-        if (j < 0) continue;
+        if (j < 0 || (uint32_t)j < begin || (uint32_t)j >= end) continue;
         float mass = 0.0f; // a label that the teacher names twice has both shares
         for (uint32_t o = 0; o < a.top; ++o) mass += id[o] == j ? q[o] : 0.0f;
         const float p = __builtin_amdgcn_exp2f(((float)z[j] - st.m) * c) / st.s;
         dz[j] = (T)(coef * (p - mass));
     }
+}
+__device__ __forceinline__ float row_coef(const DistillArgs &a, uint64_t r, const Teacher &t) {
+    const float g = a.loss_grad ? a.loss_grad[r * a.loss_grad_stride] : 1.0f;
+    return g * a.reduce * t.u * a.temperature;
+}
+// share * e of a chunk's logits
+template <typename T>
+__device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &ch, float m, float c, float share) {
+    Chunk<T> o;
+#pragma unroll
+    for (int e = 0; e < Chunk<T>::kN; ++e)
+        o.v[e] = (T)(share * __builtin_amdgcn_exp2f(((float)ch.v[e] - m) * c));
+    return o;
+}
+template <int kThreads, typename T>
+__device__ __forceinline__ void write_zeros(T *dz, uint32_t begin, uint32_t end) {
+    constexpr uint32_t kN = Chunk<T>::kN;
+    const Chunk<T> zero = {};
+    for (uint32_t at = begin + threadIdx.x * kN; at < end; at += kThreads * kN)
+        store_own(dz, at, begin, end, zero);
+}
+
+// A block per row.  With kHeld > 0 (the gradient is wanted): the row's first
+// kThreads * kHeld chunks stay in registers between the statistics and the
+// gradient, so they are read once; the rest is read again.  kHeld = 0: loss and
+// statistics alone, streamed.
+template <typename T, int kThreads, int kHeld>
+__global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
+    constexpr uint32_t kN = Chunk<T>::kN;
+    __shared__ Part parts[kThreads / 64];
+    __shared__ float q[kHeld ? kMaxTeacher : 1];
+    __shared__ int32_t id[kHeld ? kMaxTeacher : 1];
+    const uint64_t r = blockIdx.x;
+    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+    T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
+    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    constexpr uint32_t kRest = kThreads * kN * kHeld;
+    const bool read = !(a.row_weight && a.row_weight[r] == 0.0f); // the same in every thread
+    Chunk<T> held[kHeld ? kHeld : 1];
+    if (kHeld > 0 && read) { // on their way while the teacher's entries are looked at
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            held[i] = load_raw(z, (threadIdx.x + i * kThreads) * kN, 0u, a.labels, (T)-INFINITY);
+    }
+    const Teacher t = teacher_of<64>(a, r, c);
+    Part st = {0.0f, 0.0f, 0.0f};
+    if (t.counts) {
+        Part p = {-INFINITY, 0.0f, 0.0f};
+        if constexpr (kHeld > 0) {
+            if (threadIdx.x < 64u) store_shares<64>(a, r, t, c, q, id);
+            if (kRest > a.labels) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i)
+                    mask_chunk(held[i], (threadIdx.x + i * kThreads) * kN, 0u, a.labels,
+                               (T)-INFINITY);
+            }
+            absorb<false>(p, held, c);
+        }
+        if (kRest < a.labels)
+            for_chunks<kThreads, kUnroll, true>(
+                z, kRest, a.labels,
+                [&](const Chunk<T>(&ch)[kUnroll], uint32_t) { absorb<false>(p, ch, c); });
+        st = merge_block<false>(p, parts, c);
+        if (st.m == -INFINITY) st.m = 0.0f;
+    }
+    const bool live = t.counts && !(st.s == 0.0f);
+    if (a.stats && threadIdx.x == 0) a.stats[r] = make_float2(st.m, st.s);
+    if (threadIdx.x < 64u) {
+        const float loss = live ? row_loss<64>(a, r, z, t, st, c, inv_t) : 0.0f;
+        if (threadIdx.x == 0) a.loss[r] = loss;
+    }
+    if constexpr (kHeld > 0) {
+        if (!live) {
+            write_zeros<kThreads>(dz, 0, a.labels);
+            return;
+        }
+        const float coef = row_coef(a, r, t), share = coef / st.s;
+        if (kRest < a.labels)
+            map_chunks<kThreads, kUnroll>(z, dz, kRest, a.labels, [&](const Chunk<T> &ch, uint32_t) {
+                return grad_chunk(ch, st.m, c, share);
+            });
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const uint32_t at = (threadIdx.x + i * kThreads) * kN;
+            if (at < a.labels)
+                store_own(dz, at, 0u, a.labels, grad_chunk(held[i], st.m, c, share));
+        }
+        __syncthreads(); // the teacher's labels are written over what stands there
+        write_shares(a, z, dz, q, id, st, c, coef, threadIdx.x, kThreads, 0u, a.labels);
+    }
+}
+
+// Few long rows: the statistics of a slice of a row per block.
+template <typename T>
+__global__ __launch_bounds__(kStream) void part_kernel(DistillArgs a, uint32_t slices,
+                                                       uint32_t slice, Part *out) {
+    __shared__ Part parts[kStream / 64];
+    const uint64_t r = blockIdx.x / slices;
+    const uint32_t k = blockIdx.x % slices, begin = k * slice;
+    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+    const float c = (1.0f / a.temperature) * kLog2e;
+    if (a.row_weight && a.row_weight[r] == 0.0f) return; // not read, here or later
+    const Part p = merge_block<false>(
+        stream_part<false>(z, begin, min(a.labels, begin + slice), c), parts, c);
+    if (threadIdx.x == 0) out[r * slices + k] = p;
+}
+
+// The loss, and the gradient of a slice of a row per block, from the row's
+// statistics: `parts` of its slices, or a.stats where `parts` is NULL.
+template <typename T>
+__global__ __launch_bounds__(kStream) void finish_kernel(DistillArgs a, uint32_t tiles,
+                                                         uint32_t tile, const Part *parts,
+                                                         uint32_t slices) {
+    __shared__ float q[kMaxTeacher];
+    __shared__ int32_t id[kMaxTeacher];
+    const uint64_t r = blockIdx.x / tiles;
+    const uint32_t begin = (uint32_t)(blockIdx.x % tiles) * tile;
+    const uint32_t end = min(a.labels, begin + tile);
+    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+    T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
+    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    const Teacher t = teacher_of<64>(a, r, c);
+    Part st = {0.0f, 0.0f, 0.0f};
+    if (t.counts) {
+        if (parts) {
+            st = merge_parts<false>(parts + r * slices, slices, c);
+            if (st.m == -INFINITY) st.m = 0.0f;
+        } else {
+            const float2 h = a.stats[r];
+            st = {h.x, h.y, 0.0f};
+        }
+    }
+    const bool live = t.counts && !(st.s == 0.0f);
+    if (parts && begin == 0 && threadIdx.x < 64u) {
+        const float loss = live ? row_loss<64>(a, r, z, t, st, c, inv_t) : 0.0f;
+        if (threadIdx.x == 0) {
+            a.loss[r] = loss;
+            if (a.stats) a.stats[r] = make_float2(st.m, st.s);
+        }
+    }
+    if (!a.logits_grad) return;
+    if (!live) {
+        write_zeros<kStream>(dz, begin, end);
+        return;
+    }
+    if (threadIdx.x < 64u) store_shares<64>(a, r, t, c, q, id);
+    const float coef = row_coef(a, r, t), share = coef / st.s;
+    map_chunks<kStream, kUnroll>(z, dz, begin, end, [&](const Chunk<T> &ch, uint32_t) {
+        return grad_chunk(ch, st.m, c, share);
+    });
+    __syncthreads();
+    write_shares(a, z, dz, q, id, st, c, coef, threadIdx.x, kStream, begin, end);
+}
+
+// Short rows: kLanes lanes a row, the whole row in their registers (kHeld
+// chunks each), 256 / kLanes rows a block or fewer where the teacher's entries
+// fill LDS (`shares`: top floats, then top labels, for each row).
+template <typename T, int kLanes, int kHeld, bool kHaveStats>
+__global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs a, uint64_t rows) {
+    constexpr uint32_t kN = Chunk<T>::kN;
+    extern __shared__ float shares[];
+    const uint32_t g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
+    const uint64_t r = (uint64_t)blockIdx.x * (blockDim.x / kLanes) + g;
+    const bool in = r < rows;
+    float *q = shares + (size_t)g * 2 * a.top;
+    int32_t *id = reinterpret_cast<int32_t *>(q + a.top);
+    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+    T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
+    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    Teacher t = {0.0f, 0.0f, 0.0f, false};
+    Part st = {0.0f, 0.0f, 0.0f};
+    bool live = false;
+    float coef = 0.0f;
+    if (in) {
+        t = teacher_of<kLanes>(a, r, c);
+        Chunk<T> held[kHeld];
+        if (t.counts) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                held[i] = load_raw(z, (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                mask_chunk(held[i], (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+            if (kHaveStats) {
+                const float2 h = a.stats[r];
+                st = {h.x, h.y, 0.0f};
+            } else {
+                st = {-INFINITY, 0.0f, 0.0f};
+                absorb<false>(st, held, c);
+                merge_lanes<kLanes, false>(st, c);
+                if (st.m == -INFINITY) st.m = 0.0f;
+            }
+        }
+        live = t.counts && !(st.s == 0.0f);
+        if (!kHaveStats) {
+            const float loss = live ? row_loss<kLanes>(a, r, z, t, st, c, inv_t) : 0.0f;
+            if (l == 0) {
+                a.loss[r] = loss;
+                if (a.stats) a.stats[r] = make_float2(st.m, st.s);
+            }
+        }
+        if (a.logits_grad) {
+            coef = live ? row_coef(a, r, t) : 0.0f;
+            const float share = coef / st.s;
+            if (live) store_shares<kLanes>(a, r, t, c, q, id);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const uint32_t at = (l + i * kLanes) * kN;
+                if (at >= a.labels) continue;
+                Chunk<T> o = {};
+                if (live) o = grad_chunk(held[i], st.m, c, share);
+                store_own(dz, at, 0u, a.labels, o);
+            }
+        }
+    }
+    if (!a.logits_grad) return;
+    __syncthreads();
+    if (live) write_shares(a, z, dz, q, id, st, c, coef, l, kLanes, 0u, a.labels);
 }
 
 // The rows' losses in one sum, always in the same order.
@@ -200,77 +503,440 @@ __device__ __forceinline__ uint32_t logit_order(float z) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <typename T> __global__ __launch_bounds__(256) void answer_kernel(AnswerArgs a) {
-    __shared__ float shared[4];
-    __shared__ uint64_t best[4];
-    const uint64_t r = blockIdx.x;
+__device__ __forceinline__ float order_logit(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+// Keys order labels by falling logit, then by rising label; 0 is no label.
+__device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t label) {
+    return (uint64_t)order << 32 | (0xffffffffu - label);
+}
+
+constexpr uint32_t kCandidates = 512;
+
+// The k-th largest of the wavefront's 64 values, bit by bit.
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t x, uint32_t k) {
+    uint32_t t = 0;
+    for (int b = 31; b >= 0; --b) {
+        const uint32_t with = t | 1u << b;
+        if ((uint32_t)__popcll(__ballot(x >= with)) >= k) t = with;
+    }
+    return t;
+}
+
+__device__ __forceinline__ void write_answer(const AnswerArgs &a, uint64_t r, float z_label, bool named,
+                                             const Part &st, float inv_t) {
+    const bool empty = st.s == 0.0f;
+    const float log_s = logf(st.s);
+    float lp = 0.0f;
+    if (named) lp = empty ? -INFINITY : (z_label - st.m) * inv_t - log_s;
+    a.log_prob[r] = lp;
+    a.entropy[r] = empty ? 0.0f : log_s - st.w / (st.s * kLog2e);
+    if (a.stats) a.stats[r] = make_float2(empty ? 0.0f : st.m, st.s);
+}
+__device__ __forceinline__ void write_best(const AnswerArgs &a, uint64_t r, uint32_t k, uint64_t key,
+                                           const Part &st, float inv_t, float log_s) {
+    const float z = order_logit((uint32_t)(key >> 32));
+    a.top_labels[r * a.top + k] = key ? (int64_t)(0xffffffffu - (uint32_t)key) : -1;
+    a.top_log_probs[r * a.top + k] =
+        key ? (z - st.m) * inv_t - log_s : (st.s != st.s ? st.s : -INFINITY);
+}
+
+// A block per row, or per slice of one where rows are few; one pass over the
+// logits for the softmax, its entropy and each thread's largest logit.
+// The best labels: the threads form 64 groups, and the top-th largest of the
+// groups' largest logits bounds the top-th best label from below.  Only
+// threads whose largest logit reaches the bound (about `top`) look at theirs
+// again; what reaches it is ranked by counting.
+// slices > 1: Part and keys of each slice, for join_kernel.
+template <typename T>
+__global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t slices,
+                                                         uint32_t slice, Part *out,
+                                                         uint64_t *out_keys) {
+    __shared__ Part parts[kStream / 64];
+    __shared__ uint32_t groups[64];
+    __shared__ uint64_t keys[kCandidates];
+    __shared__ uint32_t found;
+    const uint64_t r = blockIdx.x / slices;
+    const uint32_t part = blockIdx.x % slices, begin = part * slice;
+    const uint32_t end = min(a.labels, begin + slice);
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
-    const RowStats st = row_stats(z, a.labels, c, shared);
-    float w = 0.0f;
-    for (uint32_t v = threadIdx.x; v < a.labels; v += 256u) {
-        const float d = ((float)z[v] - st.m) * c;
-        // fmaxf: 0, not NaN, where the exponential has underflowed
-        w += fmaxf(d, -200.0f) * __builtin_amdgcn_exp2f(d);
+    // beside its largest logit, where the thread met it, and the largest of its
+    // other steps
+    Part mine = {-INFINITY, 0.0f, 0.0f};
+    float second = -INFINITY;
+    uint32_t where = begin;
+    for_chunks<kStream, kUnroll, true>(z, begin, end, [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i)
+#pragma unroll
+            for (int e = 0; e < Chunk<T>::kN; ++e) m = fmaxf(m, (float)ch[i].v[e]);
+        second = fmaxf(second, fminf(m, mine.m));
+        where = m > mine.m ? at : where;
+        absorb<true>(mine, ch, c);
+    });
+    const uint32_t best = logit_order(mine.m);
+    if (a.top) {
+        const uint32_t o = group_all<kStream / 64>(best, [](uint32_t x, uint32_t y) { return max(x, y); });
+        if (threadIdx.x % (kStream / 64) == 0) groups[threadIdx.x / (kStream / 64)] = o;
+        if (threadIdx.x == 0) found = 0;
     }
-    w = block_sum(w, shared);
-    const float log_s = logf(st.s);
-    const bool empty = st.s == 0.0f;
+    Part st = merge_block<true>(mine, parts, c);
+    if (slices == 1 && st.m == -INFINITY) st.m = 0.0f;
     if (threadIdx.x == 0) {
-        const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
-        float lp = 0.0f;
-        if (y >= 0) lp = empty ? -INFINITY : ((float)z[y] - st.m) * inv_t - log_s;
-        a.log_prob[r] = lp;
-        a.entropy[r] = empty ? 0.0f : log_s - w / (st.s * kLog2e);
-        if (a.stats) a.stats[r] = make_float2(st.m, st.s);
+        if (slices > 1) {
+            out[r * slices + part] = st;
+        } else {
+            const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
+            write_answer(a, r, y < 0 ? 0.0f : (float)z[y], y >= 0, st, inv_t);
+        }
     }
+    if (!a.top) return;
+    const float log_s = logf(st.s);
+    const auto emit = [&](uint32_t k, uint64_t key) {
+        if (slices > 1) out_keys[(r * slices + part) * a.top + k] = key;
+        else write_best(a, r, k, key, st, inv_t, log_s);
+    };
+    const uint32_t bound = max(kth_of_wave(groups[threadIdx.x & 63u], a.top), 1u);
+    if (best >= bound) {
+        const auto collect = [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
+#pragma unroll
+            for (int i = 0; i < kUnroll; ++i)
+#pragma unroll
+                for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
+                    const uint32_t o = logit_order((float)ch[i].v[e]);
+                    if (o < bound) continue;
+                    const uint32_t k = atomicAdd(&found, 1u);
+                    const uint32_t from = place<T>(at + i * kStream * Chunk<T>::kN, begin, end);
+                    if (k < kCandidates) keys[k] = key_of(o, from + e);
+                }
+        };
+        constexpr uint32_t kStep = kStream * Chunk<T>::kN * kUnroll;
+        const bool one = logit_order(second) < bound;
+        const uint32_t first = one ? where - threadIdx.x * Chunk<T>::kN : begin;
+        for_steps<kStream, kUnroll, true>(z, first, one ? min(end, first + kStep) : end, begin, end,
+                                          collect);
+    }
+    __syncthreads();
+    const uint32_t n = found;
+    if (n <= kCandidates) {
+        for (uint32_t i = threadIdx.x; i < n; i += kStream) {
+            const uint64_t key = keys[i];
+            uint32_t rank = 0;
+            for (uint32_t o = 0; o < n; ++o) rank += keys[o] > key;
+            if (rank < a.top) emit(rank, key);
+        }
+        if (threadIdx.x >= n && threadIdx.x < a.top) emit(threadIdx.x, 0);
+        return;
+    }
+    // more labels tie at the bound than there is room for: one pass for each
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top; ++k) {
         uint64_t key = 0;
-        for (uint32_t v = threadIdx.x; v < a.labels; v += 256u) {
-            const uint64_t o = logit_order((float)z[v]);
-            const uint64_t x = o << 32 | (0xffffffffu - v);
-            if (o != 0 && x < last && x > key) key = x;
-        }
+        for_chunks<kStream, 1, true>(z, begin, end, [&](const Chunk<T>(&ch)[1], uint32_t at) {
+#pragma unroll
+            for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
+                const uint32_t o = logit_order((float)ch[0].v[e]);
+                const uint64_t x = key_of(o, place<T>(at, begin, end) + e);
+                if (o != 0 && x < last && x > key) key = x;
+            }
+        });
         for (int d = 32; d > 0; d >>= 1) {
             const uint64_t o = __shfl_xor((unsigned long long)key, d);
             key = o > key ? o : key;
         }
         __syncthreads();
-        if ((threadIdx.x & 63u) == 0) best[threadIdx.x >> 6] = key;
+        if ((threadIdx.x & 63u) == 0) keys[threadIdx.x >> 6] = key;
         __syncthreads();
-        for (int i = 0; i < 4; ++i) key = best[i] > key ? best[i] : key;
-        if (threadIdx.x == 0) {
-            const uint32_t v = 0xffffffffu - (uint32_t)key;
-            a.top_labels[r * a.top + k] = key ? (int64_t)v : -1;
-            a.top_log_probs[r * a.top + k] = key ? ((float)z[v] - st.m) * inv_t - log_s : -INFINITY;
-        }
+        for (int i = 0; i < kStream / 64; ++i) key = keys[i] > key ? keys[i] : key;
+        if (threadIdx.x == 0) emit(k, key);
         last = key;
     }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a) {
+constexpr uint32_t kMaxSlices = 32; // of a row of answers
+
+// One row of its slices: their Parts merged, and the rank of each of their
+// keys: how many keys of every slice (sorted, so by halving) stand before it.
+template <typename T>
+__global__ __launch_bounds__(kStream) void join_kernel(AnswerArgs a, uint32_t slices,
+                                                       const Part *parts, const uint64_t *keys) {
+    __shared__ uint64_t all[kMaxSlices * kMaxTop];
     const uint64_t r = blockIdx.x;
+    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    Part st = merge_parts<true>(parts + r * slices, slices, c);
+    if (st.m == -INFINITY) st.m = 0.0f;
+    if (threadIdx.x == 0) {
+        const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
+        const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+        write_answer(a, r, y < 0 ? 0.0f : (float)z[y], y >= 0, st, inv_t);
+    }
+    const uint32_t n = slices * a.top;
+    for (uint32_t i = threadIdx.x; i < n; i += kStream) all[i] = keys[r * n + i];
+    __syncthreads();
+    const float log_s = logf(st.s);
+    for (uint32_t i = threadIdx.x; i < n; i += kStream) {
+        const uint64_t key = all[i];
+        uint32_t rank = 0; // a missing key (0) counts as after every other, in its own order
+        for (uint32_t s = 0; s < slices; ++s) {
+            const uint64_t *list = all + s * a.top;
+            uint32_t lo = 0, hi = a.top;
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (list[mid] > key) lo = mid + 1;
+                else hi = mid;
+            }
+            rank += lo;
+        }
+        if (key != 0 && rank < a.top) write_best(a, r, rank, key, st, inv_t, log_s);
+    }
+    // the labels there are, where they are fewer than asked for
+    uint32_t some = 0;
+    for (uint32_t i = threadIdx.x & 63u; i < n; i += 64u) some += all[i] != 0;
+    some = group_all<64>(some, [](uint32_t x, uint32_t y) { return x + y; });
+    if (threadIdx.x >= some && threadIdx.x < a.top)
+        write_best(a, r, threadIdx.x, 0, st, inv_t, log_s);
+}
+
+// Short rows: kLanes lanes a row, in their registers.  The best labels one
+// after the other: the largest of the lanes' largest logits, then the lowest
+// label that has it.
+template <typename T, int kLanes, int kHeld>
+__global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_t rows) {
+    constexpr uint32_t kN = Chunk<T>::kN;
+    const uint32_t l = threadIdx.x % kLanes;
+    const uint64_t r = ((uint64_t)blockIdx.x * 256u + threadIdx.x) / kLanes;
+    if (r >= rows) return; // a whole group
+    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
+    const float zy = y < 0 ? 0.0f : (float)z[y];
+    Chunk<T> held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        held[i] = load_raw(z, (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        mask_chunk(held[i], (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+    Part st = {-INFINITY, 0.0f, 0.0f};
+    absorb<true>(st, held, c);
+    merge_lanes<kLanes, true>(st, c);
+    if (st.m == -INFINITY) st.m = 0.0f;
+    if (l == 0) write_answer(a, r, zy, y >= 0, st, inv_t);
+    if (!a.top) return;
+    const float log_s = logf(st.s);
+    uint32_t o[kHeld * kN];
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld * kN; ++i) o[i] = logit_order((float)held[i / kN].v[i % kN]);
+    for (uint32_t k = 0; k < a.top; ++k) {
+        uint32_t best = 0, at = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld * kN; ++i)
+            if (o[i] > best) {
+                best = o[i];
+                at = i;
+            }
+        const uint32_t top = group_all<kLanes>(best, [](uint32_t x, uint32_t w) { return max(x, w); });
+        const uint32_t label =
+            place<T>((l + at / kN * kLanes) * kN, 0u, a.labels) + at % kN;
+        const uint32_t lowest =
+            group_all<kLanes>(best == top ? label : 0xffffffffu,
+                              [](uint32_t x, uint32_t w) { return min(x, w); });
+        if (l == 0) write_best(a, r, k, top ? key_of(top, lowest) : 0, st, inv_t, log_s);
+        if (label == lowest) {
+#pragma unroll
+            for (uint32_t i = 0; i < kHeld * kN; ++i) o[i] = i == at ? 0u : o[i];
+        }
+    }
+}
+
+// kLanes lanes a row (256: a block, or a tile of a row per block).
+template <typename T, int kLanes>
+__global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, uint64_t rows,
+                                                          uint32_t tiles, uint32_t tile) {
+    const uint64_t r = kLanes == 256 ? blockIdx.x / tiles
+                                     : ((uint64_t)blockIdx.x * 256u + threadIdx.x) / kLanes;
+    if (r >= rows) return;
+    const uint32_t begin = kLanes == 256 ? (uint32_t)(blockIdx.x % tiles) * tile : 0u;
+    const uint32_t end = min(a.labels, begin + tile);
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
     const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
     const float2 st = a.stats[r];
     const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
-    const float glp = a.log_prob_grad && y >= 0 ? a.log_prob_grad[r] : 0.0f;
-    const float gh = a.entropy_grad ? a.entropy_grad[r] : 0.0f;
-    const float log_s = logf(st.y), h = a.entropy[r];
-    for (uint32_t v = threadIdx.x; v < a.labels; v += 256u) {
-        float o = 0.0f;
-        if (!(st.y == 0.0f)) {
-            const float d = ((float)z[v] - st.x) * c;
-            const float p = __builtin_amdgcn_exp2f(d) / st.y;
-            const float log_p = fmaxf(d, -200.0f) / kLog2e - log_s;
-            o = -p * (glp + gh * (log_p + h));
-            if ((int32_t)v == y) o += glp;
+    const bool live = !(st.y == 0.0f);
+    const float glp = live && a.log_prob_grad && y >= 0 ? a.log_prob_grad[r] * inv_t : 0.0f;
+    const float gh = live && a.entropy_grad ? a.entropy_grad[r] * inv_t : 0.0f;
+    // -p (glp + gh (log p + H)) = -e / S (gh ln2 d + glp + gh (H - log S))
+    const float slope = gh / kLog2e, level = glp + gh * (a.entropy[r] - logf(st.y));
+    const float inv_s = live ? -1.0f / st.y : 0.0f;
+    map_chunks<kLanes, kUnroll>(z, dz, begin, end, [&](const Chunk<T> &ch, uint32_t at) {
+        Chunk<T> o;
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::kN; ++e) {
+            const float d = ((float)ch.v[e] - st.x) * c;
+            const float p = __builtin_amdgcn_exp2f(d) * inv_s;
+            float g = live ? p * fmaf(slope, fmaxf(d, -200.0f), level) : 0.0f;
+            if ((int32_t)(at + e) == y) g += glp;
+            o.v[e] = (T)g;
         }
-        dz[v] = (T)(o * inv_t);
-    }
+        return o;
+    });
 }
+
+// ---- which kernel --------------------------------------------------------------
+
+// f(first row, rows) for windows of rows: a launch holds fewer than 2^32 threads.
+template <typename F> void for_windows(uint64_t rows, F f) {
+    constexpr uint64_t kWindow = 1ull << 22;
+    for (uint64_t r = 0; r < rows; r += kWindow) f(r, rows - r < kWindow ? rows - r : kWindow);
+}
+template <typename P> P *advance(P *p, uint64_t bytes) {
+    return p ? (P *)((uintptr_t)p + bytes) : p;
+}
+size_t id_bytes(int id_type) { return id_type == SDF_ID_I64 ? 8 : 4; }
+
+DistillArgs from_row(DistillArgs a, int type, uint64_t r) {
+    a.logits = advance(a.logits, r * a.stride * type_bytes(type));
+    a.teacher_labels = advance(a.teacher_labels, r * a.top * id_bytes(a.id_type));
+    a.teacher_logits = advance(a.teacher_logits, r * a.top * type_bytes(a.teacher_type));
+    a.row_weight = advance(a.row_weight, 4 * r);
+    a.loss_grad = advance(a.loss_grad, 4 * r * a.loss_grad_stride);
+    a.loss = advance(a.loss, 4 * r);
+    a.stats = advance(a.stats, 8 * r);
+    a.logits_grad = advance(a.logits_grad, r * a.labels * type_bytes(type));
+    return a;
+}
+AnswerArgs from_row(AnswerArgs a, int type, uint64_t r) {
+    a.logits = advance(a.logits, r * a.stride * type_bytes(type));
+    a.label_ids = advance(a.label_ids, r * id_bytes(a.id_type));
+    a.log_prob = advance(a.log_prob, 4 * r);
+    a.entropy = advance(a.entropy, 4 * r);
+    a.top_log_probs = advance(a.top_log_probs, 4 * r * a.top);
+    a.top_labels = advance(a.top_labels, 8 * r * a.top);
+    a.stats = advance(a.stats, 8 * r);
+    a.log_prob_grad = advance(a.log_prob_grad, 4 * r);
+    a.entropy_grad = advance(a.entropy_grad, 4 * r);
+    a.logits_grad = advance(a.logits_grad, r * a.labels * type_bytes(type));
+    return a;
+}
+
+// Slices for rows that are too few to fill the chip: enough blocks of at least
+// 4,096 labels each; a multiple of a chunk long.
+struct Slices {
+    uint32_t count, length;
+};
+Slices slices_of(uint64_t rows, uint64_t labels, uint32_t most) {
+    uint64_t n = 1;
+    if (rows < 512) n = 1024 / (rows ? rows : 1);
+    n = n < labels / 4096 ? n : labels / 4096;
+    n = n < most ? n : most;
+    if (n < 2) return {1, (uint32_t)labels};
+    const uint64_t length = ((labels + n - 1) / n + 7) / 8 * 8;
+    return {(uint32_t)((labels + length - 1) / length), (uint32_t)length};
+}
+constexpr uint32_t kShort = 64 * 4; // chunks of a row that a wavefront holds
+
+// f(lanes, chunks held by each) of a short row, as types
+template <int kV> struct Int {
+    static constexpr int v = kV;
+};
+template <typename T, typename F> void with_short(uint64_t labels, F f) {
+    const uint64_t chunks = (labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    if (chunks <= 8) f(Int<8>(), Int<1>());
+    else if (chunks <= 16) f(Int<16>(), Int<1>());
+    else if (chunks <= 32) f(Int<16>(), Int<2>());
+    else if (chunks <= 64) f(Int<32>(), Int<2>());
+    else if (chunks <= 128) f(Int<64>(), Int<2>());
+    else f(Int<64>(), Int<4>());
+}
+
+template <typename T, bool kHaveStats>
+void launch_short(const DistillArgs &a, uint64_t rows, hipStream_t s) {
+    with_short<T>(a.labels, [&](auto lanes, auto held) {
+        constexpr uint32_t kLanes = decltype(lanes)::v;
+        const size_t row_bytes = a.logits_grad ? 8 * (size_t)a.top : 0;
+        uint32_t threads = 256; // fewer where the teacher's entries fill LDS
+        while (threads > 64 && threads / kLanes * row_bytes > 32768) threads /= 2;
+        const uint64_t per = threads / kLanes;
+        hipLaunchKernelGGL((distill_short_kernel<T, kLanes, decltype(held)::v, kHaveStats>),
+                           dim3((unsigned)((rows + per - 1) / per)), dim3(threads),
+                           (unsigned)(per * row_bytes), s, a, rows);
+    });
+}
+
+constexpr uint32_t kTile = 32768; // labels of a block of finish_kernel
+
+template <typename T>
+void launch_finish(const DistillArgs &a, uint64_t rows, const Part *parts, uint32_t slices,
+                   hipStream_t s) {
+    // where rows are few, as many blocks as the statistics had
+    const uint32_t tile = slices > 1 ? ((a.labels + slices - 1) / slices + 7) / 8 * 8 : kTile;
+    const uint32_t tiles = a.logits_grad ? (a.labels + tile - 1) / tile : 1;
+    hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(rows * tiles)), dim3(kStream), 0, s, a,
+                       tiles, a.logits_grad ? tile : a.labels, parts, slices);
+}
+
+template <typename T>
+void launch_distill(const DistillArgs &a, uint64_t rows, Part *parts, hipStream_t s) {
+    const uint64_t chunks = (a.labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    if (chunks <= kShort) return launch_short<T, false>(a, rows, s);
+    const Slices sl = slices_of(rows, a.labels, 64);
+    if (sl.count > 1) {
+        hipLaunchKernelGGL(part_kernel<T>, dim3((unsigned)(rows * sl.count)), dim3(kStream), 0, s,
+                           a, sl.count, sl.length, parts);
+        return launch_finish<T>(a, rows, parts, sl.count, s);
+    }
+    const auto launch = [&](auto threads, auto held) {
+        hipLaunchKernelGGL((distill_kernel<T, decltype(threads)::v, decltype(held)::v>),
+                           dim3((unsigned)rows), dim3(decltype(threads)::v), 0, s, a);
+    };
+    if (!a.logits_grad) return launch(Int<kStream>(), Int<0>());
+    if (chunks <= 256 * 4) launch(Int<256>(), Int<4>());
+    else if (chunks <= 512 * 4) launch(Int<512>(), Int<4>());
+    else if (chunks <= 512 * 8) launch(Int<512>(), Int<8>());
+    else launch(Int<1024>(), Int<8>());
+}
+
+template <typename T>
+void launch_answer(const AnswerArgs &a, uint64_t rows, const Slices &sl, void *scratch,
+                   hipStream_t s) {
+    const uint64_t chunks = (a.labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    if (chunks <= kShort) {
+        with_short<T>(a.labels, [&](auto lanes, auto held) {
+            constexpr uint32_t kLanes = decltype(lanes)::v;
+            hipLaunchKernelGGL((answer_short_kernel<T, kLanes, decltype(held)::v>),
+                               dim3((unsigned)((rows * kLanes + 255) / 256)), dim3(256), 0, s, a,
+                               rows);
+        });
+        return;
+    }
+    uint64_t *keys = static_cast<uint64_t *>(scratch);
+    Part *parts = reinterpret_cast<Part *>(keys + rows * sl.count * a.top);
+    hipLaunchKernelGGL(answer_kernel<T>, dim3((unsigned)(rows * sl.count)), dim3(kStream), 0, s, a,
+                       sl.count, sl.length, parts, keys);
+    if (sl.count > 1)
+        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)rows), dim3(kStream), 0, s, a, sl.count,
+                           parts, keys);
+}
+
+template <typename T> void launch_answer_grad(const AnswerArgs &a, uint64_t rows, hipStream_t s) {
+    const uint64_t chunks = (a.labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    const auto launch = [&](auto lanes) {
+        constexpr uint32_t kLanes = decltype(lanes)::v;
+        const uint32_t tile = kLanes == 256 ? 256 * Chunk<T>::kN * kUnroll : a.labels;
+        const uint32_t tiles = (a.labels + tile - 1) / tile;
+        hipLaunchKernelGGL((answer_grad_kernel<T, kLanes>),
+                           dim3((unsigned)((rows * tiles * kLanes + 255) / 256)), dim3(256), 0, s,
+                           a, rows, tiles, tile);
+    };
+    if (chunks <= 8 * kUnroll) launch(Int<8>());
+    else if (chunks <= 64 * kUnroll) launch(Int<64>());
+    else launch(Int<256>());
+}
+
+size_t align256(size_t x) { return (x + 255u) & ~(size_t)255u; }
 
 int check_logits(const char *what, int type, const void *logits, uint64_t rows, uint64_t labels,
                  uint64_t stride, int id_type, float temperature) {
@@ -309,8 +975,8 @@ int check_distill(const char *what, int type, const void *logits, uint64_t rows,
 extern "C" {
 
 size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels) {
-    (void)labels;
-    return 4 * rows + 256;
+    const Slices sl = slices_of(rows, labels, 64);
+    return align256(4 * rows) + (sl.count > 1 ? align256(rows * sl.count * sizeof(Part)) : 0) + 256;
 }
 
 int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, uint64_t stride,
@@ -337,11 +1003,12 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
                      teacher_logits, top, temperature, row_weight, loss_grad, none ? 1u : 0u,
                      reduce, none ? loss : static_cast<float *>(scratch),
                      reinterpret_cast<float2 *>(stats), logits_grad};
-    if (rows > 0)
-        with_type(type, [&](auto t) {
-            hipLaunchKernelGGL((distill_kernel<decltype(t), false>), dim3((unsigned)rows), dim3(256),
-                               0, s, a);
+    Part *parts = reinterpret_cast<Part *>(static_cast<char *>(scratch) + align256(4 * rows));
+    with_type(type, [&](auto t) {
+        for_windows(rows, [&](uint64_t r, uint64_t n) {
+            launch_distill<decltype(t)>(from_row(a, type, r), n, parts, s);
         });
+    });
     if (!none)
         hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, a.loss, rows, reduce, loss);
     const hipError_t e = hipGetLastError();
@@ -366,18 +1033,22 @@ int sdf_distill_backward(int type, const void *logits, uint64_t rows, uint64_t l
                      reduction == SDF_REDUCE_NONE ? 1u : 0u, reduce, nullptr,
                      reinterpret_cast<float2 *>(const_cast<float *>(stats)), logits_grad};
     with_type(type, [&](auto t) {
-        hipLaunchKernelGGL((distill_kernel<decltype(t), true>), dim3((unsigned)rows), dim3(256), 0,
-                           static_cast<hipStream_t>(stream), a);
+        using T = decltype(t);
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        const bool is_short = (labels + Chunk<T>::kN - 1) / Chunk<T>::kN <= kShort;
+        for_windows(rows, [&](uint64_t r, uint64_t n) {
+            const DistillArgs w = from_row(a, type, r);
+            if (is_short) launch_short<T, true>(w, n, s);
+            else launch_finish<T>(w, n, nullptr, 0, s);
+        });
     });
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SDF_OK : hip_fail(e, "distill_backward");
 }
 
 size_t sdf_label_log_probs_scratch_bytes(uint64_t rows, uint64_t labels, uint32_t top) {
-    (void)rows;
-    (void)labels;
-    (void)top;
-    return 256;
+    const Slices sl = slices_of(rows, labels, kMaxSlices);
+    return sl.count > 1 ? align256(rows * sl.count * (sizeof(Part) + 8 * (size_t)top)) + 256 : 256;
 }
 
 int sdf_label_log_probs(int type, const void *logits, uint64_t rows, uint64_t labels,
@@ -402,8 +1073,11 @@ int sdf_label_log_probs(int type, const void *logits, uint64_t rows, uint64_t la
                     log_prob, entropy, top_log_probs, top_labels,
                     reinterpret_cast<float2 *>(stats), nullptr, nullptr, nullptr};
     with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(answer_kernel<decltype(t)>, dim3((unsigned)rows), dim3(256), 0,
-                           static_cast<hipStream_t>(stream), a);
+        const Slices sl = slices_of(rows, labels, kMaxSlices);
+        for_windows(rows, [&](uint64_t r, uint64_t n) {
+            launch_answer<decltype(t)>(from_row(a, type, r), n, sl, scratch,
+                                       static_cast<hipStream_t>(stream));
+        });
     });
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SDF_OK : hip_fail(e, "label_log_probs");
@@ -425,8 +1099,10 @@ int sdf_label_log_probs_backward(int type, const void *logits, uint64_t rows, ui
                     reinterpret_cast<float2 *>(const_cast<float *>(stats)), log_prob_grad,
                     entropy_grad, logits_grad};
     with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(answer_grad_kernel<decltype(t)>, dim3((unsigned)rows), dim3(256), 0,
-                           static_cast<hipStream_t>(stream), a);
+        for_windows(rows, [&](uint64_t r, uint64_t n) {
+            launch_answer_grad<decltype(t)>(from_row(a, type, r), n,
+                                            static_cast<hipStream_t>(stream));
+        });
     });
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SDF_OK : hip_fail(e, "label_log_probs_backward");
