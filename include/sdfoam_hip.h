@@ -626,7 +626,7 @@ int sdf_delaunay_merge_verified(const float *points, uint32_t num_points,
 /* rows[i, :] = scale * weight[i] * table[cells[i], :] (weight NULL: 1), zeros
  * where cells[i] is no cell.  table [num_cells, width] with rows table_stride
  * apart, rows [count, width] contiguous, both of `type`; fewer than 2^31 cells
- * and ids. */
+ * and ids, rows of at most 2^18 elements. */
 int sdf_cell_rows(int type, const void *table, uint64_t table_stride,
                   uint64_t num_cells, uint32_t width, int id_type,
                   const void *cells, uint64_t count, const float *weight,
