@@ -110,59 +110,94 @@ template <typename T, int kP> __global__ __launch_bounds__(256) void rows_kernel
 
 // ---- the sort of the ids: stable, least significant digit first ---------------
 
-constexpr uint32_t kTile = 4096;     // keys of one block
-constexpr uint32_t kMaxBits = 11;    // of a digit
-constexpr uint32_t kScanTiles = 16;  // threads that share a digit's tiles
+constexpr uint32_t kSortThreads = 1024;
+constexpr uint32_t kSortWaves = kSortThreads / 64;
+constexpr uint32_t kSteps = 4;                       // keys per thread
+constexpr uint32_t kTile = kSteps * kSortThreads;    // keys of one block
+constexpr uint32_t kOneBlock = 16 * kSortThreads;    // keys that one block sorts alone
+constexpr uint32_t kMaxBits = 11;                 // of a digit
+constexpr uint32_t kScanParts = 16;               // threads that share a digit's tiles
+
+// The table's gradient is cleared by extra blocks of the sort's launches, which
+// leave the memory idle: each launch clears [begin, end) of it, `each` bytes a
+// block in stores of 16.  Few large shares: beside the sort's blocks a CU has
+// room (LDS) for one of these at a time.
+struct Clear {
+    char *to;
+    uint64_t begin, end, each;
+};
+constexpr uint32_t kClearStep = kSortThreads * 16 * 4;
+constexpr uint32_t kClearBlocks = 512;
+__device__ __forceinline__ void clear_block(const Clear &c, uint32_t block) {
+    const uint64_t begin = c.begin + block * c.each;
+    const uint64_t end = begin + c.each < c.end ? begin + c.each : c.end;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (uint64_t base = begin; base < end; base += kClearStep) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint64_t at = base + (k * kSortThreads + threadIdx.x) * 16ull;
+            if (at + 16 <= end) __builtin_memcpy(c.to + at, &zero, 16);
+            else
+                for (uint64_t b = at; b < end; ++b) c.to[b] = 0;
+        }
+    }
+}
 
 struct SortPass {
-    const void *ids; // first pass: the caller's ids; NULL: keys_in, index_in
+    const void *ids; // first pass: the caller's ids; NULL: `in`
     int id_type;
     uint32_t num_cells;
-    const uint32_t *keys_in, *index_in;
-    uint32_t *keys_out, *index_out;
+    const uint2 *in; // {key, position}
+    uint2 *out;
+    // the ids' factors move with them: gathered by position, each would cost a
+    // line of memory
+    const float *weight; // the caller's, in the first pass times `scale`; NULL: none
+    float scale;
+    float *weight_out;
     uint32_t *counts; // [tiles][digits], after the scan those of the tiles before
     uint32_t *totals; // [digits]
-    uint8_t *named;   // [num_cells] whether an id names the cell: cleared in the
-                      // first pass, written in the last
-    uint32_t n, tiles, shift, bits;
-    bool clear, mark;
+    uint32_t n, tiles, shift, bits, passes;
+    uint32_t blocks; // those after them clear
+    Clear clear;
 };
 
 // no cell sorts last
-__device__ __forceinline__ uint32_t sort_key(const SortPass &p, uint32_t i) {
-    if (!p.ids) return p.keys_in[i];
+__device__ __forceinline__ uint2 sort_item(const SortPass &p, uint32_t i) {
+    if (!p.ids) return p.in[i];
     const int32_t c = load_id(p.ids, p.id_type, i, p.num_cells);
-    return c < 0 ? p.num_cells : (uint32_t)c;
+    return make_uint2(c < 0 ? p.num_cells : (uint32_t)c, i);
 }
 
-__global__ __launch_bounds__(256) void sort_count_kernel(SortPass p) {
-    __shared__ uint32_t hist[1u << kMaxBits];
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortPass p) {
+    extern __shared__ uint32_t hist[];
+    if (blockIdx.x >= p.blocks) return clear_block(p.clear, blockIdx.x - p.blocks);
     const uint32_t digits = 1u << p.bits;
-    for (uint32_t d = threadIdx.x; d < digits; d += 256u) hist[d] = 0;
-    __syncthreads();
     const uint32_t base = blockIdx.x * kTile;
-#pragma unroll 4
-    for (uint32_t j = threadIdx.x; j < kTile; j += 256u)
-        if (base + j < p.n)
-            atomicAdd(&hist[(sort_key(p, base + j) >> p.shift) & (digits - 1)], 1u);
-    if (p.clear) { // 16 bytes a thread; the array is padded to them
-        uint4 *named = reinterpret_cast<uint4 *>(p.named);
-        const uint32_t words = (p.num_cells + 15u) / 16u;
-        for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < words; i += gridDim.x * 256u)
-            named[i] = make_uint4(0, 0, 0, 0);
+    uint32_t key[kSteps];
+#pragma unroll
+    for (uint32_t r = 0; r < kSteps; ++r) {
+        const uint32_t i = base + r * kSortThreads + threadIdx.x;
+        key[r] = i < p.n ? sort_item(p, i).x : 0u;
     }
+    for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
     __syncthreads();
-    for (uint32_t d = threadIdx.x; d < digits; d += 256u)
+#pragma unroll
+    for (uint32_t r = 0; r < kSteps; ++r)
+        if (base + r * kSortThreads + threadIdx.x < p.n)
+            atomicAdd(&hist[(key[r] >> p.shift) & (digits - 1)], 1u);
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads)
         p.counts[(uint64_t)blockIdx.x * digits + d] = hist[d];
 }
 
 // Per digit, the exclusive sums over the tiles and the total: 64 digits a
-// block, kScanTiles threads each with a run of tiles.
-__global__ __launch_bounds__(64 * kScanTiles) void sort_scan_kernel(SortPass p) {
-    __shared__ uint32_t sums[kScanTiles][64];
+// block, kScanParts threads each with a run of tiles.
+__global__ __launch_bounds__(64 * kScanParts) void sort_scan_kernel(SortPass p) {
+    __shared__ uint32_t sums[kScanParts][64];
+    if (blockIdx.x >= p.blocks) return clear_block(p.clear, blockIdx.x - p.blocks);
     const uint32_t digits = 1u << p.bits;
     const uint32_t d = blockIdx.x * 64u + (threadIdx.x & 63u), part = threadIdx.x >> 6;
-    const uint32_t each = (p.tiles + kScanTiles - 1) / kScanTiles;
+    const uint32_t each = (p.tiles + kScanParts - 1) / kScanParts;
     const uint32_t lo = min(part * each, p.tiles), hi = min(lo + each, p.tiles);
     uint32_t s = 0;
     if (d < digits)
@@ -171,7 +206,7 @@ __global__ __launch_bounds__(64 * kScanTiles) void sort_scan_kernel(SortPass p) 
     sums[part][threadIdx.x & 63u] = s;
     __syncthreads();
     uint32_t before = 0, total = 0;
-    for (uint32_t k = 0; k < kScanTiles; ++k) {
+    for (uint32_t k = 0; k < kScanParts; ++k) {
         const uint32_t v = sums[k][threadIdx.x & 63u];
         if (k < part) before += v;
         total += v;
@@ -186,75 +221,164 @@ __global__ __launch_bounds__(64 * kScanTiles) void sort_scan_kernel(SortPass p) 
     }
 }
 
-// Each wavefront ranks 1,024 consecutive keys: the lanes of equal digits find
-// each other by one ballot per bit, a counter per digit in LDS carries the
-// rank from one step of 64 keys to the next.
-__global__ __launch_bounds__(256) void sort_scatter_kernel(SortPass p) {
-    __shared__ uint32_t seen[4][1u << kMaxBits];
-    __shared__ uint32_t waves[4];
+// One tile's items, and what a block needs of LDS to put them in order by a
+// digit: counters per wavefront and digit, and in their place the items.
+template <uint32_t kSteps> struct Tile {
+    uint2 item[kSteps];
+    float f[kSteps];
+};
+unsigned order_bytes(uint32_t bits, size_t item_bytes) {
+    const size_t counters = kSortWaves * sizeof(uint16_t) << bits;
+    return (unsigned)((sizeof(uint32_t) << bits) + (counters > item_bytes ? counters : item_bytes));
+}
+
+// Orders a tile of `count` items by the digit at p.shift, stably, into LDS
+// (kFactors: and their factors behind them).  Thread t has items (t / 64) * 64
+// kSteps + r * 64 + t % 64.  Each wavefront ranks its own: the lanes of equal
+// digits find each other by one ballot per bit, and the wavefront's counter of
+// the digit carries the rank from one step of 64 to the next.  to_output: also
+// shift[digit], from a place in the tile to one in the whole output.
+template <bool kFactors, uint32_t kSteps>
+__device__ __forceinline__ uint2 *order_tile(const SortPass &p, Tile<kSteps> &x, uint32_t count,
+                                             bool to_output, uint32_t *shift, uint2 *waves) {
     const uint32_t digits = 1u << p.bits;
+    uint16_t *seen = reinterpret_cast<uint16_t *>(shift + digits); // [kSortWaves][digits]
     const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
-    for (uint32_t d = threadIdx.x; d < digits; d += 256u)
-        for (uint32_t k = 0; k < 4u; ++k) seen[k][d] = 0;
-    __syncthreads();
-    const uint32_t base = blockIdx.x * kTile + w * (kTile / 4);
-    uint32_t key[16], rank[16];
+    const uint32_t base = w * (kSteps * 64);
+    constexpr uint32_t kEach = (1u << kMaxBits) / kSortThreads; // digits per thread at most
+    const uint32_t each = (digits + kSortThreads - 1) / kSortThreads, lo = threadIdx.x * each;
+    uint32_t total[kEach], earlier[kEach], here[kEach], rank[kSteps];
 #pragma unroll
-    for (uint32_t r = 0; r < 16u; ++r) {
-        const uint32_t i = base + r * 64u + lane;
-        key[r] = i < p.n ? sort_key(p, i) : 0u;
+    for (uint32_t k = 0; k < kEach; ++k) {
+        const bool has = to_output && k < each && lo + k < digits;
+        total[k] = has ? p.totals[lo + k] : 0u;
+        earlier[k] = has ? p.counts[(uint64_t)blockIdx.x * digits + lo + k] : 0u;
     }
+    uint16_t *own = seen + w * digits;
+    for (uint32_t d = lane; d < digits; d += 64u) own[d] = 0;
+    wave_sync();
 #pragma unroll
-    for (uint32_t r = 0; r < 16u; ++r) {
-        const bool in = base + r * 64u + lane < p.n;
-        const uint32_t d = (key[r] >> p.shift) & (digits - 1);
+    for (uint32_t r = 0; r < kSteps; ++r) {
+        const bool in = base + r * 64u + lane < count;
+        const uint32_t d = (x.item[r].x >> p.shift) & (digits - 1);
         uint64_t same = __ballot(in);
         for (uint32_t b = 0; b < p.bits; ++b) {
             const uint64_t set = __ballot((d >> b) & 1u);
             same &= (d >> b) & 1u ? set : ~set;
         }
         const uint32_t below = __popcll(same & ((1ull << lane) - 1ull));
-        uint32_t first = 0;
-        if (in && below == 0) first = atomicAdd(&seen[w][d], (uint32_t)__popcll(same));
-        const int leader = in ? __ffsll((unsigned long long)same) - 1 : (int)lane;
-        rank[r] = __shfl(first, leader) + below;
-        if (p.mark) { // ids of one cell stand side by side by now
-            const uint32_t left = __shfl_up(key[r], 1);
-            if (in && key[r] < p.num_cells && (lane == 0 || left != key[r])) p.named[key[r]] = 1;
-        }
+        const uint32_t so_far = own[d];
+        rank[r] = so_far + below;
+        wave_sync(); // every lane has read before the first of each digit adds
+        if (in && below == 0) own[d] = (uint16_t)(so_far + (uint32_t)__popcll(same));
+        wave_sync();
     }
     __syncthreads();
-    // where each digit starts: runs of digits / 256 of them per thread
-    const uint32_t each = (digits + 255u) / 256u, lo = threadIdx.x * each;
-    uint32_t mine = 0;
-    for (uint32_t d = lo; d < lo + each && d < digits; ++d) mine += p.totals[d];
-    uint32_t s = mine;
+    // where each digit starts: in the output (x) and in this tile (y)
+    uint2 mine = make_uint2(0u, 0u);
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+        here[k] = 0;
+        if (k < each && lo + k < digits)
+            for (uint32_t v = 0; v < kSortWaves; ++v) here[k] += seen[v * digits + lo + k];
+        mine.x += total[k];
+        mine.y += here[k];
+    }
+    uint2 s = mine;
     for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const uint32_t o = __shfl_up(s, d);
-        if (lane >= d) s += o;
+        const uint32_t a = __shfl_up(s.x, d), b = __shfl_up(s.y, d);
+        if (lane >= d) s.x += a, s.y += b;
     }
     if (lane == 63u) waves[w] = s;
     __syncthreads();
-    uint32_t start = s - mine;
-    for (uint32_t k = 0; k < w; ++k) start += waves[k];
-    for (uint32_t d = lo; d < lo + each && d < digits; ++d) {
-        uint32_t at = start + p.counts[(uint64_t)blockIdx.x * digits + d];
-        for (uint32_t k = 0; k < 4u; ++k) {
-            const uint32_t c = seen[k][d];
-            seen[k][d] = at;
-            at += c;
+    uint32_t out = s.x - mine.x, in_tile = s.y - mine.y;
+    for (uint32_t k = 0; k < w; ++k) out += waves[k].x, in_tile += waves[k].y;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+        if (k >= each || lo + k >= digits) break;
+        shift[lo + k] = out + earlier[k] - in_tile;
+        uint32_t at = in_tile;
+        for (uint32_t v = 0; v < kSortWaves; ++v) {
+            uint16_t &c = seen[v * digits + lo + k];
+            const uint32_t was = c;
+            c = (uint16_t)at;
+            at += was;
         }
-        start += p.totals[d];
+        out += total[k];
+        in_tile += here[k];
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t r = 0; r < 16u; ++r) {
-        const uint32_t i = base + r * 64u + lane;
-        if (i >= p.n) continue;
-        const uint32_t to = seen[w][(key[r] >> p.shift) & (digits - 1)] + rank[r];
-        p.keys_out[to] = key[r];
-        p.index_out[to] = p.ids ? i : p.index_in[i];
+    for (uint32_t r = 0; r < kSteps; ++r)
+        rank[r] += own[(x.item[r].x >> p.shift) & (digits - 1)];
+    __syncthreads(); // the items take the counters' place
+    uint2 *tile = reinterpret_cast<uint2 *>(seen);
+    float *factor = reinterpret_cast<float *>(tile + kSteps * kSortThreads);
+#pragma unroll
+    for (uint32_t r = 0; r < kSteps; ++r)
+        if (base + r * 64u + lane < count) {
+            tile[rank[r]] = x.item[r];
+            if (kFactors && p.weight) factor[rank[r]] = x.f[r];
+        }
+    __syncthreads();
+    return tile;
+}
+template <bool kFactors, uint32_t kSteps>
+__device__ __forceinline__ void load_tile(const SortPass &p, uint32_t begin, Tile<kSteps> &x) {
+#pragma unroll
+    for (uint32_t r = 0; r < kSteps; ++r) {
+        const uint32_t i = begin + (threadIdx.x >> 6) * (kSteps * 64) + r * 64u + (threadIdx.x & 63u);
+        x.item[r] = i < p.n ? sort_item(p, i) : make_uint2(0u, 0u);
+        x.f[r] = kFactors && p.weight && i < p.n ? p.scale * p.weight[i] : 0.0f;
     }
+}
+
+// Puts a tile in order and writes it from LDS: lanes side by side then write
+// side by side (1M ids with factors, 10-bit digits: 16 us; 22 us without).
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) {
+    extern __shared__ uint32_t shift[];
+    __shared__ uint2 waves[kSortWaves];
+    if (blockIdx.x >= p.blocks) return clear_block(p.clear, blockIdx.x - p.blocks);
+    const uint32_t begin = blockIdx.x * kTile, count = min(kTile, p.n - begin);
+    Tile<kSteps> x;
+    load_tile<true>(p, begin, x);
+    const uint2 *tile = order_tile<true>(p, x, count, true, shift, waves);
+    const float *factor = reinterpret_cast<const float *>(tile + kTile);
+#pragma unroll
+    for (uint32_t r = 0; r < kSteps; ++r) {
+        const uint32_t k = r * kSortThreads + threadIdx.x;
+        if (k >= count) break;
+        const uint2 y = tile[k];
+        const uint32_t to = k + shift[(y.x >> p.shift) & ((1u << p.bits) - 1)];
+        p.out[to] = y;
+        if (p.weight) p.weight_out[to] = factor[k];
+    }
+}
+
+// At most kSteps * kSortThreads ids: every pass in one block, without leaving
+// LDS.  The factors stay where they are: so few are read by position from L2.
+template <uint32_t kSteps>
+__global__ __launch_bounds__(kSortThreads) void sort_block_kernel(SortPass p) {
+    extern __shared__ uint32_t shift[];
+    __shared__ uint2 waves[kSortWaves];
+    if (blockIdx.x >= p.blocks) return clear_block(p.clear, blockIdx.x - p.blocks);
+    Tile<kSteps> x;
+    load_tile<false>(p, 0, x);
+    const uint2 *tile = nullptr;
+    for (uint32_t k = 0; k < p.passes; ++k) {
+        if (k > 0) {
+#pragma unroll
+            for (uint32_t r = 0; r < kSteps; ++r) {
+                const uint32_t i =
+                    (threadIdx.x >> 6) * (kSteps * 64) + r * 64u + (threadIdx.x & 63u);
+                if (i < p.n) x.item[r] = tile[i];
+            }
+            __syncthreads();
+        }
+        p.shift = k * p.bits;
+        tile = order_tile<false>(p, x, p.n, false, shift, waves);
+    }
+    for (uint32_t k = threadIdx.x; k < p.n; k += kSortThreads) p.out[k] = tile[k];
 }
 
 // ---- the sums -------------------------------------------------------------------
@@ -268,22 +392,19 @@ struct SumsArgs {
     const void *grad;
     uint64_t stride;
     uint32_t width, num_cells;
-    const uint32_t *keys, *index; // padded to whole tiles, the padding not read as ids
+    const uint2 *order; // {cell, position} of the ids, sorted by cell
     uint32_t n, tile, tiles;
-    const float *weight;
+    const float *factor; // scale and weight in the order of `order`; NULL:
+    const float *weight; // the caller's (NULL: 1), times scale
     float scale;
     float *partial; // [tiles][2][width]
     void *table_grad;
     const void *table; // with weight_grad
     uint64_t table_stride;
     float *weight_grad; // NULL: not formed here
-    const uint8_t *named;
-    uint32_t sum_blocks; // the blocks after them clear the cells that no id names
-    uint32_t clear_rows; // rows a block
-    Divisor pieces;
 };
 
-constexpr int kBatch = 8; // rows in flight per lane
+constexpr int kBatch = 4; // rows in flight per lane
 
 template <typename T, int kP, int kLanes>
 __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint32_t piece, uint32_t l) {
@@ -292,10 +413,10 @@ __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint3
     const bool mine = piece * kP < a.width; // lanes past the row hold nothing
     const uint32_t col = mine ? column<kP>(piece, a.width) : 0u;
     const uint32_t p0 = tile * a.tile, p1 = min(p0 + a.tile, a.n);
-    const uint32_t before = p0 > 0 ? a.keys[p0 - 1] : a.num_cells;
-    const uint32_t after = p1 < a.n ? a.keys[p1] : a.num_cells;
+    const uint32_t before = p0 > 0 ? a.order[p0 - 1].x : a.num_cells;
+    const uint32_t after = p1 < a.n ? a.order[p1].x : a.num_cells;
     float acc[kP] = {};
-    uint32_t cell = a.keys[p0];
+    uint32_t cell = a.order[p0].x;
     bool open = cell == before; // the first cell began in an earlier tile
     const auto flush = [&](bool goes_on) {
         if (!mine || cell >= a.num_cells) return;
@@ -316,14 +437,16 @@ __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint3
         Piece<T, kP> g[kBatch], t[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const uint32_t at = min(p + b, p1 - 1);
-            key[b] = a.keys[at];
-            index[b] = a.index[at];
+            const uint2 id = a.order[min(p + b, p1 - 1)];
+            key[b] = id.x;
+            index[b] = id.y;
+            f[b] = a.factor ? a.factor[min(p + b, p1 - 1)] : a.scale;
         }
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const bool live = p + b < p1 && key[b] < a.num_cells;
-            f[b] = live ? (a.weight ? a.scale * a.weight[index[b]] : a.scale) : 0.0f;
+            if (a.weight && !a.factor) f[b] *= a.weight[index[b]];
+            f[b] = live ? f[b] : 0.0f;
             g[b] = {};
             if (live && mine) g[b] = load_piece<T, kP>(grad + (uint64_t)index[b] * a.stride + col);
             if (a.weight_grad) {
@@ -365,32 +488,18 @@ __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint3
 
 template <typename T, int kP, int kLanes>
 __global__ __launch_bounds__(256) void sums_kernel(SumsArgs a) {
-    if (blockIdx.x < a.sum_blocks) {
-        const uint32_t tile = (blockIdx.x * 256u + threadIdx.x) / kLanes, l = threadIdx.x % kLanes;
-        if (tile < a.tiles) sum_tile<T, kP, kLanes>(a, tile, blockIdx.y * kLanes + l, l);
-        return;
-    }
-    if (blockIdx.y > 0) return;
-    const uint64_t r0 = (uint64_t)(blockIdx.x - a.sum_blocks) * a.clear_rows;
-    const uint32_t rows = (uint32_t)min((uint64_t)a.clear_rows, a.num_cells - r0);
-    const Piece<T, kP> zero = {};
-    for (uint32_t t = threadIdx.x; t < rows * a.pieces.d; t += 256u) {
-        const uint32_t row = t / a.pieces;
-        if (a.n > 0 && a.named[r0 + row]) continue;
-        store_piece<T, kP>(static_cast<T *>(a.table_grad) + (r0 + row) * a.width +
-                               column<kP>(t - row * a.pieces.d, a.width),
-                           zero);
-    }
+    const uint32_t tile = (blockIdx.x * 256u + threadIdx.x) / kLanes, l = threadIdx.x % kLanes;
+    if (tile < a.tiles) sum_tile<T, kP, kLanes>(a, tile, blockIdx.y * kLanes + l, l);
 }
 
-constexpr uint32_t kLong = 16; // tiles that one group adds by itself
-
 // The cells that go on past the tile they begin in: their tiles' sums in order.
-// A cell of more than kLong tiles is added by the whole block, every group a
-// share of its tiles.
+// A group of lanes looks at the tiles that follow its own, one a lane (16 at
+// least); where the cell goes on past those, the whole block adds its sums,
+// every group a share of the tiles.
 template <typename T, int kP, int kLanes>
 __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
     constexpr uint32_t kGroups = 256 / kLanes;
+    constexpr uint32_t kProbes = kLanes < 16 ? 16 / kLanes : 1, kNear = kProbes * kLanes;
     __shared__ uint32_t list[kGroups];
     __shared__ uint32_t listed;
     __shared__ float sums[kGroups][kLanes * kP];
@@ -400,10 +509,28 @@ __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
     const uint32_t col = mine ? column<kP>(piece, a.width) : 0u;
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    const auto slot = [&](uint32_t t, uint32_t k) {
-        return a.partial + ((uint64_t)t * 2 + k) * a.width + col;
+    const auto goes_on = [&](uint32_t t, uint32_t cell) {
+        return t < a.tiles && a.order[(uint64_t)t * a.tile].x == cell;
     };
-    const auto starts = [&](uint32_t t) { return a.keys[(uint64_t)t * a.tile]; };
+    // s += the sums of `count` tiles from `first` on, `step` apart
+    const auto add = [&](float *s, uint32_t first, uint32_t count, uint32_t step) {
+        for (uint32_t k = 0; k < count; k += 8) {
+            float x[8][kP];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                const uint32_t t = first + min(k + u, count - 1) * step;
+                __builtin_memcpy(x[u], a.partial + (uint64_t)t * 2 * a.width + col, sizeof(x[u]));
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u)
+                if (k + u < count)
+#pragma unroll
+                    for (int e = 0; e < kP; ++e) s[e] += x[u][e];
+        }
+    };
+    const auto begun = [&](float *s, uint32_t t) {
+        __builtin_memcpy(s, a.partial + ((uint64_t)t * 2 + 1) * a.width + col, kP * sizeof(float));
+    };
     const auto write = [&](uint32_t cell, const float *s) {
         if (!mine) return;
         Piece<T, kP> o;
@@ -412,47 +539,49 @@ __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
         store_piece<T, kP>(static_cast<T *>(a.table_grad) + (uint64_t)cell * a.width + col, o);
     };
     if (tile + 1 < a.tiles) {
-        const uint32_t p0 = tile * a.tile, cell = a.keys[p0 + a.tile - 1];
-        const bool whole = p0 > 0 && a.keys[p0 - 1] == cell; // then the tile is all of that cell
-        if (cell < a.num_cells && starts(tile + 1) == cell && !whole) {
-            if (tile + kLong < a.tiles && starts(tile + kLong) == cell) {
-                if (l == 0) list[atomicAdd(&listed, 1u)] = tile;
-            } else {
-                float s[kP];
+        const uint32_t p0 = tile * a.tile, cell = a.order[p0 + a.tile - 1].x;
+        const bool whole = p0 > 0 && a.order[p0 - 1].x == cell; // the tile is all of that cell
+        uint32_t near = 0; // the following tiles that begin with it: the first so many
+        if (cell < a.num_cells && !whole) {
 #pragma unroll
-                for (int e = 0; e < kP; ++e) s[e] = slot(tile, 1)[e];
-                for (uint32_t t = tile + 1; t < a.tiles && starts(t) == cell; ++t) {
-                    const float *x = slot(t, 0);
-#pragma unroll
-                    for (int e = 0; e < kP; ++e) s[e] += x[e];
-                }
-                write(cell, s);
-            }
+            for (uint32_t q = 0; q < kProbes; ++q)
+                near += goes_on(tile + 1 + q * kLanes + l, cell);
+        }
+        near = group_all<kLanes>(near, [](uint32_t x, uint32_t y) { return x + y; });
+        if (near == kNear) {
+            if (l == 0) list[atomicAdd(&listed, 1u)] = tile;
+        } else if (near > 0) {
+            float s[kP];
+            begun(s, tile);
+            add(s, tile + 1, near, 1);
+            write(cell, s);
         }
     }
     __syncthreads();
     const uint32_t n = listed; // the order of the list does not matter: each has its own cell
     for (uint32_t i = 0; i < n; ++i) {
-        const uint32_t first = list[i], cell = a.keys[(uint64_t)(first + 1) * a.tile - 1];
-        uint32_t lo = first + kLong, hi = a.tiles; // the first tile that does not start with it
-        while (lo + 1 < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (starts(mid) == cell) lo = mid;
-            else hi = mid;
+        const uint32_t first = list[i] + 1, cell = a.order[(uint64_t)first * a.tile].x;
+        // the tiles that begin with it, counted by 256 probes at a time
+        uint32_t lo = 0, range = a.tiles - first;
+        while (range > 0) {
+            const uint32_t step = (range + 255u) / 256u;
+            const uint32_t at = lo + threadIdx.x * step;
+            const uint32_t c = __syncthreads_count(threadIdx.x * step < range && goes_on(first + at, cell));
+            if (step == 1) {
+                lo += c;
+                break;
+            }
+            // the last probe that met it is `lo`; from there on, fewer than step
+            lo += (c - 1) * step;
+            range = min(step, range - (c - 1) * step);
         }
         float s[kP] = {};
-#pragma unroll 4
-        for (uint32_t t = first + 1 + g; t < hi; t += kGroups) {
-            const float *x = slot(t, 0);
-#pragma unroll
-            for (int e = 0; e < kP; ++e) s[e] += x[e];
-        }
+        if (g < lo) add(s, first + g, (lo - g + kGroups - 1) / kGroups, kGroups);
 #pragma unroll
         for (int e = 0; e < kP; ++e) sums[g][l * kP + e] = s[e];
         __syncthreads();
         if (g == 0) {
-#pragma unroll
-            for (int e = 0; e < kP; ++e) s[e] = slot(first, 1)[e];
+            begun(s, first - 1);
             for (uint32_t k = 0; k < kGroups; ++k)
 #pragma unroll
                 for (int e = 0; e < kP; ++e) s[e] += sums[k][l * kP + e];
@@ -540,7 +669,7 @@ Sort sort_of(uint64_t num_cells, uint64_t count) {
 }
 
 struct Layout {
-    size_t keys[2], index[2], counts, totals, named, partial, bytes;
+    size_t order[2], factor[2], counts, totals, partial, bytes;
 };
 Layout layout_of(int type_size, uint64_t num_cells, uint32_t width, uint64_t count) {
     const uint32_t p = 16 / type_size;
@@ -555,13 +684,10 @@ Layout layout_of(int type_size, uint64_t num_cells, uint32_t width, uint64_t cou
         at += align256(bytes);
         return was;
     };
-    for (int k = 0; k < 2; ++k) {
-        o.keys[k] = take(4 * count);
-        o.index[k] = take(4 * count);
-    }
+    for (size_t &order : o.order) order = take(8 * count);
+    for (size_t &factor : o.factor) factor = take(4 * count);
     o.counts = take(4ull * s.tiles << s.bits);
     o.totals = take(4ull << s.bits);
-    o.named = take(num_cells);
     o.partial = take(tiles * 2 * width * 4);
     o.bytes = at + 256;
     return o;
@@ -648,39 +774,72 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
     char *at = static_cast<char *>(scratch);
     const Layout lay = layout_of((int)type_bytes(type), num_cells, width, count);
     SumsArgs a = {};
-    if (sum && n > 0) {
+    if (sum) {
+        // the launches of the sort clear the gradient between them
         const Sort so = sort_of(num_cells, count);
+        const uint64_t bytes = num_cells * width * type_bytes(type);
+        const bool alone = n <= kOneBlock;
+        const uint32_t launches = alone ? 1 : 3 * so.passes;
+        const uint64_t share = (bytes / launches + kClearStep) / kClearStep * kClearStep;
+        uint64_t cleared = 0;
         SortPass p = {};
+        // blocks of the next launch: `work` of them for the sort
+        const auto with_clear = [&](uint32_t work) {
+            const uint64_t end = cleared + share < bytes ? cleared + share : bytes;
+            const uint64_t size = end - cleared;
+            const uint64_t each = (size / kClearBlocks + kClearStep) / kClearStep * kClearStep;
+            p.blocks = work;
+            p.clear = {static_cast<char *>(table_grad), cleared, end, each};
+            cleared = end;
+            return dim3((unsigned)(work + (size + each - 1) / each));
+        };
         p.ids = cells;
         p.id_type = id_type;
         p.num_cells = cells_n;
         p.counts = reinterpret_cast<uint32_t *>(at + lay.counts);
         p.totals = reinterpret_cast<uint32_t *>(at + lay.totals);
-        p.named = reinterpret_cast<uint8_t *>(at + lay.named);
         p.n = n;
         p.tiles = so.tiles;
         p.bits = so.bits;
-        for (uint32_t k = 0; k < so.passes; ++k) {
+        p.passes = so.passes;
+        const auto pass = [&](uint32_t k) {
             p.shift = k * so.bits;
-            p.clear = k == 0;
-            p.mark = k + 1 == so.passes;
-            p.keys_out = reinterpret_cast<uint32_t *>(at + lay.keys[k & 1]);
-            p.index_out = reinterpret_cast<uint32_t *>(at + lay.index[k & 1]);
-            hipLaunchKernelGGL(sort_count_kernel, dim3(so.tiles), dim3(256), 0, s, p);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3(((1u << so.bits) + 63u) / 64u),
-                               dim3(64 * kScanTiles), 0, s, p);
-            hipLaunchKernelGGL(sort_scatter_kernel, dim3(so.tiles), dim3(256), 0, s, p);
-            p.ids = nullptr;
-            p.keys_in = p.keys_out;
-            p.index_in = p.index_out;
+            p.out = reinterpret_cast<uint2 *>(at + lay.order[k & 1]);
+            p.weight = k == 0 ? weight : p.weight_out;
+            p.scale = k == 0 ? scale : 1.0f;
+            if (weight) p.weight_out = reinterpret_cast<float *>(at + lay.factor[k & 1]);
+        };
+        if (alone) {
+            pass(0);
+            const dim3 grid = with_clear(n > 0 ? 1 : 0);
+            if (n <= kTile)
+                hipLaunchKernelGGL(sort_block_kernel<kSteps>, grid, dim3(kSortThreads),
+                                   order_bytes(so.bits, 8 * kTile), s, p);
+            else
+                hipLaunchKernelGGL(sort_block_kernel<16>, grid, dim3(kSortThreads),
+                                   order_bytes(so.bits, 8 * kOneBlock), s, p);
+        } else {
+            for (uint32_t k = 0; k < so.passes; ++k) {
+                pass(k);
+                dim3 grid = with_clear(so.tiles);
+                hipLaunchKernelGGL(sort_count_kernel, grid, dim3(kSortThreads), 4u << so.bits, s, p);
+                grid = with_clear(((1u << so.bits) + 63u) / 64u);
+                hipLaunchKernelGGL(sort_scan_kernel, grid, dim3(64 * kScanParts), 0, s, p);
+                grid = with_clear(so.tiles);
+                hipLaunchKernelGGL(sort_scatter_kernel, grid, dim3(kSortThreads),
+                                   order_bytes(so.bits, 12 * kTile), s, p);
+                p.ids = nullptr;
+                p.in = p.out;
+            }
+            a.factor = p.weight_out;
         }
-        a.keys = p.keys_out;
-        a.index = p.index_out;
+        a.weight = weight;
+        a.order = p.out;
     }
     with_piece(type, width, [&](auto t, auto kp) {
         using T = decltype(t);
         constexpr int kP = decltype(kp)::v;
-        if (sum)
+        if (sum && n > 0)
             with_lanes(pieces, [&](auto lanes) {
                 constexpr int kLanes = decltype(lanes)::v;
                 a.grad = rows_grad;
@@ -690,24 +849,17 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
                 a.n = n;
                 a.tile = tile_of(count, pieces);
                 a.tiles = (n + a.tile - 1) / a.tile;
-                a.weight = weight;
                 a.scale = scale;
                 a.partial = reinterpret_cast<float *>(at + lay.partial);
                 a.table_grad = table_grad;
                 a.table = table;
                 a.table_stride = table_stride;
                 a.weight_grad = beside ? weight_grad : nullptr;
-                a.named = reinterpret_cast<const uint8_t *>(at + lay.named);
-                a.pieces = divisor(pieces);
-                a.sum_blocks = (uint32_t)(((uint64_t)a.tiles * kLanes + 255) / 256);
-                a.clear_rows = pieces < 2048 ? 2048 / pieces : 1;
-                const uint32_t clear = (cells_n + a.clear_rows - 1) / a.clear_rows;
-                const uint32_t wide = (pieces + kLanes - 1) / kLanes;
-                hipLaunchKernelGGL((sums_kernel<T, kP, kLanes>), dim3(a.sum_blocks + clear, wide),
-                                   dim3(256), 0, s, a);
+                const dim3 grid((unsigned)(((uint64_t)a.tiles * kLanes + 255) / 256),
+                                (pieces + kLanes - 1) / kLanes);
+                hipLaunchKernelGGL((sums_kernel<T, kP, kLanes>), grid, dim3(256), 0, s, a);
                 if (a.tiles > 1)
-                    hipLaunchKernelGGL((join_rows_kernel<T, kP, kLanes>), dim3(a.sum_blocks, wide),
-                                       dim3(256), 0, s, a);
+                    hipLaunchKernelGGL((join_rows_kernel<T, kP, kLanes>), grid, dim3(256), 0, s, a);
             });
         if (weight_grad && n > 0 && !beside) {
             // rows of no elements: as if no id named a cell

@@ -99,6 +99,13 @@ __device__ __forceinline__ void store_own(T *row, uint32_t at, uint32_t begin, u
         if (from + e >= at && from + e < end) row[from + e] = c.v[e];
 }
 
+// What a wavefront's lanes wrote to LDS before it, all of them see after it.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // x of the lane across: lanes of 2, 4, 8 and 16 meet through the VALU's own
 // crossbar (quads by xor; eights and sixteens mirrored, which pairs up equal
 // values once the smaller steps are done), 32 and 64 through LDS's.
