@@ -293,7 +293,7 @@ def lib() -> C.CDLL:
                                          F32, P, P, P, SZ, P]
     distill = [C.c_int, P, U64, U64, U64, C.c_int, P, C.c_int, P, U32, F32, P, C.c_int]
     L.sdf_distill_scratch_bytes.restype = SZ
-    L.sdf_distill_scratch_bytes.argtypes = [U64, U64]
+    L.sdf_distill_scratch_bytes.argtypes = [U64, U64, C.c_int]
     L.sdf_distill.restype = C.c_int
     L.sdf_distill.argtypes = distill + [P, P, P, P, P, SZ, P]
     L.sdf_distill_backward.restype = C.c_int

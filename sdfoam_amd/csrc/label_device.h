@@ -45,10 +45,31 @@ __device__ __forceinline__ int32_t load_id(const void *ids, int id_type, uint64_
 }
 
 // 16 bytes of a row: kN elements, at any address that the element type allows
-// (the hardware takes 16-byte accesses at element alignment).
+// (the hardware takes 16-byte accesses at element alignment).  Kept as it is in
+// memory: as separate values, 16-bit elements would take a register each.
 template <typename T> struct Chunk {
     static constexpr int kN = 16 / (int)sizeof(T);
-    T v[kN];
+    uint32_t w[4];
+    __device__ __forceinline__ float operator[](int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else if constexpr (__is_same(T, bf16_t))
+            return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        else return (float)__builtin_bit_cast(half_t, bits(e));
+    }
+    __device__ __forceinline__ uint16_t bits(int e) const { // of a 16-bit element
+        return (uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
+    }
+    __device__ __forceinline__ T value(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else return __builtin_bit_cast(T, bits(e));
+    }
+    __device__ __forceinline__ void set(int e, T x) {
+        if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(x);
+        else {
+            const uint32_t b = __builtin_bit_cast(uint16_t, x);
+            w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | b << 16 : (w[e / 2] & 0xffff0000u) | b;
+        }
+    }
 };
 template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *p) {
     Chunk<T> c;
@@ -58,46 +79,68 @@ template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *p)
 template <typename T> __device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
     __builtin_memcpy(p, &c, 16);
 }
-// A row's [begin, end) in chunks at begin + k kN.  Only whole chunks inside it
-// are read: one that would pass the end is read where it ends there instead
-// (place()), and its elements before `at`, which belong to the chunk before it
-// (all of them, where `at` is past the end), are set to `fill`.  A range
-// shorter than a chunk goes element by element.
-template <typename T>
-__device__ __forceinline__ uint32_t place(uint32_t at, uint32_t begin, uint32_t end) {
-    return end - begin < (uint32_t)Chunk<T>::kN ? at : min(at, end - Chunk<T>::kN);
-}
-template <typename T>
-__device__ __forceinline__ Chunk<T> load_raw(const T *row, uint32_t at, uint32_t begin,
-                                             uint32_t end, T fill) {
-    if (end - begin >= (uint32_t)Chunk<T>::kN) return load_chunk(row + place<T>(at, begin, end));
-    Chunk<T> c;
-#pragma unroll
-    for (int e = 0; e < Chunk<T>::kN; ++e) c.v[e] = at + e < end ? row[at + e] : fill;
-    return c;
-}
-template <typename T>
-__device__ __forceinline__ void mask_chunk(Chunk<T> &c, uint32_t at, uint32_t begin, uint32_t end,
-                                           T fill) {
-    const uint32_t from = place<T>(at, begin, end);
-    if (from == at) return;
-#pragma unroll
-    for (int e = 0; e < Chunk<T>::kN; ++e)
-        if (from + e < at) c.v[e] = fill;
-}
-// The chunk's own elements into a row (those that mask_chunk leaves).
-template <typename T>
-__device__ __forceinline__ void store_own(T *row, uint32_t at, uint32_t begin, uint32_t end,
-                                          const Chunk<T> &c) {
-    if (at + Chunk<T>::kN <= end) {
-        store_chunk(row + at, c);
-        return;
+// Elements [begin, end) of a row, cut into chunks at 16-byte boundaries: chunk
+// `at` (begin, begin + kN, ...) has the elements [at, at + kN) moved down by
+// `skew`, as far as they lie in the range.  (Rows of an odd number of 16-bit
+// elements read at element alignment take 1.2 times as long.)  Memory is read
+// and written in whole chunks inside the range: the first and the last begin
+// where the range begins, or end where it ends (place()), and so share elements
+// with their neighbours, which mask_chunk sets to `fill`.  A range shorter than
+// two chunks goes element by element, unskewed.
+template <typename T> struct Span {
+    static constexpr uint32_t kN = Chunk<T>::kN;
+    const T *row;
+    uint32_t begin, end, skew;
+    bool whole;
+    // begin: a multiple of kN
+    __device__ __forceinline__ Span(const T *r, uint32_t b, uint32_t e)
+        : row(r), begin(b), end(e), whole(e - b >= 2 * kN) {
+        skew = whole ? (uint32_t)(reinterpret_cast<uintptr_t>(r) & 15u) / (uint32_t)sizeof(T) : 0u;
     }
-    const uint32_t from = place<T>(at, begin, end);
+    __device__ __forceinline__ uint32_t last() const { return end + skew; } // chunks lie before it
+    __device__ __forceinline__ uint32_t first_own(uint32_t at) const {
+        return at == begin ? begin : at - skew;
+    }
+    __device__ __forceinline__ uint32_t end_own(uint32_t at) const {
+        return min(at + kN - skew, end);
+    }
+    __device__ __forceinline__ uint32_t place(uint32_t at) const {
+        return whole ? min(first_own(at), end - kN) : at;
+    }
+    // f(element of the chunk, element of the row) for the chunk's own elements
+    template <typename F> __device__ __forceinline__ void each_own(uint32_t at, F f) const {
+        const uint32_t from = place(at), lo = first_own(at), hi = end_own(at);
 #pragma unroll
-    for (int e = 0; e < Chunk<T>::kN; ++e)
-        if (from + e >= at && from + e < end) row[from + e] = c.v[e];
-}
+        for (uint32_t e = 0; e < kN; ++e)
+            if (from + e >= lo && from + e < hi) f(e, from + e);
+    }
+    __device__ __forceinline__ bool plain(uint32_t at) const { // nothing shared with a neighbour
+        return first_own(at) + kN <= end && (at != begin || skew == 0);
+    }
+    // steps of `count` chunk positions, all of them plain
+    __device__ __forceinline__ bool plain_step(uint32_t first, uint32_t elements) const {
+        return first + elements - skew <= end && (first != begin || skew == 0) && whole;
+    }
+    __device__ __forceinline__ Chunk<T> load(uint32_t at, T fill) const { // unmasked
+        if (whole) return load_chunk(row + place(at));
+        Chunk<T> c = {};
+#pragma unroll
+        for (uint32_t e = 0; e < kN; ++e) c.set(e, at + e < end ? row[at + e] : fill);
+        return c;
+    }
+    __device__ __forceinline__ void mask(Chunk<T> &c, uint32_t at, T fill) const {
+        if (plain(at)) return;
+        const uint32_t from = place(at), lo = first_own(at), hi = end_own(at);
+#pragma unroll
+        for (uint32_t e = 0; e < kN; ++e)
+            if (from + e < lo || from + e >= hi) c.set(e, fill);
+    }
+    // the chunk's own elements into another row
+    __device__ __forceinline__ void store_own(T *to, uint32_t at, const Chunk<T> &c) const {
+        if (plain(at)) store_chunk(to + place(at), c);
+        else each_own(at, [&](uint32_t e, uint32_t i) { to[i] = c.value(e); });
+    }
+};
 
 // What a wavefront's lanes wrote to LDS before it, all of them see after it.
 __device__ __forceinline__ void wave_sync() {

@@ -40,26 +40,35 @@ template <bool kEntropy> __device__ __forceinline__ void rebase(Part &p, float m
     p.s *= f;
     p.m = m;
 }
-// The elements of kU chunks into p: one change of base, then a subtraction, a
-// product, an exponential and a sum each.
-template <bool kEntropy, typename T, int kU>
-__device__ __forceinline__ void absorb(Part &p, const Chunk<T> (&ch)[kU], float c) {
-    float m = p.m;
+// The elements of kU chunks into p: for kGroup chunks at a time one change of
+// base, then a subtraction, a product, an exponential and a sum for each.
+// (A group's elements are unpacked at once: 8 held chunks of 8 in one group
+// take 138 VGPRs and leave one block of 512 threads a CU.)  The largest of them.
+template <bool kEntropy, int kGroup, typename T, int kU>
+__device__ __forceinline__ float absorb(Part &p, const Chunk<T> (&ch)[kU], float c) {
+    float largest = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kU; ++i)
+    for (int i0 = 0; i0 < kU; i0 += kGroup) {
+        float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < Chunk<T>::kN; ++e) m = fmaxf(m, (float)ch[i].v[e]);
-    rebase<kEntropy>(p, m, c);
-    const float base = m == -INFINITY ? 0.0f : m;
+        for (int i = i0; i < kU && i < i0 + kGroup; ++i)
 #pragma unroll
-    for (int i = 0; i < kU; ++i)
+            for (int e = 0; e < Chunk<T>::kN; ++e) m = fmaxf(m, ch[i][e]);
+        largest = fmaxf(largest, m);
+        m = fmaxf(m, p.m);
+        rebase<kEntropy>(p, m, c);
+        const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int e = 0; e < Chunk<T>::kN; ++e) {
-            const float d = ((float)ch[i].v[e] - base) * c;
-            const float x = __builtin_amdgcn_exp2f(d);
-            p.s += x;
-            if (kEntropy) p.w = fmaf(fmaxf(d, -200.0f), x, p.w);
-        }
+        for (int i = i0; i < kU && i < i0 + kGroup; ++i)
+#pragma unroll
+            for (int e = 0; e < Chunk<T>::kN; ++e) {
+                const float d = (ch[i][e] - base) * c;
+                const float x = __builtin_amdgcn_exp2f(d);
+                p.s += x;
+                if (kEntropy) p.w = fmaf(fmaxf(d, -200.0f), x, p.w);
+            }
+    }
+    return largest;
 }
 // One Part of the kLanes neighbouring lanes' (in all of them).
 template <int kLanes, bool kEntropy> __device__ __forceinline__ void merge_lanes(Part &p, float c) {
@@ -88,50 +97,47 @@ template <bool kEntropy> __device__ __forceinline__ Part merge_block(Part p, Par
     return merge_parts<kEntropy>(parts, blockDim.x >> 6, c);
 }
 
-// f(chunks, at) for the elements [begin, end) of a row, kU chunks of each of
-// kThreads threads at a time, chunk i at `at` + i kThreads kN; what is not a
-// chunk's own (place()) is -inf where kMask, else as it was read.
-// (for_steps: only the steps that begin in [first, last).)
+// f(chunks, at) over a span, kU chunks of each of kThreads threads at a time,
+// chunk i at `at` + i kThreads kN; what is not a chunk's own is -inf where
+// kMask, else as it was read.  Only the steps that begin in [first, last).
 template <int kThreads, int kU, bool kMask, typename T, typename F>
-__device__ __forceinline__ void for_steps(const T *z, uint32_t first, uint32_t last, uint32_t begin,
-                                          uint32_t end, F f) {
+__device__ __forceinline__ void for_steps(const Span<T> &z, uint32_t first, uint32_t last, F f) {
     constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
     for (; first < last; first += kStep * kU) {
         const uint32_t at = first + threadIdx.x % kThreads * Chunk<T>::kN;
         Chunk<T> ch[kU];
-        if (first + kStep * kU <= end) {
+        if (z.plain_step(first, kStep * kU)) {
+            const T *p = z.row + (at - z.skew);
 #pragma unroll
-            for (int i = 0; i < kU; ++i) ch[i] = load_chunk(z + at + i * kStep);
+            for (int i = 0; i < kU; ++i) ch[i] = load_chunk(p + i * kStep);
         } else {
 #pragma unroll
-            for (int i = 0; i < kU; ++i)
-                ch[i] = load_raw(z, at + i * kStep, begin, end, (T)-INFINITY);
+            for (int i = 0; i < kU; ++i) ch[i] = z.load(at + i * kStep, (T)-INFINITY);
             if (kMask) {
 #pragma unroll
-                for (int i = 0; i < kU; ++i)
-                    mask_chunk(ch[i], at + i * kStep, begin, end, (T)-INFINITY);
+                for (int i = 0; i < kU; ++i) z.mask(ch[i], at + i * kStep, (T)-INFINITY);
             }
         }
         f(ch, at);
     }
 }
 template <int kThreads, int kU, bool kMask, typename T, typename F>
-__device__ __forceinline__ void for_chunks(const T *z, uint32_t begin, uint32_t end, F f) {
-    for_steps<kThreads, kU, kMask>(z, begin, end, begin, end, f);
+__device__ __forceinline__ void for_chunks(const Span<T> &z, F f) {
+    for_steps<kThreads, kU, kMask>(z, z.begin, z.last(), f);
 }
-// row[i] = f(z[i]) chunk by chunk over [begin, end)
+// to[i] = f(z[i]) over a span, chunk by chunk
 template <int kThreads, int kU, typename T, typename F>
-__device__ __forceinline__ void map_chunks(const T *z, T *row, uint32_t begin, uint32_t end, F f) {
+__device__ __forceinline__ void map_chunks(const Span<T> &z, T *to, F f) {
     constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
-    for_chunks<kThreads, kU, false>(z, begin, end, [&](const Chunk<T>(&ch)[kU], uint32_t at) {
+    for_chunks<kThreads, kU, false>(z, [&](const Chunk<T>(&ch)[kU], uint32_t at) {
 #pragma unroll
         for (int i = 0; i < kU; ++i)
-            if (at + i * kStep < end) {
-                const uint32_t to = place<T>(at + i * kStep, begin, end);
-                const Chunk<T> o = f(ch[i], to);
+            if (at + i * kStep < z.last()) {
+                const uint32_t from = z.place(at + i * kStep);
+                const Chunk<T> o = f(ch[i], from);
                 // two threads may write one element, and then the same value
-                if (end - begin >= (uint32_t)Chunk<T>::kN) store_chunk(row + to, o);
-                else store_own(row, to, begin, end, o);
+                if (z.whole) store_chunk(to + from, o);
+                else z.store_own(to, from, o);
             }
     });
 }
@@ -139,13 +145,11 @@ __device__ __forceinline__ void map_chunks(const T *z, T *row, uint32_t begin, u
 constexpr int kStream = 256; // threads a block where rows are streamed
 constexpr int kUnroll = 4;   // chunks in flight per thread
 
-template <bool kEntropy, typename T>
-__device__ __forceinline__ Part stream_part(const T *z, uint32_t begin, uint32_t end, float c) {
-    Part p = {-INFINITY, 0.0f, 0.0f};
-    for_chunks<kStream, kUnroll, true>(z, begin, end, [&](const Chunk<T>(&ch)[kUnroll], uint32_t) {
-        absorb<kEntropy>(p, ch, c);
+template <bool kEntropy, int kThreads, typename T>
+__device__ __forceinline__ void stream_part(Part &p, const Span<T> &z, float c) {
+    for_chunks<kThreads, kUnroll, true>(z, [&](const Chunk<T>(&ch)[kUnroll], uint32_t) {
+        absorb<kEntropy, kUnroll>(p, ch, c);
     });
-    return p;
 }
 
 struct DistillArgs {
@@ -157,7 +161,7 @@ struct DistillArgs {
     int teacher_type;
     const void *teacher_logits;
     uint32_t top;
-    float temperature;
+    float temperature, inv_t, c; // T, 1 / T, log2(e) / T
     const float *row_weight;   // NULL: 1
     const float *loss_grad;    // NULL: 1
     uint32_t loss_grad_stride; // 0: one for all rows
@@ -173,96 +177,109 @@ __device__ __forceinline__ float teacher_logit(const DistillArgs &a, uint64_t i)
     return static_cast<const float *>(a.teacher_logits)[i];
 }
 
-// A row's teacher: which entries count, their softmax, and the row's factor.
-// Every group of kLanes lanes computes it for itself (a wavefront with the
-// whole row, or a few lanes that share one).
-struct Teacher {
-    float u, m, s; // row weight, largest counting logit (0: none), sum relative to it
-    bool counts;   // some entry counts and the weight is not 0
+// A row's teacher in LDS: each entry's logit (later its share q), label (-1:
+// does not count) and the row's own logit there.  Read from memory once, on
+// their way while the row itself is.
+struct Entries {
+    float *q, *z;
+    int32_t *id;
 };
+constexpr uint32_t kEntryBytes = 12;
+__device__ __forceinline__ Entries entries_at(void *shared, uint32_t top) {
+    float *q = static_cast<float *>(shared);
+    return {q, q + top, reinterpret_cast<int32_t *>(q + 2 * top)};
+}
 __device__ __forceinline__ float entry(const DistillArgs &a, uint64_t r, uint32_t k, int32_t &j) {
     j = load_id(a.teacher_labels, a.id_type, r * a.top + k, a.labels);
     const float t = j < 0 ? -INFINITY : teacher_logit(a, r * a.top + k);
     if (t == -INFINITY) j = -1;
     return t;
 }
+template <typename T>
+__device__ __forceinline__ void put_entry(const Entries &e, uint32_t k, int32_t j, float t, const T *z) {
+    e.q[k] = t;
+    e.id[k] = j;
+    e.z[k] = j < 0 ? 0.0f : (float)z[j];
+}
+// Entries `first`, `first` + step, ... from memory.
+template <typename T>
+__device__ __forceinline__ void load_entries(const DistillArgs &a, uint64_t r, const T *z,
+                                             const Entries &e, uint32_t first, uint32_t step) {
+    for (uint32_t k = first; k < a.top; k += step) {
+        int32_t j;
+        const float t = entry(a, r, k, j);
+        put_entry(e, k, j, t, z);
+    }
+}
+// The softmax of the counting entries, by every group of kLanes lanes for
+// itself.  s = 0: none counts.
+struct Teacher {
+    float m, s;
+};
 template <int kLanes>
-__device__ __forceinline__ Teacher teacher_of(const DistillArgs &a, uint64_t r, float c) {
+__device__ __forceinline__ Teacher teacher_of(const DistillArgs &a, const Entries &e) {
     const uint32_t l = threadIdx.x & (kLanes - 1);
-    Teacher t = {a.row_weight ? a.row_weight[r] : 1.0f, -INFINITY, 0.0f, false};
-    int32_t j;
-    for (uint32_t k = l; k < a.top; k += kLanes) t.m = fmaxf(t.m, entry(a, r, k, j));
+    Teacher t = {-INFINITY, 0.0f};
+    for (uint32_t k = l; k < a.top; k += kLanes) t.m = fmaxf(t.m, e.q[k]);
     t.m = group_max<kLanes>(t.m);
     if (t.m == -INFINITY) t.m = 0.0f;
     for (uint32_t k = l; k < a.top; k += kLanes)
-        t.s += __builtin_amdgcn_exp2f((entry(a, r, k, j) - t.m) * c);
+        t.s += __builtin_amdgcn_exp2f((e.q[k] - t.m) * a.c);
     t.s = group_sum<kLanes>(t.s);
-    t.counts = !(t.u == 0.0f) && !(t.s == 0.0f);
     return t;
 }
-// The counting entries' shares q and labels into LDS (label -1: none) by the
-// kLanes lanes of a group.
+// The entries' logits become their shares, by the kLanes lanes of one group
+// (when every other has read them), and sum q (log q - log p) over them.
 template <int kLanes>
-__device__ __forceinline__ void store_shares(const DistillArgs &a, uint64_t r, const Teacher &t,
-                                             float c, float *q, int32_t *id) {
-    for (uint32_t k = threadIdx.x & (kLanes - 1); k < a.top; k += kLanes) {
-        int32_t j;
-        const float x = entry(a, r, k, j);
-        q[k] = __builtin_amdgcn_exp2f((x - t.m) * c) / t.s;
-        id[k] = j;
-    }
-}
-// sum q (log q - log p) over the entries of the kLanes lanes of a group.
-template <int kLanes, typename T>
-__device__ __forceinline__ float row_loss(const DistillArgs &a, uint64_t r, const T *z,
-                                          const Teacher &t, const Part &st, float c, float inv_t) {
+__device__ __forceinline__ float shares(const DistillArgs &a, const Entries &e, const Teacher &t,
+                                        const Part &st) {
     const float log_s = logf(st.s), log_ts = logf(t.s);
     float sum = 0.0f;
     for (uint32_t k = threadIdx.x & (kLanes - 1); k < a.top; k += kLanes) {
-        int32_t j;
-        const float x = entry(a, r, k, j);
-        const float q = __builtin_amdgcn_exp2f((x - t.m) * c) / t.s;
+        const float d = e.q[k] - t.m, q = __builtin_amdgcn_exp2f(d * a.c) / t.s;
         // an entry of no mass adds nothing, whatever its label's probability
-        if (j >= 0 && !(q == 0.0f))
-            sum += q * ((x - t.m) * inv_t - log_ts - (((float)z[j] - st.m) * inv_t - log_s));
+        if (e.id[k] >= 0 && !(q == 0.0f))
+            sum += q * (d * a.inv_t - log_ts - ((e.z[k] - st.m) * a.inv_t - log_s));
+        e.q[k] = q;
     }
-    return t.u * a.temperature * a.temperature * group_sum<kLanes>(sum);
+    return group_sum<kLanes>(sum);
 }
 // The row's gradient at the teacher's labels in [begin, end), over what stands
 // there: entries `first`, `first` + `step`, ...
 template <typename T>
-__device__ __forceinline__ void write_shares(const DistillArgs &a, const T *z, T *dz, const float *q,
-                                             const int32_t *id, const Part &st, float c, float coef,
-                                             uint32_t first, uint32_t step, uint32_t begin,
-                                             uint32_t end) {
+__device__ __forceinline__ void write_shares(const DistillArgs &a, T *dz, const Entries &x,
+                                             const Part &st, float coef, uint32_t first,
+                                             uint32_t step, uint32_t begin, uint32_t end) {
     for (uint32_t k = first; k < a.top; k += step) {
-        const int32_t j = id[k];
+        const int32_t j = x.id[k];
         if (j < 0 || (uint32_t)j < begin || (uint32_t)j >= end) continue;
         float mass = 0.0f; // a label that the teacher names twice has both shares
-        for (uint32_t o = 0; o < a.top; ++o) mass += id[o] == j ? q[o] : 0.0f;
-        const float p = __builtin_amdgcn_exp2f(((float)z[j] - st.m) * c) / st.s;
+        for (uint32_t o = 0; o < a.top; ++o) mass += x.id[o] == j ? x.q[o] : 0.0f;
+        const float p = __builtin_amdgcn_exp2f((x.z[k] - st.m) * a.c) / st.s;
         dz[j] = (T)(coef * (p - mass));
     }
 }
-__device__ __forceinline__ float row_coef(const DistillArgs &a, uint64_t r, const Teacher &t) {
+__device__ __forceinline__ float row_coef(const DistillArgs &a, uint64_t r, float u) {
     const float g = a.loss_grad ? a.loss_grad[r * a.loss_grad_stride] : 1.0f;
-    return g * a.reduce * t.u * a.temperature;
+    return g * a.reduce * u * a.temperature;
+}
+__device__ __forceinline__ float row_weight(const DistillArgs &a, uint64_t r) {
+    return a.row_weight ? a.row_weight[r] : 1.0f;
 }
 // share * e of a chunk's logits
 template <typename T>
 __device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &ch, float m, float c, float share) {
-    Chunk<T> o;
+    Chunk<T> o = {};
 #pragma unroll
     for (int e = 0; e < Chunk<T>::kN; ++e)
-        o.v[e] = (T)(share * __builtin_amdgcn_exp2f(((float)ch.v[e] - m) * c));
+        o.set(e, (T)(share * __builtin_amdgcn_exp2f((ch[e] - m) * c)));
     return o;
 }
 template <int kThreads, typename T>
 __device__ __forceinline__ void write_zeros(T *dz, uint32_t begin, uint32_t end) {
-    constexpr uint32_t kN = Chunk<T>::kN;
-    const Chunk<T> zero = {};
-    for (uint32_t at = begin + threadIdx.x * kN; at < end; at += kThreads * kN)
-        store_own(dz, at, begin, end, zero);
+    const Span<T> z(dz, begin, end);
+    for (uint32_t at = begin + threadIdx.x * z.kN; at < z.last(); at += kThreads * z.kN)
+        z.store_own(dz, at, {});
 }
 
 // A block per row.  With kHeld > 0 (the gradient is wanted): the row's first
@@ -270,48 +287,54 @@ __device__ __forceinline__ void write_zeros(T *dz, uint32_t begin, uint32_t end)
 // gradient, so they are read once; the rest is read again.  kHeld = 0: loss and
 // statistics alone, streamed.
 template <typename T, int kThreads, int kHeld>
-__global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
+__global__ __launch_bounds__(kThreads)
+    __attribute__((amdgpu_waves_per_eu(kHeld > 8 ? 4 : kHeld > 4 ? 6 : 7))) void
+    distill_kernel(DistillArgs a) {
     constexpr uint32_t kN = Chunk<T>::kN;
+    extern __shared__ float shared[];
     __shared__ Part parts[kThreads / 64];
-    __shared__ float q[kHeld ? kMaxTeacher : 1];
-    __shared__ int32_t id[kHeld ? kMaxTeacher : 1];
+    const Entries e = entries_at(shared, a.top);
     const uint64_t r = blockIdx.x;
-    const T *z = static_cast<const T *>(a.logits) + r * a.stride;
+    const Span<T> z(static_cast<const T *>(a.logits) + r * a.stride, 0u, a.labels);
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
     constexpr uint32_t kRest = kThreads * kN * kHeld;
-    const bool read = !(a.row_weight && a.row_weight[r] == 0.0f); // the same in every thread
+    const float u = row_weight(a, r);
+    Teacher t = {0.0f, 0.0f};
+    Part st = {0.0f, 0.0f, 0.0f};
     Chunk<T> held[kHeld ? kHeld : 1];
-    if (kHeld > 0 && read) { // on their way while the teacher's entries are looked at
+    if (!(u == 0.0f)) { // the same in every thread
+        int32_t j = -1;
+        float logit = -INFINITY;
+        if (threadIdx.x < a.top) logit = entry(a, r, threadIdx.x, j);
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
-            held[i] = load_raw(z, (threadIdx.x + i * kThreads) * kN, 0u, a.labels, (T)-INFINITY);
-    }
-    const Teacher t = teacher_of<64>(a, r, c);
-    Part st = {0.0f, 0.0f, 0.0f};
-    if (t.counts) {
-        Part p = {-INFINITY, 0.0f, 0.0f};
-        if constexpr (kHeld > 0) {
-            if (threadIdx.x < 64u) store_shares<64>(a, r, t, c, q, id);
-            if (kRest > a.labels) {
+            held[i] = z.load((threadIdx.x + i * kThreads) * kN, (T)-INFINITY);
+        if (threadIdx.x < a.top) put_entry(e, threadIdx.x, j, logit, z.row);
+        load_entries(a, r, z.row, e, threadIdx.x + kThreads, kThreads);
+        __syncthreads();
+        t = teacher_of<64>(a, e);
+        if (!(t.s == 0.0f)) { // and this
+            Part p = {-INFINITY, 0.0f, 0.0f};
+            if constexpr (kHeld > 0) {
+                if (!z.plain_step(0u, kRest)) {
 #pragma unroll
-                for (int i = 0; i < kHeld; ++i)
-                    mask_chunk(held[i], (threadIdx.x + i * kThreads) * kN, 0u, a.labels,
-                               (T)-INFINITY);
+                    for (int i = 0; i < kHeld; ++i)
+                        z.mask(held[i], (threadIdx.x + i * kThreads) * kN, (T)-INFINITY);
+                }
+                absorb<false, 2>(p, held, a.c);
             }
-            absorb<false>(p, held, c);
+            for_steps<kThreads, kUnroll, true>(z, kRest, z.last(),
+                                               [&](const Chunk<T>(&ch)[kUnroll], uint32_t) {
+                                                   absorb<false, kUnroll>(p, ch, a.c);
+                                               });
+            st = merge_block<false>(p, parts, a.c);
+            if (st.m == -INFINITY) st.m = 0.0f;
         }
-        if (kRest < a.labels)
-            for_chunks<kThreads, kUnroll, true>(
-                z, kRest, a.labels,
-                [&](const Chunk<T>(&ch)[kUnroll], uint32_t) { absorb<false>(p, ch, c); });
-        st = merge_block<false>(p, parts, c);
-        if (st.m == -INFINITY) st.m = 0.0f;
     }
-    const bool live = t.counts && !(st.s == 0.0f);
+    const bool live = !(st.s == 0.0f);
     if (a.stats && threadIdx.x == 0) a.stats[r] = make_float2(st.m, st.s);
     if (threadIdx.x < 64u) {
-        const float loss = live ? row_loss<64>(a, r, z, t, st, c, inv_t) : 0.0f;
+        const float loss = live ? u * a.temperature * a.temperature * shares<64>(a, e, t, st) : 0.0f;
         if (threadIdx.x == 0) a.loss[r] = loss;
     }
     if constexpr (kHeld > 0) {
@@ -319,19 +342,21 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
             write_zeros<kThreads>(dz, 0, a.labels);
             return;
         }
-        const float coef = row_coef(a, r, t), share = coef / st.s;
-        if (kRest < a.labels)
-            map_chunks<kThreads, kUnroll>(z, dz, kRest, a.labels, [&](const Chunk<T> &ch, uint32_t) {
-                return grad_chunk(ch, st.m, c, share);
+        const float coef = row_coef(a, r, u), share = coef / st.s;
+        for_steps<kThreads, kUnroll, true>(
+            z, kRest, z.last(), [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
+#pragma unroll
+                for (int i = 0; i < kUnroll; ++i)
+                    if (at + i * kThreads * kN < z.last())
+                        z.store_own(dz, at + i * kThreads * kN, grad_chunk(ch[i], st.m, a.c, share));
             });
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
             const uint32_t at = (threadIdx.x + i * kThreads) * kN;
-            if (at < a.labels)
-                store_own(dz, at, 0u, a.labels, grad_chunk(held[i], st.m, c, share));
+            if (at < z.last()) z.store_own(dz, at, grad_chunk(held[i], st.m, a.c, share));
         }
         __syncthreads(); // the teacher's labels are written over what stands there
-        write_shares(a, z, dz, q, id, st, c, coef, threadIdx.x, kThreads, 0u, a.labels);
+        write_shares(a, dz, e, st, coef, threadIdx.x, kThreads, 0u, a.labels);
     }
 }
 
@@ -343,10 +368,11 @@ __global__ __launch_bounds__(kStream) void part_kernel(DistillArgs a, uint32_t s
     const uint64_t r = blockIdx.x / slices;
     const uint32_t k = blockIdx.x % slices, begin = k * slice;
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
-    const float c = (1.0f / a.temperature) * kLog2e;
+    const float c = a.c;
     if (a.row_weight && a.row_weight[r] == 0.0f) return; // not read, here or later
-    const Part p = merge_block<false>(
-        stream_part<false>(z, begin, min(a.labels, begin + slice), c), parts, c);
+    Part p = {-INFINITY, 0.0f, 0.0f};
+    stream_part<false, kStream>(p, Span<T>(z, begin, min(a.labels, begin + slice)), c);
+    p = merge_block<false>(p, parts, c);
     if (threadIdx.x == 0) out[r * slices + k] = p;
 }
 
@@ -356,31 +382,36 @@ template <typename T>
 __global__ __launch_bounds__(kStream) void finish_kernel(DistillArgs a, uint32_t tiles,
                                                          uint32_t tile, const Part *parts,
                                                          uint32_t slices) {
-    __shared__ float q[kMaxTeacher];
-    __shared__ int32_t id[kMaxTeacher];
+    extern __shared__ float shared[];
+    const Entries e = entries_at(shared, a.top);
     const uint64_t r = blockIdx.x / tiles;
     const uint32_t begin = (uint32_t)(blockIdx.x % tiles) * tile;
     const uint32_t end = min(a.labels, begin + tile);
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
-    const Teacher t = teacher_of<64>(a, r, c);
+    const float u = row_weight(a, r);
+    Teacher t = {0.0f, 0.0f};
     Part st = {0.0f, 0.0f, 0.0f};
-    if (t.counts) {
+    if (!(u == 0.0f)) {
+        load_entries(a, r, z, e, threadIdx.x, kStream);
         if (parts) {
-            st = merge_parts<false>(parts + r * slices, slices, c);
+            st = merge_parts<false>(parts + r * slices, slices, a.c);
             if (st.m == -INFINITY) st.m = 0.0f;
         } else {
             const float2 h = a.stats[r];
             st = {h.x, h.y, 0.0f};
         }
+        __syncthreads();
+        t = teacher_of<64>(a, e);
+        if (t.s == 0.0f) st.s = 0.0f;
+        __syncthreads(); // before the shares take the logits' place
     }
-    const bool live = t.counts && !(st.s == 0.0f);
-    if (parts && begin == 0 && threadIdx.x < 64u) {
-        const float loss = live ? row_loss<64>(a, r, z, t, st, c, inv_t) : 0.0f;
-        if (threadIdx.x == 0) {
+    const bool live = !(st.s == 0.0f);
+    if (threadIdx.x < 64u) {
+        const float loss = live ? u * a.temperature * a.temperature * shares<64>(a, e, t, st) : 0.0f;
+        if (parts && begin == 0 && threadIdx.x == 0) {
             a.loss[r] = loss;
-            if (a.stats) a.stats[r] = make_float2(st.m, st.s);
+            if (a.stats) a.stats[r] = make_float2(live ? st.m : 0.0f, st.s);
         }
     }
     if (!a.logits_grad) return;
@@ -388,79 +419,82 @@ __global__ __launch_bounds__(kStream) void finish_kernel(DistillArgs a, uint32_t
         write_zeros<kStream>(dz, begin, end);
         return;
     }
-    if (threadIdx.x < 64u) store_shares<64>(a, r, t, c, q, id);
-    const float coef = row_coef(a, r, t), share = coef / st.s;
-    map_chunks<kStream, kUnroll>(z, dz, begin, end, [&](const Chunk<T> &ch, uint32_t) {
-        return grad_chunk(ch, st.m, c, share);
+    const float coef = row_coef(a, r, u), share = coef / st.s;
+    map_chunks<kStream, kUnroll>(Span<T>(z, begin, end), dz, [&](const Chunk<T> &ch, uint32_t) {
+        return grad_chunk(ch, st.m, a.c, share);
     });
     __syncthreads();
-    write_shares(a, z, dz, q, id, st, c, coef, threadIdx.x, kStream, begin, end);
+    write_shares(a, dz, e, st, coef, threadIdx.x, kStream, begin, end);
 }
 
 // Short rows: kLanes lanes a row, the whole row in their registers (kHeld
 // chunks each), 256 / kLanes rows a block or fewer where the teacher's entries
-// fill LDS (`shares`: top floats, then top labels, for each row).
+// fill LDS.
 template <typename T, int kLanes, int kHeld, bool kHaveStats>
 __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs a, uint64_t rows) {
     constexpr uint32_t kN = Chunk<T>::kN;
-    extern __shared__ float shares[];
+    extern __shared__ float shared[];
     const uint32_t g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
     const uint64_t r = (uint64_t)blockIdx.x * (blockDim.x / kLanes) + g;
     const bool in = r < rows;
-    float *q = shares + (size_t)g * 2 * a.top;
-    int32_t *id = reinterpret_cast<int32_t *>(q + a.top);
+    const Entries e = entries_at(shared + (size_t)g * 3 * a.top, a.top);
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
-    Teacher t = {0.0f, 0.0f, 0.0f, false};
+    const Span<T> span(z, 0u, a.labels);
+    const float u = in ? row_weight(a, r) : 0.0f;
+    Teacher t = {0.0f, 0.0f};
     Part st = {0.0f, 0.0f, 0.0f};
-    bool live = false;
-    float coef = 0.0f;
-    if (in) {
-        t = teacher_of<kLanes>(a, r, c);
-        Chunk<T> held[kHeld];
-        if (t.counts) {
+    Chunk<T> held[kHeld];
+    if (!(u == 0.0f)) {
+        int32_t j = -1;
+        float logit = -INFINITY;
+        if (l < a.top) logit = entry(a, r, l, j);
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-                held[i] = load_raw(z, (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+        for (int i = 0; i < kHeld; ++i)
+            held[i] = span.load((l + i * kLanes) * kN, (T)-INFINITY);
+        if (l < a.top) put_entry(e, l, j, logit, z);
+        load_entries(a, r, z, e, l + kLanes, kLanes);
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-                mask_chunk(held[i], (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
-            if (kHaveStats) {
-                const float2 h = a.stats[r];
-                st = {h.x, h.y, 0.0f};
-            } else {
-                st = {-INFINITY, 0.0f, 0.0f};
-                absorb<false>(st, held, c);
-                merge_lanes<kLanes, false>(st, c);
-                if (st.m == -INFINITY) st.m = 0.0f;
-            }
-        }
-        live = t.counts && !(st.s == 0.0f);
-        if (!kHaveStats) {
-            const float loss = live ? row_loss<kLanes>(a, r, z, t, st, c, inv_t) : 0.0f;
-            if (l == 0) {
-                a.loss[r] = loss;
-                if (a.stats) a.stats[r] = make_float2(st.m, st.s);
-            }
-        }
-        if (a.logits_grad) {
-            coef = live ? row_coef(a, r, t) : 0.0f;
-            const float share = coef / st.s;
-            if (live) store_shares<kLanes>(a, r, t, c, q, id);
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                const uint32_t at = (l + i * kLanes) * kN;
-                if (at >= a.labels) continue;
-                Chunk<T> o = {};
-                if (live) o = grad_chunk(held[i], st.m, c, share);
-                store_own(dz, at, 0u, a.labels, o);
-            }
+        for (int i = 0; i < kHeld; ++i)
+            span.mask(held[i], (l + i * kLanes) * kN, (T)-INFINITY);
+        if (kHaveStats) {
+            const float2 h = a.stats[r];
+            st = {h.x, h.y, 0.0f};
+        } else {
+            st = {-INFINITY, 0.0f, 0.0f};
+            absorb<false, 2>(st, held, a.c);
+            merge_lanes<kLanes, false>(st, a.c);
+            if (st.m == -INFINITY) st.m = 0.0f;
         }
     }
+    wave_sync(); // a group's lanes are of one wavefront
+    if (!(u == 0.0f)) {
+        t = teacher_of<kLanes>(a, e);
+        if (t.s == 0.0f) st.s = 0.0f;
+    }
+    wave_sync();
+    const bool live = !(st.s == 0.0f);
+    if (live) {
+        const float sum = shares<kLanes>(a, e, t, st);
+        if (!kHaveStats && l == 0) a.loss[r] = u * a.temperature * a.temperature * sum;
+    } else if (!kHaveStats && in && l == 0) {
+        a.loss[r] = 0.0f;
+    }
+    if (!kHaveStats && a.stats && in && l == 0) a.stats[r] = make_float2(live ? st.m : 0.0f, st.s);
     if (!a.logits_grad) return;
+    const float coef = live ? row_coef(a, r, u) : 0.0f, share = coef / st.s;
+    if (in) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const uint32_t at = (l + i * kLanes) * kN;
+            if (at >= span.last()) continue;
+            Chunk<T> o = {};
+            if (live) o = grad_chunk(held[i], st.m, a.c, share);
+            span.store_own(dz, at, o);
+        }
+    }
     __syncthreads();
-    if (live) write_shares(a, z, dz, q, id, st, c, coef, l, kLanes, 0u, a.labels);
+    if (live) write_shares(a, dz, e, st, coef, l, kLanes, 0u, a.labels);
 }
 
 // The rows' losses in one sum, always in the same order.
@@ -486,7 +520,7 @@ struct AnswerArgs {
     int id_type;
     const void *label_ids;
     uint32_t top;
-    float temperature;
+    float inv_t, c; // 1 / T, log2(e) / T
     float *log_prob, *entropy; // [rows]
     float *top_log_probs;      // [rows, top]
     int64_t *top_labels;       // [rows, top]
@@ -506,6 +540,18 @@ __device__ __forceinline__ uint32_t logit_order(float z) {
 __device__ __forceinline__ float order_logit(uint32_t o) {
     return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
+// The same in 16 bits for the 16-bit types, and back.
+__device__ __forceinline__ uint32_t half_order(uint32_t bits, float z) {
+    if (!(z > -INFINITY)) return 0u;
+    if (bits == 0x8000u) bits = 0;
+    return bits & 0x8000u ? ~bits & 0xffffu : bits | 0x8000u;
+}
+template <typename T> __device__ __forceinline__ float half_value(uint32_t o) {
+    const uint16_t bits = o & 0x8000u ? (uint16_t)(o ^ 0x8000u) : (uint16_t)~o;
+    T z;
+    __builtin_memcpy(&z, &bits, 2);
+    return (float)z;
+}
 // Keys order labels by falling logit, then by rising label; 0 is no label.
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t label) {
     return (uint64_t)order << 32 | (0xffffffffu - label);
@@ -523,10 +569,9 @@ __device__ __forceinline__ uint32_t kth_of_wave(uint32_t x, uint32_t k) {
     return t;
 }
 
-__device__ __forceinline__ void write_answer(const AnswerArgs &a, uint64_t r, float z_label, bool named,
-                                             const Part &st, float inv_t) {
+__device__ __forceinline__ void write_answer(const AnswerArgs &a, uint64_t r, float z_label,
+                                             bool named, const Part &st, float inv_t, float log_s) {
     const bool empty = st.s == 0.0f;
-    const float log_s = logf(st.s);
     float lp = 0.0f;
     if (named) lp = empty ? -INFINITY : (z_label - st.m) * inv_t - log_s;
     a.log_prob[r] = lp;
@@ -560,21 +605,17 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
     const uint32_t part = blockIdx.x % slices, begin = part * slice;
     const uint32_t end = min(a.labels, begin + slice);
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    const float inv_t = a.inv_t, c = a.c;
+    const Span<T> span(z, begin, end);
     // beside its largest logit, where the thread met it, and the largest of its
     // other steps
     Part mine = {-INFINITY, 0.0f, 0.0f};
     float second = -INFINITY;
     uint32_t where = begin;
-    for_chunks<kStream, kUnroll, true>(z, begin, end, [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i)
-#pragma unroll
-            for (int e = 0; e < Chunk<T>::kN; ++e) m = fmaxf(m, (float)ch[i].v[e]);
-        second = fmaxf(second, fminf(m, mine.m));
-        where = m > mine.m ? at : where;
-        absorb<true>(mine, ch, c);
+    for_chunks<kStream, kUnroll, true>(span, [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
+        const float before = mine.m, m = absorb<true, kUnroll>(mine, ch, c);
+        second = fmaxf(second, fminf(m, before));
+        where = m > before ? at : where;
     });
     const uint32_t best = logit_order(mine.m);
     if (a.top) {
@@ -589,7 +630,7 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
             out[r * slices + part] = st;
         } else {
             const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
-            write_answer(a, r, y < 0 ? 0.0f : (float)z[y], y >= 0, st, inv_t);
+            write_answer(a, r, y < 0 ? 0.0f : (float)z[y], y >= 0, st, inv_t, logf(st.s));
         }
     }
     if (!a.top) return;
@@ -605,18 +646,16 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
             for (int i = 0; i < kUnroll; ++i)
 #pragma unroll
                 for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
-                    const uint32_t o = logit_order((float)ch[i].v[e]);
+                    const uint32_t o = logit_order(ch[i][e]);
                     if (o < bound) continue;
                     const uint32_t k = atomicAdd(&found, 1u);
-                    const uint32_t from = place<T>(at + i * kStream * Chunk<T>::kN, begin, end);
+                    const uint32_t from = span.place(at + i * kStream * Chunk<T>::kN);
                     if (k < kCandidates) keys[k] = key_of(o, from + e);
                 }
         };
-        constexpr uint32_t kStep = kStream * Chunk<T>::kN * kUnroll;
         const bool one = logit_order(second) < bound;
         const uint32_t first = one ? where - threadIdx.x * Chunk<T>::kN : begin;
-        for_steps<kStream, kUnroll, true>(z, first, one ? min(end, first + kStep) : end, begin, end,
-                                          collect);
+        for_steps<kStream, kUnroll, true>(span, first, one ? first + 1 : span.last(), collect);
     }
     __syncthreads();
     const uint32_t n = found;
@@ -634,11 +673,11 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top; ++k) {
         uint64_t key = 0;
-        for_chunks<kStream, 1, true>(z, begin, end, [&](const Chunk<T>(&ch)[1], uint32_t at) {
+        for_chunks<kStream, 1, true>(span, [&](const Chunk<T>(&ch)[1], uint32_t at) {
 #pragma unroll
             for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
-                const uint32_t o = logit_order((float)ch[0].v[e]);
-                const uint64_t x = key_of(o, place<T>(at, begin, end) + e);
+                const uint32_t o = logit_order(ch[0][e]);
+                const uint64_t x = key_of(o, span.place(at) + e);
                 if (o != 0 && x < last && x > key) key = x;
             }
         });
@@ -657,44 +696,55 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
 
 constexpr uint32_t kMaxSlices = 32; // of a row of answers
 
-// One row of its slices: their Parts merged, and the rank of each of their
-// keys: how many keys of every slice (sorted, so by halving) stand before it.
+// One row of its slices: their Parts merged, and the best of their best.  With
+// q = top / slices rounded up, the m-th largest of the slices' q-th keys has at
+// least m q keys at or above it: for m q >= top it bounds the top-th best label
+// from below.  What reaches it (about `top`) is ranked by counting.
 template <typename T>
 __global__ __launch_bounds__(kStream) void join_kernel(AnswerArgs a, uint32_t slices,
                                                        const Part *parts, const uint64_t *keys) {
+    constexpr uint32_t kEach = kMaxSlices * kMaxTop / kStream;
     __shared__ uint64_t all[kMaxSlices * kMaxTop];
+    __shared__ uint32_t found;
     const uint64_t r = blockIdx.x;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
-    Part st = merge_parts<true>(parts + r * slices, slices, c);
-    if (st.m == -INFINITY) st.m = 0.0f;
-    if (threadIdx.x == 0) {
-        const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
-        const T *z = static_cast<const T *>(a.logits) + r * a.stride;
-        write_answer(a, r, y < 0 ? 0.0f : (float)z[y], y >= 0, st, inv_t);
-    }
-    const uint32_t n = slices * a.top;
-    for (uint32_t i = threadIdx.x; i < n; i += kStream) all[i] = keys[r * n + i];
-    __syncthreads();
-    const float log_s = logf(st.s);
-    for (uint32_t i = threadIdx.x; i < n; i += kStream) {
-        const uint64_t key = all[i];
-        uint32_t rank = 0; // a missing key (0) counts as after every other, in its own order
-        for (uint32_t s = 0; s < slices; ++s) {
-            const uint64_t *list = all + s * a.top;
-            uint32_t lo = 0, hi = a.top;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (list[mid] > key) lo = mid + 1;
-                else hi = mid;
-            }
-            rank += lo;
+    const float inv_t = a.inv_t, c = a.c;
+    const uint32_t lane = threadIdx.x & 63u, n = slices * a.top;
+    if (threadIdx.x == 0) found = 0;
+    const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
+    const float zy = y < 0 ? 0.0f : (float)(static_cast<const T *>(a.logits) + r * a.stride)[y];
+    // every wavefront merges the Parts for itself, a lane each
+    Part st = {-INFINITY, 0.0f, 0.0f};
+    if (lane < slices) st = parts[r * slices + lane];
+    uint64_t mine[kEach];
+    uint32_t bound = 0;
+    if (a.top) {
+#pragma unroll
+        for (uint32_t k = 0; k < kEach; ++k) {
+            const uint32_t i = k * kStream + threadIdx.x;
+            mine[k] = i < n ? keys[r * n + i] : 0;
         }
-        if (key != 0 && rank < a.top) write_best(a, r, rank, key, st, inv_t, log_s);
+        const uint32_t q = (a.top + slices - 1) / slices;
+        bound = lane < slices ? (uint32_t)(keys[r * n + lane * a.top + q - 1] >> 32) : 0u;
+        bound = max(kth_of_wave(bound, (a.top + q - 1) / q), 1u);
     }
-    // the labels there are, where they are fewer than asked for
-    uint32_t some = 0;
-    for (uint32_t i = threadIdx.x & 63u; i < n; i += 64u) some += all[i] != 0;
-    some = group_all<64>(some, [](uint32_t x, uint32_t y) { return x + y; });
+    merge_lanes<64, true>(st, c);
+    if (st.m == -INFINITY) st.m = 0.0f;
+    if (threadIdx.x == 0) write_answer(a, r, zy, y >= 0, st, inv_t, logf(st.s));
+    if (!a.top) return;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k)
+        if ((uint32_t)(mine[k] >> 32) >= bound) all[atomicAdd(&found, 1u)] = mine[k];
+    __syncthreads();
+    const uint32_t some = found;
+    const float log_s = logf(st.s);
+    for (uint32_t i = threadIdx.x; i < some; i += kStream) {
+        const uint64_t key = all[i];
+        uint32_t rank = 0;
+        for (uint32_t o = 0; o < some; ++o) rank += all[o] > key;
+        if (rank < a.top) write_best(a, r, rank, key, st, inv_t, log_s);
+    }
+    // fewer labels than asked for
     if (threadIdx.x >= some && threadIdx.x < a.top)
         write_best(a, r, threadIdx.x, 0, st, inv_t, log_s);
 }
@@ -709,44 +759,74 @@ __global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_
     const uint64_t r = ((uint64_t)blockIdx.x * 256u + threadIdx.x) / kLanes;
     if (r >= rows) return; // a whole group
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    const float inv_t = a.inv_t, c = a.c;
     const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
     const float zy = y < 0 ? 0.0f : (float)z[y];
+    const Span<T> span(z, 0u, a.labels);
     Chunk<T> held[kHeld];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        held[i] = load_raw(z, (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+    for (int i = 0; i < kHeld; ++i) held[i] = span.load((l + i * kLanes) * kN, (T)-INFINITY);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        mask_chunk(held[i], (l + i * kLanes) * kN, 0u, a.labels, (T)-INFINITY);
+    for (int i = 0; i < kHeld; ++i) span.mask(held[i], (l + i * kLanes) * kN, (T)-INFINITY);
     Part st = {-INFINITY, 0.0f, 0.0f};
-    absorb<true>(st, held, c);
+    absorb<true, 2>(st, held, c);
     merge_lanes<kLanes, true>(st, c);
     if (st.m == -INFINITY) st.m = 0.0f;
-    if (l == 0) write_answer(a, r, zy, y >= 0, st, inv_t);
-    if (!a.top) return;
     const float log_s = logf(st.s);
-    uint32_t o[kHeld * kN];
+    if (l == 0) write_answer(a, r, zy, y >= 0, st, inv_t, log_s);
+    if (!a.top) return;
+    // lane k % kLanes keeps the k-th best until every lane has one to write
+    const auto flush = [&](uint32_t k, uint64_t key) {
+        const uint32_t last = k % kLanes;
+        if (l <= last) write_best(a, r, k - last + l, key, st, inv_t, log_s);
+    };
+    const auto greater = [](uint32_t x, uint32_t w) { return max(x, w); };
+    constexpr uint32_t kOwn = kHeld * kN;
+    if constexpr (sizeof(T) == 2) {
+        // order and label fit 32 bits (the label from the end: ties to the lowest)
+        uint32_t key[kOwn], kept = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kHeld * kN; ++i) o[i] = logit_order((float)held[i / kN].v[i % kN]);
-    for (uint32_t k = 0; k < a.top; ++k) {
-        uint32_t best = 0, at = 0;
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            const uint32_t label = span.place((l + i / kN * kLanes) * kN) + i % kN;
+            const uint32_t o = half_order(held[i / kN].bits(i % kN), held[i / kN][i % kN]);
+            key[i] = o ? o << 16 | (0xffffu - label) : 0u;
+        }
+        for (uint32_t k = 0; k < a.top; ++k) {
+            uint32_t best = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kHeld * kN; ++i)
-            if (o[i] > best) {
-                best = o[i];
-                at = i;
+            for (uint32_t i = 0; i < kOwn; ++i) best = max(best, key[i]);
+            best = group_all<kLanes>(best, greater);
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) key[i] = key[i] == best ? 0u : key[i];
+            kept = l == k % kLanes ? best : kept;
+            if (k % kLanes == kLanes - 1 || k + 1 == a.top)
+                flush(k, kept ? key_of(logit_order(half_value<T>(kept >> 16)), 0xffffu - (kept & 0xffffu))
+                              : 0);
+        }
+    } else {
+        uint32_t o[kOwn];
+        uint64_t kept = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) o[i] = logit_order(held[i / kN][i % kN]);
+        for (uint32_t k = 0; k < a.top; ++k) {
+            uint32_t best = 0, at = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i)
+                if (o[i] > best) {
+                    best = o[i];
+                    at = i;
+                }
+            const uint32_t top = group_all<kLanes>(best, greater);
+            const uint32_t label = span.place((l + at / kN * kLanes) * kN) + at % kN;
+            const uint32_t lowest =
+                group_all<kLanes>(best == top ? label : 0xffffffffu,
+                                  [](uint32_t x, uint32_t w) { return min(x, w); });
+            if (label == lowest) {
+#pragma unroll
+                for (uint32_t i = 0; i < kOwn; ++i) o[i] = i == at ? 0u : o[i];
             }
-        const uint32_t top = group_all<kLanes>(best, [](uint32_t x, uint32_t w) { return max(x, w); });
-        const uint32_t label =
-            place<T>((l + at / kN * kLanes) * kN, 0u, a.labels) + at % kN;
-        const uint32_t lowest =
-            group_all<kLanes>(best == top ? label : 0xffffffffu,
-                              [](uint32_t x, uint32_t w) { return min(x, w); });
-        if (l == 0) write_best(a, r, k, top ? key_of(top, lowest) : 0, st, inv_t, log_s);
-        if (label == lowest) {
-#pragma unroll
-            for (uint32_t i = 0; i < kHeld * kN; ++i) o[i] = i == at ? 0u : o[i];
+            if (l == k % kLanes) kept = top ? key_of(top, lowest) : 0;
+            if (k % kLanes == kLanes - 1 || k + 1 == a.top) flush(k, kept);
         }
     }
 }
@@ -762,7 +842,7 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, uint64_t
     const uint32_t end = min(a.labels, begin + tile);
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
-    const float inv_t = 1.0f / a.temperature, c = inv_t * kLog2e;
+    const float inv_t = a.inv_t, c = a.c;
     const float2 st = a.stats[r];
     const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
     const bool live = !(st.y == 0.0f);
@@ -771,15 +851,15 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, uint64_t
     // -p (glp + gh (log p + H)) = -e / S (gh ln2 d + glp + gh (H - log S))
     const float slope = gh / kLog2e, level = glp + gh * (a.entropy[r] - logf(st.y));
     const float inv_s = live ? -1.0f / st.y : 0.0f;
-    map_chunks<kLanes, kUnroll>(z, dz, begin, end, [&](const Chunk<T> &ch, uint32_t at) {
-        Chunk<T> o;
+    map_chunks<kLanes, kUnroll>(Span<T>(z, begin, end), dz, [&](const Chunk<T> &ch, uint32_t at) {
+        Chunk<T> o = {};
 #pragma unroll
         for (int e = 0; e < Chunk<T>::kN; ++e) {
-            const float d = ((float)ch.v[e] - st.x) * c;
+            const float d = (ch[e] - st.x) * c;
             const float p = __builtin_amdgcn_exp2f(d) * inv_s;
             float g = live ? p * fmaf(slope, fmaxf(d, -200.0f), level) : 0.0f;
             if ((int32_t)(at + e) == y) g += glp;
-            o.v[e] = (T)g;
+            o.set(e, (T)g);
         }
         return o;
     });
@@ -838,12 +918,17 @@ Slices slices_of(uint64_t rows, uint64_t labels, uint32_t most) {
 }
 constexpr uint32_t kShort = 64 * 4; // chunks of a row that a wavefront holds
 
+// Chunks of a row at most: one more where rows begin between 16-byte boundaries.
+template <typename T> uint64_t chunks_of(const void *logits, uint64_t stride, uint64_t labels) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(logits) & 15u) == 0 &&
+                         stride * sizeof(T) % 16 == 0;
+    return (labels + (aligned ? 0 : Chunk<T>::kN - 1) + Chunk<T>::kN - 1) / Chunk<T>::kN;
+}
 // f(lanes, chunks held by each) of a short row, as types
 template <int kV> struct Int {
     static constexpr int v = kV;
 };
-template <typename T, typename F> void with_short(uint64_t labels, F f) {
-    const uint64_t chunks = (labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+template <typename F> void with_short(uint64_t chunks, F f) {
     if (chunks <= 8) f(Int<8>(), Int<1>());
     else if (chunks <= 16) f(Int<16>(), Int<1>());
     else if (chunks <= 32) f(Int<16>(), Int<2>());
@@ -854,9 +939,9 @@ template <typename T, typename F> void with_short(uint64_t labels, F f) {
 
 template <typename T, bool kHaveStats>
 void launch_short(const DistillArgs &a, uint64_t rows, hipStream_t s) {
-    with_short<T>(a.labels, [&](auto lanes, auto held) {
+    with_short(chunks_of<T>(a.logits, a.stride, a.labels), [&](auto lanes, auto held) {
         constexpr uint32_t kLanes = decltype(lanes)::v;
-        const size_t row_bytes = a.logits_grad ? 8 * (size_t)a.top : 0;
+        const size_t row_bytes = kEntryBytes * (size_t)a.top;
         uint32_t threads = 256; // fewer where the teacher's entries fill LDS
         while (threads > 64 && threads / kLanes * row_bytes > 32768) threads /= 2;
         const uint64_t per = threads / kLanes;
@@ -874,13 +959,14 @@ void launch_finish(const DistillArgs &a, uint64_t rows, const Part *parts, uint3
     // where rows are few, as many blocks as the statistics had
     const uint32_t tile = slices > 1 ? ((a.labels + slices - 1) / slices + 7) / 8 * 8 : kTile;
     const uint32_t tiles = a.logits_grad ? (a.labels + tile - 1) / tile : 1;
-    hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(rows * tiles)), dim3(kStream), 0, s, a,
+    hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(rows * tiles)), dim3(kStream),
+                       kEntryBytes * a.top, s, a,
                        tiles, a.logits_grad ? tile : a.labels, parts, slices);
 }
 
 template <typename T>
 void launch_distill(const DistillArgs &a, uint64_t rows, Part *parts, hipStream_t s) {
-    const uint64_t chunks = (a.labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    const uint64_t chunks = chunks_of<T>(a.logits, a.stride, a.labels);
     if (chunks <= kShort) return launch_short<T, false>(a, rows, s);
     const Slices sl = slices_of(rows, a.labels, 64);
     if (sl.count > 1) {
@@ -890,21 +976,23 @@ void launch_distill(const DistillArgs &a, uint64_t rows, Part *parts, hipStream_
     }
     const auto launch = [&](auto threads, auto held) {
         hipLaunchKernelGGL((distill_kernel<T, decltype(threads)::v, decltype(held)::v>),
-                           dim3((unsigned)rows), dim3(decltype(threads)::v), 0, s, a);
+                           dim3((unsigned)rows), dim3(decltype(threads)::v), kEntryBytes * a.top, s,
+                           a);
     };
     if (!a.logits_grad) return launch(Int<kStream>(), Int<0>());
     if (chunks <= 256 * 4) launch(Int<256>(), Int<4>());
     else if (chunks <= 512 * 4) launch(Int<512>(), Int<4>());
-    else if (chunks <= 512 * 8) launch(Int<512>(), Int<8>());
-    else launch(Int<1024>(), Int<8>());
+    else if (chunks <= 512 * 9) launch(Int<512>(), Int<8>());
+    else if (chunks <= 512 * 13) launch(Int<512>(), Int<12>());
+    else launch(Int<512>(), Int<16>());
 }
 
 template <typename T>
 void launch_answer(const AnswerArgs &a, uint64_t rows, const Slices &sl, void *scratch,
                    hipStream_t s) {
-    const uint64_t chunks = (a.labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    const uint64_t chunks = chunks_of<T>(a.logits, a.stride, a.labels);
     if (chunks <= kShort) {
-        with_short<T>(a.labels, [&](auto lanes, auto held) {
+        with_short(chunks_of<T>(a.logits, a.stride, a.labels), [&](auto lanes, auto held) {
             constexpr uint32_t kLanes = decltype(lanes)::v;
             hipLaunchKernelGGL((answer_short_kernel<T, kLanes, decltype(held)::v>),
                                dim3((unsigned)((rows * kLanes + 255) / 256)), dim3(256), 0, s, a,
@@ -922,7 +1010,7 @@ void launch_answer(const AnswerArgs &a, uint64_t rows, const Slices &sl, void *s
 }
 
 template <typename T> void launch_answer_grad(const AnswerArgs &a, uint64_t rows, hipStream_t s) {
-    const uint64_t chunks = (a.labels + Chunk<T>::kN - 1) / Chunk<T>::kN;
+    const uint64_t chunks = chunks_of<T>(a.logits, a.stride, a.labels);
     const auto launch = [&](auto lanes) {
         constexpr uint32_t kLanes = decltype(lanes)::v;
         const uint32_t tile = kLanes == 256 ? 256 * Chunk<T>::kN * kUnroll : a.labels;
@@ -974,9 +1062,11 @@ int check_distill(const char *what, int type, const void *logits, uint64_t rows,
 
 extern "C" {
 
-size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels) {
+// the rows' losses where they are added up, and the Parts of slices
+size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels, int reduction) {
     const Slices sl = slices_of(rows, labels, 64);
-    return align256(4 * rows) + (sl.count > 1 ? align256(rows * sl.count * sizeof(Part)) : 0) + 256;
+    return (reduction == SDF_REDUCE_NONE ? 0 : align256(4 * rows)) +
+           (sl.count > 1 ? align256(rows * sl.count * sizeof(Part)) : 0);
 }
 
 int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, uint64_t stride,
@@ -991,8 +1081,8 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
     if (rc != SDF_OK) return rc;
     if (!loss && (rows > 0 || reduction != SDF_REDUCE_NONE))
         return fail(SDF_E_INVALID, "NULL pointer argument");
-    const size_t need = sdf_distill_scratch_bytes(rows, labels);
-    if (!scratch || scratch_bytes < need)
+    const size_t need = sdf_distill_scratch_bytes(rows, labels, reduction);
+    if (scratch_bytes < need || (need > 0 && !scratch))
         return fail(SDF_E_INVALID, "scratch must hold %zu bytes (got %zu)", need, scratch_bytes);
     if ((reinterpret_cast<uintptr_t>(scratch) & 255u) != 0)
         return fail(SDF_E_INVALID, "scratch must be 256-byte aligned");
@@ -1000,10 +1090,12 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
     const bool none = reduction == SDF_REDUCE_NONE;
     const float reduce = reduction == SDF_REDUCE_MEAN ? (float)(1.0 / (double)rows) : 1.0f;
     DistillArgs a = {logits, stride, (uint32_t)labels, id_type, teacher_labels, teacher_type,
-                     teacher_logits, top, temperature, row_weight, loss_grad, none ? 1u : 0u,
+                     teacher_logits, top, temperature, 1.0f / temperature,
+                     1.0f / temperature * kLog2e, row_weight, loss_grad, none ? 1u : 0u,
                      reduce, none ? loss : static_cast<float *>(scratch),
                      reinterpret_cast<float2 *>(stats), logits_grad};
-    Part *parts = reinterpret_cast<Part *>(static_cast<char *>(scratch) + align256(4 * rows));
+    Part *parts = reinterpret_cast<Part *>(static_cast<char *>(scratch) +
+                                           (none ? 0 : align256(4 * rows)));
     with_type(type, [&](auto t) {
         for_windows(rows, [&](uint64_t r, uint64_t n) {
             launch_distill<decltype(t)>(from_row(a, type, r), n, parts, s);
@@ -1029,13 +1121,14 @@ int sdf_distill_backward(int type, const void *logits, uint64_t rows, uint64_t l
     if (!loss_grad || !stats || !logits_grad) return fail(SDF_E_INVALID, "NULL pointer argument");
     const float reduce = reduction == SDF_REDUCE_MEAN ? (float)(1.0 / (double)rows) : 1.0f;
     DistillArgs a = {logits, stride, (uint32_t)labels, id_type, teacher_labels, teacher_type,
-                     teacher_logits, top, temperature, row_weight, loss_grad,
+                     teacher_logits, top, temperature, 1.0f / temperature,
+                     1.0f / temperature * kLog2e, row_weight, loss_grad,
                      reduction == SDF_REDUCE_NONE ? 1u : 0u, reduce, nullptr,
                      reinterpret_cast<float2 *>(const_cast<float *>(stats)), logits_grad};
     with_type(type, [&](auto t) {
         using T = decltype(t);
         hipStream_t s = static_cast<hipStream_t>(stream);
-        const bool is_short = (labels + Chunk<T>::kN - 1) / Chunk<T>::kN <= kShort;
+        const bool is_short = chunks_of<T>(logits, stride, labels) <= kShort;
         for_windows(rows, [&](uint64_t r, uint64_t n) {
             const DistillArgs w = from_row(a, type, r);
             if (is_short) launch_short<T, true>(w, n, s);
@@ -1048,7 +1141,7 @@ int sdf_distill_backward(int type, const void *logits, uint64_t rows, uint64_t l
 
 size_t sdf_label_log_probs_scratch_bytes(uint64_t rows, uint64_t labels, uint32_t top) {
     const Slices sl = slices_of(rows, labels, kMaxSlices);
-    return sl.count > 1 ? align256(rows * sl.count * (sizeof(Part) + 8 * (size_t)top)) + 256 : 256;
+    return sl.count > 1 ? align256(rows * sl.count * (sizeof(Part) + 8 * (size_t)top)) : 256;
 }
 
 int sdf_label_log_probs(int type, const void *logits, uint64_t rows, uint64_t labels,
@@ -1065,11 +1158,12 @@ int sdf_label_log_probs(int type, const void *logits, uint64_t rows, uint64_t la
     if (!label_ids || !log_prob || !entropy || (top > 0 && (!top_log_probs || !top_labels)))
         return fail(SDF_E_INVALID, "NULL pointer argument");
     const size_t need = sdf_label_log_probs_scratch_bytes(rows, labels, top);
-    if (!scratch || scratch_bytes < need)
+    if (scratch_bytes < need || (need > 0 && !scratch))
         return fail(SDF_E_INVALID, "scratch must hold %zu bytes (got %zu)", need, scratch_bytes);
     if ((reinterpret_cast<uintptr_t>(scratch) & 255u) != 0)
         return fail(SDF_E_INVALID, "scratch must be 256-byte aligned");
-    AnswerArgs a = {logits, stride, (uint32_t)labels, id_type, label_ids, top, temperature,
+    AnswerArgs a = {logits, stride, (uint32_t)labels, id_type, label_ids, top,
+                    1.0f / temperature, 1.0f / temperature * kLog2e,
                     log_prob, entropy, top_log_probs, top_labels,
                     reinterpret_cast<float2 *>(stats), nullptr, nullptr, nullptr};
     with_type(type, [&](auto t) {
@@ -1094,7 +1188,8 @@ int sdf_label_log_probs_backward(int type, const void *logits, uint64_t rows, ui
     if (rows == 0) return SDF_OK;
     if (!label_ids || !entropy || !stats || !logits_grad)
         return fail(SDF_E_INVALID, "NULL pointer argument");
-    AnswerArgs a = {logits, stride, (uint32_t)labels, id_type, label_ids, 0, temperature, nullptr,
+    AnswerArgs a = {logits, stride, (uint32_t)labels, id_type, label_ids, 0,
+                    1.0f / temperature, 1.0f / temperature * kLog2e, nullptr,
                     const_cast<float *>(entropy), nullptr, nullptr,
                     reinterpret_cast<float2 *>(const_cast<float *>(stats)), log_prob_grad,
                     entropy_grad, logits_grad};

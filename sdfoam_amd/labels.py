@@ -68,12 +68,15 @@ def _check_float32(name: str, t: torch.Tensor, shape) -> None:
     _check_shape(name, t, shape)
 
 
-def _check_devices(first: str, t: torch.Tensor, **others) -> None:
-    if t.device.type != "cuda":
+def _check_devices(first: str, t: torch.Tensor, *others) -> None:
+    """others: name, tensor or None, name, ..."""
+    device = t.device
+    if device.type != "cuda":
         raise RuntimeError(f"{first} must be on CUDA device")
-    for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise RuntimeError(f"{name} must be on the device of {first}")
+    for k in range(1, len(others), 2):
+        o = others[k]
+        if o is not None and o.device != device:
+            raise RuntimeError(f"{others[k - 1]} must be on the device of {first}")
 
 
 def _no_gradient(call: str, **tensors) -> None:
@@ -103,17 +106,26 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _call(function, device: torch.device, *args) -> None:
     """The library call on the device's current stream."""
-    if torch.cuda.current_device() == device.index:
-        check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+            status = function(*args, _raw_stream(index))
+    if status:
+        check(status)
+
+
+# the stream's handle alone, without the Stream object around it (2 us of a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_handle)
 
 
 def _scratch(nbytes: int, device: torch.device):
     """Scratch memory (kept alive by the first value) and its 256-byte aligned start.  It
     may go once the call is queued: torch gives it out again only to later work on the
     same stream."""
+    if nbytes == 0:
+        return None, None
     t = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
     return t, (t.data_ptr() + 255) & ~255
 
@@ -127,13 +139,14 @@ def _check_weight(weight, cells) -> None:
 
 
 def _rows_forward(table, cells, weight, scale) -> torch.Tensor:
-    rows = torch.empty((*cells.shape, table.size(1)), dtype=table.dtype, device=table.device)
+    device, (num_cells, width) = table.device, table.shape
+    rows = torch.empty((*cells.shape, width), dtype=table.dtype, device=device)
     t = _rows(table)
     c = cells.contiguous()
     w = None if weight is None else weight.contiguous()
-    _call(_lib.lib().sdf_cell_rows, table.device, _TYPES[table.dtype], ptr(t), t.stride(0),
-          t.size(0), t.size(1), _ID_TYPES[cells.dtype], ptr(c), c.numel(), ptr(w), scale,
-          ptr(rows))
+    _call(_lib.lib().sdf_cell_rows, device, _TYPES[table.dtype], t.data_ptr(), t.stride(0),
+          num_cells, width, _ID_TYPES[cells.dtype], c.data_ptr(), c.numel(), ptr(w), scale,
+          rows.data_ptr())
     return rows
 
 
@@ -188,7 +201,7 @@ def cell_rows(table: torch.Tensor, cells: torch.Tensor, weight: Optional[torch.T
     _element_type("table", table)
     _id_type("cells", cells)
     _check_weight(weight, cells)
-    _check_devices("table", table, cells=cells, weight=weight)
+    _check_devices("table", table, "cells", cells, "weight", weight)
     if _wants_gradient(table, weight):
         return _CellRows.apply(table, cells, weight, float(scale))
     return _rows_forward(table, cells, weight, float(scale))
@@ -215,9 +228,8 @@ def cell_rows_backward(rows_grad: torch.Tensor, cells: torch.Tensor, num_cells: 
         if table.dtype != rows_grad.dtype:
             raise RuntimeError("table and rows_grad must have the same dtype")
         _check_shape("table", table, (num_cells, rows_grad.size(-1)))
-    _check_devices("rows_grad", rows_grad, cells=cells, weight=weight, table=table)
-    with torch.no_grad():
-        return _rows_backward(rows_grad, cells, num_cells, weight, float(scale), table, True)
+    _check_devices("rows_grad", rows_grad, "cells", cells, "weight", weight, "table", table)
+    return _rows_backward(rows_grad, cells, num_cells, weight, float(scale), table, True)
 
 
 # ---- distillation ----------------------------------------------------------------------------
@@ -249,8 +261,8 @@ def _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weig
         _check_float32("row_weight", row_weight, logits.shape[:-1])
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be 'none', 'sum' or 'mean'")
-    _check_devices("logits", logits, teacher_labels=teacher_labels,
-                   teacher_logits=teacher_logits, row_weight=row_weight)
+    _check_devices("logits", logits, "teacher_labels", teacher_labels, "teacher_logits",
+                   teacher_logits, "row_weight", row_weight)
     return temperature
 
 
@@ -265,20 +277,20 @@ class _Distill:
         self.temperature, self.reduction = temperature, reduction
 
     def args(self):
-        z = self.z
-        return (_TYPES[z.dtype], ptr(z), z.size(0), z.size(1), z.stride(0),
-                _ID_TYPES[self.ids.dtype], ptr(self.ids), _TYPES[self.t.dtype], ptr(self.t),
-                self.ids.size(-1), self.temperature, ptr(self.weight),
-                _REDUCTIONS[self.reduction])
+        z, ids, t = self.z, self.ids, self.t
+        rows, labels = z.shape
+        return (_TYPES[z.dtype], z.data_ptr(), rows, labels, z.stride(0), _ID_TYPES[ids.dtype],
+                ids.data_ptr(), _TYPES[t.dtype], t.data_ptr(), ids.size(-1), self.temperature,
+                ptr(self.weight), _REDUCTIONS[self.reduction])
 
     def forward(self, shape, loss_grad=None, stats=None, logits_grad=None) -> torch.Tensor:
         dev = self.z.device
-        loss = torch.empty(shape if self.reduction == "none" else (), dtype=torch.float32,
-                           device=dev)
+        none = self.reduction == "none"
+        loss = torch.empty(shape if none else (), dtype=torch.float32, device=dev)
         L = _lib.lib()
-        nbytes = int(L.sdf_distill_scratch_bytes(self.z.size(0), self.z.size(1)))
+        nbytes = L.sdf_distill_scratch_bytes(*self.z.shape, _REDUCTIONS[self.reduction])
         keep, base = _scratch(nbytes, dev)
-        _call(L.sdf_distill, dev, *self.args(), ptr(loss_grad), ptr(loss), ptr(stats),
+        _call(L.sdf_distill, dev, *self.args(), ptr(loss_grad), loss.data_ptr(), ptr(stats),
               ptr(logits_grad), base, nbytes)
         return loss
 
@@ -343,13 +355,11 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_labels: torch.Tensor,
                                  reduction)
     if loss_grad is not None:
         _check_float32("loss_grad", loss_grad, logits.shape[:-1] if reduction == "none" else ())
-        _check_devices("logits", logits, loss_grad=loss_grad)
+        _check_devices("logits", logits, "loss_grad", loss_grad)
         loss_grad = loss_grad.contiguous()
-    with torch.no_grad():
-        a = _Distill(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction)
-        logits_grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        loss = a.forward(logits.shape[:-1], loss_grad, None, logits_grad)
-    return loss, logits_grad
+    a = _Distill(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction)
+    logits_grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return a.forward(logits.shape[:-1], loss_grad, None, logits_grad), logits_grad
 
 
 # ---- answers ---------------------------------------------------------------------------------
@@ -369,6 +379,7 @@ def _answer(logits, labels, top, temperature, stats=None):
     z = _rows(logits)
     y = labels.contiguous()
     dev, shape = logits.device, labels.shape
+    rows, count = z.shape
     log_prob = torch.empty(shape, dtype=torch.float32, device=dev)
     entropy = torch.empty(shape, dtype=torch.float32, device=dev)
     best = best_labels = None
@@ -376,11 +387,11 @@ def _answer(logits, labels, top, temperature, stats=None):
         best = torch.empty((*shape, top), dtype=torch.float32, device=dev)
         best_labels = torch.empty((*shape, top), dtype=torch.int64, device=dev)
     L = _lib.lib()
-    nbytes = int(L.sdf_label_log_probs_scratch_bytes(z.size(0), z.size(1), top))
+    nbytes = L.sdf_label_log_probs_scratch_bytes(rows, count, top)
     keep, base = _scratch(nbytes, dev)
-    _call(L.sdf_label_log_probs, dev, _TYPES[z.dtype], ptr(z), z.size(0), z.size(1), z.stride(0),
-          _ID_TYPES[y.dtype], ptr(y), top, temperature, ptr(log_prob), ptr(entropy), ptr(best),
-          ptr(best_labels), ptr(stats), base, nbytes)
+    _call(L.sdf_label_log_probs, dev, _TYPES[z.dtype], z.data_ptr(), rows, count, z.stride(0),
+          _ID_TYPES[y.dtype], y.data_ptr(), top, temperature, log_prob.data_ptr(),
+          entropy.data_ptr(), ptr(best), ptr(best_labels), ptr(stats), base, nbytes)
     return log_prob, entropy, best, best_labels
 
 
@@ -430,7 +441,7 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0,
     top = int(top)
     if not 0 <= top <= MAX_TOP:
         raise RuntimeError(f"top must be from 0 to {MAX_TOP}")
-    _check_devices("logits", logits, labels=labels)
+    _check_devices("logits", logits, "labels", labels)
     if _wants_gradient(logits):
         return LabelLogProbs(*_LabelLogProbs.apply(logits, labels, top, temperature))
     return LabelLogProbs(*_answer(logits, labels, top, temperature))
