@@ -76,8 +76,18 @@ template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *p)
     __builtin_memcpy(&c, p, 16);
     return c;
 }
-template <typename T> __device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
-    __builtin_memcpy(p, &c, 16);
+// kPast: past the caches
+template <bool kPast = false, typename T>
+__device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
+    if constexpr (kPast) {
+        typedef uint32_t Words2 __attribute__((ext_vector_type(4), aligned(2)));
+        typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
+        const Words4 w = {c.w[0], c.w[1], c.w[2], c.w[3]};
+        if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(w, reinterpret_cast<Words2 *>(p));
+        else __builtin_nontemporal_store(w, reinterpret_cast<Words4 *>(p));
+    } else {
+        __builtin_memcpy(p, &c, 16);
+    }
 }
 // Elements [begin, end) of a row, cut into chunks at 16-byte boundaries: chunk
 // `at` (begin, begin + kN, ...) has the elements [at, at + kN) moved down by
@@ -136,8 +146,9 @@ template <typename T> struct Span {
             if (from + e < lo || from + e >= hi) c.set(e, fill);
     }
     // the chunk's own elements into another row
+    template <bool kPast = false>
     __device__ __forceinline__ void store_own(T *to, uint32_t at, const Chunk<T> &c) const {
-        if (plain(at)) store_chunk(to + place(at), c);
+        if (plain(at)) store_chunk<kPast>(to + place(at), c);
         else each_own(at, [&](uint32_t e, uint32_t i) { to[i] = c.value(e); });
     }
 };

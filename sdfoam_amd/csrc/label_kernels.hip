@@ -98,13 +98,14 @@ template <bool kEntropy> __device__ __forceinline__ Part merge_block(Part p, Par
 }
 
 // f(chunks, at) over a span, kU chunks of each of kThreads threads at a time,
-// chunk i at `at` + i kThreads kN; what is not a chunk's own is -inf where
-// kMask, else as it was read.  Only the steps that begin in [first, last).
+// chunk i at `at` + i kThreads kN, and one by one where the span's end leaves
+// fewer; what is not a chunk's own is -inf where kMask, else as it was read.
+// Only the steps that begin in [first, last).
 template <int kThreads, int kU, bool kMask, typename T, typename F>
 __device__ __forceinline__ void for_steps(const Span<T> &z, uint32_t first, uint32_t last, F f) {
     constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
-    for (; first < last; first += kStep * kU) {
-        const uint32_t at = first + threadIdx.x % kThreads * Chunk<T>::kN;
+    uint32_t at = first + threadIdx.x % kThreads * Chunk<T>::kN;
+    for (; first < last && first + kStep * kU <= z.last(); first += kStep * kU, at += kStep * kU) {
         Chunk<T> ch[kU];
         if (z.plain_step(first, kStep * kU)) {
             const T *p = z.row + (at - z.skew);
@@ -120,6 +121,12 @@ __device__ __forceinline__ void for_steps(const Span<T> &z, uint32_t first, uint
         }
         f(ch, at);
     }
+    if (first >= last) return;
+    for (; at < z.last(); at += kStep) {
+        Chunk<T> ch[1] = {z.load(at, (T)-INFINITY)};
+        if (kMask) z.mask(ch[0], at, (T)-INFINITY);
+        f(ch, at);
+    }
 }
 template <int kThreads, int kU, bool kMask, typename T, typename F>
 __device__ __forceinline__ void for_chunks(const Span<T> &z, F f) {
@@ -129,9 +136,9 @@ __device__ __forceinline__ void for_chunks(const Span<T> &z, F f) {
 template <int kThreads, int kU, typename T, typename F>
 __device__ __forceinline__ void map_chunks(const Span<T> &z, T *to, F f) {
     constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
-    for_chunks<kThreads, kU, false>(z, [&](const Chunk<T>(&ch)[kU], uint32_t at) {
+    for_chunks<kThreads, kU, false>(z, [&](const auto &ch, uint32_t at) {
 #pragma unroll
-        for (int i = 0; i < kU; ++i)
+        for (int i = 0; i < (int)(sizeof(ch) / 16); ++i)
             if (at + i * kStep < z.last()) {
                 const uint32_t from = z.place(at + i * kStep);
                 const Chunk<T> o = f(ch[i], from);
@@ -147,9 +154,8 @@ constexpr int kUnroll = 4;   // chunks in flight per thread
 
 template <bool kEntropy, int kThreads, typename T>
 __device__ __forceinline__ void stream_part(Part &p, const Span<T> &z, float c) {
-    for_chunks<kThreads, kUnroll, true>(z, [&](const Chunk<T>(&ch)[kUnroll], uint32_t) {
-        absorb<kEntropy, kUnroll>(p, ch, c);
-    });
+    for_chunks<kThreads, kUnroll, true>(
+        z, [&](const auto &ch, uint32_t) { absorb<kEntropy, kUnroll>(p, ch, c); });
 }
 
 struct DistillArgs {
@@ -298,6 +304,10 @@ __global__ __launch_bounds__(kThreads)
     const Span<T> z(static_cast<const T *>(a.logits) + r * a.stride, 0u, a.labels);
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
     constexpr uint32_t kRest = kThreads * kN * kHeld;
+    // past the caches: what is written would push out what is read again
+    // (2,048 rows of 262,144: 553 -> 479 us; 16,384 of 32,768, held whole, 457
+    // -> 479)
+    constexpr bool kPast = kHeld > 8;
     const float u = row_weight(a, r);
     Teacher t = {0.0f, 0.0f};
     Part st = {0.0f, 0.0f, 0.0f};
@@ -323,10 +333,9 @@ __global__ __launch_bounds__(kThreads)
                 }
                 absorb<false, 2>(p, held, a.c);
             }
-            for_steps<kThreads, kUnroll, true>(z, kRest, z.last(),
-                                               [&](const Chunk<T>(&ch)[kUnroll], uint32_t) {
-                                                   absorb<false, kUnroll>(p, ch, a.c);
-                                               });
+            for_steps<kThreads, kUnroll, true>(
+                z, kRest, z.last(),
+                [&](const auto &ch, uint32_t) { absorb<false, kUnroll>(p, ch, a.c); });
             st = merge_block<false>(p, parts, a.c);
             if (st.m == -INFINITY) st.m = 0.0f;
         }
@@ -343,17 +352,17 @@ __global__ __launch_bounds__(kThreads)
             return;
         }
         const float coef = row_coef(a, r, u), share = coef / st.s;
-        for_steps<kThreads, kUnroll, true>(
-            z, kRest, z.last(), [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
+        for_steps<kThreads, kUnroll, true>(z, kRest, z.last(), [&](const auto &ch, uint32_t at) {
 #pragma unroll
-                for (int i = 0; i < kUnroll; ++i)
-                    if (at + i * kThreads * kN < z.last())
-                        z.store_own(dz, at + i * kThreads * kN, grad_chunk(ch[i], st.m, a.c, share));
-            });
+            for (int i = 0; i < (int)(sizeof(ch) / 16); ++i)
+                z.template store_own<kPast>(dz, at + i * kThreads * kN,
+                                            grad_chunk(ch[i], st.m, a.c, share));
+        });
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
             const uint32_t at = (threadIdx.x + i * kThreads) * kN;
-            if (at < z.last()) z.store_own(dz, at, grad_chunk(held[i], st.m, a.c, share));
+            if (at < z.last())
+                z.template store_own<kPast>(dz, at, grad_chunk(held[i], st.m, a.c, share));
         }
         __syncthreads(); // the teacher's labels are written over what stands there
         write_shares(a, dz, e, st, coef, threadIdx.x, kThreads, 0u, a.labels);
@@ -591,7 +600,8 @@ __device__ __forceinline__ void write_best(const AnswerArgs &a, uint64_t r, uint
 // The best labels: the threads form 64 groups, and the top-th largest of the
 // groups' largest logits bounds the top-th best label from below.  Only
 // threads whose largest logit reaches the bound (about `top`) look at theirs
-// again; what reaches it is ranked by counting.
+// again, and only at the one or two steps that hold it where no third does;
+// what reaches it is ranked by counting.
 // slices > 1: Part and keys of each slice, for join_kernel.
 template <typename T>
 __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t slices,
@@ -607,15 +617,18 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     const float inv_t = a.inv_t, c = a.c;
     const Span<T> span(z, begin, end);
-    // beside its largest logit, where the thread met it, and the largest of its
-    // other steps
+    // beside its largest logit, where the thread met it, the next largest step's
+    // and where, and the largest of its other steps
     Part mine = {-INFINITY, 0.0f, 0.0f};
-    float second = -INFINITY;
-    uint32_t where = begin;
-    for_chunks<kStream, kUnroll, true>(span, [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
-        const float before = mine.m, m = absorb<true, kUnroll>(mine, ch, c);
-        second = fmaxf(second, fminf(m, before));
-        where = m > before ? at : where;
+    float second = -INFINITY, third = -INFINITY;
+    uint32_t where = begin, where_second = begin;
+    for_chunks<kStream, kUnroll, true>(span, [&](const auto &ch, uint32_t at) {
+        const float first = mine.m, m = absorb<true, kUnroll>(mine, ch, c);
+        const bool leads = m > first, follows = m > second;
+        third = fmaxf(third, fminf(m, second));
+        where_second = leads ? where : follows ? at : where_second;
+        second = fmaxf(second, fminf(m, first));
+        where = leads ? at : where;
     });
     const uint32_t best = logit_order(mine.m);
     if (a.top) {
@@ -641,9 +654,9 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
     };
     const uint32_t bound = max(kth_of_wave(groups[threadIdx.x & 63u], a.top), 1u);
     if (best >= bound) {
-        const auto collect = [&](const Chunk<T>(&ch)[kUnroll], uint32_t at) {
+        const auto collect = [&](const auto &ch, uint32_t at) {
 #pragma unroll
-            for (int i = 0; i < kUnroll; ++i)
+            for (int i = 0; i < (int)(sizeof(ch) / 16); ++i)
 #pragma unroll
                 for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
                     const uint32_t o = logit_order(ch[i][e]);
@@ -653,9 +666,23 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
                     if (k < kCandidates) keys[k] = key_of(o, from + e);
                 }
         };
-        const bool one = logit_order(second) < bound;
-        const uint32_t first = one ? where - threadIdx.x * Chunk<T>::kN : begin;
-        for_steps<kStream, kUnroll, true>(span, first, one ? first + 1 : span.last(), collect);
+        if (logit_order(third) < bound) {
+            constexpr uint32_t kStep = kStream * Chunk<T>::kN;
+            const uint32_t own = threadIdx.x * Chunk<T>::kN;
+            const uint32_t steps = logit_order(second) < bound ? 1 : 2;
+            for (uint32_t k = 0; k < steps; ++k) {
+                const uint32_t at = k ? where_second : where, first = at - own;
+                if (first + kStep * kUnroll <= span.last()) {
+                    for_steps<kStream, kUnroll, true>(span, first, first + 1, collect);
+                } else {
+                    Chunk<T> ch[1] = {span.load(at, (T)-INFINITY)};
+                    span.mask(ch[0], at, (T)-INFINITY);
+                    collect(ch, at);
+                }
+            }
+        } else {
+            for_chunks<kStream, kUnroll, true>(span, collect);
+        }
     }
     __syncthreads();
     const uint32_t n = found;
@@ -760,12 +787,13 @@ __global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_
     if (r >= rows) return; // a whole group
     const T *z = static_cast<const T *>(a.logits) + r * a.stride;
     const float inv_t = a.inv_t, c = a.c;
-    const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
-    const float zy = y < 0 ? 0.0f : (float)z[y];
     const Span<T> span(z, 0u, a.labels);
     Chunk<T> held[kHeld];
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) held[i] = span.load((l + i * kLanes) * kN, (T)-INFINITY);
+    // (no branch: the row is on its way, and this load with the arithmetic)
+    const int32_t y = load_id(a.label_ids, a.id_type, r, a.labels);
+    const T zy = z[max(y, 0)];
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) span.mask(held[i], (l + i * kLanes) * kN, (T)-INFINITY);
     Part st = {-INFINITY, 0.0f, 0.0f};
@@ -773,7 +801,7 @@ __global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_
     merge_lanes<kLanes, true>(st, c);
     if (st.m == -INFINITY) st.m = 0.0f;
     const float log_s = logf(st.s);
-    if (l == 0) write_answer(a, r, zy, y >= 0, st, inv_t, log_s);
+    if (l == 0) write_answer(a, r, (float)zy, y >= 0, st, inv_t, log_s);
     if (!a.top) return;
     // lane k % kLanes keeps the k-th best until every lane has one to write
     const auto flush = [&](uint32_t k, uint64_t key) {
