@@ -140,10 +140,22 @@ template <typename T> struct Span {
     }
     __device__ __forceinline__ void mask(Chunk<T> &c, uint32_t at, T fill) const {
         if (plain(at)) return;
-        const uint32_t from = place(at), lo = first_own(at), hi = end_own(at);
+        // elements [lo, hi) of the chunk are its own (lo >= hi: none)
+        const uint32_t from = place(at);
+        const uint32_t lo = min(first_own(at) - from, kN), hi = max(end_own(at), from) - from;
+        const uint32_t own = hi > lo ? (1u << hi) - (1u << lo) : 0u; // hi <= kN
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (uint32_t e = 0; e < kN; ++e)
-            if (from + e < lo || from + e >= hi) c.set(e, fill);
+            for (uint32_t e = 0; e < kN; ++e) c.w[e] = own >> e & 1u ? c.w[e] : __builtin_bit_cast(uint32_t, fill);
+        } else {
+            const uint32_t both = __builtin_bit_cast(uint16_t, fill) * 0x10001u;
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) { // two elements' bits, as two masks of 16
+                const uint32_t bits = own >> (2 * q);
+                const uint32_t m = (bits & 1u ? 0xffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
+                c.w[q] = (c.w[q] & m) | (both & ~m);
+            }
+        }
     }
     // the chunk's own elements into another row
     template <bool kPast = false>
@@ -164,10 +176,10 @@ __device__ __forceinline__ void wave_sync() {
 // crossbar (quads by xor; eights and sixteens mirrored, which pairs up equal
 // values once the smaller steps are done), 32 and 64 through LDS's.
 template <int kStep> __device__ __forceinline__ uint32_t across(uint32_t x) {
-    if constexpr (kStep == 1) return __builtin_amdgcn_update_dpp(x, x, 0xb1, 0xf, 0xf, false);
-    else if constexpr (kStep == 2) return __builtin_amdgcn_update_dpp(x, x, 0x4e, 0xf, 0xf, false);
-    else if constexpr (kStep == 4) return __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false);
-    else if constexpr (kStep == 8) return __builtin_amdgcn_update_dpp(x, x, 0x140, 0xf, 0xf, false);
+    if constexpr (kStep == 1) return __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true);
+    else if constexpr (kStep == 2) return __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true);
+    else if constexpr (kStep == 4) return __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true);
+    else if constexpr (kStep == 8) return __builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true);
     else return (uint32_t)__shfl_xor((int)x, kStep);
 }
 template <int kStep> __device__ __forceinline__ float across(float x) {

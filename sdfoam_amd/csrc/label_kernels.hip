@@ -549,17 +549,41 @@ __device__ __forceinline__ uint32_t logit_order(float z) {
 __device__ __forceinline__ float order_logit(uint32_t o) {
     return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
-// The same in 16 bits for the 16-bit types, and back.
-__device__ __forceinline__ uint32_t half_order(uint32_t bits, float z) {
-    if (!(z > -INFINITY)) return 0u;
-    if (bits == 0x8000u) bits = 0;
-    return bits & 0x8000u ? ~bits & 0xffffu : bits | 0x8000u;
+// The same in 16 bits for two 16-bit elements side by side: sign and magnitude
+// become a two's complement number (so -0 and 0 are one) moved to be unsigned.
+// NaN of either sign and -inf are not taken out: -inf and negative NaN lie below
+// kLeast, positive NaN above +inf.
+__device__ __forceinline__ uint32_t half_orders(uint32_t w) {
+    typedef short Two __attribute__((ext_vector_type(2)));
+    const Two sign = __builtin_bit_cast(Two, w) >> 15;
+    const Two magnitude = __builtin_bit_cast(Two, w & 0x7fff7fffu);
+    return __builtin_bit_cast(uint32_t, (Two)((magnitude ^ sign) - sign)) ^ 0x80008000u;
 }
-template <typename T> __device__ __forceinline__ float half_value(uint32_t o) {
-    const uint16_t bits = o & 0x8000u ? (uint16_t)(o ^ 0x8000u) : (uint16_t)~o;
-    T z;
-    __builtin_memcpy(&z, &bits, 2);
-    return (float)z;
+template <typename T> struct HalfOrder {
+    static constexpr uint32_t kInf = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+    static constexpr uint32_t kLeast = 0x8000u - kInf + 1u; // of the lowest finite value
+    static constexpr uint32_t kMost = 0x8000u + kInf;       // of +inf
+    static __device__ __forceinline__ float value(uint32_t o) {
+        const uint16_t bits = (uint16_t)(o >= 0x8000u ? o - 0x8000u : 0x8000u + (0x8000u - o));
+        return (float)__builtin_bit_cast(T, bits);
+    }
+};
+// Largest first.
+template <int kCount> __device__ __forceinline__ void sort_falling(uint32_t (&x)[kCount]) {
+    // Batcher's odd-even merge sort
+#pragma unroll
+    for (int p = 1; p < kCount; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < kCount; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < kCount && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t a = x[i + j], b = x[i + j + k];
+                        x[i + j] = max(a, b);
+                        x[i + j + k] = min(a, b);
+                    }
 }
 // Keys order labels by falling logit, then by rising label; 0 is no label.
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t label) {
@@ -568,14 +592,16 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t label) {
 
 constexpr uint32_t kCandidates = 512;
 
-// The k-th largest of the wavefront's 64 values, bit by bit.
-__device__ __forceinline__ uint32_t kth_of_wave(uint32_t x, uint32_t k) {
+// A bound from below on the k-th largest of the wavefront's 64 orders, bit by
+// bit: its upper half, which is all of it for bfloat16.  At least that of the
+// lowest finite logit.
+__device__ __forceinline__ uint32_t bound_of_wave(uint32_t x, uint32_t k) {
     uint32_t t = 0;
-    for (int b = 31; b >= 0; --b) {
+    for (int b = 31; b >= 16; --b) {
         const uint32_t with = t | 1u << b;
         if ((uint32_t)__popcll(__ballot(x >= with)) >= k) t = with;
     }
-    return t;
+    return max(t, 0x00800000u);
 }
 
 __device__ __forceinline__ void write_answer(const AnswerArgs &a, uint64_t r, float z_label,
@@ -584,15 +610,20 @@ __device__ __forceinline__ void write_answer(const AnswerArgs &a, uint64_t r, fl
     float lp = 0.0f;
     if (named) lp = empty ? -INFINITY : (z_label - st.m) * inv_t - log_s;
     a.log_prob[r] = lp;
-    a.entropy[r] = empty ? 0.0f : log_s - st.w / (st.s * kLog2e);
+    a.entropy[r] = empty ? 0.0f : log_s - st.w * __builtin_amdgcn_rcpf(st.s * kLog2e);
     if (a.stats) a.stats[r] = make_float2(empty ? 0.0f : st.m, st.s);
+}
+__device__ __forceinline__ void write_best(const AnswerArgs &a, uint64_t r, uint32_t k, bool any,
+                                           float z, uint32_t label, const Part &st, float inv_t,
+                                           float log_s) {
+    a.top_labels[r * a.top + k] = any ? (int64_t)label : -1;
+    a.top_log_probs[r * a.top + k] =
+        any ? (z - st.m) * inv_t - log_s : (st.s != st.s ? st.s : -INFINITY);
 }
 __device__ __forceinline__ void write_best(const AnswerArgs &a, uint64_t r, uint32_t k, uint64_t key,
                                            const Part &st, float inv_t, float log_s) {
-    const float z = order_logit((uint32_t)(key >> 32));
-    a.top_labels[r * a.top + k] = key ? (int64_t)(0xffffffffu - (uint32_t)key) : -1;
-    a.top_log_probs[r * a.top + k] =
-        key ? (z - st.m) * inv_t - log_s : (st.s != st.s ? st.s : -INFINITY);
+    write_best(a, r, k, key != 0, order_logit((uint32_t)(key >> 32)), 0xffffffffu - (uint32_t)key, st,
+               inv_t, log_s);
 }
 
 // A block per row, or per slice of one where rows are few; one pass over the
@@ -652,15 +683,16 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
         if (slices > 1) out_keys[(r * slices + part) * a.top + k] = key;
         else write_best(a, r, k, key, st, inv_t, log_s);
     };
-    const uint32_t bound = max(kth_of_wave(groups[threadIdx.x & 63u], a.top), 1u);
+    const uint32_t bound = bound_of_wave(groups[threadIdx.x & 63u], a.top);
+    const float least = order_logit(bound);
     if (best >= bound) {
         const auto collect = [&](const auto &ch, uint32_t at) {
 #pragma unroll
             for (int i = 0; i < (int)(sizeof(ch) / 16); ++i)
 #pragma unroll
                 for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
+                    if (!(ch[i][e] >= least)) continue;
                     const uint32_t o = logit_order(ch[i][e]);
-                    if (o < bound) continue;
                     const uint32_t k = atomicAdd(&found, 1u);
                     const uint32_t from = span.place(at + i * kStream * Chunk<T>::kN);
                     if (k < kCandidates) keys[k] = key_of(o, from + e);
@@ -752,7 +784,7 @@ __global__ __launch_bounds__(kStream) void join_kernel(AnswerArgs a, uint32_t sl
         }
         const uint32_t q = (a.top + slices - 1) / slices;
         bound = lane < slices ? (uint32_t)(keys[r * n + lane * a.top + q - 1] >> 32) : 0u;
-        bound = max(kth_of_wave(bound, (a.top + q - 1) / q), 1u);
+        bound = bound_of_wave(bound, (a.top + q - 1) / q);
     }
     merge_lanes<64, true>(st, c);
     if (st.m == -INFINITY) st.m = 0.0f;
@@ -801,39 +833,59 @@ __global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_
     merge_lanes<kLanes, true>(st, c);
     if (st.m == -INFINITY) st.m = 0.0f;
     const float log_s = logf(st.s);
-    if (l == 0) write_answer(a, r, (float)zy, y >= 0, st, inv_t, log_s);
-    if (!a.top) return;
+    // (the rest is written last: a wait for a load waits for earlier stores too)
+    const auto done = [&]() {
+        if (l == 0) write_answer(a, r, (float)zy, y >= 0, st, inv_t, log_s);
+    };
+    if (!a.top) return done();
     // lane k % kLanes keeps the k-th best until every lane has one to write
-    const auto flush = [&](uint32_t k, uint64_t key) {
+    const auto flush = [&](uint32_t k, bool any, float best, uint32_t label) {
         const uint32_t last = k % kLanes;
-        if (l <= last) write_best(a, r, k - last + l, key, st, inv_t, log_s);
+        if (l <= last) write_best(a, r, k - last + l, any, best, label, st, inv_t, log_s);
     };
     const auto greater = [](uint32_t x, uint32_t w) { return max(x, w); };
     constexpr uint32_t kOwn = kHeld * kN;
     if constexpr (sizeof(T) == 2) {
         // order and label fit 32 bits (the label from the end: ties to the lowest)
+        using Order = HalfOrder<T>;
         uint32_t key[kOwn], kept = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kOwn; ++i) {
-            const uint32_t label = span.place((l + i / kN * kLanes) * kN) + i % kN;
-            const uint32_t o = half_order(held[i / kN].bits(i % kN), held[i / kN][i % kN]);
-            key[i] = o ? o << 16 | (0xffffu - label) : 0u;
+        for (uint32_t i = 0; i < kOwn; i += 2) {
+            const uint32_t label = 0xffffu - span.place((l + i / kN * kLanes) * kN) - i % kN;
+            const uint32_t o = half_orders(held[i / kN].w[i % kN / 2]);
+            key[i] = o << 16 | label;
+            key[i + 1] = (o & 0xffff0000u) | (label - 1u);
         }
+        if (st.s != st.s) { // of a row that may hold NaN: those are never the best
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) key[i] = key[i] >> 16 > Order::kMost ? 0u : key[i];
+        }
+        constexpr bool kSorted = kOwn <= 8; // else taking out the best is less work
+        if constexpr (kSorted) sort_falling(key);
         for (uint32_t k = 0; k < a.top; ++k) {
-            uint32_t best = 0;
+            uint32_t best = key[0];
+            if constexpr (!kSorted) {
 #pragma unroll
-            for (uint32_t i = 0; i < kOwn; ++i) best = max(best, key[i]);
+                for (uint32_t i = 1; i < kOwn; ++i) best = max(best, key[i]);
+            }
             best = group_all<kLanes>(best, greater);
+            if constexpr (kSorted) {
+                if (key[0] == best) {
 #pragma unroll
-            for (uint32_t i = 0; i < kOwn; ++i) key[i] = key[i] == best ? 0u : key[i];
+                    for (uint32_t i = 0; i + 1 < kOwn; ++i) key[i] = key[i + 1];
+                    key[kOwn - 1] = 0u;
+                }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < kOwn; ++i) key[i] = key[i] == best ? 0u : key[i];
+            }
             kept = l == k % kLanes ? best : kept;
             if (k % kLanes == kLanes - 1 || k + 1 == a.top)
-                flush(k, kept ? key_of(logit_order(half_value<T>(kept >> 16)), 0xffffu - (kept & 0xffffu))
-                              : 0);
+                flush(k, kept >> 16 >= Order::kLeast, Order::value(kept >> 16),
+                      0xffffu - (kept & 0xffffu));
         }
     } else {
-        uint32_t o[kOwn];
-        uint64_t kept = 0;
+        uint32_t o[kOwn], kept = 0, kept_label = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kOwn; ++i) o[i] = logit_order(held[i / kN][i % kN]);
         for (uint32_t k = 0; k < a.top; ++k) {
@@ -853,10 +905,13 @@ __global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_
 #pragma unroll
                 for (uint32_t i = 0; i < kOwn; ++i) o[i] = i == at ? 0u : o[i];
             }
-            if (l == k % kLanes) kept = top ? key_of(top, lowest) : 0;
-            if (k % kLanes == kLanes - 1 || k + 1 == a.top) flush(k, kept);
+            kept = l == k % kLanes ? top : kept;
+            kept_label = l == k % kLanes ? lowest : kept_label;
+            if (k % kLanes == kLanes - 1 || k + 1 == a.top)
+                flush(k, kept != 0, order_logit(kept), kept_label);
         }
     }
+    done();
 }
 
 // kLanes lanes a row (256: a block, or a tile of a row per block).
