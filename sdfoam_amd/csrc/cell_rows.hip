@@ -31,6 +31,16 @@ template <typename T, int kP>
 __device__ __forceinline__ void store_piece(T *p, const Piece<T, kP> &c) {
     __builtin_memcpy(p, &c, sizeof(c));
 }
+// Read or written once: past the caches (single elements: as above).
+template <typename T, int kP> __device__ __forceinline__ Piece<T, kP> load_piece_past(const T *p) {
+    if constexpr (sizeof(Piece<T, kP>) == 16) return load_past<Piece<T, kP>, sizeof(T)>(p);
+    else return load_piece<T, kP>(p);
+}
+template <typename T, int kP>
+__device__ __forceinline__ void store_piece_past(T *p, const Piece<T, kP> &c) {
+    if constexpr (sizeof(c) == 16) store_past<sizeof(T)>(p, c);
+    else store_piece<T, kP>(p, c);
+}
 template <int kP> __device__ __forceinline__ uint32_t column(uint32_t piece, uint32_t width) {
     return min(piece * kP, width - kP);
 }
@@ -74,7 +84,8 @@ constexpr uint32_t kMaxWidth = 1u << 18; // of a row: Divisor's range
 
 // One lane per piece of a row, kUnroll of them in flight: bound by the bytes of
 // the rows read and written (the ids come once per row, from L1 after that).
-template <typename T, int kP> __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
+template <typename T, int kP, bool kPast>
+__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     const T *table = static_cast<const T *>(a.table);
     T *out = static_cast<T *>(a.rows);
     const uint64_t r0 = a.first + block_of_xcd(blockIdx.x, gridDim.x) * a.per;
@@ -103,7 +114,9 @@ template <typename T, int kP> __global__ __launch_bounds__(256) void rows_kernel
             Piece<T, kP> o;
 #pragma unroll
             for (int e = 0; e < kP; ++e) o.v[e] = (T)(cell[u] < 0 ? 0.0f : f[u] * (float)p[u].v[e]);
-            store_piece<T, kP>(out + (r0 + row[u]) * a.width + col[u], o);
+            T *to = out + (r0 + row[u]) * a.width + col[u];
+            if constexpr (kPast) store_piece_past<T, kP>(to, o);
+            else store_piece<T, kP>(to, o);
         }
     }
 }
@@ -120,7 +133,8 @@ constexpr uint32_t kScanParts = 16;               // threads that share a digit'
 
 // The table's gradient is cleared by extra blocks of the sort's launches, which
 // leave the memory idle: each launch clears [begin, end) of it, `each` bytes a
-// block in stores of 16.  Few large shares: beside the sort's blocks a CU has
+// block in stores of 16, past the caches (which would otherwise be full of
+// zeros when the sums begin: 120 -> 96 us for 268 MB).  Few large shares: beside the sort's blocks a CU has
 // room (LDS) for one of these at a time.
 struct Clear {
     char *to;
@@ -136,7 +150,7 @@ __device__ __forceinline__ void clear_block(const Clear &c, uint32_t block) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
             const uint64_t at = base + (k * kSortThreads + threadIdx.x) * 16ull;
-            if (at + 16 <= end) __builtin_memcpy(c.to + at, &zero, 16);
+            if (at + 16 <= end) store_past<2>(c.to + at, zero);
             else
                 for (uint64_t b = at; b < end; ++b) c.to[b] = 0;
         }
@@ -448,7 +462,7 @@ __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint3
             if (a.weight && !a.factor) f[b] *= a.weight[index[b]];
             f[b] = live ? f[b] : 0.0f;
             g[b] = {};
-            if (live && mine) g[b] = load_piece<T, kP>(grad + (uint64_t)index[b] * a.stride + col);
+            if (live && mine) g[b] = load_piece_past<T, kP>(grad + (uint64_t)index[b] * a.stride + col);
             if (a.weight_grad) {
                 t[b] = {};
                 if (live && mine)
@@ -723,6 +737,10 @@ int sdf_cell_rows(int type, const void *table, uint64_t table_stride, uint64_t n
     const uint32_t pieces = pieces_of(type, width);
     RowsArgs a = {table, table_stride, (uint32_t)num_cells, width, divisor(pieces), cells, id_type,
                   0, count, 1, weight, scale, rows};
+    // Rows that no cache would keep for their reader are written past them
+    // (1.92M rows of 49 floats, 376 MB: 135 -> 98 us; 1M of 64 bfloat16, 134 MB:
+    // 51 -> 44; 16,384 of 2,048 halves, 67 MB: 23.9 and 24.4).
+    const bool past = count * width * type_bytes(type) >= 128ull << 20;
     // 1,024 pieces a block, or 256 where that leaves CUs without one
     const uint64_t items = count * pieces < 1024 * 1024 ? 256 : 1024;
     a.per = (uint32_t)(items / pieces > 0 ? items / pieces : 1);
@@ -730,9 +748,12 @@ int sdf_cell_rows(int type, const void *table, uint64_t table_stride, uint64_t n
         for (uint64_t r = 0; r < count; r += kWindow * a.per) {
             a.first = r;
             a.count = count - r < kWindow * a.per ? count - r : kWindow * a.per;
-            hipLaunchKernelGGL((rows_kernel<decltype(t), decltype(p)::v>),
-                               dim3((unsigned)((a.count + a.per - 1) / a.per)), dim3(256), 0,
-                               static_cast<hipStream_t>(stream), a);
+            const dim3 grid((unsigned)((a.count + a.per - 1) / a.per));
+            hipStream_t s = static_cast<hipStream_t>(stream);
+            using T = decltype(t);
+            constexpr int kP = decltype(p)::v;
+            if (past) hipLaunchKernelGGL((rows_kernel<T, kP, true>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((rows_kernel<T, kP, false>), grid, dim3(256), 0, s, a);
         }
     });
     const hipError_t e = hipGetLastError();

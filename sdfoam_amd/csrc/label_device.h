@@ -76,19 +76,34 @@ template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T *p)
     __builtin_memcpy(&c, p, 16);
     return c;
 }
-// kPast: past the caches
-template <bool kPast = false, typename T>
-__device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
-    if constexpr (kPast) {
-        typedef uint32_t Words2 __attribute__((ext_vector_type(4), aligned(2)));
-        typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
-        const Words4 w = {c.w[0], c.w[1], c.w[2], c.w[3]};
-        if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(w, reinterpret_cast<Words2 *>(p));
-        else __builtin_nontemporal_store(w, reinterpret_cast<Words4 *>(p));
-    } else {
-        __builtin_memcpy(p, &c, 16);
-    }
+template <typename T> __device__ __forceinline__ void store_chunk(T *p, const Chunk<T> &c) {
+    __builtin_memcpy(p, &c, 16);
 }
+
+// 16 bytes that are read or written once, past the caches, at the alignment of
+// an element of kElement bytes.
+template <int kElement> struct Past;
+template <> struct Past<2> {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct Past<4> {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <int kElement, typename V> __device__ __forceinline__ void store_past(void *p, const V &v) {
+    static_assert(sizeof(V) == 16, "16 bytes");
+    typename Past<kElement>::Words w;
+    __builtin_memcpy(&w, &v, 16);
+    __builtin_nontemporal_store(w, static_cast<typename Past<kElement>::Words *>(p));
+}
+template <typename V, int kElement> __device__ __forceinline__ V load_past(const void *p) {
+    static_assert(sizeof(V) == 16, "16 bytes");
+    const auto w =
+        __builtin_nontemporal_load(static_cast<const typename Past<kElement>::Words *>(p));
+    V v;
+    __builtin_memcpy(&v, &w, 16);
+    return v;
+}
+
 // Elements [begin, end) of a row, cut into chunks at 16-byte boundaries: chunk
 // `at` (begin, begin + kN, ...) has the elements [at, at + kN) moved down by
 // `skew`, as far as they lie in the range.  (Rows of an odd number of 16-bit
@@ -160,8 +175,10 @@ template <typename T> struct Span {
     // the chunk's own elements into another row
     template <bool kPast = false>
     __device__ __forceinline__ void store_own(T *to, uint32_t at, const Chunk<T> &c) const {
-        if (plain(at)) store_chunk<kPast>(to + place(at), c);
-        else each_own(at, [&](uint32_t e, uint32_t i) { to[i] = c.value(e); });
+        if (plain(at)) {
+            if constexpr (kPast) store_past<sizeof(T)>(to + place(at), c);
+            else store_chunk(to + place(at), c);
+        } else each_own(at, [&](uint32_t e, uint32_t i) { to[i] = c.value(e); });
     }
 };
 
