@@ -104,6 +104,16 @@ template <typename V, int kElement> __device__ __forceinline__ V load_past(const
     return v;
 }
 
+template <bool kOnce, typename T> __device__ __forceinline__ Chunk<T> load_chunk_if(const T *p) {
+    if constexpr (kOnce) return load_past<Chunk<T>, sizeof(T)>(p);
+    else return load_chunk(p);
+}
+template <bool kPast, typename T>
+__device__ __forceinline__ void store_chunk_if(T *p, const Chunk<T> &c) {
+    if constexpr (kPast) store_past<sizeof(T)>(p, c);
+    else store_chunk(p, c);
+}
+
 // Elements [begin, end) of a row, cut into chunks at 16-byte boundaries: chunk
 // `at` (begin, begin + kN, ...) has the elements [at, at + kN) moved down by
 // `skew`, as far as they lie in the range.  (Rows of an odd number of 16-bit
@@ -146,8 +156,10 @@ template <typename T> struct Span {
     __device__ __forceinline__ bool plain_step(uint32_t first, uint32_t elements) const {
         return first + elements - skew <= end && (first != begin || skew == 0) && whole;
     }
-    __device__ __forceinline__ Chunk<T> load(uint32_t at, T fill) const { // unmasked
-        if (whole) return load_chunk(row + place(at));
+    // unmasked; kOnce: past the caches
+    template <bool kOnce = false>
+    __device__ __forceinline__ Chunk<T> load(uint32_t at, T fill) const {
+        if (whole) return load_chunk_if<kOnce>(row + place(at));
         Chunk<T> c = {};
 #pragma unroll
         for (uint32_t e = 0; e < kN; ++e) c.set(e, at + e < end ? row[at + e] : fill);
@@ -175,10 +187,8 @@ template <typename T> struct Span {
     // the chunk's own elements into another row
     template <bool kPast = false>
     __device__ __forceinline__ void store_own(T *to, uint32_t at, const Chunk<T> &c) const {
-        if (plain(at)) {
-            if constexpr (kPast) store_past<sizeof(T)>(to + place(at), c);
-            else store_chunk(to + place(at), c);
-        } else each_own(at, [&](uint32_t e, uint32_t i) { to[i] = c.value(e); });
+        if (plain(at)) store_chunk_if<kPast>(to + place(at), c);
+        else each_own(at, [&](uint32_t e, uint32_t i) { to[i] = c.value(e); });
     }
 };
 

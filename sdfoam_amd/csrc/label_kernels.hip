@@ -100,8 +100,9 @@ template <bool kEntropy> __device__ __forceinline__ Part merge_block(Part p, Par
 // f(chunks, at) over a span, kU chunks of each of kThreads threads at a time,
 // chunk i at `at` + i kThreads kN, and one by one where the span's end leaves
 // fewer; what is not a chunk's own is -inf where kMask, else as it was read.
-// Only the steps that begin in [first, last).
-template <int kThreads, int kU, bool kMask, typename T, typename F>
+// kOnce: past the caches, for what is not read again (8,192 rows of 65,536: 190
+// -> 164 us, 6.6 TB/s).  Only the steps that begin in [first, last).
+template <int kThreads, int kU, bool kMask, bool kOnce, typename T, typename F>
 __device__ __forceinline__ void for_steps(const Span<T> &z, uint32_t first, uint32_t last, F f) {
     constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
     uint32_t at = first + threadIdx.x % kThreads * Chunk<T>::kN;
@@ -110,10 +111,11 @@ __device__ __forceinline__ void for_steps(const Span<T> &z, uint32_t first, uint
         if (z.plain_step(first, kStep * kU)) {
             const T *p = z.row + (at - z.skew);
 #pragma unroll
-            for (int i = 0; i < kU; ++i) ch[i] = load_chunk(p + i * kStep);
+            for (int i = 0; i < kU; ++i) ch[i] = load_chunk_if<kOnce>(p + i * kStep);
         } else {
 #pragma unroll
-            for (int i = 0; i < kU; ++i) ch[i] = z.load(at + i * kStep, (T)-INFINITY);
+            for (int i = 0; i < kU; ++i)
+                ch[i] = z.template load<kOnce>(at + i * kStep, (T)-INFINITY);
             if (kMask) {
 #pragma unroll
                 for (int i = 0; i < kU; ++i) z.mask(ch[i], at + i * kStep, (T)-INFINITY);
@@ -123,27 +125,27 @@ __device__ __forceinline__ void for_steps(const Span<T> &z, uint32_t first, uint
     }
     if (first >= last) return;
     for (; at < z.last(); at += kStep) {
-        Chunk<T> ch[1] = {z.load(at, (T)-INFINITY)};
+        Chunk<T> ch[1] = {z.template load<kOnce>(at, (T)-INFINITY)};
         if (kMask) z.mask(ch[0], at, (T)-INFINITY);
         f(ch, at);
     }
 }
-template <int kThreads, int kU, bool kMask, typename T, typename F>
+template <int kThreads, int kU, bool kMask, bool kOnce, typename T, typename F>
 __device__ __forceinline__ void for_chunks(const Span<T> &z, F f) {
-    for_steps<kThreads, kU, kMask>(z, z.begin, z.last(), f);
+    for_steps<kThreads, kU, kMask, kOnce>(z, z.begin, z.last(), f);
 }
-// to[i] = f(z[i]) over a span, chunk by chunk
-template <int kThreads, int kU, typename T, typename F>
+// to[i] = f(z[i]) over a span, chunk by chunk, z read for the last time
+template <int kThreads, int kU, bool kPast, typename T, typename F>
 __device__ __forceinline__ void map_chunks(const Span<T> &z, T *to, F f) {
     constexpr uint32_t kStep = kThreads * Chunk<T>::kN;
-    for_chunks<kThreads, kU, false>(z, [&](const auto &ch, uint32_t at) {
+    for_chunks<kThreads, kU, false, true>(z, [&](const auto &ch, uint32_t at) {
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(ch) / 16); ++i)
             if (at + i * kStep < z.last()) {
                 const uint32_t from = z.place(at + i * kStep);
                 const Chunk<T> o = f(ch[i], from);
                 // two threads may write one element, and then the same value
-                if (z.whole) store_chunk(to + from, o);
+                if (z.whole) store_chunk_if<kPast>(to + from, o);
                 else z.store_own(to, from, o);
             }
     });
@@ -154,7 +156,7 @@ constexpr int kUnroll = 4;   // chunks in flight per thread
 
 template <bool kEntropy, int kThreads, typename T>
 __device__ __forceinline__ void stream_part(Part &p, const Span<T> &z, float c) {
-    for_chunks<kThreads, kUnroll, true>(
+    for_chunks<kThreads, kUnroll, true, false>(
         z, [&](const auto &ch, uint32_t) { absorb<kEntropy, kUnroll>(p, ch, c); });
 }
 
@@ -281,18 +283,19 @@ __device__ __forceinline__ Chunk<T> grad_chunk(const Chunk<T> &ch, float m, floa
         o.set(e, (T)(share * __builtin_amdgcn_exp2f((ch[e] - m) * c)));
     return o;
 }
-template <int kThreads, typename T>
+template <int kThreads, bool kPast, typename T>
 __device__ __forceinline__ void write_zeros(T *dz, uint32_t begin, uint32_t end) {
     const Span<T> z(dz, begin, end);
     for (uint32_t at = begin + threadIdx.x * z.kN; at < z.last(); at += kThreads * z.kN)
-        z.store_own(dz, at, {});
+        z.template store_own<kPast>(dz, at, {});
 }
 
 // A block per row.  With kHeld > 0 (the gradient is wanted): the row's first
 // kThreads * kHeld chunks stay in registers between the statistics and the
 // gradient, so they are read once; the rest is read again.  kHeld = 0: loss and
-// statistics alone, streamed.
-template <typename T, int kThreads, int kHeld>
+// statistics alone, streamed.  kPast: the gradient is written past the caches,
+// or, with kHeld = 0, no backward will read the logits again.
+template <typename T, int kThreads, int kHeld, bool kPast>
 __global__ __launch_bounds__(kThreads)
     __attribute__((amdgpu_waves_per_eu(kHeld > 8 ? 4 : kHeld > 4 ? 6 : 7))) void
     distill_kernel(DistillArgs a) {
@@ -304,10 +307,6 @@ __global__ __launch_bounds__(kThreads)
     const Span<T> z(static_cast<const T *>(a.logits) + r * a.stride, 0u, a.labels);
     T *dz = static_cast<T *>(a.logits_grad) + r * a.labels;
     constexpr uint32_t kRest = kThreads * kN * kHeld;
-    // past the caches: what is written would push out what is read again
-    // (2,048 rows of 262,144: 553 -> 479 us; 16,384 of 32,768, held whole, 457
-    // -> 479)
-    constexpr bool kPast = kHeld > 8;
     const float u = row_weight(a, r);
     Teacher t = {0.0f, 0.0f};
     Part st = {0.0f, 0.0f, 0.0f};
@@ -318,7 +317,7 @@ __global__ __launch_bounds__(kThreads)
         if (threadIdx.x < a.top) logit = entry(a, r, threadIdx.x, j);
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
-            held[i] = z.load((threadIdx.x + i * kThreads) * kN, (T)-INFINITY);
+            held[i] = z.template load<true>((threadIdx.x + i * kThreads) * kN, (T)-INFINITY);
         if (threadIdx.x < a.top) put_entry(e, threadIdx.x, j, logit, z.row);
         load_entries(a, r, z.row, e, threadIdx.x + kThreads, kThreads);
         __syncthreads();
@@ -333,7 +332,7 @@ __global__ __launch_bounds__(kThreads)
                 }
                 absorb<false, 2>(p, held, a.c);
             }
-            for_steps<kThreads, kUnroll, true>(
+            for_steps<kThreads, kUnroll, true, kHeld == 0 && kPast>(
                 z, kRest, z.last(),
                 [&](const auto &ch, uint32_t) { absorb<false, kUnroll>(p, ch, a.c); });
             st = merge_block<false>(p, parts, a.c);
@@ -348,11 +347,11 @@ __global__ __launch_bounds__(kThreads)
     }
     if constexpr (kHeld > 0) {
         if (!live) {
-            write_zeros<kThreads>(dz, 0, a.labels);
+            write_zeros<kThreads, kPast>(dz, 0, a.labels);
             return;
         }
         const float coef = row_coef(a, r, u), share = coef / st.s;
-        for_steps<kThreads, kUnroll, true>(z, kRest, z.last(), [&](const auto &ch, uint32_t at) {
+        for_steps<kThreads, kUnroll, true, true>(z, kRest, z.last(), [&](const auto &ch, uint32_t at) {
 #pragma unroll
             for (int i = 0; i < (int)(sizeof(ch) / 16); ++i)
                 z.template store_own<kPast>(dz, at + i * kThreads * kN,
@@ -387,7 +386,7 @@ __global__ __launch_bounds__(kStream) void part_kernel(DistillArgs a, uint32_t s
 
 // The loss, and the gradient of a slice of a row per block, from the row's
 // statistics: `parts` of its slices, or a.stats where `parts` is NULL.
-template <typename T>
+template <typename T, bool kPast>
 __global__ __launch_bounds__(kStream) void finish_kernel(DistillArgs a, uint32_t tiles,
                                                          uint32_t tile, const Part *parts,
                                                          uint32_t slices) {
@@ -425,11 +424,11 @@ __global__ __launch_bounds__(kStream) void finish_kernel(DistillArgs a, uint32_t
     }
     if (!a.logits_grad) return;
     if (!live) {
-        write_zeros<kStream>(dz, begin, end);
+        write_zeros<kStream, kPast>(dz, begin, end);
         return;
     }
     const float coef = row_coef(a, r, u), share = coef / st.s;
-    map_chunks<kStream, kUnroll>(Span<T>(z, begin, end), dz, [&](const Chunk<T> &ch, uint32_t) {
+    map_chunks<kStream, kUnroll, kPast>(Span<T>(z, begin, end), dz, [&](const Chunk<T> &ch, uint32_t) {
         return grad_chunk(ch, st.m, a.c, share);
     });
     __syncthreads();
@@ -633,8 +632,10 @@ __device__ __forceinline__ void write_best(const AnswerArgs &a, uint64_t r, uint
 // threads whose largest logit reaches the bound (about `top`) look at theirs
 // again, and only at the one or two steps that hold it where no third does;
 // what reaches it is ranked by counting.
-// slices > 1: Part and keys of each slice, for join_kernel.
-template <typename T>
+// slices > 1: Part and keys of each slice, for join_kernel.  kOnce: no backward
+// will read the logits again (2,048 rows of 50,021 floats with their gradient:
+// 221 us past the caches, 207 through them).
+template <typename T, bool kOnce>
 __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t slices,
                                                          uint32_t slice, Part *out,
                                                          uint64_t *out_keys) {
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
     Part mine = {-INFINITY, 0.0f, 0.0f};
     float second = -INFINITY, third = -INFINITY;
     uint32_t where = begin, where_second = begin;
-    for_chunks<kStream, kUnroll, true>(span, [&](const auto &ch, uint32_t at) {
+    for_chunks<kStream, kUnroll, true, kOnce>(span, [&](const auto &ch, uint32_t at) {
         const float first = mine.m, m = absorb<true, kUnroll>(mine, ch, c);
         const bool leads = m > first, follows = m > second;
         third = fmaxf(third, fminf(m, second));
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
             for (uint32_t k = 0; k < steps; ++k) {
                 const uint32_t at = k ? where_second : where, first = at - own;
                 if (first + kStep * kUnroll <= span.last()) {
-                    for_steps<kStream, kUnroll, true>(span, first, first + 1, collect);
+                    for_steps<kStream, kUnroll, true, false>(span, first, first + 1, collect);
                 } else {
                     Chunk<T> ch[1] = {span.load(at, (T)-INFINITY)};
                     span.mask(ch[0], at, (T)-INFINITY);
@@ -713,7 +714,7 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
                 }
             }
         } else {
-            for_chunks<kStream, kUnroll, true>(span, collect);
+            for_chunks<kStream, kUnroll, true, false>(span, collect);
         }
     }
     __syncthreads();
@@ -732,7 +733,7 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top; ++k) {
         uint64_t key = 0;
-        for_chunks<kStream, 1, true>(span, [&](const Chunk<T>(&ch)[1], uint32_t at) {
+        for_chunks<kStream, 1, true, false>(span, [&](const Chunk<T>(&ch)[1], uint32_t at) {
 #pragma unroll
             for (uint32_t e = 0; e < (uint32_t)Chunk<T>::kN; ++e) {
                 const uint32_t o = logit_order(ch[0][e]);
@@ -915,7 +916,7 @@ __global__ __launch_bounds__(256) void answer_short_kernel(AnswerArgs a, uint64_
 }
 
 // kLanes lanes a row (256: a block, or a tile of a row per block).
-template <typename T, int kLanes>
+template <typename T, int kLanes, bool kPast>
 __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, uint64_t rows,
                                                           uint32_t tiles, uint32_t tile) {
     const uint64_t r = kLanes == 256 ? blockIdx.x / tiles
@@ -934,7 +935,7 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, uint64_t
     // -p (glp + gh (log p + H)) = -e / S (gh ln2 d + glp + gh (H - log S))
     const float slope = gh / kLog2e, level = glp + gh * (a.entropy[r] - logf(st.y));
     const float inv_s = live ? -1.0f / st.y : 0.0f;
-    map_chunks<kLanes, kUnroll>(Span<T>(z, begin, end), dz, [&](const Chunk<T> &ch, uint32_t at) {
+    map_chunks<kLanes, kUnroll, kPast>(Span<T>(z, begin, end), dz, [&](const Chunk<T> &ch, uint32_t at) {
         Chunk<T> o = {};
 #pragma unroll
         for (int e = 0; e < Chunk<T>::kN; ++e) {
@@ -1007,6 +1008,12 @@ template <typename T> uint64_t chunks_of(const void *logits, uint64_t stride, ui
                          stride * sizeof(T) % 16 == 0;
     return (labels + (aligned ? 0 : Chunk<T>::kN - 1) + Chunk<T>::kN - 1) / Chunk<T>::kN;
 }
+// Gradients that no cache would keep for their reader are written past them
+// (1 GB, 2,048 rows of 262,144 bfloat16: 553 -> 475 us, 16,384 of 32,768: 454 ->
+// 412; 256 MiB, 4,096 of 32,768, a third of the rows masked: 97 -> 104).
+template <typename T> bool past_caches(uint64_t rows, uint64_t labels) {
+    return rows * labels * sizeof(T) > 256ull << 20;
+}
 // f(lanes, chunks held by each) of a short row, as types
 template <int kV> struct Int {
     static constexpr int v = kV;
@@ -1042,9 +1049,9 @@ void launch_finish(const DistillArgs &a, uint64_t rows, const Part *parts, uint3
     // where rows are few, as many blocks as the statistics had
     const uint32_t tile = slices > 1 ? ((a.labels + slices - 1) / slices + 7) / 8 * 8 : kTile;
     const uint32_t tiles = a.logits_grad ? (a.labels + tile - 1) / tile : 1;
-    hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(rows * tiles)), dim3(kStream),
-                       kEntryBytes * a.top, s, a,
-                       tiles, a.logits_grad ? tile : a.labels, parts, slices);
+    const auto kernel = past_caches<T>(rows, a.labels) ? finish_kernel<T, true> : finish_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * tiles)), dim3(kStream), kEntryBytes * a.top, s,
+                       a, tiles, a.logits_grad ? tile : a.labels, parts, slices);
 }
 
 template <typename T>
@@ -1057,17 +1064,25 @@ void launch_distill(const DistillArgs &a, uint64_t rows, Part *parts, hipStream_
                            a, sl.count, sl.length, parts);
         return launch_finish<T>(a, rows, parts, sl.count, s);
     }
-    const auto launch = [&](auto threads, auto held) {
-        hipLaunchKernelGGL((distill_kernel<T, decltype(threads)::v, decltype(held)::v>),
-                           dim3((unsigned)rows), dim3(decltype(threads)::v), kEntryBytes * a.top, s,
-                           a);
+    const auto launch = [&](auto threads, auto held, auto past) {
+        constexpr int kThreads = decltype(threads)::v;
+        hipLaunchKernelGGL((distill_kernel<T, kThreads, decltype(held)::v, decltype(past)::v != 0>),
+                           dim3((unsigned)rows), dim3(kThreads), kEntryBytes * a.top, s, a);
     };
-    if (!a.logits_grad) return launch(Int<kStream>(), Int<0>());
-    if (chunks <= 256 * 4) launch(Int<256>(), Int<4>());
-    else if (chunks <= 512 * 4) launch(Int<512>(), Int<4>());
-    else if (chunks <= 512 * 9) launch(Int<512>(), Int<8>());
-    else if (chunks <= 512 * 13) launch(Int<512>(), Int<12>());
-    else launch(Int<512>(), Int<16>());
+    if (!a.logits_grad) {
+        if (a.stats) return launch(Int<kStream>(), Int<0>(), Int<0>());
+        return launch(Int<kStream>(), Int<0>(), Int<1>());
+    }
+    // The fewest held chunks that leave little to read again.
+    const auto launch_held = [&](auto past) {
+        if (chunks <= 256 * 4) launch(Int<256>(), Int<4>(), past);
+        else if (chunks <= 512 * 4) launch(Int<512>(), Int<4>(), past);
+        else if (chunks <= 512 * 9) launch(Int<512>(), Int<8>(), past);
+        else if (chunks <= 512 * 13) launch(Int<512>(), Int<12>(), past);
+        else launch(Int<512>(), Int<16>(), past);
+    };
+    if (past_caches<T>(rows, a.labels)) launch_held(Int<1>());
+    else launch_held(Int<0>());
 }
 
 template <typename T>
@@ -1085,8 +1100,9 @@ void launch_answer(const AnswerArgs &a, uint64_t rows, const Slices &sl, void *s
     }
     uint64_t *keys = static_cast<uint64_t *>(scratch);
     Part *parts = reinterpret_cast<Part *>(keys + rows * sl.count * a.top);
-    hipLaunchKernelGGL(answer_kernel<T>, dim3((unsigned)(rows * sl.count)), dim3(kStream), 0, s, a,
-                       sl.count, sl.length, parts, keys);
+    const auto kernel = a.stats ? answer_kernel<T, false> : answer_kernel<T, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * sl.count)), dim3(kStream), 0, s, a, sl.count,
+                       sl.length, parts, keys);
     if (sl.count > 1)
         hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)rows), dim3(kStream), 0, s, a, sl.count,
                            parts, keys);
@@ -1098,9 +1114,10 @@ template <typename T> void launch_answer_grad(const AnswerArgs &a, uint64_t rows
         constexpr uint32_t kLanes = decltype(lanes)::v;
         const uint32_t tile = kLanes == 256 ? 256 * Chunk<T>::kN * kUnroll : a.labels;
         const uint32_t tiles = (a.labels + tile - 1) / tile;
-        hipLaunchKernelGGL((answer_grad_kernel<T, kLanes>),
-                           dim3((unsigned)((rows * tiles * kLanes + 255) / 256)), dim3(256), 0, s,
-                           a, rows, tiles, tile);
+        const auto kernel = past_caches<T>(rows, a.labels) ? answer_grad_kernel<T, kLanes, true>
+                                                           : answer_grad_kernel<T, kLanes, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows * tiles * kLanes + 255) / 256)), dim3(256),
+                           0, s, a, rows, tiles, tile);
     };
     if (chunks <= 8 * kUnroll) launch(Int<8>());
     else if (chunks <= 64 * kUnroll) launch(Int<64>());
