@@ -70,12 +70,12 @@ def _check_float32(name: str, t: torch.Tensor, shape) -> None:
 
 def _check_devices(first: str, t: torch.Tensor, *others) -> None:
     """others: name, tensor or None, name, ..."""
-    device = t.device
-    if device.type != "cuda":
+    device = t.get_device()
+    if device < 0:
         raise RuntimeError(f"{first} must be on CUDA device")
     for k in range(1, len(others), 2):
         o = others[k]
-        if o is not None and o.device != device:
+        if o is not None and o.get_device() != device:
             raise RuntimeError(f"{others[k - 1]} must be on the device of {first}")
 
 
@@ -93,24 +93,32 @@ def _wants_gradient(*tensors) -> bool:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., D] as [R, D] whose rows are contiguous, without a copy where the layout
     allows it."""
-    d = t.size(-1)
+    shape = t.shape
+    d = shape[-1]
     if d > 1 and t.stride(-1) != 1:
         t = t.contiguous()
-    if t.dim() == 2:
+    if len(shape) == 2:
         return t
     rows = 1
-    for k in t.shape[:-1]:
+    for k in shape[:-1]:
         rows *= k
     return t.reshape(rows, d)
 
 
-def _call(function, device: torch.device, *args) -> None:
-    """The library call on the device's current stream."""
-    index = device.index
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type, not written."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _call(function, t: torch.Tensor, *args) -> None:
+    """The library call on the current stream of t's device."""
+    index = t.get_device()
     if index == torch.cuda.current_device():
         status = function(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = function(*args, _raw_stream(index))
     if status:
         check(status)
@@ -144,7 +152,7 @@ def _rows_forward(table, cells, weight, scale) -> torch.Tensor:
     t = _rows(table)
     c = cells.contiguous()
     w = None if weight is None else weight.contiguous()
-    _call(_lib.lib().sdf_cell_rows, device, _TYPES[table.dtype], t.data_ptr(), t.stride(0),
+    _call(_lib.lib().sdf_cell_rows, t, _TYPES[table.dtype], t.data_ptr(), t.stride(0),
           num_cells, width, _ID_TYPES[cells.dtype], c.data_ptr(), c.numel(), ptr(w), scale,
           rows.data_ptr())
     return rows
@@ -166,7 +174,7 @@ def _rows_backward(rows_grad, cells, num_cells, weight, scale, table, need_table
     L = _lib.lib()
     nbytes = int(L.sdf_cell_rows_backward_scratch_bytes(num_cells, width, c.numel()))
     keep, base = _scratch(nbytes, dev)
-    _call(L.sdf_cell_rows_backward, dev, _TYPES[rows_grad.dtype], ptr(g), g.stride(0), ptr(t),
+    _call(L.sdf_cell_rows_backward, g, _TYPES[rows_grad.dtype], ptr(g), g.stride(0), ptr(t),
           0 if t is None else t.stride(0), num_cells, width, _ID_TYPES[cells.dtype], ptr(c),
           c.numel(), ptr(w), scale, ptr(table_grad), ptr(weight_grad), base, nbytes)
     return table_grad, weight_grad
@@ -236,9 +244,9 @@ def cell_rows_backward(rows_grad: torch.Tensor, cells: torch.Tensor, num_cells: 
 
 
 def _check_logits(logits, temperature) -> float:
+    _element_type("logits", logits)
     if logits.dim() < 1:
         raise RuntimeError("logits must have at least 1 dimension")
-    _element_type("logits", logits)
     if logits.size(-1) == 0:
         raise RuntimeError("logits must have at least one label")
     temperature = float(temperature)
@@ -251,14 +259,15 @@ def _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weig
     temperature = _check_logits(logits, temperature)
     _id_type("teacher_labels", teacher_labels)
     _element_type("teacher_logits", teacher_logits)
-    if teacher_labels.dim() != logits.dim() or teacher_labels.shape[:-1] != logits.shape[:-1]:
-        raise RuntimeError(f"teacher_labels had shape {list(teacher_labels.shape)}, expected "
-                           f"{list(logits.shape[:-1])} and a last dimension")
-    _check_shape("teacher_logits", teacher_logits, teacher_labels.shape)
-    if teacher_labels.size(-1) > MAX_TEACHER:
+    shape, lead = teacher_labels.shape, logits.shape[:-1]
+    if shape[:-1] != lead or not shape:
+        raise RuntimeError(f"teacher_labels had shape {list(shape)}, expected {list(lead)} "
+                           "and a last dimension")
+    _check_shape("teacher_logits", teacher_logits, shape)
+    if shape[-1] > MAX_TEACHER:
         raise RuntimeError(f"at most {MAX_TEACHER} teacher logits per row")
     if row_weight is not None:
-        _check_float32("row_weight", row_weight, logits.shape[:-1])
+        _check_float32("row_weight", row_weight, lead)
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be 'none', 'sum' or 'mean'")
     _check_devices("logits", logits, "teacher_labels", teacher_labels, "teacher_logits",
@@ -266,41 +275,40 @@ def _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weig
     return temperature
 
 
-class _Distill:
-    """The arguments that both directions share, laid out for the library."""
+def _distill_args(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction):
+    """The arguments that both directions share, laid out for the library: first what has
+    to stay alive until the call is queued."""
+    z, ids, t = _rows(logits), teacher_labels.contiguous(), teacher_logits.contiguous()
+    w = None if row_weight is None else row_weight.contiguous()
+    rows, labels = z.shape
+    return (z, ids, t, w), (
+        _TYPES[z.dtype], z.data_ptr(), rows, labels, z.stride(0), _ID_TYPES[ids.dtype],
+        ids.data_ptr(), _TYPES[t.dtype], t.data_ptr(), ids.size(-1), temperature, ptr(w),
+        _REDUCTIONS[reduction])
 
-    def __init__(self, logits, teacher_labels, teacher_logits, temperature, row_weight, reduction):
-        self.z = _rows(logits)
-        self.ids = teacher_labels.contiguous()
-        self.t = teacher_logits.contiguous()
-        self.weight = None if row_weight is None else row_weight.contiguous()
-        self.temperature, self.reduction = temperature, reduction
 
-    def args(self):
-        z, ids, t = self.z, self.ids, self.t
-        rows, labels = z.shape
-        return (_TYPES[z.dtype], z.data_ptr(), rows, labels, z.stride(0), _ID_TYPES[ids.dtype],
-                ids.data_ptr(), _TYPES[t.dtype], t.data_ptr(), ids.size(-1), self.temperature,
-                ptr(self.weight), _REDUCTIONS[self.reduction])
-
-    def forward(self, shape, loss_grad=None, stats=None, logits_grad=None) -> torch.Tensor:
-        dev = self.z.device
-        none = self.reduction == "none"
-        loss = torch.empty(shape if none else (), dtype=torch.float32, device=dev)
-        L = _lib.lib()
-        nbytes = L.sdf_distill_scratch_bytes(*self.z.shape, _REDUCTIONS[self.reduction])
-        keep, base = _scratch(nbytes, dev)
-        _call(L.sdf_distill, dev, *self.args(), ptr(loss_grad), loss.data_ptr(), ptr(stats),
-              ptr(logits_grad), base, nbytes)
-        return loss
+def _distill_forward(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction,
+                     loss_grad=None, stats=None, logits_grad=None) -> torch.Tensor:
+    keep, args = _distill_args(logits, teacher_labels, teacher_logits, temperature, row_weight,
+                               reduction)
+    dev = logits.device
+    loss = torch.empty(logits.shape[:-1] if reduction == "none" else (), dtype=torch.float32,
+                       device=dev)
+    L = _lib.lib()
+    nbytes = L.sdf_distill_scratch_bytes(args[2], args[3], args[12])
+    scratch, base = _scratch(nbytes, dev)
+    _call(L.sdf_distill, logits, *args, ptr(loss_grad), loss.data_ptr(), ptr(stats),
+          ptr(logits_grad), base, nbytes)
+    return loss
 
 
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_labels, teacher_logits, temperature, row_weight, reduction):
-        a = _Distill(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction)
-        stats = torch.empty((a.z.size(0), 2), dtype=torch.float32, device=logits.device)
-        loss = a.forward(logits.shape[:-1], stats=stats)
+        rows = logits.numel() // logits.size(-1)
+        stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
+        loss = _distill_forward(logits, teacher_labels, teacher_logits, temperature, row_weight,
+                                reduction, stats=stats)
         ctx.save_for_backward(logits, teacher_labels, teacher_logits, row_weight, stats)
         ctx.temperature, ctx.reduction = temperature, reduction
         return loss
@@ -309,11 +317,11 @@ class _DistillLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, loss_grad):
         logits, teacher_labels, teacher_logits, row_weight, stats = ctx.saved_tensors
-        a = _Distill(logits, teacher_labels, teacher_logits, ctx.temperature, row_weight,
-                     ctx.reduction)
+        keep, args = _distill_args(logits, teacher_labels, teacher_logits, ctx.temperature,
+                                   row_weight, ctx.reduction)
         g = loss_grad.contiguous()
-        logits_grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _call(_lib.lib().sdf_distill_backward, logits.device, *a.args(), ptr(g), ptr(stats),
+        logits_grad = _like(logits)
+        _call(_lib.lib().sdf_distill_backward, logits, *args, ptr(g), ptr(stats),
               ptr(logits_grad))
         return logits_grad, None, None, None, None, None
 
@@ -338,8 +346,8 @@ def distill_loss(logits: torch.Tensor, teacher_labels: torch.Tensor,
     if _wants_gradient(logits):
         return _DistillLoss.apply(logits, teacher_labels, teacher_logits, temperature, row_weight,
                                   reduction)
-    a = _Distill(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction)
-    return a.forward(logits.shape[:-1])
+    return _distill_forward(logits, teacher_labels, teacher_logits, temperature, row_weight,
+                            reduction)
 
 
 def distill_loss_and_grad(logits: torch.Tensor, teacher_labels: torch.Tensor,
@@ -357,9 +365,9 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_labels: torch.Tensor,
         _check_float32("loss_grad", loss_grad, logits.shape[:-1] if reduction == "none" else ())
         _check_devices("logits", logits, "loss_grad", loss_grad)
         loss_grad = loss_grad.contiguous()
-    a = _Distill(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction)
-    logits_grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    return a.forward(logits.shape[:-1], loss_grad, None, logits_grad), logits_grad
+    logits_grad = _like(logits)
+    return _distill_forward(logits, teacher_labels, teacher_logits, temperature, row_weight,
+                            reduction, loss_grad, None, logits_grad), logits_grad
 
 
 # ---- answers ---------------------------------------------------------------------------------
@@ -381,7 +389,7 @@ def _answer(logits, labels, top, temperature, stats=None):
     dev, shape = logits.device, labels.shape
     rows, count = z.shape
     log_prob = torch.empty(shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(log_prob)
     best = best_labels = None
     if top:
         best = torch.empty((*shape, top), dtype=torch.float32, device=dev)
@@ -389,7 +397,7 @@ def _answer(logits, labels, top, temperature, stats=None):
     L = _lib.lib()
     nbytes = L.sdf_label_log_probs_scratch_bytes(rows, count, top)
     keep, base = _scratch(nbytes, dev)
-    _call(L.sdf_label_log_probs, dev, _TYPES[z.dtype], z.data_ptr(), rows, count, z.stride(0),
+    _call(L.sdf_label_log_probs, z, _TYPES[z.dtype], z.data_ptr(), rows, count, z.stride(0),
           _ID_TYPES[y.dtype], y.data_ptr(), top, temperature, log_prob.data_ptr(),
           entropy.data_ptr(), ptr(best), ptr(best_labels), ptr(stats), base, nbytes)
     return log_prob, entropy, best, best_labels
@@ -418,8 +426,8 @@ class _LabelLogProbs(torch.autograd.Function):
         y = labels.contiguous()
         g = None if log_prob_grad is None else log_prob_grad.contiguous()
         h = None if entropy_grad is None else entropy_grad.contiguous()
-        logits_grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _call(_lib.lib().sdf_label_log_probs_backward, logits.device, _TYPES[z.dtype], ptr(z),
+        logits_grad = _like(logits)
+        _call(_lib.lib().sdf_label_log_probs_backward, logits, _TYPES[z.dtype], ptr(z),
               z.size(0), z.size(1), z.stride(0), _ID_TYPES[y.dtype], ptr(y), ctx.temperature,
               ptr(entropy), ptr(stats), ptr(g), ptr(h), ptr(logits_grad))
         return logits_grad, None, None, None
