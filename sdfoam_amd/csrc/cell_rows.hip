@@ -79,7 +79,7 @@ struct RowsArgs {
 };
 
 constexpr int kUnroll = 4;
-constexpr uint64_t kWindow = 1ull << 22; // blocks a launch: it holds fewer than 2^32 threads
+constexpr uint64_t kWindow = 1ull << 18; // blocks a launch: it holds fewer than 2^32 threads
 constexpr uint32_t kMaxWidth = 1u << 18; // of a row: Divisor's range
 
 // One lane per piece of a row, kUnroll of them in flight: bound by the bytes of

@@ -267,6 +267,27 @@ def test_rows_past_32_bits(dev):
     assert int((tg != 0).any(1).sum()) == 3
 
 
+def test_rows_of_more_than_one_launch(dev):
+    """More rows than one launch takes: 270,000 of 8,192 elements, and the weights' gradient
+    alone of 1.1 million ids."""
+    say("rows of more than one launch")
+    g = torch.Generator().manual_seed(5)
+    table = torch.randn((50, 8192), generator=g).to(torch.bfloat16).to(dev)
+    ids = torch.randint(-1, 50, (270_000,), generator=g).to(dev)
+    out = sdfoam_amd.cell_rows(table, ids)
+    ref = torch.cat([table, torch.zeros((1, 8192), dtype=torch.bfloat16, device=dev)])
+    for k in range(0, 270_000, 30_000):
+        assert torch.equal(out[k:k + 30_000], ref[ids[k:k + 30_000]])
+    del out
+    table = torch.randn((50, 3), generator=g)
+    ids = torch.randint(-1, 50, (1_100_000,), generator=g)
+    up = torch.randn((1_100_000, 3), generator=g)
+    w = torch.rand(1_100_000, generator=g).to(dev).requires_grad_()
+    sdfoam_amd.cell_rows(table.to(dev), ids.to(dev), w).backward(up.to(dev))
+    prod = torch.where((ids >= 0)[:, None], table[ids.clamp(min=0)].double(), 0.0) * up.double()
+    near(w.grad, prod.sum(1), 6 * U * prod.abs().sum(1))
+
+
 # ---- logits ------------------------------------------------------------------------------
 
 
@@ -690,6 +711,32 @@ def test_logits_past_32_bits(dev):
     assert torch.allclose(la[-4:], lb, rtol=1e-5)
     # one rounding of bf16 apart at most
     assert torch.all((da[-4:].float() - db.float()).abs() <= 2.0 ** -7 * db.float().abs() + 1e-30)
+
+
+def test_rows_of_logits_of_more_than_one_launch(dev):
+    """4.2 million rows of 5 labels: the last rows as if alone."""
+    say("more rows than a launch takes")
+    rows, labels = (1 << 22) + 77, 5
+    g = torch.Generator().manual_seed(2)
+    z = torch.randn((rows, labels), generator=g).to(dev)
+    j = torch.randint(-1, labels, (rows, 2), generator=g).to(dev)
+    t = torch.randn((rows, 2), generator=g).to(dev)
+    w = torch.rand(rows, generator=g).to(dev)
+    up = torch.randn(rows, generator=g).to(dev)
+    y = j[:, 0].contiguous()
+    last = slice(rows - 100, rows)
+
+    def work(s):
+        loss, dz = sdfoam_amd.distill_loss_and_grad(z[s], j[s], t[s], 1.0, w[s], "none", up[s])
+        leaf = z[s].detach().requires_grad_()
+        a = sdfoam_amd.label_log_probs(leaf, y[s], 3)
+        back, = torch.autograd.grad((a.log_prob, a.entropy), leaf, (up[s], w[s]))
+        other = z[s].detach().requires_grad_()
+        sdfoam_amd.distill_loss(other, j[s], t[s], 1.0, w[s], "none").backward(up[s])
+        return [loss, dz, a.log_prob, a.entropy, a.top_log_probs, a.top_labels, back, other.grad]
+
+    for x, alone in zip(work(slice(0, rows)), work(last)):
+        assert torch.equal(x[last], alone)
 
 
 # ---- streams and graphs ----------------------------------------------------------------------

@@ -117,6 +117,8 @@ def test_c_cell_rows():
     _refused(rows(out=None), b"NULL pointer")
     _refused(rows(table=p + 2), b"aligned to their elements")
     assert rows(count=0, ids=None, out=None) == 0
+    rc = L.sdf_cell_rows(0, p, 4, 5, (1 << 18) + 1, 0, p, 3, None, 1.0, p, None)
+    _refused(rc, b"rows of at most 2^18 elements")
 
     def back(type=0, grad=p, table=None, cells=5, ids=p, count=3, tg=p, wg=None, scratch=p,
              nbytes=None):
