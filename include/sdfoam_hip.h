@@ -612,7 +612,7 @@ int sdf_delaunay_merge_verified(const float *points, uint32_t num_points,
  * either signedness) of the arrays below.  An id outside [0, limit) -- negative,
  * 0xffffffff as the trace writes it, or too large -- names no cell or label.
  * Strides are in elements; rows themselves are contiguous.  Scratch is 256-byte
- * aligned. */
+ * aligned, and may be NULL where its size is 0. */
 #define SDF_TYPE_F32 0
 #define SDF_TYPE_F16 1
 #define SDF_TYPE_BF16 2
@@ -659,7 +659,7 @@ int sdf_cell_rows_backward(int type, const void *rows_grad,
  * sdf_distill_backward.  logits_grad [rows, labels] contiguous (NULL: not
  * wanted): the gradient, times loss_grad ([rows] for SDF_REDUCE_NONE, else one
  * value; NULL: 1). */
-size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels);
+size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels, int reduction);
 int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels,
                 uint64_t stride, int id_type, const void *teacher_labels,
                 int teacher_type, const void *teacher_logits, uint32_t top,

@@ -505,20 +505,49 @@ __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs a, uint6
     if (live) write_shares(a, dz, e, st, coef, l, kLanes, 0u, a.labels);
 }
 
-// The rows' losses in one sum, always in the same order.
-__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ loss,
-                                                        uint64_t rows, float scale,
+// The rows' losses in one sum, always in the same order: each block a share of
+// them, 32 in flight per thread; one block where they are few, else the blocks'
+// sums are added by a second launch of one (160,000 rows: 7 us, 44 with one load
+// at a time in one block).
+constexpr uint64_t kSumRows = 1 << 15; // of a block
+template <typename V>
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const V *__restrict__ loss, uint64_t rows,
+                                                        uint64_t each, float scale,
+                                                        double *__restrict__ partial,
                                                         float *__restrict__ out) {
     __shared__ double part[16];
+    const uint64_t begin = blockIdx.x * each, end = begin + each < rows ? begin + each : rows;
     double s = 0.0;
-    for (uint64_t r = threadIdx.x; r < rows; r += 1024u) s += (double)loss[r];
+    for (uint64_t r = begin + threadIdx.x; r < end; r += 1024u * 32u) {
+        V x[32];
+#pragma unroll
+        for (uint32_t k = 0; k < 32u; ++k) // no branches: all of them on their way at once
+            x[k] = loss[r + k * 1024u < end ? r + k * 1024u : end - 1];
+#pragma unroll
+        for (uint32_t k = 0; k < 32u; ++k) s += r + k * 1024u < end ? (double)x[k] : 0.0;
+    }
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x != 0) return;
     s = 0.0;
     for (int k = 0; k < 16; ++k) s += part[k];
-    *out = (float)(s * (double)scale);
+    if (out) *out = (float)(s * (double)scale);
+    else partial[blockIdx.x] = s;
+}
+uint64_t sum_blocks(uint64_t rows) { return (rows + kSumRows - 1) / kSumRows; }
+void launch_loss_sum(const float *loss, uint64_t rows, float scale, double *partial, float *out,
+                     hipStream_t s) {
+    const uint64_t blocks = sum_blocks(rows);
+    if (blocks <= 1) {
+        hipLaunchKernelGGL(loss_sum_kernel<float>, dim3(1), dim3(1024), 0, s, loss, rows, rows, scale,
+                           partial, out);
+        return;
+    }
+    hipLaunchKernelGGL(loss_sum_kernel<float>, dim3((unsigned)blocks), dim3(1024), 0, s, loss, rows,
+                       kSumRows, scale, partial, static_cast<float *>(nullptr));
+    hipLaunchKernelGGL(loss_sum_kernel<double>, dim3(1), dim3(1024), 0, s, partial, blocks, blocks,
+                       scale, partial, out);
 }
 
 struct AnswerArgs {
@@ -591,14 +620,18 @@ __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t label) {
 
 constexpr uint32_t kCandidates = 512;
 
-// A bound from below on the k-th largest of the wavefront's 64 orders, bit by
-// bit: its upper half, which is all of it for bfloat16.  At least that of the
+// A bound from below on the k-th largest of the wavefront's 64 kEach orders, bit
+// by bit: its upper half, which is all of it for bfloat16.  At least that of the
 // lowest finite logit.
-__device__ __forceinline__ uint32_t bound_of_wave(uint32_t x, uint32_t k) {
+template <int kEach>
+__device__ __forceinline__ uint32_t bound_of_wave(const uint32_t (&x)[kEach], uint32_t k) {
     uint32_t t = 0;
     for (int b = 31; b >= 16; --b) {
         const uint32_t with = t | 1u << b;
-        if ((uint32_t)__popcll(__ballot(x >= with)) >= k) t = with;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n += (uint32_t)__popcll(__ballot(x[i] >= with));
+        if (n >= k) t = with;
     }
     return max(t, 0x00800000u);
 }
@@ -627,11 +660,11 @@ __device__ __forceinline__ void write_best(const AnswerArgs &a, uint64_t r, uint
 
 // A block per row, or per slice of one where rows are few; one pass over the
 // logits for the softmax, its entropy and each thread's largest logit.
-// The best labels: the threads form 64 groups, and the top-th largest of the
-// groups' largest logits bounds the top-th best label from below.  Only
-// threads whose largest logit reaches the bound (about `top`) look at theirs
-// again, and only at the one or two steps that hold it where no third does;
-// what reaches it is ranked by counting.
+// The best labels: the top-th largest of the threads' largest logits bounds the
+// top-th best label from below (the threads are more than `top`).  Only threads
+// whose largest logit reaches the bound (about `top`) look at theirs again, and
+// only at the one or two steps that hold it where no third does; what reaches
+// it is ranked by counting.
 // slices > 1: Part and keys of each slice, for join_kernel.  kOnce: no backward
 // will read the logits again (2,048 rows of 50,021 floats with their gradient:
 // 221 us past the caches, 207 through them).
@@ -640,7 +673,8 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
                                                          uint32_t slice, Part *out,
                                                          uint64_t *out_keys) {
     __shared__ Part parts[kStream / 64];
-    __shared__ uint32_t groups[64];
+    constexpr int kEach = kStream / 64;
+    __shared__ uint32_t bests[kStream];
     __shared__ uint64_t keys[kCandidates];
     __shared__ uint32_t found;
     const uint64_t r = blockIdx.x / slices;
@@ -663,11 +697,8 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
         where = leads ? at : where;
     });
     const uint32_t best = logit_order(mine.m);
-    if (a.top) {
-        const uint32_t o = group_all<kStream / 64>(best, [](uint32_t x, uint32_t y) { return max(x, y); });
-        if (threadIdx.x % (kStream / 64) == 0) groups[threadIdx.x / (kStream / 64)] = o;
-        if (threadIdx.x == 0) found = 0;
-    }
+    bests[threadIdx.x] = best;
+    if (threadIdx.x == 0) found = 0;
     Part st = merge_block<true>(mine, parts, c);
     if (slices == 1 && st.m == -INFINITY) st.m = 0.0f;
     if (threadIdx.x == 0) {
@@ -684,7 +715,10 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
         if (slices > 1) out_keys[(r * slices + part) * a.top + k] = key;
         else write_best(a, r, k, key, st, inv_t, log_s);
     };
-    const uint32_t bound = bound_of_wave(groups[threadIdx.x & 63u], a.top);
+    uint32_t of_threads[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) of_threads[k] = bests[k * 64u + (threadIdx.x & 63u)];
+    const uint32_t bound = bound_of_wave(of_threads, a.top);
     const float least = order_logit(bound);
     if (best >= bound) {
         const auto collect = [&](const auto &ch, uint32_t at) {
@@ -729,7 +763,47 @@ __global__ __launch_bounds__(kStream) void answer_kernel(AnswerArgs a, uint32_t 
         if (threadIdx.x >= n && threadIdx.x < a.top) emit(threadIdx.x, 0);
         return;
     }
-    // more labels tie at the bound than there is room for: one pass for each
+    // More labels reach the bound than there is room for.  Where `top` threads and
+    // more have the row's largest logit, as in a row of one value, the first
+    // `top` labels that have it are the answer: in order, counted as they come.
+    uint32_t peak = 0, equal = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) peak = max(peak, of_threads[k]);
+    peak = group_all<64>(peak, [](uint32_t x, uint32_t y) { return max(x, y); });
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) equal += (uint32_t)__popcll(__ballot(of_threads[k] == peak));
+    if (equal >= a.top) {
+        const float largest = order_logit(peak);
+        uint32_t *counts = reinterpret_cast<uint32_t *>(keys); // [2][wavefronts]
+        uint32_t have = 0, turn = 0;
+        for (uint32_t first = begin; have < a.top && first < span.last();
+             first += kStream * Chunk<T>::kN, turn ^= kStream / 64) {
+            const uint32_t at = first + threadIdx.x * Chunk<T>::kN;
+            uint32_t bits = 0;
+            if (at < span.last()) {
+                Chunk<T> ch = span.load(at, (T)-INFINITY);
+                span.mask(ch, at, (T)-INFINITY);
+#pragma unroll
+                for (int e = 0; e < Chunk<T>::kN; ++e) bits |= (ch[e] == largest ? 1u : 0u) << e;
+            }
+            uint32_t upto = __popc(bits);
+            for (uint32_t d = 1; d < 64u; d <<= 1) {
+                const uint32_t o = __shfl_up(upto, d);
+                if ((threadIdx.x & 63u) >= d) upto += o;
+            }
+            if ((threadIdx.x & 63u) == 63u) counts[turn + (threadIdx.x >> 6)] = upto;
+            __syncthreads();
+            uint32_t rank = have + upto - __popc(bits);
+            for (uint32_t w = 0; w < kStream / 64u; ++w) {
+                if (w < threadIdx.x >> 6) rank += counts[turn + w];
+                have += counts[turn + w];
+            }
+            for (; bits != 0 && rank < a.top; bits &= bits - 1u, ++rank)
+                emit(rank, key_of(peak, span.place(at) + __ffs(bits) - 1));
+        }
+        return;
+    }
+    // Else one pass for each.
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top; ++k) {
         uint64_t key = 0;
@@ -784,8 +858,9 @@ __global__ __launch_bounds__(kStream) void join_kernel(AnswerArgs a, uint32_t sl
             mine[k] = i < n ? keys[r * n + i] : 0;
         }
         const uint32_t q = (a.top + slices - 1) / slices;
-        bound = lane < slices ? (uint32_t)(keys[r * n + lane * a.top + q - 1] >> 32) : 0u;
-        bound = bound_of_wave(bound, (a.top + q - 1) / q);
+        const uint32_t of_slices[1] = {
+            lane < slices ? (uint32_t)(keys[r * n + lane * a.top + q - 1] >> 32) : 0u};
+        bound = bound_of_wave(of_slices, (a.top + q - 1) / q);
     }
     merge_lanes<64, true>(st, c);
     if (st.m == -INFINITY) st.m = 0.0f;
@@ -1125,6 +1200,9 @@ template <typename T> void launch_answer_grad(const AnswerArgs &a, uint64_t rows
 }
 
 size_t align256(size_t x) { return (x + 255u) & ~(size_t)255u; }
+size_t sum_bytes(uint64_t rows) {
+    return align256(4 * rows) + (sum_blocks(rows) > 1 ? align256(8 * sum_blocks(rows)) : 0);
+}
 
 int check_logits(const char *what, int type, const void *logits, uint64_t rows, uint64_t labels,
                  uint64_t stride, int id_type, float temperature) {
@@ -1162,10 +1240,11 @@ int check_distill(const char *what, int type, const void *logits, uint64_t rows,
 
 extern "C" {
 
-// the rows' losses where they are added up, and the Parts of slices
+// the rows' losses and their blocks' sums where they are added up, and the Parts
+// of slices
 size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels, int reduction) {
     const Slices sl = slices_of(rows, labels, 64);
-    return (reduction == SDF_REDUCE_NONE ? 0 : align256(4 * rows)) +
+    return (reduction == SDF_REDUCE_NONE ? 0 : sum_bytes(rows)) +
            (sl.count > 1 ? align256(rows * sl.count * sizeof(Part)) : 0);
 }
 
@@ -1195,14 +1274,16 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
                      reduce, none ? loss : static_cast<float *>(scratch),
                      reinterpret_cast<float2 *>(stats), logits_grad};
     Part *parts = reinterpret_cast<Part *>(static_cast<char *>(scratch) +
-                                           (none ? 0 : align256(4 * rows)));
+                                           (none ? 0 : sum_bytes(rows)));
     with_type(type, [&](auto t) {
         for_windows(rows, [&](uint64_t r, uint64_t n) {
             launch_distill<decltype(t)>(from_row(a, type, r), n, parts, s);
         });
     });
     if (!none)
-        hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, a.loss, rows, reduce, loss);
+        launch_loss_sum(a.loss, rows, reduce,
+                        reinterpret_cast<double *>(static_cast<char *>(scratch) + align256(4 * rows)),
+                        loss, s);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SDF_OK : hip_fail(e, "distill");
 }

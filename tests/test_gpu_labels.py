@@ -609,6 +609,36 @@ def test_answers_ties(dev, labels):
             check_answer(dev, z, y, top, 1.0, dtype, grads=False)
 
 
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+def test_distill_sums_of_many_rows(dev, reduction):
+    """300,000 rows: the sum of the rows' own losses, each rounded to fp32, in 64 bits."""
+    g = torch.Generator().manual_seed(3)
+    z = torch.randn((300_000, 7), generator=g).to(dev)
+    j = torch.randint(-1, 7, (300_000, 2), generator=g).to(dev)
+    t = torch.randn((300_000, 2), generator=g).to(dev)
+    rows = sdfoam_amd.distill_loss(z, j, t, reduction="none").double().sum().cpu()
+    got = sdfoam_amd.distill_loss(z, j, t, reduction=reduction)
+    near(got, rows if reduction == "sum" else rows / 300_000, 2 * U * rows.abs()
+         if reduction == "sum" else 2 * U * rows.abs() / 300_000)
+
+
+def test_answers_first_of_many_equal(dev):
+    """The largest logit many times over, its first labels late in the row."""
+    for labels in (5003, 70_001, 100_003):
+        for dtype in TYPES:
+            z, g = logits_case(4, labels, dtype)
+            z[0, labels // 3:] = 20.0
+            z[1, labels - 700:] = 20.0
+            z[2, ::3] = 20.0
+            z[3] = -5.0
+            y = torch.randint(labels, (4,), generator=g)
+            big = z.repeat(200, 1)
+            for top in (1, 8, 64):
+                check_answer(dev, z, y, top, 1.0, dtype, grads=False)
+                a = sdfoam_amd.label_log_probs(big.to(dev), y.repeat(200).to(dev), top)
+                assert torch.equal(a.top_labels.cpu(), best_reference(z, top).repeat(200, 1))
+
+
 @pytest.mark.parametrize("labels", [37, 1000, 5003, 70_001, 140_000])
 def test_answers_masks(dev, labels):
     """Few labels allowed, spread or side by side; none; the label itself masked."""
