@@ -84,6 +84,8 @@ constexpr uint32_t kMaxWidth = 1u << 18; // of a row: Divisor's range
 
 // One lane per piece of a row, kUnroll of them in flight: bound by the bytes of
 // the rows read and written (the ids come once per row, from L1 after that).
+// 1.92M rows of 49 floats, 460 MB: 77 to 109 us; 8 pieces in flight a lane or 2
+// are slower (165, 142 against 136 before the writes went past the caches).
 template <typename T, int kP, bool kPast>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
     const T *table = static_cast<const T *>(a.table);
@@ -182,6 +184,8 @@ __device__ __forceinline__ uint2 sort_item(const SortPass &p, uint32_t i) {
     return make_uint2(c < 0 ? p.num_cells : (uint32_t)c, i);
 }
 
+// How often each digit occurs in each tile (1M ids: 7 us, with its share of the
+// clearing, as is the scan).
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortPass p) {
     extern __shared__ uint32_t hist[];
     if (blockIdx.x >= p.blocks) return clear_block(p.clear, blockIdx.x - p.blocks);
@@ -348,7 +352,9 @@ __device__ __forceinline__ void load_tile(const SortPass &p, uint32_t begin, Til
 }
 
 // Puts a tile in order and writes it from LDS: lanes side by side then write
-// side by side (1M ids with factors, 10-bit digits: 16 us; 22 us without).
+// side by side (1M ids with factors, 10-bit digits: 16 us, 22 without; 19 with a
+// share of the clearing).  Bound by the pieces of lines it writes: tiles of 8,192
+// would write longer ones, but on half the CUs (22 us).
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) {
     extern __shared__ uint32_t shift[];
     __shared__ uint2 waves[kSortWaves];
@@ -371,6 +377,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass p) 
 
 // At most kSteps * kSortThreads ids: every pass in one block, without leaving
 // LDS.  The factors stay where they are: so few are read by position from L2.
+// 16,381 ids: 35 us alone, 50 beside the clearing of 268 MB; 4,096: 11.
 template <uint32_t kSteps>
 __global__ __launch_bounds__(kSortThreads) void sort_block_kernel(SortPass p) {
     extern __shared__ uint32_t shift[];
@@ -402,6 +409,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_block_kernel(SortPass p) {
 // is summed and written there.  Of a cell that goes on in other tiles, each
 // tile keeps its sum in fp32: slot 0 where the cell began in an earlier tile,
 // slot 1 where it begins here; join_rows_kernel adds them.
+// Bound by the bytes: 1M rows of 64 bfloat16 in 300,000 cells, weights'
+// gradient beside: 68 us for about 300 MB (111 when each id's weight was
+// gathered by its position); 16,381 rows of 2,048 halves: 28.
 struct SumsArgs {
     const void *grad;
     uint64_t stride;
@@ -418,7 +428,7 @@ struct SumsArgs {
     float *weight_grad; // NULL: not formed here
 };
 
-constexpr int kBatch = 4; // rows in flight per lane
+constexpr int kBatch = 4; // rows in flight per lane (8: 100 VGPRs, half the waves, 167 us for 117)
 
 template <typename T, int kP, int kLanes>
 __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint32_t piece, uint32_t l) {
@@ -509,7 +519,8 @@ __global__ __launch_bounds__(256) void sums_kernel(SumsArgs a) {
 // The cells that go on past the tile they begin in: their tiles' sums in order.
 // A group of lanes looks at the tiles that follow its own, one a lane (16 at
 // least); where the cell goes on past those, the whole block adds its sums,
-// every group a share of the tiles.
+// every group a share of the tiles.  Bound by latency: 9 us for 1M rows of 64, 12
+// for 16,381 of 2,048, one cell of them in 125 tiles.
 template <typename T, int kP, int kLanes>
 __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
     constexpr uint32_t kGroups = 256 / kLanes;
@@ -605,28 +616,49 @@ __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
     }
 }
 
-// The weights' gradient by itself, a wavefront per id: where the table's is not
-// wanted, or a row is wider than a wavefront holds.
-template <typename T, int kP>
+// The weights' gradient by itself, where the table's is not wanted or a row is
+// wider than a wavefront holds: kLanes lanes an id, kUnroll ids at a time.  Bound
+// by the two rows that each id reads (1M ids, rows of 64 bfloat16, 268 MB: 56
+// us; a wavefront per id took 280).
+template <typename T, int kP, int kLanes>
 __global__ __launch_bounds__(256) void weight_grad_kernel(RowsArgs a, const T *__restrict__ grad,
                                                           uint64_t grad_stride,
                                                           float *__restrict__ weight_grad) {
-    const uint64_t i = a.first + (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
-    if (i >= a.first + a.count) return;
-    const int32_t c = load_id(a.cells, a.id_type, i, a.num_cells);
-    float s = 0.0f;
-    if (c >= 0)
-        for (uint32_t k = threadIdx.x & 63u; k < a.pieces.d; k += 64u) {
-            const uint32_t col = column<kP>(k, a.width);
-            const auto x = load_piece<T, kP>(grad + i * grad_stride + col);
-            const auto y = load_piece<T, kP>(static_cast<const T *>(a.table) +
-                                             (uint64_t)c * a.stride + col);
+    const uint32_t l = threadIdx.x % kLanes;
+    const uint64_t first =
+        a.first + ((uint64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes) * kUnroll;
+    const uint64_t end = a.first + a.count;
+    if (first >= end) return; // a whole group
+    int32_t cell[kUnroll];
+    float s[kUnroll];
 #pragma unroll
-            for (int e = 0; e < kP; ++e)
-                if (col + e >= k * kP) s = fmaf((float)x.v[e], (float)y.v[e], s);
+    for (int u = 0; u < kUnroll; ++u) {
+        const uint64_t i = first + u < end ? first + u : end - 1;
+        cell[u] = load_id(a.cells, a.id_type, i, a.num_cells);
+        s[u] = 0.0f;
+    }
+    for (uint32_t k = l; k < a.pieces.d; k += kLanes) {
+        const uint32_t col = column<kP>(k, a.width);
+        Piece<T, kP> x[kUnroll], y[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            x[u] = {};
+            y[u] = {};
+            if (cell[u] < 0 || first + u >= end) continue;
+            x[u] = load_piece_past<T, kP>(grad + (first + u) * grad_stride + col);
+            y[u] = load_piece<T, kP>(static_cast<const T *>(a.table) + (uint64_t)cell[u] * a.stride + col);
         }
-    s = group_sum<64>(s);
-    if ((threadIdx.x & 63u) == 0) weight_grad[i] = a.scale * s;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int e = 0; e < kP; ++e) // elements that two lanes hold count once
+                if (col + e >= k * kP) s[u] = fmaf((float)x[u].v[e], (float)y[u].v[e], s[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const float sum = group_sum<kLanes>(s[u]);
+        if (l == u % kLanes && first + u < end) weight_grad[first + u] = a.scale * sum;
+    }
 }
 
 // ---- which kernel --------------------------------------------------------------
@@ -887,13 +919,18 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
             RowsArgs w = {table, table_stride, width ? cells_n : 0u, width,
                           divisor(width ? pieces : 1u), cells, id_type, 0, count, 1, nullptr, scale,
                           nullptr};
-            for (uint64_t r = 0; r < count; r += 4 * kWindow) {
-                w.first = r;
-                w.count = count - r < 4 * kWindow ? count - r : 4 * kWindow;
-                hipLaunchKernelGGL((weight_grad_kernel<T, kP>), dim3((unsigned)((w.count + 3) / 4)),
-                                   dim3(256), 0, s, w, static_cast<const T *>(rows_grad),
-                                   rows_grad_stride, weight_grad);
-            }
+            with_lanes(pieces, [&](auto lanes) {
+                constexpr int kLanes = decltype(lanes)::v;
+                constexpr uint64_t kIds = 256 / kLanes * kUnroll; // of a block
+                for (uint64_t r = 0; r < count; r += kIds * kWindow) {
+                    w.first = r;
+                    w.count = count - r < kIds * kWindow ? count - r : kIds * kWindow;
+                    hipLaunchKernelGGL((weight_grad_kernel<T, kP, kLanes>),
+                                       dim3((unsigned)((w.count + kIds - 1) / kIds)), dim3(256), 0,
+                                       s, w, static_cast<const T *>(rows_grad), rows_grad_stride,
+                                       weight_grad);
+                }
+            });
         }
     });
     const hipError_t e = hipGetLastError();
