@@ -1222,8 +1222,9 @@ int check_logits(const char *what, int type, const void *logits, uint64_t rows, 
     if (labels == 0 || labels >= (1ull << 31))
         return fail(SDF_E_INVALID, "%s takes 1 to 2^31 - 1 labels", what);
     if (rows >= (1ull << 31)) return fail(SDF_E_INVALID, "%s takes fewer than 2^31 rows", what);
-    if (!(temperature > 0.0f) || temperature > 3.0e38f)
-        return fail(SDF_E_INVALID, "%s: temperature must be positive and finite", what);
+    if (!(temperature >= 1.0e-38f) || temperature > 3.0e38f) // (1 / T is formed)
+        return fail(SDF_E_INVALID, "%s: temperature must be positive and finite, as its reciprocal",
+                    what);
     if (rows > 0 && !logits) return fail(SDF_E_INVALID, "NULL pointer argument");
     (void)stride;
     if ((reinterpret_cast<uintptr_t>(logits) & (type_bytes(type) - 1)) != 0)

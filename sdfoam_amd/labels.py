@@ -250,8 +250,8 @@ def _check_logits(logits, temperature) -> float:
     if logits.size(-1) == 0:
         raise RuntimeError("logits must have at least one label")
     temperature = float(temperature)
-    if not 0.0 < temperature <= 3.0e38:
-        raise RuntimeError("temperature must be positive and finite")
+    if not 1.0e-38 <= temperature <= 3.0e38:
+        raise RuntimeError("temperature must be positive and finite, as its reciprocal in float32")
     return temperature
 
 

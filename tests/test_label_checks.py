@@ -200,3 +200,15 @@ def test_c_label_log_probs():
     _refused(back(z=None), b"NULL pointer")
     _refused(back(entropy=None), b"NULL pointer")
     _refused(back(out=None), b"NULL pointer")
+
+
+def test_temperature_without_a_reciprocal():
+    z, j = torch.zeros(3, 7), ids(3, 2)
+    for bad in (1e-39, 1e-60):
+        with pytest.raises(RuntimeError, match="temperature must be positive and finite"):
+            sdfoam_amd.distill_loss(z, j, torch.zeros(3, 2), bad)
+        with pytest.raises(RuntimeError, match="temperature must be positive and finite"):
+            sdfoam_amd.label_log_probs(z, ids(3), 0, bad)
+    keep, p = _memory()
+    _refused(_lib.lib().sdf_label_log_probs(0, p, 3, 7, 7, 0, p, 0, 1e-39, p, p, None, None, None, p,
+                                            1024, None), b"temperature must be positive and finite")
