@@ -130,14 +130,19 @@ constexpr uint32_t kSortWaves = kSortThreads / 64;
 constexpr uint32_t kSteps = 4;                       // keys per thread
 constexpr uint32_t kTile = kSteps * kSortThreads;    // keys of one block
 constexpr uint32_t kOneBlock = 16 * kSortThreads;    // keys that one block sorts alone
-constexpr uint32_t kMaxBits = 11;                 // of a digit
-constexpr uint32_t kScanParts = 16;               // threads that share a digit's tiles
+constexpr uint32_t kMaxBits = 11;                    // of a digit
+constexpr uint32_t kScanParts = 16;                  // threads that share a digit's tiles
+// Up to so many tiles, and with a digit per thread, each tile's block adds up the
+// counts of all tiles itself, for the scan's launch (100,000 cells: 32,000 ids 37 ->
+// 35 us, 131,072 43 -> 38, 500,000 59 -> 60; two digits per thread: 64 -> 82 for
+// 262,144 ids in 2M cells).
+constexpr uint32_t kFewTiles = 64;
 
 // The table's gradient is cleared by extra blocks of the sort's launches, which
 // leave the memory idle: each launch clears [begin, end) of it, `each` bytes a
 // block in stores of 16, past the caches (which would otherwise be full of
-// zeros when the sums begin: 120 -> 96 us for 268 MB).  Few large shares: beside the sort's blocks a CU has
-// room (LDS) for one of these at a time.
+// zeros when the sums begin: 120 -> 96 us for 268 MB).  Few large shares: beside
+// the sort's blocks a CU has room (LDS) for one of these at a time.
 struct Clear {
     char *to;
     uint64_t begin, end, each;
@@ -173,6 +178,7 @@ struct SortPass {
     uint32_t *counts; // [tiles][digits], after the scan those of the tiles before
     uint32_t *totals; // [digits]
     uint32_t n, tiles, shift, bits, passes;
+    bool scanned;    // counts and totals; else counts as they were made, and no totals
     uint32_t blocks; // those after them clear
     Clear clear;
 };
@@ -269,8 +275,17 @@ __device__ __forceinline__ uint2 *order_tile(const SortPass &p, Tile<kSteps> &x,
 #pragma unroll
     for (uint32_t k = 0; k < kEach; ++k) {
         const bool has = to_output && k < each && lo + k < digits;
-        total[k] = has ? p.totals[lo + k] : 0u;
-        earlier[k] = has ? p.counts[(uint64_t)blockIdx.x * digits + lo + k] : 0u;
+        total[k] = has && p.scanned ? p.totals[lo + k] : 0u;
+        earlier[k] = has && p.scanned ? p.counts[(uint64_t)blockIdx.x * digits + lo + k] : 0u;
+    }
+    if (to_output && !p.scanned && lo < digits) { // one digit per thread then
+        const uint32_t *counts = p.counts + lo;
+#pragma unroll 16
+        for (uint32_t t = 0; t < p.tiles; ++t) {
+            const uint32_t c = counts[(uint64_t)t * digits];
+            total[0] += c;
+            earlier[0] += t < blockIdx.x ? c : 0u;
+        }
     }
     uint16_t *own = seen + w * digits;
     for (uint32_t d = lane; d < digits; d += 64u) own[d] = 0;
@@ -832,7 +847,8 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
         const Sort so = sort_of(num_cells, count);
         const uint64_t bytes = num_cells * width * type_bytes(type);
         const bool alone = n <= kOneBlock;
-        const uint32_t launches = alone ? 1 : 3 * so.passes;
+        const bool scan = so.tiles > kFewTiles || (1u << so.bits) > kSortThreads;
+        const uint32_t launches = alone ? 1 : (scan ? 3 : 2) * so.passes;
         const uint64_t share = (bytes / launches + kClearStep) / kClearStep * kClearStep;
         uint64_t cleared = 0;
         SortPass p = {};
@@ -855,6 +871,7 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
         p.tiles = so.tiles;
         p.bits = so.bits;
         p.passes = so.passes;
+        p.scanned = scan;
         const auto pass = [&](uint32_t k) {
             p.shift = k * so.bits;
             p.out = reinterpret_cast<uint2 *>(at + lay.order[k & 1]);
@@ -876,8 +893,10 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
                 pass(k);
                 dim3 grid = with_clear(so.tiles);
                 hipLaunchKernelGGL(sort_count_kernel, grid, dim3(kSortThreads), 4u << so.bits, s, p);
-                grid = with_clear(((1u << so.bits) + 63u) / 64u);
-                hipLaunchKernelGGL(sort_scan_kernel, grid, dim3(64 * kScanParts), 0, s, p);
+                if (scan) {
+                    grid = with_clear(((1u << so.bits) + 63u) / 64u);
+                    hipLaunchKernelGGL(sort_scan_kernel, grid, dim3(64 * kScanParts), 0, s, p);
+                }
                 grid = with_clear(so.tiles);
                 hipLaunchKernelGGL(sort_scatter_kernel, grid, dim3(kSortThreads),
                                    order_bytes(so.bits, 12 * kTile), s, p);

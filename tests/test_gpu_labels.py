@@ -252,6 +252,22 @@ def test_rows_differences(dev):
         assert abs(diff - float((gradient.cpu().double() * d.double()).sum())) <= 40 * U * size
 
 
+@pytest.mark.parametrize("cells", [900, 2000, 70_000])
+@pytest.mark.parametrize("count", [16_384, 16_385, 262_144, 262_145])
+def test_rows_gradient_at_the_sorts_limits(dev, cells, count):
+    """Whole numbers, so that every sum is exact: the counts at which the sort of the ids
+    takes another form, with one and two digits a thread and one and two passes."""
+    say("rows, sort", cells, count)
+    g = torch.Generator().manual_seed(count + cells)
+    ids = torch.randint(-1, cells, (count,), generator=g)
+    up = torch.randint(-9, 10, (count, 3), generator=g).float()
+    weight = torch.randint(1, 4, (count,), generator=g).float()
+    got, _ = sdfoam_amd.cell_rows_backward(up.to(dev), ids.to(dev), cells, weight.to(dev))
+    sums = torch.zeros((cells + 1, 3)).index_add_(0, torch.where(ids < 0, cells, ids),
+                                                  up * weight[:, None])
+    assert torch.equal(got.cpu(), sums[:cells])
+
+
 def test_rows_past_32_bits(dev):
     """Tables and gradients of more than 2^32 bytes and 2^31 elements."""
     cells, width = 1_100_003, 2048
