@@ -129,13 +129,18 @@ constexpr uint32_t kSortThreads = 1024;
 constexpr uint32_t kSortWaves = kSortThreads / 64;
 constexpr uint32_t kSteps = 4;                       // keys per thread
 constexpr uint32_t kTile = kSteps * kSortThreads;    // keys of one block
-constexpr uint32_t kOneBlock = 16 * kSortThreads;    // keys that one block sorts alone
+// One block sorts up to a tile alone, and up to kOneBlock keys where the clearing
+// beside it takes as long (see below): 16,381 ids in 65,536 cells, 67 MB of them 53 us
+// for 43 with several blocks, 134 MB 65 for 57, 201 MB 76 for 75, 268 MB 86 for 91.
+constexpr uint32_t kOneBlock = 16 * kSortThreads;
+constexpr uint64_t kOneBlockClears = 192ull << 20;
 constexpr uint32_t kMaxBits = 11;                    // of a digit
+constexpr uint32_t kFewTilesBits = 10;               // where tiles are few
 constexpr uint32_t kScanParts = 16;                  // threads that share a digit's tiles
-// Up to so many tiles, and with a digit per thread, each tile's block adds up the
-// counts of all tiles itself, for the scan's launch (100,000 cells: 32,000 ids 37 ->
-// 35 us, 131,072 43 -> 38, 500,000 59 -> 60; two digits per thread: 64 -> 82 for
-// 262,144 ids in 2M cells).
+// Up to so many tiles, each tile's block adds up the counts of all tiles itself, a
+// digit per thread, for the scan's launch (100,000 cells: 32,000 ids 37 -> 35 us,
+// 131,072 43 -> 38, 500,000 59 -> 60; 2M cells in three passes of 7 bits for two of
+// 11 with their scans: 262,144 ids 64 -> 59, 1M 97 -> 103).
 constexpr uint32_t kFewTiles = 64;
 
 // The table's gradient is cleared by extra blocks of the sort's launches, which
@@ -533,16 +538,19 @@ __global__ __launch_bounds__(256) void sums_kernel(SumsArgs a) {
 
 // The cells that go on past the tile they begin in: their tiles' sums in order.
 // A group of lanes looks at the tiles that follow its own, one a lane (16 at
-// least); where the cell goes on past those, the whole block adds its sums,
-// every group a share of the tiles.  Bound by latency: 9 us for 1M rows of 64, 12
-// for 16,381 of 2,048, one cell of them in 125 tiles.
+// least) and on to 64 while all are that cell's; where it goes on past those, the
+// whole block adds its sums, every group a share of the tiles.  Bound by latency:
+// 9 us for 1M rows of 64, 12 for 16,381 of 2,048, one cell of them in 125 tiles.
+// (Blocks for all that pass 16 tiles: the gradient of 262,144 rows of 8 in 2,000
+// cells 158 us for 43, of 200,000 rows of 32 in 100 cells 30 for 33.)
 template <typename T, int kP, int kLanes>
 __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
     constexpr uint32_t kGroups = 256 / kLanes;
-    constexpr uint32_t kProbes = kLanes < 16 ? 16 / kLanes : 1, kNear = kProbes * kLanes;
+    constexpr uint32_t kProbes = kLanes < 16 ? 16 / kLanes : 1, kRound = kProbes * kLanes;
+    constexpr uint32_t kNear = 64;
     __shared__ uint32_t list[kGroups];
     __shared__ uint32_t listed;
-    __shared__ float sums[kGroups][kLanes * kP];
+    __shared__ float sums[4][kLanes * kP]; // of the wavefronts
     const uint32_t g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
     const uint32_t tile = blockIdx.x * kGroups + g, piece = blockIdx.y * kLanes + l;
     const bool mine = piece * kP < a.width;
@@ -583,11 +591,14 @@ __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
         const bool whole = p0 > 0 && a.order[p0 - 1].x == cell; // the tile is all of that cell
         uint32_t near = 0; // the following tiles that begin with it: the first so many
         if (cell < a.num_cells && !whole) {
+            for (uint32_t k = 0; k < kNear && near == k; k += kRound) {
+                uint32_t n = 0;
 #pragma unroll
-            for (uint32_t q = 0; q < kProbes; ++q)
-                near += goes_on(tile + 1 + q * kLanes + l, cell);
+                for (uint32_t q = 0; q < kProbes; ++q)
+                    n += goes_on(tile + 1 + k + q * kLanes + l, cell);
+                near += group_all<kLanes>(n, [](uint32_t x, uint32_t y) { return x + y; });
+            }
         }
-        near = group_all<kLanes>(near, [](uint32_t x, uint32_t y) { return x + y; });
         if (near == kNear) {
             if (l == 0) list[atomicAdd(&listed, 1u)] = tile;
         } else if (near > 0) {
@@ -617,12 +628,18 @@ __global__ __launch_bounds__(256) void join_rows_kernel(SumsArgs a) {
         }
         float s[kP] = {};
         if (g < lo) add(s, first + g, (lo - g + kGroups - 1) / kGroups, kGroups);
+        // the wavefront's groups, then the wavefronts
 #pragma unroll
-        for (int e = 0; e < kP; ++e) sums[g][l * kP + e] = s[e];
+        for (int e = 0; e < kP; ++e) {
+#pragma unroll
+            for (int d = kLanes; d < 64; d *= 2) s[e] += __shfl_xor(s[e], d);
+            if ((threadIdx.x & 63u) < (uint32_t)kLanes) sums[threadIdx.x >> 6][l * kP + e] = s[e];
+        }
         __syncthreads();
         if (g == 0) {
             begun(s, first - 1);
-            for (uint32_t k = 0; k < kGroups; ++k)
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
 #pragma unroll
                 for (int e = 0; e < kP; ++e) s[e] += sums[k][l * kP + e];
             write(cell, s);
@@ -718,14 +735,17 @@ uint32_t tile_of(uint64_t count, uint32_t pieces) {
 
 struct Sort {
     uint32_t passes, bits, tiles;
+    bool scan;
 };
 Sort sort_of(uint64_t num_cells, uint64_t count) {
     uint32_t bits = 1; // of the largest key, num_cells
     while ((num_cells >> bits) != 0) ++bits;
     Sort s;
-    s.passes = (bits + kMaxBits - 1) / kMaxBits;
-    s.bits = (bits + s.passes - 1) / s.passes;
     s.tiles = (uint32_t)((count + kTile - 1) / kTile);
+    s.scan = s.tiles > kFewTiles;
+    const uint32_t most = s.scan ? kMaxBits : kFewTilesBits;
+    s.passes = (bits + most - 1) / most;
+    s.bits = (bits + s.passes - 1) / s.passes;
     return s;
 }
 
@@ -846,9 +866,8 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
         // the launches of the sort clear the gradient between them
         const Sort so = sort_of(num_cells, count);
         const uint64_t bytes = num_cells * width * type_bytes(type);
-        const bool alone = n <= kOneBlock;
-        const bool scan = so.tiles > kFewTiles || (1u << so.bits) > kSortThreads;
-        const uint32_t launches = alone ? 1 : (scan ? 3 : 2) * so.passes;
+        const bool alone = n <= kTile || (n <= kOneBlock && bytes >= kOneBlockClears);
+        const uint32_t launches = alone ? 1 : (so.scan ? 3 : 2) * so.passes;
         const uint64_t share = (bytes / launches + kClearStep) / kClearStep * kClearStep;
         uint64_t cleared = 0;
         SortPass p = {};
@@ -871,7 +890,7 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
         p.tiles = so.tiles;
         p.bits = so.bits;
         p.passes = so.passes;
-        p.scanned = scan;
+        p.scanned = so.scan;
         const auto pass = [&](uint32_t k) {
             p.shift = k * so.bits;
             p.out = reinterpret_cast<uint2 *>(at + lay.order[k & 1]);
@@ -893,7 +912,7 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
                 pass(k);
                 dim3 grid = with_clear(so.tiles);
                 hipLaunchKernelGGL(sort_count_kernel, grid, dim3(kSortThreads), 4u << so.bits, s, p);
-                if (scan) {
+                if (so.scan) {
                     grid = with_clear(((1u << so.bits) + 63u) / 64u);
                     hipLaunchKernelGGL(sort_scan_kernel, grid, dim3(64 * kScanParts), 0, s, p);
                 }

@@ -268,6 +268,25 @@ def test_rows_gradient_at_the_sorts_limits(dev, cells, count):
     assert torch.equal(got.cpu(), sums[:cells])
 
 
+@pytest.mark.parametrize("width", [1, 3, 8, 24, 61, 200, 700])
+def test_rows_gradient_of_long_runs(dev, width):
+    """Whole numbers, so that every sum is exact: cells that 1 to 6,000 ids name, the ids of
+    a cell beside each other and spread."""
+    say("rows, runs", width)
+    g = torch.Generator().manual_seed(width)
+    runs = torch.cat([torch.arange(1, 40), torch.arange(40, 800, 37),
+                      torch.tensor([511, 512, 513, 519, 520, 527, 528, 1023, 6000, 1, 3000])])
+    cells = len(runs)
+    ids = torch.repeat_interleave(torch.arange(cells), runs)
+    up = torch.randint(-9, 10, (len(ids), width), generator=g).float()
+    for order in (torch.arange(len(ids)), torch.randperm(len(ids), generator=g)):
+        for dtype in (torch.float32, torch.bfloat16):
+            got, _ = sdfoam_amd.cell_rows_backward(up[order].to(dtype).to(dev),
+                                                   ids[order].to(dev), cells)
+            sums = torch.zeros((cells, width)).index_add_(0, ids, up)
+            assert torch.equal(got.cpu(), sums.to(dtype))
+
+
 def test_rows_past_32_bits(dev):
     """Tables and gradients of more than 2^32 bytes and 2^31 elements."""
     cells, width = 1_100_003, 2048
