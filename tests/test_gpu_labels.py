@@ -480,6 +480,23 @@ def test_distill_masks(dev, labels):
         near(leaf.grad, grad, gt, dtype)
 
 
+@pytest.mark.parametrize("top", [1, 2, 3, 5, 7, 65, 255, 1022, 1024])
+def test_distill_labels_named_often(dev, top):
+    """Teachers whose entries name a few labels over and over, at odd counts of entries."""
+    say("distill named often", top)
+    for labels, named in ((40, 3), (3001, 40), (70_001, 500)):
+        z, g = logits_case(5, labels, torch.float32, seed=top)
+        ids = torch.randint(named, (5, top), generator=g) * (labels // named)
+        t = torch.randn((5, top), generator=g)
+        loss, grad, lt, gt = distill_reference(z, ids, t, 1.5, None, "none")
+        got, dz = sdfoam_amd.distill_loss_and_grad(z.to(dev), ids.to(dev), t.to(dev), 1.5,
+                                                   reduction="none")
+        near(got, loss, lt)
+        # a sum of up to `top` shares, one after the other, may be off by top U of it; gt
+        # holds 64 U of it at least
+        near(dz, grad, gt * (1 + top / 64), torch.float32)
+
+
 @pytest.mark.parametrize("labels", [37, 5003, 70_001])
 def test_distill_nan_reaches_the_loss(dev, labels):
     for at in (0, labels // 2, labels - 1):
