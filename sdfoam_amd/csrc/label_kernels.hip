@@ -1084,7 +1084,9 @@ AnswerArgs from_row(AnswerArgs a, int type, uint64_t r) {
 }
 
 // Slices for rows that are too few to fill the chip: enough blocks of at least
-// 4,096 labels each; a multiple of a chunk long.
+// 4,096 labels each; a multiple of a chunk long.  Made once of all rows of a
+// call, as the size of the scratch is: a window's own rows may be few where the
+// call's are many, and have no room for its Parts then.
 struct Slices {
     uint32_t count, length;
 };
@@ -1097,6 +1099,7 @@ Slices slices_of(uint64_t rows, uint64_t labels, uint32_t most) {
     const uint64_t length = ((labels + n - 1) / n + 7) / 8 * 8;
     return {(uint32_t)((labels + length - 1) / length), (uint32_t)length};
 }
+constexpr uint32_t kDistillSlices = 64;
 constexpr uint32_t kShort = 64 * 4; // chunks of a row that a wavefront holds
 
 // Chunks of a row at most: one more where rows begin between 16-byte boundaries.
@@ -1152,10 +1155,10 @@ void launch_finish(const DistillArgs &a, uint64_t rows, const Part *parts, uint3
 }
 
 template <typename T>
-void launch_distill(const DistillArgs &a, uint64_t rows, Part *parts, hipStream_t s) {
+void launch_distill(const DistillArgs &a, uint64_t rows, const Slices &sl, Part *parts,
+                    hipStream_t s) {
     const uint64_t chunks = chunks_of<T>(a.logits, a.stride, a.labels);
     if (chunks <= kShort) return launch_short<T, false>(a, rows, s);
-    const Slices sl = slices_of(rows, a.labels, 64);
     if (sl.count > 1) {
         hipLaunchKernelGGL(part_kernel<T>, dim3((unsigned)(rows * sl.count)), dim3(kStream), 0, s,
                            a, sl.count, sl.length, parts);
@@ -1266,7 +1269,7 @@ extern "C" {
 // the rows' losses and their blocks' sums where they are added up, and the Parts
 // of slices
 size_t sdf_distill_scratch_bytes(uint64_t rows, uint64_t labels, int reduction) {
-    const Slices sl = slices_of(rows, labels, 64);
+    const Slices sl = slices_of(rows, labels, kDistillSlices);
     return (reduction == SDF_REDUCE_NONE ? 0 : sum_bytes(rows)) +
            (sl.count > 1 ? align256(rows * sl.count * sizeof(Part)) : 0);
 }
@@ -1298,9 +1301,10 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
                      reinterpret_cast<float2 *>(stats), logits_grad};
     Part *parts = reinterpret_cast<Part *>(static_cast<char *>(scratch) +
                                            (none ? 0 : sum_bytes(rows)));
+    const Slices sl = slices_of(rows, labels, kDistillSlices);
     with_type(type, [&](auto t) {
         for_windows(rows, [&](uint64_t r, uint64_t n) {
-            launch_distill<decltype(t)>(from_row(a, type, r), n, parts, s);
+            launch_distill<decltype(t)>(from_row(a, type, r), n, sl, parts, s);
         });
     });
     if (!none)

@@ -821,6 +821,25 @@ def test_rows_of_logits_of_more_than_one_launch(dev):
         assert torch.equal(x[last], alone)
 
 
+def test_distill_few_long_rows_after_a_full_launch(dev):
+    """77 rows more than one launch takes, of a length at which 77 rows by themselves are cut
+    into slices: the call's scratch holds none.  One row's logits, expanded, so that they
+    take no memory; an entry a row, of share 1: its loss is -log p of its label."""
+    rows, labels = (1 << 22) + 77, 8200
+    say("distill, few long rows after a full launch")
+    z, g = logits_case(1, labels, torch.bfloat16)
+    j = torch.randint(labels, (rows, 1), generator=g)
+    log_p, _, err = softmax64(z, 1.0)
+    loss = -log_p[0][j[:, 0]]
+    tol = 4 * (err + 17 * U) * (2 + loss.abs())
+    zd, jd = z.to(dev).expand(rows, labels), j.to(dev)
+    t = torch.zeros((rows, 1), device=dev)
+    near(sdfoam_amd.distill_loss(zd, jd, t, reduction="none"), loss, tol)
+    for reduction, scale in (("sum", 1.0), ("mean", 1.0 / rows)):
+        got = sdfoam_amd.distill_loss(zd, jd, t, reduction=reduction)
+        near(got, loss.sum() * scale, (tol.sum() + 2 * U * loss.abs().sum()) * scale)
+
+
 # ---- streams and graphs ----------------------------------------------------------------------
 
 
