@@ -17,7 +17,8 @@ in float32 and rounded to the output's type once.  Cells and labels are uint32, 
 int64; one that is negative, 0xffffffff (what the trace writes for a ray that ends in no
 cell) or too large names none.  Rows of a table or of logits may be strided (a slice of
 padded rows is read in place); other layouts are copied.  Results are the same on every
-run: no sum's order is left to chance.
+run: no sum's order is left to chance.  Derivatives are reverse-mode and of the first order;
+tensors with a forward-mode tangent are refused.
 """
 
 from __future__ import annotations
@@ -25,6 +26,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -84,6 +86,16 @@ def _no_gradient(call: str, **tensors) -> None:
         for name, t in tensors.items():
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{call} has no gradient for {name}: detach it")
+
+
+def _no_tangent(call: str, **tensors) -> None:
+    """Refuses dual tensors: their tangents would not reach the results, and requires_grad
+    does not show them."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of every dual_level
+        return
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{call} has no forward-mode derivative for {name}: detach it")
 
 
 def _wants_gradient(*tensors) -> bool:
@@ -191,6 +203,7 @@ class _CellRows(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, rows_grad):
+        _no_tangent("cell_rows", gradient=rows_grad)
         cells, weight, table = ctx.saved_tensors
         table_grad, weight_grad = _rows_backward(rows_grad, cells, ctx.num_cells, weight,
                                                  ctx.scale, table, ctx.needs_input_grad[0])
@@ -209,6 +222,7 @@ def cell_rows(table: torch.Tensor, cells: torch.Tensor, weight: Optional[torch.T
     _element_type("table", table)
     _id_type("cells", cells)
     _check_weight(weight, cells)
+    _no_tangent("cell_rows", table=table, weight=weight)
     _check_devices("table", table, "cells", cells, "weight", weight)
     if _wants_gradient(table, weight):
         return _CellRows.apply(table, cells, weight, float(scale))
@@ -236,6 +250,7 @@ def cell_rows_backward(rows_grad: torch.Tensor, cells: torch.Tensor, num_cells: 
         if table.dtype != rows_grad.dtype:
             raise RuntimeError("table and rows_grad must have the same dtype")
         _check_shape("table", table, (num_cells, rows_grad.size(-1)))
+    _no_tangent("cell_rows_backward", rows_grad=rows_grad, weight=weight, table=table)
     _check_devices("rows_grad", rows_grad, "cells", cells, "weight", weight, "table", table)
     return _rows_backward(rows_grad, cells, num_cells, weight, float(scale), table, True)
 
@@ -255,7 +270,8 @@ def _check_logits(logits, temperature) -> float:
     return temperature
 
 
-def _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weight, reduction):
+def _check_distill(call, logits, teacher_labels, teacher_logits, temperature, row_weight,
+                   reduction):
     temperature = _check_logits(logits, temperature)
     _id_type("teacher_labels", teacher_labels)
     _element_type("teacher_logits", teacher_logits)
@@ -270,6 +286,7 @@ def _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weig
         _check_float32("row_weight", row_weight, lead)
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be 'none', 'sum' or 'mean'")
+    _no_tangent(call, logits=logits, teacher_logits=teacher_logits, row_weight=row_weight)
     _check_devices("logits", logits, "teacher_labels", teacher_labels, "teacher_logits",
                    teacher_logits, "row_weight", row_weight)
     return temperature
@@ -316,6 +333,7 @@ class _DistillLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, loss_grad):
+        _no_tangent("distill_loss", gradient=loss_grad)
         logits, teacher_labels, teacher_logits, row_weight, stats = ctx.saved_tensors
         keep, args = _distill_args(logits, teacher_labels, teacher_logits, ctx.temperature,
                                    row_weight, ctx.reduction)
@@ -340,8 +358,8 @@ def distill_loss(logits: torch.Tensor, teacher_labels: torch.Tensor,
     read.  A row without an entry, or whose logits are all -inf, has loss 0 and no gradient.
     Returns float32: the rows' losses ("none"), their "sum", or their "mean" over all rows.
     Differentiable in ``logits``."""
-    temperature = _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weight,
-                                 reduction)
+    temperature = _check_distill("distill_loss", logits, teacher_labels, teacher_logits,
+                                 temperature, row_weight, reduction)
     _no_gradient("distill_loss", teacher_logits=teacher_logits, row_weight=row_weight)
     if _wants_gradient(logits):
         return _DistillLoss.apply(logits, teacher_labels, teacher_logits, temperature, row_weight,
@@ -359,8 +377,9 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_labels: torch.Tensor,
 
     loss_grad (float32, the shape of the loss; default 1) is the gradient that reaches the
     loss from above, such as a loss scale: it is applied before the gradient is rounded."""
-    temperature = _check_distill(logits, teacher_labels, teacher_logits, temperature, row_weight,
-                                 reduction)
+    _no_tangent("distill_loss_and_grad", loss_grad=loss_grad)
+    temperature = _check_distill("distill_loss_and_grad", logits, teacher_labels, teacher_logits,
+                                 temperature, row_weight, reduction)
     if loss_grad is not None:
         _check_float32("loss_grad", loss_grad, logits.shape[:-1] if reduction == "none" else ())
         _check_devices("logits", logits, "loss_grad", loss_grad)
@@ -421,6 +440,8 @@ class _LabelLogProbs(torch.autograd.Function):
     def backward(ctx, log_prob_grad, entropy_grad, best_grad, best_labels_grad):
         if log_prob_grad is None and entropy_grad is None:
             return None, None, None, None
+        for g in (log_prob_grad, entropy_grad):
+            _no_tangent("label_log_probs", gradient=g)
         logits, labels, entropy, stats = ctx.saved_tensors
         z = _rows(logits)
         y = labels.contiguous()
@@ -449,6 +470,7 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0,
     top = int(top)
     if not 0 <= top <= MAX_TOP:
         raise RuntimeError(f"top must be from 0 to {MAX_TOP}")
+    _no_tangent("label_log_probs", logits=logits)
     _check_devices("logits", logits, "labels", labels)
     if _wants_gradient(logits):
         return LabelLogProbs(*_LabelLogProbs.apply(logits, labels, top, temperature))

@@ -840,6 +840,27 @@ def test_distill_few_long_rows_after_a_full_launch(dev):
         near(got, loss.sum() * scale, (tol.sum() + 2 * U * loss.abs().sum()) * scale)
 
 
+def test_tangents_that_reach_a_backward(dev):
+    """Inputs without a tangent, gradients with one: refused, not lost."""
+    from torch.autograd import forward_ad
+
+    j = torch.zeros((3, 2), dtype=torch.int64, device=dev)
+    y = j[:, 0].contiguous()
+    calls = [lambda x: sdfoam_amd.cell_rows(x, y),
+             lambda x: sdfoam_amd.distill_loss(x, j, j.float(), reduction="none"),
+             lambda x: sdfoam_amd.label_log_probs(x, y).log_prob,
+             lambda x: sdfoam_amd.label_log_probs(x, y).entropy]
+    for call in calls:
+        x = torch.randn((3, 7), device=dev).requires_grad_()
+        out = call(x)
+        with forward_ad.dual_level():
+            one = torch.ones_like(out)
+            with pytest.raises(RuntimeError, match="has no forward-mode derivative for gradient"):
+                out.backward(forward_ad.make_dual(one, one))
+        call(x).backward(one)
+        assert x.grad is not None
+
+
 # ---- streams and graphs ----------------------------------------------------------------------
 
 

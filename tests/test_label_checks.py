@@ -212,3 +212,42 @@ def test_temperature_without_a_reciprocal():
     keep, p = _memory()
     _refused(_lib.lib().sdf_label_log_probs(0, p, 3, 7, 7, 0, p, 0, 1e-39, p, p, None, None, None, p,
                                             1024, None), b"temperature must be positive and finite")
+
+
+def test_tangents_are_refused():
+    """A dual tensor has requires_grad False; its tangent must not be lost without a word,
+    with the recording of gradients on or off.  The same tensors pass outside of a level and
+    as primals."""
+    from torch.autograd import forward_ad
+
+    table, z, j, t, w = torch.zeros(5, 4), torch.zeros(3, 7), ids(3, 2), torch.zeros(3, 2), torch.ones(3)
+    calls = {  # arguments that derivatives reach, by name
+        "cell_rows": (lambda x: sdfoam_amd.cell_rows(x["table"], ids(3), x["weight"]),
+                      {"table": table, "weight": w}),
+        "cell_rows_backward": (
+            lambda x: sdfoam_amd.cell_rows_backward(x["rows_grad"], ids(3), 5, x["weight"],
+                                                    table=x["table"]),
+            {"rows_grad": torch.zeros(3, 4), "weight": w, "table": table}),
+        "distill_loss": (
+            lambda x: sdfoam_amd.distill_loss(x["logits"], j, x["teacher_logits"], 1.0,
+                                              x["row_weight"]),
+            {"logits": z, "teacher_logits": t, "row_weight": w}),
+        "distill_loss_and_grad": (
+            lambda x: sdfoam_amd.distill_loss_and_grad(x["logits"], j, x["teacher_logits"], 1.0,
+                                                       x["row_weight"], "none", x["loss_grad"]),
+            {"logits": z, "teacher_logits": t, "row_weight": w, "loss_grad": w.clone()}),
+        "label_log_probs": (lambda x: sdfoam_amd.label_log_probs(x["logits"], ids(3)),
+                            {"logits": z}),
+    }
+    for call, (f, plain) in calls.items():
+        for name in plain:
+            for enabled in (True, False):
+                with forward_ad.dual_level(), torch.set_grad_enabled(enabled):
+                    dual = forward_ad.make_dual(plain[name], torch.ones_like(plain[name]))
+                    with pytest.raises(RuntimeError, match=f"{call} has no forward-mode "
+                                                           f"derivative for {name}: detach it"):
+                        f({**plain, name: dual})
+                    with pytest.raises(RuntimeError, match="must be on CUDA device"):
+                        f({**plain, name: dual.detach()})
+        with pytest.raises(RuntimeError, match="must be on CUDA device"):
+            f(plain)
