@@ -236,7 +236,7 @@ def cell_rows_backward(rows_grad: torch.Tensor, cells: torch.Tensor, num_cells: 
 
     rows_grad [*cells.shape, D]; table_grad [num_cells, D] of its type, zeros for cells that
     no id names; weight_grad (float32, the shape of ``cells``) where ``table`` is given,
-    else None."""
+    else None.  Neither carries a graph."""
     _element_type("rows_grad", rows_grad)
     _id_type("cells", cells)
     if rows_grad.dim() != cells.dim() + 1 or rows_grad.shape[:-1] != cells.shape:
@@ -286,6 +286,7 @@ def _check_distill(call, logits, teacher_labels, teacher_logits, temperature, ro
         _check_float32("row_weight", row_weight, lead)
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be 'none', 'sum' or 'mean'")
+    _no_gradient(call, teacher_logits=teacher_logits, row_weight=row_weight)
     _no_tangent(call, logits=logits, teacher_logits=teacher_logits, row_weight=row_weight)
     _check_devices("logits", logits, "teacher_labels", teacher_labels, "teacher_logits",
                    teacher_logits, "row_weight", row_weight)
@@ -360,7 +361,6 @@ def distill_loss(logits: torch.Tensor, teacher_labels: torch.Tensor,
     Differentiable in ``logits``."""
     temperature = _check_distill("distill_loss", logits, teacher_labels, teacher_logits,
                                  temperature, row_weight, reduction)
-    _no_gradient("distill_loss", teacher_logits=teacher_logits, row_weight=row_weight)
     if _wants_gradient(logits):
         return _DistillLoss.apply(logits, teacher_labels, teacher_logits, temperature, row_weight,
                                   reduction)
@@ -376,7 +376,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_labels: torch.Tensor,
     logits_grad)``, logits_grad of the logits' shape and type.
 
     loss_grad (float32, the shape of the loss; default 1) is the gradient that reaches the
-    loss from above, such as a loss scale: it is applied before the gradient is rounded."""
+    loss from above, such as a loss scale: it is applied before the gradient is rounded.
+    Neither result carries a graph."""
     _no_tangent("distill_loss_and_grad", loss_grad=loss_grad)
     temperature = _check_distill("distill_loss_and_grad", logits, teacher_labels, teacher_logits,
                                  temperature, row_weight, reduction)

@@ -251,3 +251,16 @@ def test_tangents_are_refused():
                         f({**plain, name: dual.detach()})
         with pytest.raises(RuntimeError, match="must be on CUDA device"):
             f(plain)
+
+
+@pytest.mark.parametrize("call", [sdfoam_amd.distill_loss, sdfoam_amd.distill_loss_and_grad])
+def test_distill_refuses_what_it_has_no_gradient_for(call):
+    z, j, t, w = torch.zeros(3, 7), ids(3, 2), torch.zeros(3, 2), torch.ones(3)
+    for name, leaf in (("teacher_logits", t), ("row_weight", w)):
+        args = {"teacher_logits": t, "row_weight": w, name: leaf.clone().requires_grad_()}
+        with pytest.raises(RuntimeError, match=f"{call.__name__} has no gradient for {name}: detach it"):
+            call(z, j, **args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="logits must be on CUDA device"):
+            call(z, j, **args)
+    with pytest.raises(RuntimeError, match="logits must be on CUDA device"):
+        call(z.requires_grad_(), j, t, 1.0, w)
