@@ -636,7 +636,8 @@ int sdf_cell_rows(int type, const void *table, uint64_t table_stride,
  * row written: zeros for cells that no id names; NULL: not wanted) and, where
  * weight_grad is not NULL, weight_grad[i] = scale * <table[cells[i], :], rows_grad[i, :]> (fp32, 0
  * for no cell; table is read for it only).  Each cell's rows are summed in fp32
- * in an order that the ids alone decide. */
+ * in an order that the ids alone decide.  Scratch is for table_grad; without it
+ * none is asked for. */
 size_t sdf_cell_rows_backward_scratch_bytes(uint64_t num_cells, uint32_t width,
                                             uint64_t count);
 int sdf_cell_rows_backward(int type, const void *rows_grad,

@@ -842,17 +842,19 @@ int sdf_cell_rows_backward(int type, const void *rows_grad, uint64_t rows_grad_s
     if (rc != SDF_OK) return rc;
     if (!table_grad && !weight_grad) return SDF_OK;
     if ((count > 0 && !cells) ||
-        (count > 0 && width > 0 && !rows_grad) || !scratch ||
+        (count > 0 && width > 0 && !rows_grad) || (table_grad && !scratch) ||
         (weight_grad && num_cells > 0 && width > 0 && !table))
         return fail(SDF_E_INVALID, "NULL pointer argument");
-    const size_t need = sdf_cell_rows_backward_scratch_bytes(num_cells, width, count);
+    // (the weights' gradient by itself needs no scratch)
+    const size_t need =
+        table_grad ? sdf_cell_rows_backward_scratch_bytes(num_cells, width, count) : 0;
     if (scratch_bytes < need)
         return fail(SDF_E_INVALID, "scratch must hold %zu bytes (got %zu)", need, scratch_bytes);
     const size_t e_size = type_bytes(type);
     if (misaligned(rows_grad, e_size) || misaligned(table, e_size) || misaligned(table_grad, e_size))
         return fail(SDF_E_INVALID,
                     "cell_rows_backward: rows and tables must be aligned to their elements");
-    if (misaligned(scratch, 256)) return fail(SDF_E_INVALID, "scratch must be 256-byte aligned");
+    if (table_grad && misaligned(scratch, 256)) return fail(SDF_E_INVALID, "scratch must be 256-byte aligned");
     hipStream_t s = static_cast<hipStream_t>(stream);
     const uint32_t n = (uint32_t)count, cells_n = (uint32_t)num_cells;
     const uint32_t pieces = pieces_of(type, width);

@@ -184,7 +184,9 @@ def _rows_backward(rows_grad, cells, num_cells, weight, scale, table, need_table
     if table is not None:
         weight_grad = torch.empty(cells.shape, dtype=torch.float32, device=dev)
     L = _lib.lib()
-    nbytes = int(L.sdf_cell_rows_backward_scratch_bytes(num_cells, width, c.numel()))
+    nbytes = 0
+    if need_table:
+        nbytes = int(L.sdf_cell_rows_backward_scratch_bytes(num_cells, width, c.numel()))
     keep, base = _scratch(nbytes, dev)
     _call(L.sdf_cell_rows_backward, g, _TYPES[rows_grad.dtype], ptr(g), g.stride(0), ptr(t),
           0 if t is None else t.stride(0), num_cells, width, _ID_TYPES[cells.dtype], ptr(c),

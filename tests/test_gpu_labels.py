@@ -323,6 +323,24 @@ def test_rows_of_more_than_one_launch(dev):
     near(w.grad, prod.sum(1), 6 * U * prod.abs().sum(1))
 
 
+def test_weights_gradient_alone_takes_no_workspace(dev):
+    """The weights' gradient by itself allocates that gradient and nothing beside it."""
+    g = torch.Generator().manual_seed(6)
+    table, up = torch.randn((50, 512), generator=g), torch.randn((20_000, 512), generator=g)
+    ids = torch.randint(-1, 50, (20_000,), generator=g)
+    w = torch.rand(20_000, generator=g).to(dev).requires_grad_()
+    out = sdfoam_amd.cell_rows(table.to(dev), ids.to(dev), w)
+    ud = up.to(dev)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out.backward(ud)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before <= 4 * 20_000 + 4096
+    prod = torch.where((ids >= 0)[:, None], table[ids.clamp(min=0)].double(), 0.0) * up.double()
+    near(w.grad, prod.sum(1), 515 * U * prod.abs().sum(1))
+
+
 # ---- logits ------------------------------------------------------------------------------
 
 

@@ -264,3 +264,16 @@ def test_distill_refuses_what_it_has_no_gradient_for(call):
             call(z, j, **args)
     with pytest.raises(RuntimeError, match="logits must be on CUDA device"):
         call(z.requires_grad_(), j, t, 1.0, w)
+
+
+def test_c_weights_gradient_takes_no_scratch():
+    L = _lib.lib()
+    keep, p = _memory()
+
+    def back(table_grad, scratch, nbytes):  # of no ids: nothing is launched for the weights
+        return L.sdf_cell_rows_backward(0, p, 4, p, 4, 5, 4, 0, p, 0, None, 1.0, table_grad, p, scratch,
+                                        nbytes, None)
+
+    assert back(None, None, 0) != _lib.SDF_E_INVALID
+    _refused(back(p, None, 1 << 20), b"NULL pointer")
+    _refused(back(p, p, 0), b"scratch must hold")
