@@ -169,7 +169,7 @@ struct DistillArgs {
     int teacher_type;
     const void *teacher_logits;
     uint32_t top;
-    float temperature, inv_t, c; // T, 1 / T, log2(e) / T
+    float temperature, c; // T, log2(e) / T
     const float *row_weight;   // NULL: 1
     const float *loss_grad;    // NULL: 1
     uint32_t loss_grad_stride; // 0: one for all rows
@@ -237,7 +237,10 @@ __device__ __forceinline__ Teacher teacher_of(const DistillArgs &a, const Entrie
     return t;
 }
 // The entries' logits become their shares, by the kLanes lanes of one group
-// (when every other has read them), and sum q (log q - log p) over them.
+// (when every other has read them), and T sum q (log q - log p) over them, the
+// row's loss over u T.  (The T goes into the sum: what it multiplies is a
+// difference of logits over T, and T^2 by itself is 0 or infinite in fp32 for
+// temperatures below 1e-23 and above 1e19.)
 template <int kLanes>
 __device__ __forceinline__ float shares(const DistillArgs &a, const Entries &e, const Teacher &t,
                                         const Part &st) {
@@ -247,7 +250,7 @@ __device__ __forceinline__ float shares(const DistillArgs &a, const Entries &e, 
         const float d = e.q[k] - t.m, q = __builtin_amdgcn_exp2f(d * a.c) / t.s;
         // an entry of no mass adds nothing, whatever its label's probability
         if (e.id[k] >= 0 && !(q == 0.0f))
-            sum += q * (d * a.inv_t - log_ts - ((e.z[k] - st.m) * a.inv_t - log_s));
+            sum += q * (d - (e.z[k] - st.m) + a.temperature * (log_s - log_ts));
         e.q[k] = q;
     }
     return group_sum<kLanes>(sum);
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(kThreads)
     const bool live = !(st.s == 0.0f);
     if (a.stats && threadIdx.x == 0) a.stats[r] = make_float2(st.m, st.s);
     if (threadIdx.x < 64u) {
-        const float loss = live ? u * a.temperature * a.temperature * shares<64>(a, e, t, st) : 0.0f;
+        const float loss = live ? u * a.temperature * shares<64>(a, e, t, st) : 0.0f;
         if (threadIdx.x == 0) a.loss[r] = loss;
     }
     if constexpr (kHeld > 0) {
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(kStream) void finish_kernel(DistillArgs a, uint32_t
     }
     const bool live = !(st.s == 0.0f);
     if (threadIdx.x < 64u) {
-        const float loss = live ? u * a.temperature * a.temperature * shares<64>(a, e, t, st) : 0.0f;
+        const float loss = live ? u * a.temperature * shares<64>(a, e, t, st) : 0.0f;
         if (parts && begin == 0 && threadIdx.x == 0) {
             a.loss[r] = loss;
             if (a.stats) a.stats[r] = make_float2(live ? st.m : 0.0f, st.s);
@@ -500,7 +503,7 @@ __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs a, uint6
     const bool live = !(st.s == 0.0f);
     if (live) {
         const float sum = shares<kLanes>(a, e, t, st);
-        if (!kHaveStats && l == 0) a.loss[r] = u * a.temperature * a.temperature * sum;
+        if (!kHaveStats && l == 0) a.loss[r] = u * a.temperature * sum;
     } else if (!kHaveStats && in && l == 0) {
         a.loss[r] = 0.0f;
     }
@@ -1295,8 +1298,8 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
     const bool none = reduction == SDF_REDUCE_NONE;
     const float reduce = reduction == SDF_REDUCE_MEAN ? (float)(1.0 / (double)rows) : 1.0f;
     DistillArgs a = {logits, stride, (uint32_t)labels, id_type, teacher_labels, teacher_type,
-                     teacher_logits, top, temperature, 1.0f / temperature,
-                     1.0f / temperature * kLog2e, row_weight, loss_grad, none ? 1u : 0u,
+                     teacher_logits, top, temperature, 1.0f / temperature * kLog2e, row_weight,
+                     loss_grad, none ? 1u : 0u,
                      reduce, none ? loss : static_cast<float *>(scratch),
                      reinterpret_cast<float2 *>(stats), logits_grad};
     Part *parts = reinterpret_cast<Part *>(static_cast<char *>(scratch) +
@@ -1329,8 +1332,8 @@ int sdf_distill_backward(int type, const void *logits, uint64_t rows, uint64_t l
     if (!loss_grad || !stats || !logits_grad) return fail(SDF_E_INVALID, "NULL pointer argument");
     const float reduce = reduction == SDF_REDUCE_MEAN ? (float)(1.0 / (double)rows) : 1.0f;
     DistillArgs a = {logits, stride, (uint32_t)labels, id_type, teacher_labels, teacher_type,
-                     teacher_logits, top, temperature, 1.0f / temperature,
-                     1.0f / temperature * kLog2e, row_weight, loss_grad,
+                     teacher_logits, top, temperature, 1.0f / temperature * kLog2e, row_weight,
+                     loss_grad,
                      reduction == SDF_REDUCE_NONE ? 1u : 0u, reduce, nullptr,
                      reinterpret_cast<float2 *>(const_cast<float *>(stats)), logits_grad};
     with_type(type, [&](auto t) {

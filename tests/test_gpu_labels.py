@@ -879,6 +879,29 @@ def test_tangents_that_reach_a_backward(dev):
         assert x.grad is not None
 
 
+@pytest.mark.parametrize("labels", [40, 5003, 70_001])
+def test_distill_far_temperatures(dev, labels):
+    """Temperatures whose square fp32 does not hold, or barely: the loss is that of the
+    formula where fp32 holds it."""
+    say("distill, far temperatures", labels)
+    z, g = logits_case(5, labels, torch.float32)
+    ids = torch.randint(labels, (5, 6), generator=g)
+    t = torch.randn((5, 6), generator=g)
+    weight = torch.tensor([1.0, 0.5, 0.0, 2.0, 1.5])
+    for temperature in (1e-36, 1e-30, 1e-20, 1e10, 1e18):
+        loss, grad, lt, gt = distill_reference(z, ids, t, temperature, weight, "none")
+        args = (z.to(dev), ids.to(dev), t.to(dev), temperature, weight.to(dev), "none")
+        got, dz = sdfoam_amd.distill_loss_and_grad(*args)
+        near(got, loss, lt)
+        near(dz, grad, gt)
+        near(sdfoam_amd.distill_loss(*args), loss, lt)
+    # one label: no distance, at any temperature
+    one = torch.zeros((3, 1), dtype=torch.int64, device=dev)
+    for temperature in (1e-38, 1e20, 3e38):
+        loss, dz = sdfoam_amd.distill_loss_and_grad(one + 2.5, one, one.float(), temperature)
+        assert float(loss) == 0 and not dz.any()
+
+
 # ---- streams and graphs ----------------------------------------------------------------------
 
 
