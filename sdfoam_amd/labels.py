@@ -42,6 +42,7 @@ _REDUCTIONS = {"none": _lib.SDF_REDUCE_NONE, "sum": _lib.SDF_REDUCE_SUM,
 
 MAX_TEACHER = 1024  # a teacher's logits per row
 MAX_TOP = 64  # best labels per row
+MAX_WIDTH = 1 << 18  # elements of a cell's row
 
 
 def _element_type(name: str, t: torch.Tensor) -> int:
@@ -153,6 +154,11 @@ def _scratch(nbytes: int, device: torch.device):
 # ---- rows of cells ------------------------------------------------------------------------
 
 
+def _check_width(call: str, width: int) -> None:
+    if width > MAX_WIDTH:  # here: the library's argument has 32 bits
+        raise RuntimeError(f"{call} takes rows of at most 2^18 elements")
+
+
 def _check_weight(weight, cells) -> None:
     if weight is not None:
         _check_float32("weight", weight, cells.shape)
@@ -223,6 +229,7 @@ def cell_rows(table: torch.Tensor, cells: torch.Tensor, weight: Optional[torch.T
         raise RuntimeError("table must have 2 dimensions")
     _element_type("table", table)
     _id_type("cells", cells)
+    _check_width("cell_rows", table.size(1))
     _check_weight(weight, cells)
     _no_tangent("cell_rows", table=table, weight=weight)
     _check_devices("table", table, "cells", cells, "weight", weight)
@@ -244,6 +251,7 @@ def cell_rows_backward(rows_grad: torch.Tensor, cells: torch.Tensor, num_cells: 
     if rows_grad.dim() != cells.dim() + 1 or rows_grad.shape[:-1] != cells.shape:
         raise RuntimeError(f"rows_grad had shape {list(rows_grad.shape)}, "
                            f"expected {list(cells.shape)} and a last dimension")
+    _check_width("cell_rows_backward", rows_grad.size(-1))
     num_cells = int(num_cells)
     if num_cells < 0:
         raise RuntimeError("num_cells must not be negative")

@@ -277,3 +277,18 @@ def test_c_weights_gradient_takes_no_scratch():
     assert back(None, None, 0) != _lib.SDF_E_INVALID
     _refused(back(p, None, 1 << 20), b"NULL pointer")
     _refused(back(p, p, 0), b"scratch must hold")
+
+
+@pytest.mark.parametrize("width", [(1 << 18) + 1, (1 << 32) + 4])
+def test_rows_too_wide(width):
+    """Also where the width's lower 32 bits alone would be a width."""
+    wide = torch.zeros(1, 1).expand(1, width)
+    with pytest.raises(RuntimeError, match=r"cell_rows takes rows of at most 2\^18 elements"):
+        sdfoam_amd.cell_rows(wide, ids(1))
+    with pytest.raises(RuntimeError, match=r"cell_rows_backward takes rows of at most 2\^18 elements"):
+        sdfoam_amd.cell_rows_backward(wide, ids(1), 3)
+    fits = wide[:, :1 << 18]
+    with pytest.raises(RuntimeError, match="table must be on CUDA device"):
+        sdfoam_amd.cell_rows(fits, ids(1))
+    with pytest.raises(RuntimeError, match="rows_grad must be on CUDA device"):
+        sdfoam_amd.cell_rows_backward(fits, ids(1), 3)
