@@ -510,7 +510,8 @@ __device__ __forceinline__ void sum_tile(const SumsArgs &a, uint32_t tile, uint3
                 for (int e = 0; e < kP; ++e)
                     if ((uint32_t)e >= own) s = fmaf((float)g[b].v[e], (float)t[b].v[e], s);
                 s = group_sum<kLanes>(s);
-                if (l == b % kLanes && p + b < p1) a.weight_grad[index[b]] = a.scale * s;
+                if (l == b % kLanes && p + b < p1) // (no cell: 0 whatever the scale)
+                    a.weight_grad[index[b]] = key[b] < a.num_cells ? a.scale * s : 0.0f;
             }
         }
 #pragma unroll
@@ -689,7 +690,8 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(RowsArgs a, const T *_
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         const float sum = group_sum<kLanes>(s[u]);
-        if (l == u % kLanes && first + u < end) weight_grad[first + u] = a.scale * sum;
+        if (l == u % kLanes && first + u < end) // (no cell: 0 whatever the scale)
+            weight_grad[first + u] = cell[u] < 0 ? 0.0f : a.scale * sum;
     }
 }
 

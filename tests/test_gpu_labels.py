@@ -341,6 +341,23 @@ def test_weights_gradient_alone_takes_no_workspace(dev):
     near(w.grad, prod.sum(1), 515 * U * prod.abs().sum(1))
 
 
+@pytest.mark.parametrize("width", [3, 64, 1000])
+def test_rows_of_no_cell_at_any_scale(dev, width):
+    """A scale that has overflown reaches the rows of cells, and those of no cell stay 0."""
+    ids = torch.tensor([1, -1, 0, 7, -1], device=dev)
+    none = (ids < 0) | (ids >= 4)
+    table, up = torch.ones((4, width), device=dev), torch.ones((5, width), device=dev)
+    for scale in (math.inf, math.nan):
+        w = torch.ones(5, device=dev).requires_grad_()
+        out = sdfoam_amd.cell_rows(table, ids, w, scale)
+        assert not out[none].any() and not out[~none].isfinite().any()
+        out.backward(up)  # the weights' gradient by itself
+        tg, wg = sdfoam_amd.cell_rows_backward(up, ids, 4, w.detach(), scale, table=table)
+        for x in (wg, w.grad):
+            assert not x[none].any() and not x[~none].isfinite().any()
+        assert not tg[2:].any() and not tg[:2].isfinite().any()
+
+
 # ---- logits ------------------------------------------------------------------------------
 
 
