@@ -130,8 +130,10 @@ constexpr uint32_t kSortWaves = kSortThreads / 64;
 constexpr uint32_t kSteps = 4;                       // keys per thread
 constexpr uint32_t kTile = kSteps * kSortThreads;    // keys of one block
 // One block sorts up to a tile alone, and up to kOneBlock keys where the clearing
-// beside it takes as long (see below): 16,381 ids in 65,536 cells, 67 MB of them 53 us
-// for 43 with several blocks, 134 MB 65 for 57, 201 MB 76 for 75, 268 MB 86 for 91.
+// beside it takes as long.  Several blocks for one there: 6,000 ids in 1M cells of 49
+// floats 62 -> 50 us, 12,000 in 1M of 64 71 -> 66, 16,384 in 2M of 64 108 -> 100; rows
+// of 2,048 halves, 8,000 ids in 65,536 cells 94 -> 88, 16,381 98 -> 92, but 16,384 in
+// 65,429 85 -> 89; beside 134 MB, below the limit, 10,000 64 -> 64, 16,384 69 -> 75.
 constexpr uint32_t kOneBlock = 16 * kSortThreads;
 constexpr uint64_t kOneBlockClears = 192ull << 20;
 constexpr uint32_t kMaxBits = 11;                    // of a digit

@@ -358,6 +358,30 @@ def test_rows_of_no_cell_at_any_scale(dev, width):
         assert not tg[2:].any() and not tg[:2].isfinite().any()
 
 
+@pytest.mark.parametrize("count", [4096, 4097, 10_001, 16_383, 16_384, 16_385])
+def test_rows_gradient_beside_a_large_table(dev, count):
+    """Whole numbers, so that every sum is exact.  50,000 x 1,024 floats are cleared (195
+    MiB): beside so much one block sorts up to 16,384 ids, 16 a thread."""
+    say("rows, one block beside a large table", count)
+    g = torch.Generator().manual_seed(count)
+    cells, width = 50_000, 1024
+    up = torch.randint(-9, 10, (count, width), generator=g).float()
+    weight = torch.randint(1, 4, (count,), generator=g).float()
+    few = torch.randint(3, (count,), generator=g) * 20_000
+    for ids in (torch.randint(-1, cells, (count,), generator=g),
+                torch.where(torch.rand(count, generator=g) < 0.6, few,
+                            torch.randint(-3000, cells, (count,), generator=g)),
+                torch.arange(count).flip(0) * 3, torch.full((count,), cells - 1)):
+        for w in (None, weight):
+            got, _ = sdfoam_amd.cell_rows_backward(up.to(dev), ids.to(dev), cells,
+                                                   None if w is None else w.to(dev))
+            live = ids >= 0
+            sums = torch.zeros((cells, width), device=dev)
+            terms = up if w is None else up * w[:, None]
+            sums.index_add_(0, ids[live].to(dev), terms[live].to(dev))
+            assert torch.equal(got, sums)
+
+
 # ---- logits ------------------------------------------------------------------------------
 
 
