@@ -1130,13 +1130,21 @@ template <typename F> void with_short(uint64_t chunks, F f) {
     else f(Int<64>(), Int<4>());
 }
 
+constexpr size_t kEntriesLds = 32768; // of a block of short rows
+
 template <typename T, bool kHaveStats>
 void launch_short(const DistillArgs &a, uint64_t rows, hipStream_t s) {
-    with_short(chunks_of<T>(a.logits, a.stride, a.labels), [&](auto lanes, auto held) {
+    const size_t row_bytes = kEntryBytes * (size_t)a.top;
+    // At least as many lanes a row as leave a wavefront's rows that room for their
+    // teacher's entries: 8 up to 341 of them, 16 up to 682, then 32 (20,000 rows of 20
+    // floats at 8 lanes: 400 entries 186 -> 124 us, 700 550 -> 171, 1,024 1,470 -> 332).
+    uint64_t chunks = chunks_of<T>(a.logits, a.stride, a.labels);
+    if (64 / 16 * row_bytes > kEntriesLds) chunks = chunks > 33 ? chunks : 33;
+    else if (64 / 8 * row_bytes > kEntriesLds) chunks = chunks > 9 ? chunks : 9;
+    with_short(chunks, [&](auto lanes, auto held) {
         constexpr uint32_t kLanes = decltype(lanes)::v;
-        const size_t row_bytes = kEntryBytes * (size_t)a.top;
         uint32_t threads = 256; // fewer where the teacher's entries fill LDS
-        while (threads > 64 && threads / kLanes * row_bytes > 32768) threads /= 2;
+        while (threads > 64 && threads / kLanes * row_bytes > kEntriesLds) threads /= 2;
         const uint64_t per = threads / kLanes;
         hipLaunchKernelGGL((distill_short_kernel<T, kLanes, decltype(held)::v, kHaveStats>),
                            dim3((unsigned)((rows + per - 1) / per)), dim3(threads),

@@ -943,6 +943,27 @@ def test_distill_far_temperatures(dev, labels):
         assert float(loss) == 0 and not dz.any()
 
 
+@pytest.mark.parametrize("top", [341, 342, 682, 683, 1024])
+def test_distill_more_entries_than_labels(dev, top):
+    """Short rows whose teacher's entries fill LDS: labels named often, entries that name
+    none, and rows that end inside a block."""
+    say("distill, more entries than labels", top)
+    for dtype, sizes in ((torch.float32, (1, 5, 31, 32, 33, 100)), (torch.bfloat16, (64, 120))):
+        for labels in sizes:
+            for rows in (1, 77):
+                z, g = logits_case(rows, labels, dtype, seed=top)
+                ids, t = teacher_case(rows, labels, top, g)
+                loss, grad, lt, gt = distill_reference(z, ids, t, 1.5, None, "none")
+                zd = z.to(dev).requires_grad_()
+                args = (ids.to(dev), t.to(dev), 1.5, None, "none")
+                got, dz = sdfoam_amd.distill_loss_and_grad(zd.detach(), *args)
+                near(got, loss, lt)
+                # (a sum of up to `top` shares: as above)
+                near(dz, grad, gt * (1 + top / 64), dtype)
+                sdfoam_amd.distill_loss(zd, *args).backward(torch.ones(rows, device=dev))
+                near(zd.grad, grad, gt * (1 + top / 64), dtype)
+
+
 # ---- streams and graphs ----------------------------------------------------------------------
 
 
