@@ -296,7 +296,8 @@ def _check_distill(call, logits, teacher_labels, teacher_logits, temperature, ro
         _check_float32("row_weight", row_weight, lead)
     if reduction not in _REDUCTIONS:
         raise RuntimeError("reduction must be 'none', 'sum' or 'mean'")
-    _no_gradient(call, teacher_logits=teacher_logits, row_weight=row_weight)
+    if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
+        _no_gradient(call, teacher_logits=teacher_logits, row_weight=row_weight)
     _no_tangent(call, logits=logits, teacher_logits=teacher_logits, row_weight=row_weight)
     _check_devices("logits", logits, "teacher_labels", teacher_labels, "teacher_logits",
                    teacher_logits, "row_weight", row_weight)
@@ -388,7 +389,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_labels: torch.Tensor,
     loss_grad (float32, the shape of the loss; default 1) is the gradient that reaches the
     loss from above, such as a loss scale: it is applied before the gradient is rounded.
     Neither result carries a graph."""
-    _no_tangent("distill_loss_and_grad", loss_grad=loss_grad)
+    if loss_grad is not None:
+        _no_tangent("distill_loss_and_grad", loss_grad=loss_grad)
     temperature = _check_distill("distill_loss_and_grad", logits, teacher_labels, teacher_logits,
                                  temperature, row_weight, reduction)
     if loss_grad is not None:
