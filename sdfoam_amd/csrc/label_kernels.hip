@@ -1241,7 +1241,7 @@ size_t sum_bytes(uint64_t rows) {
 }
 
 int check_logits(const char *what, int type, const void *logits, uint64_t rows, uint64_t labels,
-                 uint64_t stride, int id_type, float temperature) {
+                 int id_type, float temperature) {
     if (!known_type(type)) return fail(SDF_E_INVALID, "%s: unknown element type %d", what, type);
     if (!known_id_type(id_type)) return fail(SDF_E_INVALID, "%s: unknown id type %d", what, id_type);
     if (labels == 0 || labels >= (1ull << 31))
@@ -1251,16 +1251,15 @@ int check_logits(const char *what, int type, const void *logits, uint64_t rows, 
         return fail(SDF_E_INVALID, "%s: temperature must be positive and finite, as its reciprocal",
                     what);
     if (rows > 0 && !logits) return fail(SDF_E_INVALID, "NULL pointer argument");
-    (void)stride;
     if ((reinterpret_cast<uintptr_t>(logits) & (type_bytes(type) - 1)) != 0)
         return fail(SDF_E_INVALID, "%s: logits must be aligned to their elements", what);
     return SDF_OK;
 }
 
 int check_distill(const char *what, int type, const void *logits, uint64_t rows, uint64_t labels,
-                  uint64_t stride, int id_type, const void *teacher_labels, int teacher_type,
+                  int id_type, const void *teacher_labels, int teacher_type,
                   const void *teacher_logits, uint32_t top, float temperature, int reduction) {
-    const int rc = check_logits(what, type, logits, rows, labels, stride, id_type, temperature);
+    const int rc = check_logits(what, type, logits, rows, labels, id_type, temperature);
     if (rc != SDF_OK) return rc;
     if (!known_type(teacher_type))
         return fail(SDF_E_INVALID, "%s: unknown element type %d", what, teacher_type);
@@ -1291,7 +1290,7 @@ int sdf_distill(int type, const void *logits, uint64_t rows, uint64_t labels, ui
                 const float *row_weight, int reduction, const float *loss_grad, float *loss,
                 float *stats, void *logits_grad, void *scratch, size_t scratch_bytes,
                 void *stream) {
-    const int rc = check_distill("distill", type, logits, rows, labels, stride, id_type,
+    const int rc = check_distill("distill", type, logits, rows, labels, id_type,
                                  teacher_labels, teacher_type, teacher_logits, top, temperature,
                                  reduction);
     if (rc != SDF_OK) return rc;
@@ -1332,7 +1331,7 @@ int sdf_distill_backward(int type, const void *logits, uint64_t rows, uint64_t l
                          float temperature, const float *row_weight, int reduction,
                          const float *loss_grad, const float *stats, void *logits_grad,
                          void *stream) {
-    const int rc = check_distill("distill_backward", type, logits, rows, labels, stride, id_type,
+    const int rc = check_distill("distill_backward", type, logits, rows, labels, id_type,
                                  teacher_labels, teacher_type, teacher_logits, top, temperature,
                                  reduction);
     if (rc != SDF_OK) return rc;
@@ -1368,8 +1367,7 @@ int sdf_label_log_probs(int type, const void *logits, uint64_t rows, uint64_t la
                         float temperature, float *log_prob, float *entropy, float *top_log_probs,
                         int64_t *top_labels, float *stats, void *scratch, size_t scratch_bytes,
                         void *stream) {
-    const int rc = check_logits("label_log_probs", type, logits, rows, labels, stride, id_type,
-                                temperature);
+    const int rc = check_logits("label_log_probs", type, logits, rows, labels, id_type, temperature);
     if (rc != SDF_OK) return rc;
     if (top > kMaxTop)
         return fail(SDF_E_INVALID, "label_log_probs returns at most %u best labels", kMaxTop);
@@ -1401,8 +1399,8 @@ int sdf_label_log_probs_backward(int type, const void *logits, uint64_t rows, ui
                                  float temperature, const float *entropy, const float *stats,
                                  const float *log_prob_grad, const float *entropy_grad,
                                  void *logits_grad, void *stream) {
-    const int rc = check_logits("label_log_probs_backward", type, logits, rows, labels, stride,
-                                id_type, temperature);
+    const int rc = check_logits("label_log_probs_backward", type, logits, rows, labels, id_type,
+                                temperature);
     if (rc != SDF_OK) return rc;
     if (rows == 0) return SDF_OK;
     if (!label_ids || !entropy || !stats || !logits_grad)
