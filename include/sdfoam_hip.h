@@ -700,6 +700,125 @@ int sdf_label_log_probs_backward(int type, const void *logits, uint64_t rows,
                                  const float *entropy_grad, void *logits_grad,
                                  void *stream);
 
+/* ---- heads of label fields (no counterpart in the reference) ----------
+ *
+ * What a label field's head needs beyond one linear layer: rows in the order of
+ * the experts that a router chose for them, the experts' products, a shared
+ * projection with a low-rank adapter of each row's own beside it, and the
+ * gradients of all of these.  Types, ids, strides and scratch as above; every
+ * sum is held in fp32, and its order is the same on every run. */
+#define SDF_MAX_EXPERTS 2048u
+#define SDF_MAX_ADAPTERS 2048u
+#define SDF_MAX_RANK 256u
+
+/* The order of `count` entries (row i's k-th choice is entry choices * i + k) by
+ * expert, those of one expert as they came: places[e] is where entry e stands,
+ * or -1 - place for an entry that names no expert (those stand last), and
+ * offsets [num_experts + 1] where each expert's begin; offsets[num_experts]
+ * entries name one.  Fewer than 2^31 entries. */
+size_t sdf_expert_order_scratch_bytes(uint64_t count, uint32_t num_experts);
+int sdf_expert_order(int id_type, const void *experts, uint64_t count,
+                     uint32_t num_experts, int32_t *places, int32_t *offsets,
+                     void *scratch, size_t scratch_bytes, void *stream);
+
+/* sorted[places[choices * i + k], :] = rows[i, :] for the count rows; zeros at
+ * the places of entries that name no expert.  sorted [count * choices, width] is
+ * contiguous; places outside of it are left out. */
+int sdf_expert_rows(int type, const void *rows, uint64_t rows_stride,
+                    uint64_t count, uint32_t choices, uint32_t width,
+                    const int32_t *places, void *sorted, void *stream);
+
+/* out[i, :] = sum over k of weight[i, k] * sorted[places[choices * i + k], :],
+ * entries that name no expert left out (weight NULL: 1).  out contiguous. */
+int sdf_expert_combine(int type, const void *sorted, uint64_t sorted_stride,
+                       uint64_t count, uint32_t choices, uint32_t width,
+                       const int32_t *places, const float *weight, void *out,
+                       void *stream);
+
+/* Gradients of sdf_expert_combine: sorted_grad (contiguous; zeros at the places
+ * of entries that name no expert) and weight_grad [count, choices], either NULL
+ * where it is not wanted; sorted is read for weight_grad only. */
+int sdf_expert_combine_backward(int type, const void *out_grad,
+                                uint64_t out_grad_stride, const void *sorted,
+                                uint64_t sorted_stride, uint64_t count,
+                                uint32_t choices, uint32_t width,
+                                const int32_t *places, const float *weight,
+                                void *sorted_grad, float *weight_grad,
+                                void *stream);
+
+/* out[p, :] = rows[p, :] weight[g]^T for the places p of expert g, offsets[g] to
+ * offsets[g + 1]; zeros for those past offsets[num_experts].  rows [count, width],
+ * weight [num_experts, out_width, width] and out [count, out_width] contiguous
+ * but for the rows' stride; offsets on the device, ascending from 0 (what they
+ * hold past `count` is taken for count). */
+size_t sdf_expert_linear_scratch_bytes(uint64_t count, uint32_t num_experts,
+                                       uint32_t width, uint32_t out_width);
+int sdf_expert_linear(int type, const void *rows, uint64_t rows_stride,
+                      uint64_t count, uint32_t num_experts, uint32_t width,
+                      uint32_t out_width, const void *weight,
+                      const int32_t *offsets, void *out, void *scratch,
+                      size_t scratch_bytes, void *stream);
+
+/* Gradients of sdf_expert_linear, either NULL where it is not wanted: rows_grad
+ * (zeros past offsets[num_experts]) and weight_grad (zeros for an expert without
+ * rows). */
+size_t sdf_expert_linear_backward_scratch_bytes(uint64_t count,
+                                                uint32_t num_experts,
+                                                uint32_t width,
+                                                uint32_t out_width);
+int sdf_expert_linear_backward(int type, const void *out_grad,
+                               uint64_t out_grad_stride, const void *rows,
+                               uint64_t rows_stride, uint64_t count,
+                               uint32_t num_experts, uint32_t width,
+                               uint32_t out_width, const void *weight,
+                               const int32_t *offsets, void *rows_grad,
+                               void *weight_grad, void *scratch,
+                               size_t scratch_bytes, void *stream);
+
+/* out[i, :] = weight rows[i, :] + scale * up[a] (down[a] rows[i, :]), a the
+ * adapter that adapters[i] names; the first term alone where it names none.
+ * weight [out_width, width], down [num_adapters, rank, width], up [num_adapters,
+ * out_width, rank]. */
+size_t sdf_adapter_linear_scratch_bytes(uint64_t count, uint32_t width,
+                                        uint32_t out_width,
+                                        uint32_t num_adapters, uint32_t rank);
+int sdf_adapter_linear(int type, const void *rows, uint64_t rows_stride,
+                       uint64_t count, uint32_t width, uint32_t out_width,
+                       const void *weight, uint64_t weight_stride, int id_type,
+                       const void *adapters, uint32_t num_adapters,
+                       uint32_t rank, const void *down, const void *up,
+                       float scale, void *out, void *scratch,
+                       size_t scratch_bytes, void *stream);
+
+/* Gradients of sdf_adapter_linear, each contiguous and of `type`, NULL where it is
+ * not wanted; zeros for an adapter without rows. */
+size_t sdf_adapter_linear_backward_scratch_bytes(uint64_t count, uint32_t width,
+                                                 uint32_t out_width,
+                                                 uint32_t num_adapters,
+                                                 uint32_t rank);
+int sdf_adapter_linear_backward(
+    int type, const void *out_grad, uint64_t out_grad_stride, const void *rows,
+    uint64_t rows_stride, uint64_t count, uint32_t width, uint32_t out_width,
+    const void *weight, uint64_t weight_stride, int id_type,
+    const void *adapters, uint32_t num_adapters, uint32_t rank,
+    const void *down, const void *up, float scale, void *rows_grad,
+    void *weight_grad, void *down_grad, void *up_grad, void *scratch,
+    size_t scratch_bytes, void *stream);
+
+/* *norm (on the device) = scale * the Euclidean norm of all gradients together,
+ * and, unless out is NULL, out[t] = scale * min(1, max_norm / (*norm + 1e-6)) *
+ * gradients[t].  The arrays are the host's, read before the call returns:
+ * num_tensors types, device addresses and numbers of elements (fewer than 2^40
+ * in all); out[t] of the gradient's type or float32, the gradient itself or
+ * memory that no gradient and no other result lies on.  A norm that is not
+ * finite leaves results that are not (infinite: 0 times each element; NaN: NaN). */
+size_t sdf_clip_gradients_scratch_bytes(uint32_t num_tensors);
+int sdf_clip_gradients(uint32_t num_tensors, const int *types,
+                       const void *const *gradients, const uint64_t *counts,
+                       const int *out_types, void *const *out, float max_norm,
+                       float scale, float *norm, void *scratch,
+                       size_t scratch_bytes, void *stream);
+
 /* ---- measurement and test hooks (no counterpart in the reference) ----- */
 
 /* Per-ray walk statistics of the forward (backward = 0) or backward

@@ -86,6 +86,21 @@ EXPORTS = (
     "sdf_label_log_probs_scratch_bytes",
     "sdf_label_log_probs",
     "sdf_label_log_probs_backward",
+    "sdf_expert_order_scratch_bytes",
+    "sdf_expert_order",
+    "sdf_expert_rows",
+    "sdf_expert_combine",
+    "sdf_expert_combine_backward",
+    "sdf_expert_linear_scratch_bytes",
+    "sdf_expert_linear",
+    "sdf_expert_linear_backward_scratch_bytes",
+    "sdf_expert_linear_backward",
+    "sdf_adapter_linear_scratch_bytes",
+    "sdf_adapter_linear",
+    "sdf_adapter_linear_backward_scratch_bytes",
+    "sdf_adapter_linear_backward",
+    "sdf_clip_gradients_scratch_bytes",
+    "sdf_clip_gradients",
     "sdf_trace_walk_stats",
     "sdf_debug_fpmath",
     "sdf_set_timing",
@@ -306,6 +321,39 @@ def lib() -> C.CDLL:
     L.sdf_label_log_probs_backward.restype = C.c_int
     L.sdf_label_log_probs_backward.argtypes = [C.c_int, P, U64, U64, U64, C.c_int, P, F32, P, P,
                                                P, P, P, P]
+    L.sdf_expert_order_scratch_bytes.restype = SZ
+    L.sdf_expert_order_scratch_bytes.argtypes = [U64, U32]
+    L.sdf_expert_order.restype = C.c_int
+    L.sdf_expert_order.argtypes = [C.c_int, P, U64, U32, P, P, P, SZ, P]
+    L.sdf_expert_rows.restype = C.c_int
+    L.sdf_expert_rows.argtypes = [C.c_int, P, U64, U64, U32, U32, P, P, P]
+    L.sdf_expert_combine.restype = C.c_int
+    L.sdf_expert_combine.argtypes = [C.c_int, P, U64, U64, U32, U32, P, P, P, P]
+    L.sdf_expert_combine_backward.restype = C.c_int
+    L.sdf_expert_combine_backward.argtypes = [C.c_int, P, U64, P, U64, U64, U32, U32, P, P, P, P,
+                                              P]
+    L.sdf_expert_linear_scratch_bytes.restype = SZ
+    L.sdf_expert_linear_scratch_bytes.argtypes = [U64, U32, U32, U32]
+    L.sdf_expert_linear.restype = C.c_int
+    L.sdf_expert_linear.argtypes = [C.c_int, P, U64, U64, U32, U32, U32, P, P, P, P, SZ, P]
+    L.sdf_expert_linear_backward_scratch_bytes.restype = SZ
+    L.sdf_expert_linear_backward_scratch_bytes.argtypes = [U64, U32, U32, U32]
+    L.sdf_expert_linear_backward.restype = C.c_int
+    L.sdf_expert_linear_backward.argtypes = [C.c_int, P, U64, P, U64, U64, U32, U32, U32, P, P, P,
+                                             P, P, SZ, P]
+    adapter = [P, U64, U64, U32, U32, P, U64, C.c_int, P, U32, U32, P, P, F32]
+    L.sdf_adapter_linear_scratch_bytes.restype = SZ
+    L.sdf_adapter_linear_scratch_bytes.argtypes = [U64, U32, U32, U32, U32]
+    L.sdf_adapter_linear.restype = C.c_int
+    L.sdf_adapter_linear.argtypes = [C.c_int] + adapter + [P, P, SZ, P]
+    L.sdf_adapter_linear_backward_scratch_bytes.restype = SZ
+    L.sdf_adapter_linear_backward_scratch_bytes.argtypes = [U64, U32, U32, U32, U32]
+    L.sdf_adapter_linear_backward.restype = C.c_int
+    L.sdf_adapter_linear_backward.argtypes = [C.c_int, P, U64] + adapter + [P, P, P, P, P, SZ, P]
+    L.sdf_clip_gradients_scratch_bytes.restype = SZ
+    L.sdf_clip_gradients_scratch_bytes.argtypes = [U32]
+    L.sdf_clip_gradients.restype = C.c_int
+    L.sdf_clip_gradients.argtypes = [U32, P, P, P, P, P, F32, F32, P, P, SZ, P]
     L.sdf_trace_walk_stats.restype = C.c_int
     L.sdf_trace_walk_stats.argtypes = [
         C.c_int, C.POINTER(TraceSettings), C.c_int, U32, P, P, U32, P, P, U32, P, P, P,

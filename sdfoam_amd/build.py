@@ -25,7 +25,8 @@ ARCH = os.environ.get("SDFOAM_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = ["trace_kernels.hip", "render_kernels.hip", "aabb_kernels.hip", "nn_sorted.hip", "order_kernels.hip", "delaunay_tables.hip",
            "delaunay_gpu.hip", "batch_fetcher.hip", "triangulation_kernels.hip",
-           "cell_rows.hip", "label_kernels.hip", "capi.hip"]
+           "cell_rows.hip", "label_kernels.hip", "expert_rows.hip", "products.hip",
+           "adapters.hip", "gradient_norm.hip", "capi.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

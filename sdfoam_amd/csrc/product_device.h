@@ -1,0 +1,295 @@
+// Tiles of matrix products for rows in groups: what products.hip and adapters.hip run.
+//
+// Two forms, over 128 bytes of the inner dimension at a time (64 elements of 16 bits, 32
+// floats), fp32 accumulators in the matrix units:
+//
+//   rows:     out[m, n] = sum_k a[m, k] b_g[n, k]   for the rows m of group g
+//   weights:  out_g[m, n] = sum over rows k of group g of a[k, m] b[k, n]
+//
+// Either operand may lie with k along its rows or across them; the tile in LDS always has
+// k along its rows (an operand that lies across is turned in registers on its way there),
+// so that every wave reads its fragments as 16 bytes a lane.  Chunks of 16 bytes are
+// swizzled: chunk c of row r lies at c ^ ((r ^ r >> 3) & 7), which keeps reads (32 rows,
+// the same chunk) and turned writes (every 4th or 8th row) off each other's banks.
+#pragma once
+
+#include "head_device.h"
+
+namespace sdfoam_hip {
+namespace head {
+
+using namespace label;
+
+typedef float F16x __attribute__((ext_vector_type(16)));
+typedef float F4x __attribute__((ext_vector_type(4)));
+typedef half_t H8 __attribute__((ext_vector_type(8)));
+typedef bf16_t B8 __attribute__((ext_vector_type(8)));
+
+// D[i][j] += sum over k of a's row i times b's row j, from 16 bytes a lane of each.  32x32:
+// lane l has row l % 32 and chunk l / 32 of two; 16x16: row l % 16, chunk l / 16 of four.
+// Element e of a lane's chunk meets element e of the other's, so it does not matter which
+// k of the operands the chunks are, as long as both have the same.  Lane l gets column
+// j = l % 32 (l % 16) and rows 8 (v / 4) + 4 (l / 32) + v % 4 (4 (l / 16) + v).
+template <typename T> __device__ __forceinline__ void mma32(F16x &d, const Chunk<T> &a, const Chunk<T> &b) {
+    if constexpr (__is_same(T, half_t))
+        d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), d, 0, 0, 0);
+    else if constexpr (__is_same(T, bf16_t))
+        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), d, 0, 0, 0);
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], d, 0, 0, 0);
+}
+template <typename T> __device__ __forceinline__ void mma16(F4x &d, const Chunk<T> &a, const Chunk<T> &b) {
+    if constexpr (__is_same(T, half_t))
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), d, 0, 0, 0);
+    else if constexpr (__is_same(T, bf16_t))
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), d, 0, 0, 0);
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], d, 0, 0, 0);
+}
+
+// kN elements as they lie in memory, at any address that the element type allows.
+template <typename T, int kN> struct Few {
+    T v[kN];
+};
+template <typename T, int kN> __device__ __forceinline__ Few<T, kN> load_few(const T *p) {
+    Few<T, kN> c;
+    __builtin_memcpy(&c, p, sizeof(c));
+    return c;
+}
+// the elements [0, have) of them, the others 0
+template <typename T, int kN>
+__device__ __forceinline__ Few<T, kN> load_some(const T *p, uint32_t have) {
+    if (have >= kN) return load_few<T, kN>(p);
+    Few<T, kN> c;
+#pragma unroll
+    for (uint32_t e = 0; e < kN; ++e) c.v[e] = e < have ? p[e] : (T)0.0f;
+    return c;
+}
+template <typename T, int kN>
+__device__ __forceinline__ void store_some(T *p, const Few<T, kN> &c, uint32_t have) {
+    if (have >= kN) __builtin_memcpy(p, &c, sizeof(c));
+    else
+#pragma unroll
+        for (uint32_t e = 0; e < kN; ++e)
+            if (e < have) p[e] = c.v[e];
+}
+
+// Rows of group g: [offsets[g], offsets[g + 1]); those behind the last group's are a group
+// of their own, `groups`, whose rows of the result are 0.  offsets NULL: one group has all.
+struct Groups {
+    const int32_t *offsets;
+    uint32_t groups;
+    uint32_t total; // rows
+    __device__ __forceinline__ uint32_t at(uint32_t g) const {
+        const int32_t v = offsets[g]; // whatever the caller's array holds stays in range
+        return v < 0 ? 0u : min((uint32_t)v, total);
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t g) const { return offsets ? at(g) : 0u; }
+    __device__ __forceinline__ uint32_t end(uint32_t g) const {
+        return !offsets || g == groups ? total : at(g + 1);
+    }
+};
+
+struct TileOfRows {
+    uint32_t group, first, rows; // rows [first, first + rows); group `groups`: none
+};
+
+// The `tile`-th tile of kRows rows, counted group by group; false where there are fewer.
+// Every thread of the block calls it; `lds` has room for 8 + 4 words.
+template <int kRows, int kThreads>
+__device__ __forceinline__ bool find_tile(const Groups &g, uint32_t tile, uint32_t *lds,
+                                          TileOfRows &t) {
+    if (!g.offsets) {
+        t.group = 0;
+        t.first = tile * kRows;
+        if (t.first >= g.total) return false;
+        t.rows = min((uint32_t)kRows, g.total - t.first);
+        return true;
+    }
+    const uint32_t keys = g.groups + 1;
+    const uint32_t each = (keys + kThreads - 1) / kThreads;
+    const uint32_t lo = min(threadIdx.x * each, keys), hi = min(lo + each, keys);
+    uint32_t sum = 0;
+    for (uint32_t k = lo; k < hi; ++k) {
+        const uint32_t b = g.begin(k), e = g.end(k);
+        sum += e > b ? (e - b + kRows - 1) / kRows : 0u;
+    }
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t run = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t v = __shfl_up(run, d);
+        if ((int)lane >= d) run += v;
+    }
+    if (lane == 63) lds[wave] = run;
+    if (threadIdx.x == 0) lds[8] = ~0u;
+    __syncthreads();
+    for (uint32_t w = 0; w < wave; ++w) run += lds[w];
+    if (tile < run && tile >= run - sum) {
+        uint32_t left = tile - (run - sum);
+        for (uint32_t k = lo; k < hi; ++k) {
+            const uint32_t b = g.begin(k), e = g.end(k);
+            const uint32_t n = e > b ? (e - b + kRows - 1) / kRows : 0u;
+            if (left < n) {
+                lds[8] = k;
+                lds[9] = b + left * kRows;
+                lds[10] = min((uint32_t)kRows, e - (b + left * kRows));
+                break;
+            }
+            left -= n;
+        }
+    }
+    __syncthreads();
+    t.group = lds[8];
+    t.first = lds[9];
+    t.rows = lds[10];
+    return t.group != ~0u;
+}
+// no more tiles than this
+inline uint64_t tiles_of_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t tile) {
+    const uint64_t most = (rows + tile - 1) / tile;
+    const uint64_t some = rows < (uint64_t)groups + 1 ? rows : (uint64_t)groups + 1;
+    return grouped ? most + some : most;
+}
+
+struct Operand {
+    const void *base;
+    uint64_t stride;       // between rows
+    uint64_t group_stride; // between the groups' matrices; 0: one for all
+    const int32_t *index;  // the row at a place; NULL: the place itself
+};
+
+// What a row's adapter adds to its product: sum_r inner[place, r] outer_g[n, r], g the
+// row's group (adapters.hip).
+struct Beside {
+    const float *inner; // [places][pitch]; NULL: nothing beside
+    uint32_t rank, pitch;
+    const void *outer; // [groups] of [n][rank], or across: [rank][n]
+    uint64_t group_stride, stride;
+    const int32_t *group_of; // of a place, -1: none
+};
+
+struct ProductArgs {
+    Operand a, b;
+    Groups groups;
+    uint32_t m, n; // rows form: n alone; weights form: both
+    uint32_t n_out; // columns written, those past n as 0 (at most as many tiles); 0: n
+    uint32_t k;    // rows form
+    uint32_t splits, k_each; // of the inner dimension; k_each: a multiple of 64
+    void *out;
+    uint64_t out_stride;
+    const int32_t *out_index; // rows form: the row of the result for a place; NULL: itself
+    float *partial;           // splits > 1: [split][rows or group m][n], unscaled
+    float scale;
+    Beside beside;
+    uint32_t tiles_n;
+};
+
+// ---- tiles on their way to LDS ---------------------------------------------------------
+
+template <typename T> struct TileOf {
+    static constexpr int kK = 128 / sizeof(T); // elements of k
+    static constexpr int kC = 16 / sizeof(T);  // of a chunk
+};
+__device__ __forceinline__ uint32_t place_in_lds(uint32_t row, uint32_t chunk) {
+    return row * 128u + ((chunk ^ ((row ^ row >> 3) & 7u)) << 4);
+}
+
+// kRows rows with k along them: 8 threads a row.  Rows past the end repeat the last (what
+// becomes of them is not stored).
+template <typename T, int kRows, int kThreads> struct Along {
+    static constexpr int kPer = kRows * 8 / kThreads;
+    const T *row[kPer];
+    Chunk<T> c[kPer];
+    __device__ __forceinline__ void begin(const Operand &o, uint64_t group, uint32_t first,
+                                          uint32_t rows) {
+        const T *base = static_cast<const T *>(o.base) + group * o.group_stride;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const uint32_t r = first + min(threadIdx.x / 8 + j * (kThreads / 8), rows - 1);
+            row[j] = base + (uint64_t)(o.index ? (uint32_t)o.index[r] : r) * o.stride;
+        }
+    }
+    __device__ __forceinline__ void load(uint32_t k0, uint32_t end) {
+        const uint32_t k = k0 + (threadIdx.x & 7u) * TileOf<T>::kC;
+        if (k0 + TileOf<T>::kK <= end) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) c[j] = load_chunk(row[j] + k);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                c[j] = __builtin_bit_cast(Chunk<T>, load_some<T, TileOf<T>::kC>(
+                                                        row[j] + k, end > k ? end - k : 0u));
+        }
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            *reinterpret_cast<Chunk<T> *>(
+                lds + place_in_lds(threadIdx.x / 8 + j * (kThreads / 8), threadIdx.x & 7u)) = c[j];
+    }
+};
+
+// kRows columns of rows k of type S: a thread has 4 rows k by as many columns as 16 bytes
+// hold of the wider type, and turns them.  Rows and columns past the end are 0.
+template <typename T, typename S, int kRows, int kThreads> struct Across {
+    static constexpr int kN = TileOf<T>::kC;      // columns a thread
+    static constexpr int kAcross = kRows / kN;    // threads across
+    static constexpr int kTasks = kAcross * (TileOf<T>::kK / 4);
+    static constexpr int kPer = (kTasks + kThreads - 1) / kThreads;
+    const S *base;
+    uint64_t stride;
+    const int32_t *index;
+    uint32_t columns, first;
+    Few<S, kN> c[kPer][4];
+    __device__ __forceinline__ void begin(const Operand &o, uint64_t group, uint32_t first_column,
+                                          uint32_t all_columns) {
+        base = static_cast<const S *>(o.base) + group * o.group_stride;
+        stride = o.stride;
+        index = o.index;
+        first = first_column;
+        columns = all_columns;
+    }
+    __device__ __forceinline__ void load(uint32_t k0, uint32_t end) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const uint32_t task = threadIdx.x + j * kThreads;
+            if (kTasks % kThreads && task >= kTasks) break;
+            const uint32_t n = first + task % kAcross * kN, k = k0 + task / kAcross * 4;
+            const uint32_t have = n < columns ? columns - n : 0u;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (k + i < end && have) {
+                    const uint64_t r = index ? (uint32_t)index[k + i] : k + i;
+                    c[j][i] = load_some<S, kN>(base + r * stride + n, have);
+                } else {
+                    c[j][i] = {};
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const uint32_t task = threadIdx.x + j * kThreads;
+            if (kTasks % kThreads && task >= kTasks) break;
+            const uint32_t n = task % kAcross * kN, k = task / kAcross * 4;
+#pragma unroll
+            for (uint32_t e = 0; e < kN; ++e) {
+                Few<T, 4> t;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (__is_same(T, S)) t.v[i] = c[j][i].v[e];
+                    else t.v[i] = (T)(float)c[j][i].v[e];
+                }
+                *reinterpret_cast<Few<T, 4> *>(lds + place_in_lds(n + e, k * sizeof(T) / 16) +
+                                               k * sizeof(T) % 16) = t;
+            }
+        }
+    }
+};
+
+} // namespace head
+} // namespace sdfoam_hip

@@ -1,0 +1,28 @@
+// Host side of the products of rows in groups (products.hip).
+#pragma once
+
+#include "product_device.h"
+
+namespace sdfoam_hip {
+namespace head {
+
+// How a product is cut: tiles of the result, parts of the inner dimension, and the scratch
+// that the parts' sums take.
+struct Plan {
+    uint64_t tiles;
+    uint32_t tiles_n, splits, k_each;
+    size_t bytes;
+};
+// rows form: 128 x 128 (skinny: 128 x 32, results in fp32) of rows x n, k summed over
+Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_t k, bool skinny);
+// weights form: per group m x n, its rows summed over; narrow: 32 of m (a is fp32) or of n (b is)
+Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool narrow_m, bool narrow_n);
+
+hipError_t product_rows(int type, ProductArgs p, const Plan &plan, bool across, bool skinny,
+                        bool out_float, hipStream_t s);
+hipError_t product_weights(int type, ProductArgs p, const Plan &plan, bool narrow_m, bool narrow_n,
+                           hipStream_t s);
+int check_blocks(const char *call, const Plan &plan);
+
+} // namespace head
+} // namespace sdfoam_hip
