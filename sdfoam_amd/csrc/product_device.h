@@ -72,7 +72,7 @@ __device__ __forceinline__ void store_some(T *p, const Few<T, kN> &c, uint32_t h
     if (have >= kN) __builtin_memcpy(p, &c, sizeof(c));
     else
 #pragma unroll
-        for (uint32_t e = 0; e < kN; ++e)
+        for (uint32_t e = 0; e < kN - 1; ++e)
             if (e < have) p[e] = c.v[e];
 }
 
@@ -93,60 +93,71 @@ struct Groups {
 };
 
 struct TileOfRows {
-    uint32_t group, first, rows; // rows [first, first + rows); group `groups`: none
+    uint32_t group, first, rows; // rows [first, first + rows); group `groups`: none of them
 };
 
-// The `tile`-th tile of kRows rows, counted group by group; false where there are fewer.
-// Every thread of the block calls it; `lds` has room for 8 + 4 words.
-template <int kRows, int kThreads>
-__device__ __forceinline__ bool find_tile(const Groups &g, uint32_t tile, uint32_t *lds,
-                                          TileOfRows &t) {
-    if (!g.offsets) {
-        t.group = 0;
-        t.first = tile * kRows;
-        if (t.first >= g.total) return false;
-        t.rows = min((uint32_t)kRows, g.total - t.first);
-        return true;
+// Tiles of kRows rows, counted group by group.  count(): of all groups; find(): the
+// `tile`-th one.  Every thread of the block calls both; `lds` has room for 20 words.
+template <int kRows, int kThreads> struct TilesOfRows {
+    const Groups &g;
+    uint32_t *lds;
+    uint32_t lo, hi, before, sum; // a run of groups a thread, and the tiles before and in it
+    __device__ __forceinline__ static uint32_t tiles(uint32_t b, uint32_t e) {
+        return e > b ? (e - b + kRows - 1) / kRows : 0u;
     }
-    const uint32_t keys = g.groups + 1;
-    const uint32_t each = (keys + kThreads - 1) / kThreads;
-    const uint32_t lo = min(threadIdx.x * each, keys), hi = min(lo + each, keys);
-    uint32_t sum = 0;
-    for (uint32_t k = lo; k < hi; ++k) {
-        const uint32_t b = g.begin(k), e = g.end(k);
-        sum += e > b ? (e - b + kRows - 1) / kRows : 0u;
-    }
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t run = sum;
+    __device__ __forceinline__ TilesOfRows(const Groups &groups, uint32_t *words)
+        : g(groups), lds(words) {}
+    __device__ __forceinline__ uint32_t count() {
+        if (!g.offsets) return tiles(0, g.total);
+        const uint32_t keys = g.groups + 1, each = (keys + kThreads - 1) / kThreads;
+        lo = min(threadIdx.x * each, keys);
+        hi = min(lo + each, keys);
+        sum = 0;
+        for (uint32_t k = lo; k < hi; ++k) sum += tiles(g.begin(k), g.end(k));
+        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        uint32_t run = sum;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t v = __shfl_up(run, d);
-        if ((int)lane >= d) run += v;
-    }
-    if (lane == 63) lds[wave] = run;
-    if (threadIdx.x == 0) lds[8] = ~0u;
-    __syncthreads();
-    for (uint32_t w = 0; w < wave; ++w) run += lds[w];
-    if (tile < run && tile >= run - sum) {
-        uint32_t left = tile - (run - sum);
-        for (uint32_t k = lo; k < hi; ++k) {
-            const uint32_t b = g.begin(k), e = g.end(k);
-            const uint32_t n = e > b ? (e - b + kRows - 1) / kRows : 0u;
-            if (left < n) {
-                lds[8] = k;
-                lds[9] = b + left * kRows;
-                lds[10] = min((uint32_t)kRows, e - (b + left * kRows));
-                break;
-            }
-            left -= n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t v = __shfl_up(run, d);
+            if ((int)lane >= d) run += v;
         }
+        if (lane == 63) lds[wave] = run;
+        __syncthreads();
+        uint32_t all = 0;
+        for (uint32_t w = 0; w < kThreads / 64; ++w) {
+            if (w == wave) before = all + run - sum;
+            all += lds[w];
+        }
+        return __builtin_amdgcn_readfirstlane(all); // the same in every lane
     }
-    __syncthreads();
-    t.group = lds[8];
-    t.first = lds[9];
-    t.rows = lds[10];
-    return t.group != ~0u;
-}
+    __device__ __forceinline__ TileOfRows find(uint32_t tile) {
+        TileOfRows t;
+        if (!g.offsets) {
+            t.group = 0;
+            t.first = tile * kRows;
+            t.rows = min((uint32_t)kRows, g.total - t.first);
+            return t;
+        }
+        if (tile >= before && tile - before < sum) {
+            uint32_t left = tile - before;
+            for (uint32_t k = lo; k < hi; ++k) {
+                const uint32_t b = g.begin(k), e = g.end(k), n = tiles(b, e);
+                if (left < n) {
+                    lds[16] = k;
+                    lds[17] = b + left * kRows;
+                    lds[18] = min((uint32_t)kRows, e - (b + left * kRows));
+                    break;
+                }
+                left -= n;
+            }
+        }
+        __syncthreads();
+        t.group = __builtin_amdgcn_readfirstlane(lds[16]);
+        t.first = __builtin_amdgcn_readfirstlane(lds[17]);
+        t.rows = __builtin_amdgcn_readfirstlane(lds[18]);
+        return t;
+    }
+};
 // no more tiles than this
 inline uint64_t tiles_of_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t tile) {
     const uint64_t most = (rows + tile - 1) / tile;
@@ -187,12 +198,159 @@ struct ProductArgs {
     uint32_t tiles_n;
 };
 
-// ---- tiles on their way to LDS ---------------------------------------------------------
+// ---- large tiles: LDS as memory has it ----------------------------------------------------
+//
+// kRows rows (along) or columns (across) of 128 bytes of k: as many bytes either way.  Each
+// wave brings 1 KB at a time, 16 bytes a lane, straight into LDS where 16-byte pieces line
+// up (kDirect), through registers where they do not.  LDS takes a wave's 16 bytes a lane in
+// the order of the lanes, so the swizzle is in which piece a lane fetches:
+//
+//   along:  [row][128 bytes], piece c of row r at c ^ (r / 2 & 7): 16 rows' same piece on
+//           all banks
+//   across: [k][kRows], 16 bits: piece c of row k at c ^ 2 ((k & 3) + 4 (k / 8 & 1)), which
+//           keeps the 8 rows that a transposing read takes at a time off each other's banks;
+//           floats: at c ^ 8 (k / 4 & 1), for the two that a read of 64 words takes
+
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0}; // what pieces past the end are read from
 
 template <typename T> struct TileOf {
     static constexpr int kK = 128 / sizeof(T); // elements of k
-    static constexpr int kC = 16 / sizeof(T);  // of a chunk
+    static constexpr int kC = 16 / sizeof(T);  // of a piece
 };
+
+// A wave's 16 bytes a lane to LDS from `at` (the same in every lane) on, on their way until
+// the wave waits for its loads (landed()).  As an instruction of its own: were it a builtin,
+// the compiler would wait for it before every read of LDS that it cannot tell apart.
+__device__ __forceinline__ void to_lds(const void *from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(at), "v"(from)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
+}
+
+template <typename T, bool kAcross, int kRows, int kWaves, bool kDirect> struct Feed {
+    static constexpr int kPer = kRows / 8 / kWaves; // pieces a lane
+    static constexpr int kC = TileOf<T>::kC, kK = TileOf<T>::kK;
+    static constexpr int kRowBytes = kAcross ? kRows * (int)sizeof(T) : 128;
+    const T *p[kPer];
+    uint64_t stride;
+    uint32_t columns; // across: from the lane's first column on
+    Chunk<T> c[kDirect ? 1 : kPer];
+
+    // where in the tile the lane's j-th piece lies: its row of LDS and its place there
+    __device__ __forceinline__ static uint32_t wave() {
+        return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    }
+    __device__ __forceinline__ static uint32_t lds_row(int j) {
+        return ((wave() * kPer + j) * 1024u + (threadIdx.x & 63u) * 16u) / kRowBytes;
+    }
+    __device__ __forceinline__ static uint32_t swizzle(uint32_t row) {
+        if constexpr (!kAcross) return row >> 1 & 7u;
+        else if constexpr (sizeof(T) == 2) return ((row & 3u) | (row >> 3 & 1u) << 2) << 1;
+        else return (row >> 2 & 1u) << 3;
+    }
+    __device__ __forceinline__ static uint32_t piece(int j) {
+        return (((threadIdx.x & 63u) * 16u) % kRowBytes / 16u) ^ swizzle(lds_row(j));
+    }
+
+    // along: rows [first, first + rows), by the operand's index; across: columns from `first` of `rows` in all
+    __device__ __forceinline__ void begin(const Operand &o, uint64_t group, uint32_t first,
+                                          uint32_t rows, uint32_t k0) {
+        const T *base = static_cast<const T *>(o.base) + group * o.group_stride;
+        stride = o.stride;
+        columns = kAcross ? rows - first : rows;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if constexpr (!kAcross) {
+                const uint32_t r = first + min(lds_row(j), rows - 1);
+                p[j] = base + (uint64_t)(o.index ? (uint32_t)o.index[r] : r) * stride + k0 + piece(j) * kC;
+            } else {
+                p[j] = base + (uint64_t)(k0 + lds_row(j)) * stride + first + piece(j) * kC;
+            }
+        }
+    }
+
+    // of the tile at k, the lane's pieces; k0 as in begin()
+    __device__ __forceinline__ void load(char *lds, uint32_t k, uint32_t k0, uint32_t end) {
+        const uint64_t on = kAcross ? (uint64_t)(k - k0) * stride : k - k0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const T *from = p[j] + on;
+            uint32_t have;
+            if constexpr (!kAcross) {
+                const uint32_t at = k + piece(j) * kC;
+                have = end > at ? end - at : 0u;
+            } else {
+                const uint32_t at = k + lds_row(j), n = piece(j) * kC;
+                have = at < end && n < columns ? columns - n : 0u;
+            }
+            if constexpr (kDirect)
+                to_lds(have ? static_cast<const void *>(from) : kZeros,
+                       lds_address(lds) + (wave() * kPer + j) * 1024u);
+            else
+                c[j] = __builtin_bit_cast(Chunk<T>, load_some<T, kC>(from, have));
+        }
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+        if constexpr (!kDirect)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                *reinterpret_cast<uint4 *>(lds + (wave() * kPer + j) * 1024u + (threadIdx.x & 63u) * 16u) =
+                    __builtin_bit_cast(uint4, c[j]);
+    }
+};
+
+// Fragments of 32 rows (columns) from `first` (a multiple of 64; of 128 for more than two)
+// on, of the 32 bytes of k at step kk.  What the swizzle changes with i or kk are bits that
+// nothing else has: one address each.
+template <typename T, bool kAcross, int kRows, int kFragments> struct Fragments {
+    static constexpr int kRowBytes = kAcross ? kRows * (int)sizeof(T) : 128;
+    static constexpr int kAt = kAcross ? kFragments : 4;
+    uint32_t at[kAt];
+    __device__ __forceinline__ explicit Fragments(uint32_t first) {
+        const uint32_t lane = threadIdx.x & 63u, half = lane >> 5, q = lane & 15u;
+#pragma unroll
+        for (uint32_t i = 0; i < kAt; ++i) {
+            if constexpr (!kAcross) {
+                at[i] = (first + (lane & 31u)) * 128u + (((2u * i + half) ^ (lane >> 1 & 7u)) << 4);
+            } else if constexpr (sizeof(T) == 2) {
+                // 16 lanes read 4 rows k of 16 columns; each gets its column's 4
+                const uint32_t n = first + i * 32u + (lane >> 4 & 1u) * 16u + (q & 3u) * 4u;
+                at[i] = (half * 8u + (q >> 2)) * kRowBytes +
+                        (((n >> 3) ^ (((q >> 2) | half << 2) << 1)) << 4) + (n & 7u) * 2u;
+            } else {
+                const uint32_t n = first + i * 32u + (lane & 31u);
+                at[i] = half * 4u * kRowBytes + (((n >> 2) ^ half << 3) << 4) + (n & 3u) * 4u;
+            }
+        }
+    }
+    __device__ __forceinline__ Chunk<T> read(const char *lds, int i, int kk) const {
+        Chunk<T> c;
+        if constexpr (!kAcross) {
+            c = __builtin_bit_cast(Chunk<T>, *reinterpret_cast<const uint4 *>(lds + at[kk] + i * 4096u));
+        } else if constexpr (sizeof(T) == 2) {
+            typedef short S4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) S4 LdsS4;
+            S4 v[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                v[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (LdsS4 *)(lds + at[i] + (kk * 16 + s * 4) * kRowBytes));
+            __builtin_memcpy(&c, v, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                c.w[e] = *reinterpret_cast<const uint32_t *>(lds + at[i] + (kk * 8 + e) * kRowBytes);
+        }
+        return c;
+    }
+};
+
+// ---- narrow tiles: turned on their way to LDS ---------------------------------------------
 __device__ __forceinline__ uint32_t place_in_lds(uint32_t row, uint32_t chunk) {
     return row * 128u + ((chunk ^ ((row ^ row >> 3) & 7u)) << 4);
 }
@@ -227,8 +385,9 @@ template <typename T, int kRows, int kThreads> struct Along {
     __device__ __forceinline__ void store(char *lds) const {
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
-            *reinterpret_cast<Chunk<T> *>(
-                lds + place_in_lds(threadIdx.x / 8 + j * (kThreads / 8), threadIdx.x & 7u)) = c[j];
+            *reinterpret_cast<uint4 *>(
+                lds + place_in_lds(threadIdx.x / 8 + j * (kThreads / 8), threadIdx.x & 7u)) =
+                __builtin_bit_cast(uint4, c[j]);
     }
 };
 

@@ -11,6 +11,7 @@ namespace head {
 struct Plan {
     uint64_t tiles;
     uint32_t tiles_n, splits, k_each;
+    bool large; // tiles of 256 x 256, else 128 x 128
     size_t bytes;
 };
 // rows form: 128 x 128 (skinny: 128 x 32, results in fp32) of rows x n, k summed over
