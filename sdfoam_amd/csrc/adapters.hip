@@ -21,6 +21,41 @@ using namespace sdfoam_hip::head;
 
 namespace {
 
+// h of few rows, in the order they come: a wave for each of a row's values.  Beside the
+// matrix of ranks that the rows share, a row of `down` is read by no more than the rows of
+// its adapter; 64 rows of 2,048 bf16, rank 16: bound by the launch.
+struct FewRows {
+    const void *rows, *ids, *down;
+    uint64_t stride;
+    int id_type;
+    uint32_t width, adapters, rank, pitch;
+    float scale;
+    float *inner;
+    int32_t *group_of;
+};
+constexpr uint32_t kFewRows = 64;
+
+template <typename T> __global__ __launch_bounds__(256) void few_rows_kernel(FewRows f) {
+    constexpr uint32_t kC = Chunk<T>::kN;
+    const uint32_t row = blockIdx.x, lane = threadIdx.x & 63u, r = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const int32_t a = load_id(f.ids, f.id_type, row, f.adapters);
+    if (blockIdx.y == 0 && threadIdx.x == 0) f.group_of[row] = a;
+    float sum = 0.0f;
+    if (a >= 0 && r < f.rank) {
+        const T *x = static_cast<const T *>(f.rows) + row * f.stride;
+        const T *d = static_cast<const T *>(f.down) + ((uint64_t)a * f.rank + r) * f.width;
+#pragma unroll 4
+        for (uint32_t k = lane * kC; k < f.width; k += 64 * kC) {
+            const uint32_t have = f.width - k;
+            const Few<T, kC> u = load_some<T, kC>(x + k, have), v = load_some<T, kC>(d + k, have);
+#pragma unroll
+            for (uint32_t e = 0; e < kC; ++e) sum = fmaf((float)u.v[e], (float)v.v[e], sum);
+        }
+    }
+    sum = group_sum<64>(sum);
+    if (lane == 0 && r < f.pitch) f.inner[row * f.pitch + r] = f.scale * sum;
+}
+
 struct Layout {
     size_t order, entries, group_of, offsets, inner, back, partial, bytes;
     uint32_t pitch;
@@ -33,6 +68,11 @@ struct Sizes {
     bool beside() const { return count > 0 && adapters > 0 && rank > 0; }
 };
 
+// few rows for each adapter, and few enough that their sums in fp32 cost little
+bool one_each(const Sizes &z) { return z.count <= 1024 && z.count < 8ull * z.adapters; }
+
+bool few(const Sizes &z, bool backward) { return !backward && z.count <= kFewRows; }
+
 Layout layout(const Sizes &z, bool backward) {
     Layout l = {};
     size_t at = 0, partial = 0;
@@ -44,26 +84,34 @@ Layout layout(const Sizes &z, bool backward) {
     const auto also = [&](const Plan &p) {
         if (p.bytes > partial) partial = p.bytes;
     };
-    if (z.beside()) {
+    if (z.beside() && few(z, backward)) {
+        l.pitch = (z.rank + 15) / 16 * 16;
+        l.group_of = take(z.count * 4);
+        l.inner = take(z.count * l.pitch * 4);
+    } else if (z.beside()) {
         l.pitch = (z.rank + 15) / 16 * 16;
         l.order = take(order_scratch_bytes(z.count, z.adapters));
         l.entries = take(z.count * 4);
         l.group_of = take(z.count * 4);
         l.offsets = take((z.adapters + 1ull) * 4);
         l.inner = take(z.count * l.pitch * 4);
-        also(l.inner_plan = plan_rows(z.count, z.adapters, true, l.pitch, z.width, true));
+        also(l.inner_plan = plan_rows(z.count, z.adapters, true, l.pitch, z.width, false, true));
         if (backward) {
             l.back = take(z.count * l.pitch * 4);
-            also(l.back_plan = plan_rows(z.count, z.adapters, true, l.pitch, z.out_width, true));
+            also(l.back_plan = plan_rows(z.count, z.adapters, true, l.pitch, z.out_width, true, true));
             also(l.down_plan = plan_weights(z.count, z.adapters, z.rank, z.width, true, false));
             also(l.up_plan = plan_weights(z.count, z.adapters, z.out_width, z.rank, false, true));
         }
     }
+    const auto product = [&](uint32_t n, uint32_t k, bool across) {
+        const Plan plan = plan_rows(z.count, 1, false, n, k, across, false);
+        return z.beside() && one_each(z) ? late(plan, z.count, n) : plan;
+    };
     if (backward) {
-        also(l.rows_plan = plan_rows(z.count, 1, false, z.width, z.out_width, false));
+        also(l.rows_plan = product(z.width, z.out_width, true));
         also(l.weight_plan = plan_weights(z.count, 1, z.out_width, z.width, false, false));
     } else {
-        also(l.out_plan = plan_rows(z.count, 1, false, z.out_width, z.width, false));
+        also(l.out_plan = product(z.out_width, z.width, false));
     }
     l.partial = take(partial);
     l.bytes = at;
@@ -154,10 +202,23 @@ int sdf_adapter_linear(int type, const void *rows, uint64_t rows_stride, uint64_
     for (const Plan *plan : {&l.inner_plan, &l.out_plan})
         if ((rc = check_blocks("sdf_adapter_linear", *plan)) != SDF_OK) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    Ordered o;
-    hipError_t e = order_rows(l, z, id_type, adapters, static_cast<char *>(scratch), o, s);
-    if (e == hipSuccess && z.beside())
-        e = low_rank(type, l.inner_plan, z, o, l, rows, rows_stride, width, down, false, scale, o.inner, s);
+    Ordered o = {};
+    hipError_t e = hipSuccess;
+    if (z.beside() && few(z, false)) {
+        char *at = static_cast<char *>(scratch);
+        o.inner = reinterpret_cast<float *>(at + l.inner);
+        o.group_of = reinterpret_cast<int32_t *>(at + l.group_of);
+        o.partial = reinterpret_cast<float *>(at + l.partial);
+        const FewRows f = {rows, adapters, down, rows_stride, id_type, width, num_adapters, rank, l.pitch,
+                           scale, o.inner, o.group_of};
+        const dim3 grid((uint32_t)count, l.pitch / 4);
+        with_type(type, [&](auto t) { few_rows_kernel<decltype(t)><<<grid, 256, 0, s>>>(f); });
+        e = hipGetLastError();
+    } else {
+        e = order_rows(l, z, id_type, adapters, static_cast<char *>(scratch), o, s);
+        if (e == hipSuccess && z.beside())
+            e = low_rank(type, l.inner_plan, z, o, l, rows, rows_stride, width, down, false, scale, o.inner, s);
+    }
     if (e == hipSuccess) {
         ProductArgs p = {};
         p.a = {rows, rows_stride, 0, o.entries};

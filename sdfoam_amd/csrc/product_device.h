@@ -189,10 +189,11 @@ struct ProductArgs {
     uint32_t n_out; // columns written, those past n as 0 (at most as many tiles); 0: n
     uint32_t k;    // rows form
     uint32_t splits, k_each; // of the inner dimension; k_each: a multiple of 64
+    bool parts;              // the sums go to `partial` and are joined from there
     void *out;
     uint64_t out_stride;
     const int32_t *out_index; // rows form: the row of the result for a place; NULL: itself
-    float *partial;           // splits > 1: [split][rows or group m][n], unscaled
+    float *partial;           // [split][rows or group m][n], unscaled
     float scale;
     Beside beside;
     uint32_t tiles_n;
@@ -222,10 +223,7 @@ template <typename T> struct TileOf {
 // the wave waits for its loads (landed()).  As an instruction of its own: were it a builtin,
 // the compiler would wait for it before every read of LDS that it cannot tell apart.
 __device__ __forceinline__ void to_lds(const void *from, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :
-                 : "s"(at), "v"(from)
-                 : "memory", "m0");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(at), "v"(from) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const char *p) {

@@ -12,14 +12,22 @@ struct Plan {
     uint64_t tiles;
     uint32_t tiles_n, splits, k_each;
     bool large; // tiles of 256 x 256, else 128 x 128
+    uint32_t thin_m, thin_n; // few rows a group: tiles of 16 thin_m x 16 thin_n; 0: not so
+    bool late; // the rows' adapters are added when the parts are joined
     size_t bytes;
 };
-// rows form: 128 x 128 (skinny: 128 x 32, results in fp32) of rows x n, k summed over
-Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_t k, bool skinny);
+// rows form: rows x n, k summed over, b across k or along it (skinny: tiles of 128 x 32,
+// results in fp32)
+Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_t k, bool across,
+               bool skinny);
 // weights form: per group m x n, its rows summed over; narrow: 32 of m (a is fp32) or of n (b is)
 Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool narrow_m, bool narrow_n);
 
-hipError_t product_rows(int type, ProductArgs p, const Plan &plan, bool across, bool skinny,
+// the same plan with the adapters added late: where rows have an adapter each, more or less,
+// every row's is read by threads of its own (64 rows of 2,048 -> 32,768 bf16 and rank 16)
+Plan late(Plan plan, uint64_t rows, uint32_t n);
+
+hipError_t product_rows(int type, const ProductArgs &p, const Plan &plan, bool across, bool skinny,
                         bool out_float, hipStream_t s);
 hipError_t product_weights(int type, ProductArgs p, const Plan &plan, bool narrow_m, bool narrow_n,
                            hipStream_t s);

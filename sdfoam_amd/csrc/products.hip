@@ -23,8 +23,64 @@ struct LoaderOf<true, T, S, kRows, kThreads> {
     typedef Across<T, S, kRows, kThreads> type;
 };
 
-// What the rows' adapters add to 32 rows of kTn x 32 columns from n0 on: a lane has row m0 +
-// mi.  One adapter of the 32 rows' after the other, floats in the matrix units.
+// What the rows' adapters add to 32 rows of kTn x 32 columns from n0 on, in one of two ways:
+// by the matrix units, one adapter of the 32 rows' after the other, where they have few
+// (add_beside; a lane has row m0 + mi, as the accumulators do), and for each row by itself
+// where they have many (beside_of_rows).  One after the other, each waits for its values: 200
+// rows, an adapter each, of 2,048 -> 32,768 bf16 and rank 16 took 247 us, 48 without them.
+constexpr uint32_t kFewAdapters = 3;
+__device__ __forceinline__ bool few_adapters(const ProductArgs &p, uint32_t m0, uint32_t rows, uint32_t mi) {
+    const int32_t mine = mi < rows ? p.beside.group_of[m0 + mi] : -1;
+    uint64_t left = __ballot(mine >= 0);
+#pragma unroll
+    for (uint32_t k = 0; k < kFewAdapters; ++k)
+        if (left) left &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __ffsll((long long)left) - 1));
+    return left == 0;
+}
+
+// Column n of kRows rows from `place` on (the last of `rows` again where there are fewer),
+// their values on their way together; the rows are the same in every lane, `groups` has
+// theirs from lane `from` on.
+template <typename S, bool kAcross, int kRows>
+__device__ __forceinline__ void beside_of_rows(const ProductArgs &p, uint32_t place, uint32_t rows,
+                                               int32_t groups, uint32_t from, uint32_t n, float *sum) {
+    const S *outer[kRows];
+    const float *inner[kRows];
+    bool some[kRows];
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+        const uint32_t at = place + min(i, rows - 1);
+        const int32_t g = __builtin_amdgcn_readlane(groups, from + min(i, rows - 1));
+        some[i] = g >= 0;
+        outer[i] = static_cast<const S *>(p.beside.outer) + (uint64_t)max(g, 0) * p.beside.group_stride +
+                   (kAcross ? n : (uint64_t)n * p.beside.stride);
+        inner[i] = p.beside.inner + (uint64_t)at * p.beside.pitch;
+        sum[i] = 0.0f;
+    }
+    constexpr uint32_t kE = 8;
+    for (uint32_t r = 0; r < p.beside.rank; r += kE) { // inner is 0 past the rank
+        const uint32_t have = p.beside.rank - r;
+        Few<S, kE> o[kRows];
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; ++i) {
+            if constexpr (kAcross) {
+#pragma unroll
+                for (uint32_t e = 0; e < kE; ++e)
+                    o[i].v[e] = e < have ? outer[i][(uint64_t)(r + e) * p.beside.stride] : (S)0.0f;
+            } else {
+                o[i] = load_some<S, kE>(outer[i] + r, have);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < kE; ++e) sum[i] = fmaf((float)o[i].v[e], inner[i][r + e], sum[i]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i)
+        if (!some[i]) sum[i] = 0.0f;
+}
+
 template <typename S, bool kAcross, int kTn>
 __device__ __forceinline__ void add_beside(const ProductArgs &p, uint32_t m0, uint32_t rows,
                                            uint32_t mi, uint32_t n0, F16x *acc) {
@@ -184,11 +240,45 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
     char *turn = lds + wave * kTurn;
     const uint64_t rows = kWeights ? (uint64_t)p.groups.groups * p.m : p.groups.total;
     const uint64_t row0 = kWeights ? (uint64_t)group * p.m + m0 : m0;
+    uint32_t by_row = 0; // bit i: its rows' adapters are added row by row
     if constexpr (!kWeights)
         if (p.beside.inner && split == 0)
 #pragma unroll
-            for (int i = 0; i < kTm; ++i)
-                add_beside<T, kAcrossB, kTn>(p, m0, rows_m, wm + i * 32 + l32, n0 + wn, acc[i]);
+            for (int i = 0; i < kTm; ++i) {
+                if (few_adapters(p, m0, rows_m, wm + i * 32 + l32))
+                    add_beside<T, kAcrossB, kTn>(p, m0, rows_m, wm + i * 32 + l32, n0 + wn, acc[i]);
+                else by_row |= 1u << i;
+            }
+    // rows whose adapters are added one by one: a lane has a column
+    const auto write_rows = [&](auto t, const F16x *sums, uint32_t first, auto row_at, float scale) {
+        typedef decltype(t) O;
+        constexpr uint32_t kFloats = kTn * 32 + 4;
+        float *turned = reinterpret_cast<float *>(turn);
+        wave_sync();
+#pragma unroll
+        for (int j = 0; j < kTn; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                Few<float, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.v[e] = sums[j][q * 4 + e];
+                *reinterpret_cast<Few<float, 4> *>(turned + l32 * kFloats + j * 32 + q * 8 + half * 4) = o;
+            }
+        wave_sync();
+        const uint32_t n = n0 + wn + lane, rows_here = first < rows_m ? min(32u, rows_m - first) : 0u;
+        static_assert(kTn * 32 == 64, "a lane for each column");
+        const int32_t groups = l32 < rows_here ? p.beside.group_of[m0 + first + l32] : -1;
+        if (n >= p.n) return;
+        constexpr uint32_t kBatch = 4;
+        for (uint32_t r = 0; r < rows_here; r += kBatch) {
+            float extra[kBatch];
+            beside_of_rows<T, kAcrossB, kBatch>(p, m0 + first + r, rows_here - r, groups, r, n, extra);
+#pragma unroll
+            for (uint32_t i = 0; i < kBatch; ++i)
+                if (r + i < rows_here)
+                    row_at(row0 + first + r + i)[n] = (O)(scale * (turned[(r + i) * kFloats + lane] + extra[i]));
+        }
+    };
     const auto write = [&](auto t, const F16x *sums, uint32_t first, auto row_at, float scale) {
         typedef decltype(t) O;
         constexpr uint32_t kE = 16 / sizeof(O), kPieces = kTn * 32 / kE;
@@ -220,17 +310,22 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
                 for (uint32_t e = 0; e < have; ++e) to[e] = from[e];
         }
     };
-    if (p.splits > 1) {
+    if (p.parts) {
 #pragma unroll
-        for (int i = 0; i < kTm; ++i)
-            write(0.0f, acc[i], wm + i * 32,
-                  [&](uint64_t row) { return p.partial + (split * rows + row) * p.n_out; }, 1.0f);
+        for (int i = 0; i < kTm; ++i) {
+            const auto row_at = [&](uint64_t row) { return p.partial + (split * rows + row) * p.n_out; };
+            if (!kWeights && (by_row >> i & 1u)) write_rows(0.0f, acc[i], wm + i * 32, row_at, 1.0f);
+            else write(0.0f, acc[i], wm + i * 32, row_at, 1.0f);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < kTm; ++i)
-            write(T(), acc[i], wm + i * 32, [&](uint64_t row) {
+        for (int i = 0; i < kTm; ++i) {
+            const auto row_at = [&](uint64_t row) {
                 return static_cast<T *>(p.out) + (p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride;
-            }, p.scale);
+            };
+            if (!kWeights && (by_row >> i & 1u)) write_rows(T(), acc[i], wm + i * 32, row_at, p.scale);
+            else write(T(), acc[i], wm + i * 32, row_at, p.scale);
+        }
     }
 }
 
@@ -347,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs p) {
                 Few<float, 4> sum;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum.v[e] = n + e < p.n ? acc[i][j][q * 4 + e] : 0.0f;
-                if (p.splits > 1) {
+                if (p.parts) {
                     const uint64_t rows = kWeights ? (uint64_t)p.groups.groups * p.m : p.groups.total;
                     store_some<float, 4>(p.partial + (split * rows + row) * p.n_out + n, sum, p.n_out - n);
                 } else {
@@ -361,7 +456,7 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs p) {
     }
 }
 
-// The splits' sums in order.  rows x n floats a split; four columns a thread.
+// The parts' sums in order.  rows x n floats a part; four columns a thread.
 template <typename O> __global__ __launch_bounds__(256) void join_kernel(ProductArgs p, uint64_t rows) {
     const uint32_t quads = (p.n_out + 3) / 4;
     const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
@@ -379,6 +474,141 @@ template <typename O> __global__ __launch_bounds__(256) void join_kernel(Product
 #pragma unroll
     for (int e = 0; e < 4; ++e) o.v[e] = (O)(p.scale * sum[e]);
     store_some<O, 4>(to, o, have);
+}
+
+// The same with what the rows' adapters add, where the tiles left that out (Plan::late): a
+// column a thread, so that neighbours read neighbouring values (four columns a thread, 128
+// bytes from one lane to the next: 152 us for 200 rows of 32,768 and rank 16).
+template <typename O, bool kAcross> __global__ __launch_bounds__(256) void join_late_kernel(ProductArgs p) {
+    const uint32_t row = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= p.n) return;
+    float sum = 0.0f, extra = 0.0f;
+    for (uint32_t s = 0; s < p.splits; ++s) sum += p.partial[((uint64_t)s * gridDim.y + row) * p.n + n];
+    const int32_t g = p.beside.group_of[row];
+    if (g >= 0) {
+        const O *outer = static_cast<const O *>(p.beside.outer) + (uint64_t)g * p.beside.group_stride;
+        const float *inner = p.beside.inner + (uint64_t)row * p.beside.pitch;
+        if constexpr (kAcross) {
+#pragma unroll 16
+            for (uint32_t r = 0; r < p.beside.rank; ++r)
+                extra = fmaf((float)outer[(uint64_t)r * p.beside.stride + n], inner[r], extra);
+        } else {
+            constexpr uint32_t kE = 8;
+#pragma unroll 4
+            for (uint32_t r = 0; r < p.beside.rank; r += kE) { // inner is 0 past the rank
+                const Few<O, kE> o = load_some<O, kE>(outer + (uint64_t)n * p.beside.stride + r, p.beside.rank - r);
+#pragma unroll
+                for (uint32_t e = 0; e < kE; ++e) extra = fmaf((float)o.v[e], inner[r + e], extra);
+            }
+        }
+    }
+    static_cast<O *>(p.out)[(p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride + n] = (O)(p.scale * (sum + extra));
+}
+
+// ---- few rows a group --------------------------------------------------------------------
+//
+// 16 kMt rows by 16 kNt columns a block; each of four waves has a quarter of the inner
+// dimension and reads its operands straight into registers, 128 bytes of a row at a time,
+// since no other wave of the block needs them.  Bound by the bytes of the matrices; the
+// rows come from L2, as often as there are tiles of columns.
+constexpr int kThinWaves = 4;
+
+template <typename T, int kMt, int kNt>
+__global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ProductArgs p) {
+    constexpr uint32_t kC = TileOf<T>::kC, kStep = TileOf<T>::kK; // a lane has two pieces a step
+    constexpr int kAhead = kMt * kNt <= 2 ? 4 : kMt * kNt <= 8 ? 2 : 1; // steps in flight
+    __shared__ F4x sums[kThinWaves][kMt * kNt][64];
+    __shared__ uint32_t found[20];
+    const uint32_t tile_n = blockIdx.x % p.tiles_n, tile_m = blockIdx.x / p.tiles_n;
+    TilesOfRows<16 * kMt, 64 * kThinWaves> tiles(p.groups, found);
+    if (tile_m >= tiles.count()) return;
+    const TileOfRows t = tiles.find(tile_m);
+    const bool none = p.groups.offsets && t.group == p.groups.groups; // rows of no group: zeros
+    const uint32_t k_all = none ? 0u : p.k, n0 = tile_n * (16 * kNt);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, l16 = lane & 15u, q = lane >> 4;
+    const T *x[kMt], *w[kNt];
+#pragma unroll
+    for (int i = 0; i < kMt; ++i) {
+        const uint32_t r = t.first + min(i * 16 + l16, t.rows - 1);
+        x[i] = static_cast<const T *>(p.a.base) + (uint64_t)(p.a.index ? (uint32_t)p.a.index[r] : r) * p.a.stride;
+    }
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+        w[j] = static_cast<const T *>(p.b.base) + (none ? 0u : t.group) * p.b.group_stride +
+               (uint64_t)min(n0 + j * 16 + l16, p.n - 1) * p.b.stride;
+    const uint32_t steps = (k_all + kStep - 1) / kStep, each = (steps + kThinWaves - 1) / kThinWaves;
+    const uint32_t k_begin = min(wave * each * kStep, k_all), k_end = min(k_begin + each * kStep, k_all);
+    F4x acc[kMt][kNt] = {};
+    uint32_t k = k_begin;
+    for (; k + kAhead * kStep <= k_end; k += kAhead * kStep) {
+        Chunk<T> fx[kAhead][kMt][2], fw[kAhead][kNt][2];
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t at = k + s * kStep + (q * 2 + h) * kC;
+#pragma unroll
+                for (int j = 0; j < kNt; ++j) fw[s][j][h] = load_chunk(w[j] + at);
+#pragma unroll
+                for (int i = 0; i < kMt; ++i) fx[s][i][h] = load_chunk(x[i] + at);
+            }
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                    for (int j = 0; j < kNt; ++j) mma16<T>(acc[i][j], fw[s][j][h], fx[s][i][h]);
+    }
+    for (; k < k_end; k += kStep)
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t at = k + (q * 2 + h) * kC, have = k_end > at ? k_end - at : 0u;
+            Chunk<T> fx[kMt], fw[kNt];
+#pragma unroll
+            for (int j = 0; j < kNt; ++j) fw[j] = __builtin_bit_cast(Chunk<T>, load_some<T, kC>(w[j] + at, have));
+#pragma unroll
+            for (int i = 0; i < kMt; ++i) fx[i] = __builtin_bit_cast(Chunk<T>, load_some<T, kC>(x[i] + at, have));
+#pragma unroll
+            for (int i = 0; i < kMt; ++i)
+#pragma unroll
+                for (int j = 0; j < kNt; ++j) mma16<T>(acc[i][j], fw[j], fx[i]);
+        }
+#pragma unroll
+    for (int i = 0; i < kMt; ++i)
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) sums[wave][i * kNt + j][lane] = acc[i][j];
+    __syncthreads();
+    // an element of the result a thread, its row's adapter read for it alone: of few rows
+    // each has its own, as often as not
+#pragma unroll 4
+    for (uint32_t c = 0; c < kMt * kNt; ++c) {
+        const uint32_t at = c * 256 + threadIdx.x, m = at / (16 * kNt), nn = at % (16 * kNt), n = n0 + nn;
+        if (m >= t.rows || n >= p.n) continue;
+        const uint32_t place = t.first + m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kThinWaves; ++v)
+            sum += sums[v][m / 16 * kNt + nn / 16][m % 16 + nn % 16 / 4 * 16][nn % 4];
+        const int32_t g = p.beside.inner ? p.beside.group_of[place] : -1;
+        if (g >= 0) {
+            const T *outer = static_cast<const T *>(p.beside.outer) + (uint64_t)g * p.beside.group_stride +
+                             (uint64_t)n * p.beside.stride;
+            const float *h = p.beside.inner + (uint64_t)place * p.beside.pitch;
+            float extra = 0.0f;
+#pragma unroll 2
+            for (uint32_t r = 0; r < p.beside.rank; r += kC) { // h is 0 past the rank
+                const Few<T, kC> o = load_some<T, kC>(outer + r, p.beside.rank - r);
+                const Few<float, kC> hr = load_few<float, kC>(h + r);
+#pragma unroll
+                for (uint32_t e = 0; e < kC; ++e) extra = fmaf((float)o.v[e], hr.v[e], extra);
+            }
+            sum += extra;
+        }
+        const uint64_t row = p.out_index ? (uint32_t)p.out_index[place] : place;
+        static_cast<T *>(p.out)[row * p.out_stride + n] = (T)(p.scale * sum);
+    }
 }
 
 constexpr uint64_t kMaxBlocks = 1ull << 23;
@@ -402,6 +632,19 @@ void launch_tiles(const ProductArgs &p, const Plan &plan, bool direct, hipStream
     else launch_tiles_as<T, kWeights, kAcross, false>(p, plan, s);
 }
 
+template <typename T> void launch_thin(const ProductArgs &p, const Plan &plan, hipStream_t s) {
+    const uint32_t grid = (uint32_t)plan.tiles, block = 64 * kThinWaves;
+    switch (plan.thin_m * 8 + plan.thin_n) {
+    case 9: thin_kernel<T, 1, 1><<<grid, block, 0, s>>>(p); break;
+    case 10: thin_kernel<T, 1, 2><<<grid, block, 0, s>>>(p); break;
+    case 17: thin_kernel<T, 2, 1><<<grid, block, 0, s>>>(p); break;
+    case 18: thin_kernel<T, 2, 2><<<grid, block, 0, s>>>(p); break;
+    case 33: thin_kernel<T, 4, 1><<<grid, block, 0, s>>>(p); break;
+    case 34: thin_kernel<T, 4, 2><<<grid, block, 0, s>>>(p); break;
+    default: thin_kernel<T, 4, 4><<<grid, block, 0, s>>>(p); break;
+    }
+}
+
 template <typename O> hipError_t join(const ProductArgs &p, uint64_t rows, hipStream_t s) {
     const uint64_t threads = rows * ((p.n_out + 3) / 4);
     join_kernel<O><<<(uint32_t)((threads + 255) / 256), 256, 0, s>>>(p, rows);
@@ -420,8 +663,23 @@ bool take_large(uint64_t large, uint64_t small) {
     return 3 * ((large + 255) / 256) <= 2 * ((small + 511) / 512);
 }
 
-Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_t k, bool skinny) {
+Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_t k, bool across,
+               bool skinny) {
     Plan plan = {};
+    const uint64_t each = grouped && groups > 0 ? (rows + groups - 1) / groups : rows;
+    if (!skinny && !across && each <= 32) {
+        plan.thin_m = each <= 16 ? 1 : 2;
+        const uint64_t tiles_m = tiles_of_rows(rows, groups, grouped, 16 * plan.thin_m);
+        // wider where there are columns enough for every CU: the rows are read less often
+        plan.thin_n = plan.thin_m < 2 ? plan.thin_m : 2;
+        if (plan.thin_n < 2 && tiles_m * (n / 32) >= 1024) plan.thin_n = 2;
+        while (plan.thin_n > 1 && tiles_m * ((n + 16 * plan.thin_n - 1) / (16 * plan.thin_n)) < 256)
+            plan.thin_n /= 2;
+        plan.tiles_n = (n + 16 * plan.thin_n - 1) / (16 * plan.thin_n);
+        plan.tiles = tiles_m * plan.tiles_n;
+        plan.splits = 1;
+        return plan;
+    }
     plan.large = !skinny && take_large(tiles_of_rows(rows, groups, grouped, 256) * ((n + 255) / 256),
                                        tiles_of_rows(rows, groups, grouped, 128) * ((n + 127) / 128));
     const uint32_t km = plan.large ? 256 : 128, kn = skinny ? 32 : km;
@@ -458,17 +716,30 @@ Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool n
     return plan;
 }
 
-hipError_t product_rows(int type, ProductArgs p, const Plan &plan, bool across, bool skinny,
+Plan late(Plan plan, uint64_t rows, uint32_t n) {
+    if (plan.thin_m || plan.late) return plan;
+    plan.late = true;
+    plan.bytes = round_up(plan.splits * rows * n * 4);
+    return plan;
+}
+
+hipError_t product_rows(int type, const ProductArgs &args, const Plan &plan, bool across, bool skinny,
                         bool out_float, hipStream_t s) {
     if (plan.tiles == 0) return hipSuccess;
+    ProductArgs p = args;
+    p.parts = plan.splits > 1 || plan.late;
+    if (p.parts && !p.partial) return hipErrorInvalidValue; // the caller's layout
     p.tiles_n = plan.tiles_n;
     if (p.n_out == 0) p.n_out = p.n;
     p.splits = plan.splits;
     p.k_each = plan.k_each;
+    if (plan.late) p.beside.inner = nullptr;
     const dim3 grid((uint32_t)plan.tiles, plan.splits);
     return with_type(type, [&](auto t) {
         typedef decltype(t) T;
-        if (skinny) {
+        if (plan.thin_m) {
+            launch_thin<T>(p, plan, s);
+        } else if (skinny) {
             if (across) product_kernel<T, T, T, false, true, 128, 32, 4, 1, float><<<grid, kThreads, 0, s>>>(p);
             else product_kernel<T, T, T, false, false, 128, 32, 4, 1, float><<<grid, kThreads, 0, s>>>(p);
         } else {
@@ -476,8 +747,15 @@ hipError_t product_rows(int type, ProductArgs p, const Plan &plan, bool across, 
             if (across) launch_tiles<T, false, true>(p, plan, direct, s);
             else launch_tiles<T, false, false>(p, plan, direct, s);
         }
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess || plan.splits == 1) return e;
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || !p.parts) return e;
+        if (plan.late && args.beside.inner) {
+            p.beside = args.beside;
+            const dim3 blocks((p.n + 255) / 256, p.groups.total); // at most 1,024 rows
+            if (across) join_late_kernel<T, true><<<blocks, 256, 0, s>>>(p);
+            else join_late_kernel<T, false><<<blocks, 256, 0, s>>>(p);
+            return hipGetLastError();
+        }
         return out_float ? join<float>(p, p.groups.total, s) : join<T>(p, p.groups.total, s);
     });
 }
@@ -485,6 +763,8 @@ hipError_t product_rows(int type, ProductArgs p, const Plan &plan, bool across, 
 hipError_t product_weights(int type, ProductArgs p, const Plan &plan, bool narrow_m, bool narrow_n,
                            hipStream_t s) {
     if (plan.tiles == 0) return hipSuccess;
+    p.parts = plan.splits > 1;
+    if (p.parts && !p.partial) return hipErrorInvalidValue; // the caller's layout
     p.tiles_n = plan.tiles_n;
     if (p.n_out == 0) p.n_out = p.n;
     p.splits = plan.splits;
@@ -527,7 +807,7 @@ extern "C" {
 size_t sdf_expert_linear_scratch_bytes(uint64_t count, uint32_t num_experts, uint32_t width,
                                        uint32_t out_width) {
     if (count >= 1ull << 31 || num_experts > SDF_MAX_EXPERTS) return 0;
-    return plan_rows(count, num_experts, true, out_width, width, false).bytes;
+    return plan_rows(count, num_experts, true, out_width, width, false, false).bytes;
 }
 
 int sdf_expert_linear(int type, const void *rows, uint64_t rows_stride, uint64_t count,
@@ -539,7 +819,7 @@ int sdf_expert_linear(int type, const void *rows, uint64_t rows_stride, uint64_t
     if (count == 0 || out_width == 0) return SDF_OK;
     if (!offsets || !out || (width > 0 && (!rows || (num_experts > 0 && !weight))))
         return fail(SDF_E_INVALID, "NULL pointer argument");
-    const Plan plan = plan_rows(count, num_experts, true, out_width, width, false);
+    const Plan plan = plan_rows(count, num_experts, true, out_width, width, false, false);
     if ((rc = check_scratch(scratch, scratch_bytes, plan.bytes)) != SDF_OK) return rc;
     if ((rc = check_blocks("sdf_expert_linear", plan)) != SDF_OK) return rc;
     ProductArgs p = {};
@@ -559,7 +839,7 @@ int sdf_expert_linear(int type, const void *rows, uint64_t rows_stride, uint64_t
 size_t sdf_expert_linear_backward_scratch_bytes(uint64_t count, uint32_t num_experts,
                                                 uint32_t width, uint32_t out_width) {
     if (count >= 1ull << 31 || num_experts > SDF_MAX_EXPERTS || num_experts == 0) return 0;
-    const size_t a = plan_rows(count, num_experts, true, width, out_width, false).bytes;
+    const size_t a = plan_rows(count, num_experts, true, width, out_width, true, false).bytes;
     const size_t b = plan_weights(count, num_experts, out_width, width, false, false).bytes;
     return a > b ? a : b; // one after the other
 }
@@ -587,7 +867,7 @@ int sdf_expert_linear_backward(int type, const void *out_grad, uint64_t out_grad
     p.partial = static_cast<float *>(scratch);
     p.scale = 1.0f;
     if (want_rows) {
-        const Plan plan = plan_rows(count, num_experts, true, width, out_width, false);
+        const Plan plan = plan_rows(count, num_experts, true, width, out_width, true, false);
         if ((rc = check_blocks("sdf_expert_linear_backward", plan)) != SDF_OK) return rc;
         p.a = {out_grad, out_grad_stride, 0, nullptr};
         p.b = {weight, width, (uint64_t)out_width * width, nullptr};
