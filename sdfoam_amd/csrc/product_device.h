@@ -186,7 +186,7 @@ struct ProductArgs {
     Operand a, b;
     Groups groups;
     uint32_t m, n; // rows form: n alone; weights form: both
-    uint32_t n_out; // columns written, those past n as 0 (at most as many tiles); 0: n
+    uint32_t n_out; // narrow rows: columns written, those past n as 0 (at most as many tiles); 0: n
     uint32_t k;    // rows form
     uint32_t splits, k_each; // of the inner dimension; k_each: a multiple of 64
     bool parts;              // the sums go to `partial` and are joined from there
@@ -194,7 +194,7 @@ struct ProductArgs {
     uint64_t out_stride;
     const int32_t *out_index; // rows form: the row of the result for a place; NULL: itself
     float *partial;           // [split][rows or group m][n], unscaled
-    float scale;
+    float scale;              // narrow tiles and their joining; 1 for all others
     Beside beside;
     uint32_t tiles_n;
 };

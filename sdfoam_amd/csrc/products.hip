@@ -29,8 +29,7 @@ struct LoaderOf<true, T, S, kRows, kThreads> {
 // where they have many (beside_of_rows).  One after the other, each waits for its values: 200
 // rows, an adapter each, of 2,048 -> 32,768 bf16 and rank 16 took 247 us, 48 without them.
 constexpr uint32_t kFewAdapters = 3;
-__device__ __forceinline__ bool few_adapters(const ProductArgs &p, uint32_t m0, uint32_t rows, uint32_t mi) {
-    const int32_t mine = mi < rows ? p.beside.group_of[m0 + mi] : -1;
+__device__ __forceinline__ bool few_adapters(int32_t mine) {
     uint64_t left = __ballot(mine >= 0);
 #pragma unroll
     for (uint32_t k = 0; k < kFewAdapters; ++k)
@@ -83,10 +82,9 @@ __device__ __forceinline__ void beside_of_rows(const ProductArgs &p, uint32_t pl
 
 template <typename S, bool kAcross, int kTn>
 __device__ __forceinline__ void add_beside(const ProductArgs &p, uint32_t m0, uint32_t rows,
-                                           uint32_t mi, uint32_t n0, F16x *acc) {
+                                           uint32_t mi, int32_t mine, uint32_t n0, F16x *acc) {
     const uint32_t lane = threadIdx.x & 63u, l32 = lane & 31u, half = lane >> 5;
     const uint32_t place = m0 + min(mi, rows - 1);
-    const int32_t mine = mi < rows ? p.beside.group_of[place] : -1;
     uint64_t left = __ballot(mine >= 0);
     const float *inner = p.beside.inner + (uint64_t)place * p.beside.pitch + half * 4;
     while (left) {
@@ -123,6 +121,79 @@ __device__ __forceinline__ void add_beside(const ProductArgs &p, uint32_t m0, ui
     }
 }
 
+// A wave's 32 rows of kTn x 32 columns from n0 on, turned in LDS of its own (a lane has one
+// row, l32, and runs of 4 columns) to be written in pieces of 16 bytes side by side.  Rows
+// [0, rows) are written, the l32-th to row_at(to_row of lane l32).
+template <int kTn> constexpr uint32_t turn_bytes() { return 32 * (kTn * 32 * 4 + 16); }
+
+template <typename O, int kTn, typename RowAt>
+__device__ __forceinline__ void write_rows(const ProductArgs &p, char *turn, const F16x *sums, uint32_t rows,
+                                           uint32_t n0, int32_t to_row, RowAt row_at) {
+    constexpr uint32_t kE = 16 / sizeof(O), kPieces = kTn * 32 / kE;
+    constexpr uint32_t kBytes = kTn * 32 * sizeof(O) + 16;
+    const uint32_t lane = threadIdx.x & 63u, l32 = lane & 31u, half = lane >> 5;
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < kTn; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t n = j * 32 + q * 8 + half * 4;
+            Few<O, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = (O)sums[j][q * 4 + e];
+            *reinterpret_cast<Few<O, 4> *>(turn + l32 * kBytes + n * sizeof(O)) = o;
+        }
+    wave_sync();
+#pragma unroll
+    for (uint32_t t = 0; t < kPieces / 2; ++t) {
+        const uint32_t at = t * 64 + lane, r = at / kPieces, n = at % kPieces * kE;
+        const O *from = reinterpret_cast<const O *>(turn + r * kBytes) + n;
+        const int32_t row = __shfl(to_row, r);
+        if (r >= rows || n0 + n >= p.n) continue;
+        O *to = row_at(row) + n0 + n;
+        const uint32_t have = p.n - (n0 + n);
+        if (have >= kE) __builtin_memcpy(to, from, 16);
+        else
+#pragma unroll 1
+            for (uint32_t e = 0; e < have; ++e) to[e] = from[e];
+    }
+}
+
+// The same with the rows' adapters added one by one; a lane has a column.  The first row is
+// at `place`, lane l32 has the l32-th row's adapter.
+template <typename S, bool kAcross, typename O, int kTn, typename RowAt>
+__device__ __forceinline__ void write_by_row(const ProductArgs &p, char *turn, const F16x *sums, uint32_t place,
+                                             uint32_t rows, uint32_t n0, int32_t to_row, int32_t adapters,
+                                             RowAt row_at) {
+    static_assert(kTn * 32 == 64, "a lane for each column");
+    constexpr uint32_t kFloats = kTn * 32 + 4;
+    const uint32_t lane = threadIdx.x & 63u, l32 = lane & 31u, half = lane >> 5;
+    float *turned = reinterpret_cast<float *>(turn);
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < kTn; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            Few<float, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = sums[j][q * 4 + e];
+            *reinterpret_cast<Few<float, 4> *>(turned + l32 * kFloats + j * 32 + q * 8 + half * 4) = o;
+        }
+    wave_sync();
+    const uint32_t n = n0 + lane;
+    if (n >= p.n) return;
+    constexpr uint32_t kBatch = 4;
+    for (uint32_t r = 0; r < rows; r += kBatch) {
+        float extra[kBatch];
+        beside_of_rows<S, kAcross, kBatch>(p, place + r, rows - r, adapters, r, n, extra);
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; ++i)
+            if (r + i < rows)
+                row_at(__builtin_amdgcn_readlane(to_row, r + i))[n] =
+                    (O)(turned[(r + i) * kFloats + lane] + extra[i]);
+    }
+}
+
 constexpr uint32_t kXcds = 8;
 // Blocks go to the XCDs in turn; of `tiles_m` x tiles_n tiles each XCD takes a run, kGroup
 // tiles of rows by all of the columns at a time, so that its L2 holds what its blocks share.
@@ -144,6 +215,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
     constexpr int kWaves = kWavesM * kWavesN, kBlock = 64 * kWaves;
     constexpr int kTm = kM / kWavesM / 32, kTn = kN / kWavesN / 32, kK = TileOf<T>::kK;
     constexpr uint32_t kTile = (kM + kN) * 128;
+    constexpr uint32_t kTurn = turn_bytes<kTn>();
     __shared__ __attribute__((aligned(16))) char lds[2 * kTile];
     __shared__ uint32_t found[20];
     Feed<T, kWeights, kM, kWaves, kDirect> a;
@@ -193,8 +265,17 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
 
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t wm = wave % kWavesM * (kTm * 32), wn = wave / kWavesM * (kTn * 32);
-    const uint32_t l32 = lane & 31u, half = lane >> 5;
+    const uint32_t l32 = lane & 31u;
     F16x acc[kTm][kTn] = {};
+    // what the end needs of the rows, on its way meanwhile: where each goes, its adapter
+    int32_t groups[kTm], goes_to[kTm];
+    if constexpr (!kWeights)
+#pragma unroll
+        for (int i = 0; i < kTm; ++i) {
+            const uint32_t mi = wm + i * 32 + l32, place = m0 + min(mi, rows_m - 1);
+            groups[i] = p.beside.inner && split == 0 && mi < rows_m ? p.beside.group_of[place] : -1;
+            goes_to[i] = p.out_index && !p.parts ? p.out_index[place] : (int32_t)place;
+        }
     const Fragments<T, kWeights, kM, kTm> of_a(wm);
     const Fragments<T, kWeights || kAcrossB, kN, kTn> of_b(wn);
     if (k_begin < k_end) {
@@ -233,98 +314,38 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
         __syncthreads();
     }
 
-    // a lane has one row of the result (l32) and runs of 4 columns of it; a wave turns 32
-    // rows at a time in LDS of its own, to write each in pieces of 16 bytes side by side
-    constexpr uint32_t kTurn = 32 * (kTn * 32 * 4 + 16);
     static_assert(kWaves * kTurn <= sizeof(lds), "room for each wave");
     char *turn = lds + wave * kTurn;
     const uint64_t rows = kWeights ? (uint64_t)p.groups.groups * p.m : p.groups.total;
-    const uint64_t row0 = kWeights ? (uint64_t)group * p.m + m0 : m0;
     uint32_t by_row = 0; // bit i: its rows' adapters are added row by row
     if constexpr (!kWeights)
         if (p.beside.inner && split == 0)
 #pragma unroll
             for (int i = 0; i < kTm; ++i) {
-                if (few_adapters(p, m0, rows_m, wm + i * 32 + l32))
-                    add_beside<T, kAcrossB, kTn>(p, m0, rows_m, wm + i * 32 + l32, n0 + wn, acc[i]);
+                if (few_adapters(groups[i]))
+                    add_beside<T, kAcrossB, kTn>(p, m0, rows_m, wm + i * 32 + l32, groups[i], n0 + wn, acc[i]);
                 else by_row |= 1u << i;
             }
-    // rows whose adapters are added one by one: a lane has a column
-    const auto write_rows = [&](auto t, const F16x *sums, uint32_t first, auto row_at, float scale) {
-        typedef decltype(t) O;
-        constexpr uint32_t kFloats = kTn * 32 + 4;
-        float *turned = reinterpret_cast<float *>(turn);
-        wave_sync();
 #pragma unroll
-        for (int j = 0; j < kTn; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                Few<float, 4> o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = sums[j][q * 4 + e];
-                *reinterpret_cast<Few<float, 4> *>(turned + l32 * kFloats + j * 32 + q * 8 + half * 4) = o;
-            }
-        wave_sync();
-        const uint32_t n = n0 + wn + lane, rows_here = first < rows_m ? min(32u, rows_m - first) : 0u;
-        static_assert(kTn * 32 == 64, "a lane for each column");
-        const int32_t groups = l32 < rows_here ? p.beside.group_of[m0 + first + l32] : -1;
-        if (n >= p.n) return;
-        constexpr uint32_t kBatch = 4;
-        for (uint32_t r = 0; r < rows_here; r += kBatch) {
-            float extra[kBatch];
-            beside_of_rows<T, kAcrossB, kBatch>(p, m0 + first + r, rows_here - r, groups, r, n, extra);
-#pragma unroll
-            for (uint32_t i = 0; i < kBatch; ++i)
-                if (r + i < rows_here)
-                    row_at(row0 + first + r + i)[n] = (O)(scale * (turned[(r + i) * kFloats + lane] + extra[i]));
-        }
-    };
-    const auto write = [&](auto t, const F16x *sums, uint32_t first, auto row_at, float scale) {
-        typedef decltype(t) O;
-        constexpr uint32_t kE = 16 / sizeof(O), kPieces = kTn * 32 / kE;
-        constexpr uint32_t kBytes = kTn * 32 * sizeof(O) + 16;
-        wave_sync();
-#pragma unroll
-        for (int j = 0; j < kTn; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t n = j * 32 + q * 8 + half * 4;
-                Few<O, 4> o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    o.v[e] = n0 + wn + n + e < p.n ? (O)(scale * sums[j][q * 4 + e]) : (O)0.0f;
-                *reinterpret_cast<Few<O, 4> *>(turn + l32 * kBytes + n * sizeof(O)) = o;
-            }
-        wave_sync();
-#pragma unroll
-        for (uint32_t t = 0; t < kPieces / 2; ++t) {
-            const uint32_t at = t * 64 + lane, r = at / kPieces, n = at % kPieces * kE;
-            const uint32_t m = first + r;
-            const O *from = reinterpret_cast<const O *>(turn + r * kBytes) + n;
-            if (m >= rows_m || n0 + wn + n >= p.n_out) continue;
-            O *to = row_at(row0 + m) + n0 + wn + n;
-            const uint32_t have = p.n_out - (n0 + wn + n);
-            if (have >= kE) __builtin_memcpy(to, from, 16);
-            else
-#pragma unroll 1
-                for (uint32_t e = 0; e < have; ++e) to[e] = from[e];
-        }
-    };
-    if (p.parts) {
-#pragma unroll
-        for (int i = 0; i < kTm; ++i) {
-            const auto row_at = [&](uint64_t row) { return p.partial + (split * rows + row) * p.n_out; };
-            if (!kWeights && (by_row >> i & 1u)) write_rows(0.0f, acc[i], wm + i * 32, row_at, 1.0f);
-            else write(0.0f, acc[i], wm + i * 32, row_at, 1.0f);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kTm; ++i) {
-            const auto row_at = [&](uint64_t row) {
-                return static_cast<T *>(p.out) + (p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride;
+    for (int i = 0; i < kTm; ++i) {
+        const uint32_t first = wm + i * 32;
+        int32_t to_row = (int32_t)(m0 + first + l32), adapters = -1; // of the lane's row
+        if constexpr (!kWeights) to_row = goes_to[i], adapters = groups[i];
+        const uint32_t left = first < rows_m ? min(32u, rows_m - first) : 0u; // of the 32 rows
+        if (p.parts) {
+            const auto row_at = [&](int32_t row) {
+                return p.partial + (split * rows + (kWeights ? (uint64_t)group * p.m : 0) + (uint32_t)row) * p.n;
             };
-            if (!kWeights && (by_row >> i & 1u)) write_rows(T(), acc[i], wm + i * 32, row_at, p.scale);
-            else write(T(), acc[i], wm + i * 32, row_at, p.scale);
+            if (!kWeights && (by_row >> i & 1u))
+                write_by_row<T, kAcrossB, float, kTn>(p, turn, acc[i], m0 + first, left, n0 + wn, to_row, adapters, row_at);
+            else write_rows<float, kTn>(p, turn, acc[i], left, n0 + wn, to_row, row_at);
+        } else {
+            const auto row_at = [&](int32_t row) {
+                return static_cast<T *>(p.out) + ((kWeights ? (uint64_t)group * p.m : 0) + (uint32_t)row) * p.out_stride;
+            };
+            if (!kWeights && (by_row >> i & 1u))
+                write_by_row<T, kAcrossB, T, kTn>(p, turn, acc[i], m0 + first, left, n0 + wn, to_row, adapters, row_at);
+            else write_rows<T, kTn>(p, turn, acc[i], left, n0 + wn, to_row, row_at);
         }
     }
 }
@@ -430,7 +451,8 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs p) {
         const uint32_t mi = wm + i * 32 + l32;
         if constexpr (!kWeights)
             if (p.beside.inner && split == 0)
-                add_beside<SB, kAcrossB, kTn>(p, m0, rows_m, mi, n0 + wn, acc[i]);
+                add_beside<SB, kAcrossB, kTn>(p, m0, rows_m, mi, mi < rows_m ? p.beside.group_of[m0 + mi] : -1,
+                                              n0 + wn, acc[i]);
         if (mi >= rows_m) continue;
         const uint64_t row = kWeights ? (uint64_t)group * p.m + m0 + mi : m0 + mi;
 #pragma unroll
@@ -502,7 +524,66 @@ template <typename O, bool kAcross> __global__ __launch_bounds__(256) void join_
             }
         }
     }
-    static_cast<O *>(p.out)[(p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride + n] = (O)(p.scale * (sum + extra));
+    static_cast<O *>(p.out)[(p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride + n] = (O)(sum + extra);
+}
+
+// ---- a short inner dimension -------------------------------------------------------------
+//
+// At most 128 bytes of it: a wave keeps 32 rows in registers and goes over the columns, 64 at
+// a time, their fragments from the caches while the 64 before are written, without LDS but to
+// turn what it writes and without waiting for another wave.  Bound by what it reads and
+// writes; tiles wait in turn for rows, columns and each other.
+constexpr uint32_t kShortWaves = 4, kShortRows = 32 * kShortWaves;
+
+template <typename T> __global__ __launch_bounds__(64 * kShortWaves, 3) void short_kernel(ProductArgs p, uint32_t columns) {
+    constexpr uint32_t kC = TileOf<T>::kC, kPieces = 4;
+    __shared__ __attribute__((aligned(16))) char turns[kShortWaves * turn_bytes<2>()];
+    __shared__ uint32_t found[20];
+    TilesOfRows<kShortRows, 64 * kShortWaves> tiles(p.groups, found);
+    if (blockIdx.x >= tiles.count()) return;
+    const TileOfRows t = tiles.find(blockIdx.x);
+    const bool none = p.groups.offsets && t.group == p.groups.groups; // rows of no group: zeros
+    const uint32_t lane = threadIdx.x & 63u, l32 = lane & 31u, half = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave * 32 >= t.rows) return;
+    const uint32_t m0 = t.first + wave * 32, rows = min(32u, t.rows - wave * 32), k_all = none ? 0u : p.k;
+    char *turn = turns + wave * turn_bytes<2>();
+    const uint32_t place = m0 + min(l32, rows - 1);
+    // pieces 2 kk + half of a row, of zeros past the end
+    const auto pieces = [&](const T *row, Chunk<T> *c) {
+#pragma unroll
+        for (uint32_t kk = 0; kk < kPieces; ++kk) {
+            const uint32_t at = (2 * kk + half) * kC;
+            c[kk] = __builtin_bit_cast(Chunk<T>, load_some<T, kC>(row + at, k_all > at ? k_all - at : 0u));
+        }
+    };
+    const T *w = static_cast<const T *>(p.b.base) + (none ? 0u : t.group) * p.b.group_stride;
+    const uint32_t from = blockIdx.y * columns, to = min(from + columns, p.n);
+    Chunk<T> fa[kPieces], fb[2][kPieces];
+    pieces(static_cast<const T *>(p.a.base) + (uint64_t)(p.a.index ? (uint32_t)p.a.index[place] : place) * p.a.stride, fa);
+    const auto bring = [&](uint32_t n0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) pieces(w + (uint64_t)min(n0 + j * 32 + l32, p.n - 1) * p.b.stride, fb[j]);
+    };
+    bring(from);
+    const int32_t group = p.beside.inner && l32 < rows ? p.beside.group_of[place] : -1;
+    const int32_t goes_to = p.out_index ? p.out_index[place] : (int32_t)place;
+    const bool few = few_adapters(group);
+    for (uint32_t n0 = from; n0 < to; n0 += 64) {
+        F16x acc[2] = {};
+#pragma unroll
+        for (uint32_t kk = 0; kk < kPieces; ++kk)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma32<T>(acc[j], fb[j][kk], fa[kk]);
+        if (n0 + 64 < to) bring(n0 + 64);
+        const auto row_at = [&](int32_t row) { return static_cast<T *>(p.out) + (uint32_t)row * p.out_stride; };
+        if (few) {
+            if (p.beside.inner) add_beside<T, false, 2>(p, m0, rows, l32, group, n0, acc);
+            write_rows<T, 2>(p, turn, acc, rows, n0, goes_to, row_at);
+        } else {
+            write_by_row<T, false, T, 2>(p, turn, acc, m0, rows, n0, goes_to, group, row_at);
+        }
+    }
 }
 
 // ---- few rows a group --------------------------------------------------------------------
@@ -607,7 +688,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ProductArgs p) {
             sum += extra;
         }
         const uint64_t row = p.out_index ? (uint32_t)p.out_index[place] : place;
-        static_cast<T *>(p.out)[row * p.out_stride + n] = (T)(p.scale * sum);
+        static_cast<T *>(p.out)[row * p.out_stride + n] = (T)sum;
     }
 }
 
@@ -680,7 +761,7 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
         plan.splits = 1;
         return plan;
     }
-    plan.large = !skinny && take_large(tiles_of_rows(rows, groups, grouped, 256) * ((n + 255) / 256),
+    plan.large = !skinny && k > 256 && take_large(tiles_of_rows(rows, groups, grouped, 256) * ((n + 255) / 256),
                                        tiles_of_rows(rows, groups, grouped, 128) * ((n + 127) / 128));
     const uint32_t km = plan.large ? 256 : 128, kn = skinny ? 32 : km;
     plan.tiles_n = (n + kn - 1) / kn;
@@ -688,8 +769,8 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
     // few tiles: the inner dimension in several parts, of 512 elements at least, until the
     // chip has a block for each of its places
     plan.splits = 1;
-    if (plan.tiles > 0 && !plan.large && plan.tiles < 256) {
-        const uint64_t want = 512 / plan.tiles, most = k / 512;
+    if (plan.tiles > 0 && !plan.large && plan.tiles < (skinny ? 768 : 256)) {
+        const uint64_t want = (skinny ? 1536 : 512) / plan.tiles, most = k / (skinny ? 256 : 512);
         plan.splits = (uint32_t)(want < most ? want : most);
         if (plan.splits < 1) plan.splits = 1;
     }
@@ -707,8 +788,10 @@ Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool n
     plan.tiles_n = (n + kn - 1) / kn;
     plan.tiles = (uint64_t)groups * ((m + km - 1) / km) * plan.tiles_n;
     plan.splits = 1;
-    if (plan.tiles > 0 && !plan.large && plan.tiles < 256) {
-        const uint64_t want = 512 / plan.tiles, most = rows / groups / 256;
+    // narrow ones wait for memory more than they multiply: more blocks, shorter parts
+    const bool narrow = narrow_m || narrow_n;
+    if (plan.tiles > 0 && !plan.large && plan.tiles < (narrow ? 768 : 256)) {
+        const uint64_t want = (narrow ? 1536 : 512) / plan.tiles, most = rows / groups / (narrow ? 96 : 256);
         plan.splits = (uint32_t)(want < most ? want : most);
         if (plan.splits < 1) plan.splits = 1;
     }
@@ -739,6 +822,13 @@ hipError_t product_rows(int type, const ProductArgs &args, const Plan &plan, boo
         typedef decltype(t) T;
         if (plan.thin_m) {
             launch_thin<T>(p, plan, s);
+        } else if (!skinny && !across && !p.parts && p.k <= TileOf<T>::kK) {
+            // a share of the columns each, so many that the chip has waves enough
+            const uint64_t tiles = tiles_of_rows(p.groups.total, p.groups.groups, p.groups.offsets != nullptr, kShortRows);
+            const uint64_t shares = 2048 / tiles + 1, steps = (p.n + 63) / 64;
+            const uint32_t columns = 64 * (uint32_t)((steps + shares - 1) / shares);
+            const dim3 blocks((uint32_t)tiles, (p.n + columns - 1) / columns);
+            short_kernel<T><<<blocks, 64 * kShortWaves, 0, s>>>(p, columns);
         } else if (skinny) {
             if (across) product_kernel<T, T, T, false, true, 128, 32, 4, 1, float><<<grid, kThreads, 0, s>>>(p);
             else product_kernel<T, T, T, false, false, 128, 32, 4, 1, float><<<grid, kThreads, 0, s>>>(p);
