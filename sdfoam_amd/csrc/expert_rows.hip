@@ -286,6 +286,14 @@ template <typename T, int kP>
 __device__ __forceinline__ void store_piece(T *p, const Piece<T, kP> &c) {
     __builtin_memcpy(p, &c, sizeof(c));
 }
+// Rows that fill the caches go past them.  131,072 rows of 1,024 bf16 written from 16,384:
+// 89 -> 54 us.
+constexpr uint64_t kPastBytes = 128ull << 20;
+template <bool kPast, typename T, int kP>
+__device__ __forceinline__ void store_piece_if(T *p, const Piece<T, kP> &c) {
+    if constexpr (kPast && sizeof(c) == 16) store_past<sizeof(T)>(p, c);
+    else store_piece<T, kP>(p, c);
+}
 
 // A group of `lanes` per row; a lane has every lanes-th piece of it.
 #define ROW_OF_GROUP                                                                       \
@@ -293,7 +301,7 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T, kP> &c) {
     const uint32_t lane = threadIdx.x % a.lanes;                                           \
     const uint32_t pieces = (a.width + kP - 1) / kP
 
-template <typename T, int kP> __global__ __launch_bounds__(256) void spread_kernel(RowArgs a) {
+template <typename T, int kP, bool kPast> __global__ __launch_bounds__(256) void spread_kernel(RowArgs a) {
     ROW_OF_GROUP;
     if (i >= a.rows) return;
     const T *x = static_cast<const T *>(a.in) + i * a.stride;
@@ -304,7 +312,7 @@ template <typename T, int kP> __global__ __launch_bounds__(256) void spread_kern
             const int32_t p = a.places[i * a.choices + k];
             const uint64_t at = p < 0 ? -1 - (int64_t)p : p;
             if (at >= a.entries) continue; // no place of these rows
-            store_piece<T, kP>(static_cast<T *>(a.out) + at * a.width + col, p < 0 ? zero : v);
+            store_piece_if<kPast, T, kP>(static_cast<T *>(a.out) + at * a.width + col, p < 0 ? zero : v);
         }
     }
 }
@@ -332,7 +340,7 @@ template <typename T, int kP> __global__ __launch_bounds__(256) void combine_ker
     }
 }
 
-template <typename T, int kP>
+template <typename T, int kP, bool kPast>
 __global__ __launch_bounds__(256) void combine_backward_kernel(RowArgs a) {
     ROW_OF_GROUP;
     const bool in_range = i < a.rows;
@@ -353,7 +361,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(RowArgs a) {
 #pragma unroll
                         for (int e = 0; e < kP; ++e)
                             o.v[e] = (T)(p < 0 ? 0.0f : w * (float)v.v[e]);
-                        store_piece<T, kP>(static_cast<T *>(a.out) + at * a.width + col, o);
+                        store_piece_if<kPast, T, kP>(static_cast<T *>(a.out) + at * a.width + col, o);
                     }
                     if (a.sorted && p >= 0) {
                         const Piece<T, kP> y = load_piece<T, kP>(
@@ -453,8 +461,10 @@ int sdf_expert_rows(int type, const void *rows, uint64_t rows_stride, uint64_t c
         with_pieces(type, a, s, [&](auto t, RowArgs &b, uint64_t i, uint32_t blocks, bool whole) {
             typedef decltype(t) T;
             b.in = static_cast<const T *>(a.in) + i * a.stride;
-            if (whole) spread_kernel<T, 16 / sizeof(T)><<<blocks, 256, 0, s>>>(b);
-            else spread_kernel<T, 1><<<blocks, 256, 0, s>>>(b);
+            const bool past = a.entries * a.width * sizeof(T) >= kPastBytes;
+            if (whole && past) spread_kernel<T, 16 / sizeof(T), true><<<blocks, 256, 0, s>>>(b);
+            else if (whole) spread_kernel<T, 16 / sizeof(T), false><<<blocks, 256, 0, s>>>(b);
+            else spread_kernel<T, 1, false><<<blocks, 256, 0, s>>>(b);
         });
     return e == hipSuccess ? SDF_OK : hip_fail(e, "expert_rows");
 }
@@ -517,8 +527,10 @@ int sdf_expert_combine_backward(int type, const void *out_grad, uint64_t out_gra
         with_pieces(type, a, s, [&](auto t, RowArgs &b, uint64_t i, uint32_t blocks, bool whole) {
             typedef decltype(t) T;
             b.in = static_cast<const T *>(a.in) + i * a.stride;
-            if (whole) combine_backward_kernel<T, 16 / sizeof(T)><<<blocks, 256, 0, s>>>(b);
-            else combine_backward_kernel<T, 1><<<blocks, 256, 0, s>>>(b);
+            const bool past = a.entries * a.width * sizeof(T) >= kPastBytes;
+            if (whole && past) combine_backward_kernel<T, 16 / sizeof(T), true><<<blocks, 256, 0, s>>>(b);
+            else if (whole) combine_backward_kernel<T, 16 / sizeof(T), false><<<blocks, 256, 0, s>>>(b);
+            else combine_backward_kernel<T, 1, false><<<blocks, 256, 0, s>>>(b);
         });
     return e == hipSuccess ? SDF_OK : hip_fail(e, "expert_combine_backward");
 }

@@ -4,9 +4,8 @@
 //   factor = scale min(1, max_norm / (norm + 1e-6))        out = factor g
 //
 // Squares are added in fp64: those of floats below 1e-19 or above 1e19 leave fp32's range,
-// and memory is the bound all the same.  The tensors' addresses travel in the launch's
-// arguments, kTensors a launch: nothing is copied to the device beforehand, a captured
-// graph keeps them.  Every block's share is decided by the sizes alone, and the blocks'
+// and memory is the bound all the same.  The tensors' addresses travel in the launches'
+// arguments: nothing is copied to the device beforehand, a captured graph keeps them.  Every block's share is decided by the sizes alone, and the blocks'
 // sums are added in order: every run gives the same.
 #include <algorithm>
 #include <new>
@@ -22,35 +21,57 @@ namespace {
 
 constexpr uint32_t kThreads = 512;
 constexpr uint32_t kChunk = 16384; // elements a block takes at a time
-constexpr uint32_t kTensors = 96;
-constexpr uint32_t kBlocks = 1024; // a launch
-// Up to so many blocks' sums, every block that scales adds them up itself; more are
-// added by a launch of their own.
-constexpr uint32_t kFewSums = 4096;
+constexpr uint32_t kBlocks = 1024; // a launch: four a CU, all of them there at once
+constexpr uint32_t kTensors = 96;  // that a launch's arguments hold
 
-struct Tensors {
-    const void *in[kTensors];
-    void *out[kTensors];
-    uint64_t count[kTensors];
-    uint32_t chunk[kTensors + 1]; // chunks before each tensor's
-    uint8_t type[kTensors], out_type[kTensors];
-    uint32_t tensors;
-};
+constexpr uint32_t kPastChunks = (128u << 20) / 4 / kChunk; // 128 MiB of floats
 
-struct Piece {
-    uint32_t tensor;
-    uint64_t first, count;
+struct Entry {
+    const void *in;
+    void *out;
+    uint64_t count;
+    uint32_t chunk; // chunks before the tensor's
+    uint8_t type, out_type;
 };
-__device__ __forceinline__ Piece piece_of(const Tensors &t, uint32_t chunk) {
-    uint32_t lo = 0, hi = t.tensors; // chunk[lo] <= chunk < chunk[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (t.chunk[mid] <= chunk) lo = mid;
+// Few tensors come with the arguments; more are written to a table first, kTensors a launch,
+// so that one launch goes over all of them (four launches each way for 300 tensors of 500M
+// bf16 elements: 955 us).
+struct Few {
+    Entry e[kTensors];
+    uint32_t tensors, chunks;
+};
+struct Many {
+    const Entry *e;
+    uint32_t tensors, chunks;
+};
+__global__ __launch_bounds__(64) void table_kernel(Few t, Entry *to) {
+    for (uint32_t i = threadIdx.x; i < t.tensors; i += 64) to[i] = t.e[i];
+}
+
+// f(tensor, first element, elements) for the block's run of chunks, in order or from its end:
+// what the last pass read last is then still in the caches.
+template <bool kBack, typename Source, typename F>
+__device__ __forceinline__ void each_chunk(const Source &t, F f) {
+    const uint32_t each = (t.chunks + gridDim.x - 1) / gridDim.x;
+    const uint32_t begin = min(blockIdx.x * each, t.chunks), end = min(begin + each, t.chunks);
+    if (begin == end) return;
+    const uint32_t start = kBack ? end - 1 : begin;
+    uint32_t at = 0, hi = t.tensors; // e[at].chunk <= start < e[hi].chunk
+    while (hi - at > 1) {
+        const uint32_t mid = (at + hi) / 2;
+        if (t.e[mid].chunk <= start) at = mid;
         else hi = mid;
     }
-    const uint64_t first = (uint64_t)(chunk - t.chunk[lo]) * kChunk;
-    const uint64_t left = t.count[lo] - first;
-    return {lo, first, left < kChunk ? left : kChunk};
+    for (uint32_t k = 0; k < end - begin; ++k) {
+        const uint32_t c = kBack ? end - 1 - k : begin + k;
+        if (kBack)
+            while (t.e[at].chunk > c) --at;
+        else
+            while (at + 1 < t.tensors && t.e[at + 1].chunk <= c) ++at;
+        const uint64_t first = (uint64_t)(c - t.e[at].chunk) * kChunk;
+        const uint64_t left = t.e[at].count - first;
+        f(t.e[at], first, (uint32_t)(left < kChunk ? left : kChunk));
+    }
 }
 
 __device__ __forceinline__ double block_sum(double x, double *lds) {
@@ -65,31 +86,29 @@ __device__ __forceinline__ double block_sum(double x, double *lds) {
 
 template <typename T> __device__ __forceinline__ double squares(const T *p, uint32_t n) {
     constexpr uint32_t kN = Chunk<T>::kN;
-    double s = 0.0;
+    double s[4] = {};
     const uint32_t whole = n / kN;
 #pragma unroll 4
     for (uint32_t c = threadIdx.x; c < whole; c += kThreads) {
         const Chunk<T> v = load_chunk(p + (uint64_t)c * kN);
 #pragma unroll
-        for (uint32_t e = 0; e < kN; ++e) s = fma((double)v[e], (double)v[e], s);
+        for (uint32_t e = 0; e < kN; ++e) s[e % 4] = fma((double)v[e], (double)v[e], s[e % 4]);
     }
     for (uint32_t i = whole * kN + threadIdx.x; i < n; i += kThreads) {
         const double v = (double)(float)p[i];
-        s = fma(v, v, s);
+        s[0] = fma(v, v, s[0]);
     }
-    return s;
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-__global__ __launch_bounds__(kThreads) void squares_kernel(Tensors t, double *sums) {
+template <typename Source> __global__ __launch_bounds__(kThreads) void squares_kernel(Source t, double *sums) {
     __shared__ double lds[kThreads / 64];
     double s = 0.0;
-    for (uint32_t c = blockIdx.x; c < t.chunk[t.tensors]; c += gridDim.x) {
-        const Piece k = piece_of(t, c);
-        const uint32_t n = (uint32_t)k.count;
-        if (t.type[k.tensor] == SDF_TYPE_F32) s += squares(static_cast<const float *>(t.in[k.tensor]) + k.first, n);
-        else if (t.type[k.tensor] == SDF_TYPE_F16) s += squares(static_cast<const half_t *>(t.in[k.tensor]) + k.first, n);
-        else s += squares(static_cast<const bf16_t *>(t.in[k.tensor]) + k.first, n);
-    }
+    each_chunk<false>(t, [&](const Entry &k, uint64_t first, uint32_t n) {
+        if (k.type == SDF_TYPE_F32) s += squares(static_cast<const float *>(k.in) + first, n);
+        else if (k.type == SDF_TYPE_F16) s += squares(static_cast<const half_t *>(k.in) + first, n);
+        else s += squares(static_cast<const bf16_t *>(k.in) + first, n);
+    });
     s = block_sum(s, lds);
     if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
@@ -100,93 +119,69 @@ __device__ __forceinline__ double total_of(const double *sums, uint32_t n, doubl
     return block_sum(s, lds);
 }
 
-__global__ __launch_bounds__(kThreads) void norm_kernel(const double *sums, uint32_t n, float scale,
-                                                        float *norm, double *total) {
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double *sums, uint32_t n, float scale, float *norm) {
     __shared__ double lds[kThreads / 64];
     const double s = total_of(sums, n, lds);
-    if (threadIdx.x == 0) {
-        if (norm) *norm = (float)((double)scale * sqrt(s));
-        if (total) *total = s;
-    }
+    if (threadIdx.x == 0) *norm = (float)((double)scale * sqrt(s));
 }
 
+// 16 bytes of the result a thread, so that a wavefront writes whole lines; large results past
+// the caches.
 template <typename T, typename O>
-__device__ __forceinline__ void scaled(const T *p, O *o, uint32_t n, float f) {
-    constexpr uint32_t kN = Chunk<T>::kN;
+__device__ __forceinline__ void scaled(const void *in, void *out, uint64_t first, uint32_t n, float f, bool past) {
+    constexpr uint32_t kN = 16 / sizeof(O);
+    struct In {
+        T v[kN];
+    };
+    struct Out {
+        O v[kN];
+    };
+    const T *p = static_cast<const T *>(in) + first;
+    O *o = static_cast<O *>(out) + first;
+    // whole pieces begin where the result's 128 bytes do
+    const uint32_t head = min(n, (uint32_t)(-reinterpret_cast<uintptr_t>(o) & 127u) / (uint32_t)sizeof(O));
+    if (threadIdx.x < head) o[threadIdx.x] = (O)(f * (float)p[threadIdx.x]);
+    p += head, o += head, n -= head;
     const uint32_t whole = n / kN;
+    const auto go = [&](auto store) {
 #pragma unroll 4
-    for (uint32_t c = threadIdx.x; c < whole; c += kThreads) {
-        const Chunk<T> v = load_chunk(p + (uint64_t)c * kN);
-        O r[kN];
+        for (uint32_t c = threadIdx.x; c < whole; c += kThreads) {
+            In v;
+            __builtin_memcpy(&v, p + (uint64_t)c * kN, sizeof(v));
+            Out r;
 #pragma unroll
-        for (uint32_t e = 0; e < kN; ++e) r[e] = (O)(f * v[e]);
-        __builtin_memcpy(o + (uint64_t)c * kN, r, sizeof(r));
-    }
+            for (uint32_t e = 0; e < kN; ++e) r.v[e] = (O)(f * (float)v.v[e]);
+            store(o + (uint64_t)c * kN, r);
+        }
+    };
+    if (past) go([](O *to, const Out &r) { store_past<sizeof(O)>(to, r); });
+    else go([](O *to, const Out &r) { __builtin_memcpy(to, &r, sizeof(r)); });
     for (uint32_t i = whole * kN + threadIdx.x; i < n; i += kThreads) o[i] = (O)(f * (float)p[i]);
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(Tensors t, const double *sums, uint32_t n,
-                                                         float scale, float max_norm, float *norm) {
+// Every block adds the other pass's sums itself, in the same order (8 KB from L2).
+template <typename Source>
+__global__ __launch_bounds__(kThreads) void scale_kernel(Source t, const double *sums, uint32_t n, float scale,
+                                                         float max_norm, float *norm) {
     __shared__ double lds[kThreads / 64];
     const double size = (double)scale * sqrt(total_of(sums, n, lds));
     double c = (double)max_norm / (size + 1e-6);
     c = c > 1.0 ? 1.0 : c; // NaN stays
     const float f = (float)(scale * c);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)size;
-    for (uint32_t c = blockIdx.x; c < t.chunk[t.tensors]; c += gridDim.x) {
-        const Piece k = piece_of(t, c);
-        const uint32_t count = (uint32_t)k.count;
-        const void *in = t.in[k.tensor];
-        void *out = t.out[k.tensor];
-        if (in == out && f == 1.0f) continue;
-        const int type = t.type[k.tensor];
-        if (type == SDF_TYPE_F32)
-            scaled(static_cast<const float *>(in) + k.first, static_cast<float *>(out) + k.first, count, f);
-        else if (t.out_type[k.tensor] == SDF_TYPE_F32) {
-            if (type == SDF_TYPE_F16)
-                scaled(static_cast<const half_t *>(in) + k.first, static_cast<float *>(out) + k.first, count, f);
-            else
-                scaled(static_cast<const bf16_t *>(in) + k.first, static_cast<float *>(out) + k.first, count, f);
-        } else if (type == SDF_TYPE_F16)
-            scaled(static_cast<const half_t *>(in) + k.first, static_cast<half_t *>(out) + k.first, count, f);
-        else
-            scaled(static_cast<const bf16_t *>(in) + k.first, static_cast<bf16_t *>(out) + k.first, count, f);
-    }
+    const bool past = t.chunks >= kPastChunks;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)size;
+    each_chunk<true>(t, [&](const Entry &k, uint64_t first, uint32_t n) {
+        if (k.in == k.out && f == 1.0f) return;
+        if (k.type == SDF_TYPE_F32) scaled<float, float>(k.in, k.out, first, n, f, past);
+        else if (k.type == SDF_TYPE_F16) {
+            if (k.out_type == SDF_TYPE_F32) scaled<half_t, float>(k.in, k.out, first, n, f, past);
+            else scaled<half_t, half_t>(k.in, k.out, first, n, f, past);
+        } else if (k.out_type == SDF_TYPE_F32) scaled<bf16_t, float>(k.in, k.out, first, n, f, past);
+        else scaled<bf16_t, bf16_t>(k.in, k.out, first, n, f, past);
+    });
 }
 
 constexpr uint64_t kMaxElements = 1ull << 40; // of all tensors: 32 bits count the chunks
-
-// kTensors tensors that have elements a launch; f(the tensors, the blocks of the launch).
-template <typename F>
-hipError_t each_launch(uint32_t n, const int *types, const void *const *in, const int *out_types,
-                       void *const *out, const uint64_t *counts, F f) {
-    Tensors t;
-    t.tensors = 0;
-    t.chunk[0] = 0;
-    const auto flush = [&]() -> hipError_t {
-        if (t.tensors == 0) return hipSuccess;
-        const uint32_t chunks = t.chunk[t.tensors];
-        f(t, chunks < kBlocks ? chunks : kBlocks);
-        t.tensors = 0;
-        return hipGetLastError();
-    };
-    for (uint32_t i = 0; i < n; ++i) {
-        if (counts[i] == 0) continue;
-        const uint64_t chunks = (counts[i] + kChunk - 1) / kChunk;
-        if (t.tensors == kTensors) {
-            const hipError_t e = flush();
-            if (e != hipSuccess) return e;
-        }
-        const uint32_t k = t.tensors++;
-        t.in[k] = in[i];
-        t.out[k] = out ? out[i] : nullptr;
-        t.count[k] = counts[i];
-        t.type[k] = (uint8_t)types[i];
-        t.out_type[k] = (uint8_t)(out ? out_types[i] : types[i]);
-        t.chunk[k + 1] = t.chunk[k] + (uint32_t)chunks;
-    }
-    return flush();
-}
 
 int check_tensors(uint32_t n, const int *types, const void *const *in, const uint64_t *counts) {
     if (n > 0 && (!types || !in || !counts)) return fail(SDF_E_INVALID, "NULL pointer argument");
@@ -233,14 +228,22 @@ int check_apart(uint32_t n, const int *types, const void *const *in, const int *
     return SDF_OK;
 }
 
-uint64_t sums_of(uint32_t n) { return ((uint64_t)n / kTensors + 2) * kBlocks; }
+template <typename Source>
+hipError_t run(const Source &t, bool scales, float max_norm, float scale, float *norm, double *sums,
+               hipStream_t s) {
+    const uint32_t blocks = t.chunks < kBlocks ? t.chunks : kBlocks;
+    if (blocks > 0) squares_kernel<<<blocks, kThreads, 0, s>>>(t, sums);
+    if (scales && blocks > 0) scale_kernel<<<blocks, kThreads, 0, s>>>(t, sums, blocks, scale, max_norm, norm);
+    else norm_kernel<<<1, kThreads, 0, s>>>(sums, blocks, scale, norm);
+    return hipGetLastError();
+}
 
 } // namespace
 
 extern "C" {
 
 size_t sdf_clip_gradients_scratch_bytes(uint32_t num_tensors) {
-    return round_up((sums_of(num_tensors) + 1) * 8);
+    return round_up(kBlocks * 8) + (num_tensors > kTensors ? round_up((size_t)num_tensors * sizeof(Entry)) : 0);
 }
 
 int sdf_clip_gradients(uint32_t num_tensors, const int *types, const void *const *gradients,
@@ -265,31 +268,31 @@ int sdf_clip_gradients(uint32_t num_tensors, const int *types, const void *const
         return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     double *sums = static_cast<double *>(scratch);
-    const double *from = sums;
-    const uint64_t room = sums_of(num_tensors);
-    uint32_t n = 0;
-    hipError_t e = each_launch(num_tensors, types, gradients, nullptr, nullptr, counts,
-                               [&](const Tensors &t, uint32_t blocks) {
-                                   squares_kernel<<<blocks, kThreads, 0, s>>>(t, sums + n);
-                                   n += blocks;
-                               });
-    bool said = false;
-    if (e == hipSuccess && out && n > 0) {
-        if (n > kFewSums) {
-            norm_kernel<<<1, kThreads, 0, s>>>(sums, n, scale, nullptr, sums + room);
-            from = sums + room;
-            n = 1;
+    Entry *table = reinterpret_cast<Entry *>(static_cast<char *>(scratch) + round_up(kBlocks * 8));
+    Few t;
+    t.tensors = 0;
+    uint32_t chunks = 0, written = 0;
+    hipError_t e = hipSuccess;
+    for (uint32_t i = 0; i < num_tensors && e == hipSuccess; ++i) {
+        if (counts[i] == 0) continue;
+        if (t.tensors == kTensors) {
+            table_kernel<<<1, 64, 0, s>>>(t, table + written);
+            e = hipGetLastError();
+            written += kTensors;
+            t.tensors = 0;
         }
-        e = each_launch(num_tensors, types, gradients, out_types, out, counts,
-                        [&](const Tensors &t, uint32_t blocks) {
-                            scale_kernel<<<blocks, kThreads, 0, s>>>(t, from, n, scale, max_norm,
-                                                                     said ? nullptr : norm);
-                            said = true;
-                        });
+        t.e[t.tensors++] = {gradients[i], out ? out[i] : nullptr, counts[i], chunks, (uint8_t)types[i],
+                            (uint8_t)(out ? out_types[i] : types[i])};
+        chunks += (uint32_t)((counts[i] + kChunk - 1) / kChunk);
     }
-    if (e == hipSuccess && !said) {
-        norm_kernel<<<1, kThreads, 0, s>>>(sums, n, scale, norm, nullptr);
+    t.chunks = chunks;
+    if (e == hipSuccess && written > 0) {
+        table_kernel<<<1, 64, 0, s>>>(t, table + written);
         e = hipGetLastError();
+        if (e == hipSuccess)
+            e = run(Many{table, written + t.tensors, chunks}, out != nullptr, max_norm, scale, norm, sums, s);
+    } else if (e == hipSuccess) {
+        e = run(t, out != nullptr, max_norm, scale, norm, sums, s);
     }
     return e == hipSuccess ? SDF_OK : hip_fail(e, "clip_gradients");
 }

@@ -31,29 +31,21 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _gradients(call: str, gradients: Iterable[Optional[torch.Tensor]]):
-    if isinstance(gradients, torch.Tensor):
-        gradients = [gradients]
-    tensors = list(gradients)
-    device = None
-    for g in tensors:
-        if g is None:
-            continue
+    tensors = [gradients] if isinstance(gradients, torch.Tensor) else list(gradients)
+    some = [g for g in tensors if g is not None]
+    if not some:
+        raise RuntimeError("gradients must hold at least one tensor")
+    for g in some:
         _element_type("gradients", g)
-        _no_tangent(call, gradients=g)
         if not g.is_contiguous() and g.numel() > 0 and not _dense(g):
             raise RuntimeError("gradients must fill their memory without gaps or overlaps")
-    for g in tensors:
-        if g is None:
-            continue
-        if g.get_device() < 0:
-            raise RuntimeError("gradients must be on CUDA device")
-        if device is None:
-            device = g.device
-        elif g.device != device:
-            raise RuntimeError("gradients must be on one device")
-    if device is None:
-        raise RuntimeError("gradients must hold at least one tensor")
-    return tensors, device
+        _no_tangent(call, gradients=g)
+    device = some[0].get_device()
+    for g in some:
+        if g.get_device() != device or device < 0:
+            raise RuntimeError("gradients must be on CUDA device" if g.get_device() < 0
+                               else "gradients must be on one device")
+    return tensors, some[0].device
 
 
 def _run(gradients, out, max_norm, scale, device) -> torch.Tensor:
@@ -81,7 +73,6 @@ def _check_scale(scale) -> float:
     return scale
 
 
-@torch.no_grad()
 def gradient_norm(gradients: Iterable[Optional[torch.Tensor]], scale: float = 1.0) -> torch.Tensor:
     """``scale`` times the Euclidean norm of all gradients together (float32, on their
     device).  gradients: tensors of any shapes, empty ones and None (a parameter without a
@@ -91,7 +82,6 @@ def gradient_norm(gradients: Iterable[Optional[torch.Tensor]], scale: float = 1.
     return _run([g for g in tensors if g is not None], None, 0.0, scale, device)
 
 
-@torch.no_grad()
 def clip_gradients(gradients: Iterable[Optional[torch.Tensor]], max_norm: float,
                    scale: float = 1.0,
                    out: Optional[Iterable[Optional[torch.Tensor]]] = None) -> torch.Tensor:
