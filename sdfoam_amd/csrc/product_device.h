@@ -236,7 +236,8 @@ template <typename T, bool kAcross, int kRows, int kWaves, bool kDirect> struct 
     static constexpr int kRowBytes = kAcross ? kRows * (int)sizeof(T) : 128;
     const T *p[kPer];
     uint64_t stride;
-    uint32_t columns; // across: from the lane's first column on
+    uint32_t columns; // across: from the tile's first column on
+    bool tiny;        // rows of less than a piece
     Chunk<T> c[kDirect ? 1 : kPer];
 
     // where in the tile the lane's j-th piece lies: its row of LDS and its place there
@@ -255,12 +256,14 @@ template <typename T, bool kAcross, int kRows, int kWaves, bool kDirect> struct 
         return (((threadIdx.x & 63u) * 16u) % kRowBytes / 16u) ^ swizzle(lds_row(j));
     }
 
-    // along: rows [first, first + rows), by the operand's index; across: columns from `first` of `rows` in all
+    // along: rows [first, first + rows), by the operand's index; across: columns from `first`
+    // of `rows` in all.  length: elements of a row.
     __device__ __forceinline__ void begin(const Operand &o, uint64_t group, uint32_t first,
-                                          uint32_t rows, uint32_t k0) {
+                                          uint32_t rows, uint32_t k0, uint32_t length) {
         const T *base = static_cast<const T *>(o.base) + group * o.group_stride;
         stride = o.stride;
         columns = kAcross ? rows - first : rows;
+        tiny = length < kC;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             if constexpr (!kAcross) {
@@ -272,33 +275,52 @@ template <typename T, bool kAcross, int kRows, int kWaves, bool kDirect> struct 
         }
     }
 
-    // of the tile at k, the lane's pieces; k0 as in begin()
+    // how many elements of the lane's j-th piece of the tile at k there are, or more
+    __device__ __forceinline__ uint32_t there(int j, uint32_t k, uint32_t end) const {
+        if constexpr (!kAcross) {
+            const uint32_t at = k + piece(j) * kC;
+            return end > at ? end - at : 0u;
+        } else {
+            const uint32_t at = k + lds_row(j), n = piece(j) * kC;
+            return at < end && n < columns ? columns - n : 0u;
+        }
+    }
+
+    // of the tile at k, the lane's pieces; k0 as in begin().  A piece that the row's end cuts
+    // is read where it ends there and moved down (store()): every piece is one read, without a
+    // branch (element by element, the waits of the cut pieces held up all others: TN of 8,192
+    // rows of 1,000 x 5,003 bf16 182 TFLOP/s).
     __device__ __forceinline__ void load(char *lds, uint32_t k, uint32_t k0, uint32_t end) {
         const uint64_t on = kAcross ? (uint64_t)(k - k0) * stride : k - k0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const T *from = p[j] + on;
-            uint32_t have;
-            if constexpr (!kAcross) {
-                const uint32_t at = k + piece(j) * kC;
-                have = end > at ? end - at : 0u;
-            } else {
-                const uint32_t at = k + lds_row(j), n = piece(j) * kC;
-                have = at < end && n < columns ? columns - n : 0u;
-            }
-            if constexpr (kDirect)
+            const uint32_t have = there(j, k, end);
+            if constexpr (kDirect) {
                 to_lds(have ? static_cast<const void *>(from) : kZeros,
                        lds_address(lds) + (wave() * kPer + j) * 1024u);
-            else
+            } else if (tiny) {
                 c[j] = __builtin_bit_cast(Chunk<T>, load_some<T, kC>(from, have));
+            } else {
+                const void *at = have >= kC ? from : have ? from - (kC - have) : static_cast<const void *>(kZeros);
+                __builtin_memcpy(&c[j], at, 16);
+            }
         }
     }
-    __device__ __forceinline__ void store(char *lds) const {
+    __device__ __forceinline__ void store(char *lds, uint32_t k, uint32_t end) {
         if constexpr (!kDirect)
 #pragma unroll
-            for (int j = 0; j < kPer; ++j)
+            for (int j = 0; j < kPer; ++j) {
+                const uint32_t have = there(j, k, end);
+                const bool cut = !tiny && have > 0 && have < kC;
+                if (__ballot(cut)) { // the piece ends with the elements that there are: down with them
+                    typedef unsigned __int128 U128;
+                    const U128 all = __builtin_bit_cast(U128, c[j]);
+                    if (cut) c[j] = __builtin_bit_cast(Chunk<T>, all >> ((kC - have) * 8 * sizeof(T)));
+                }
                 *reinterpret_cast<uint4 *>(lds + (wave() * kPer + j) * 1024u + (threadIdx.x & 63u) * 16u) =
                     __builtin_bit_cast(uint4, c[j]);
+            }
     }
 };
 

@@ -239,8 +239,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
         const uint32_t from = min(k_begin + split * each, k_end);
         k_end = min(from + each, k_end);
         k_begin = from;
-        a.begin(p.a, 0, m0, p.m, k_begin);
-        b.begin(p.b, 0, n0, p.n, k_begin);
+        a.begin(p.a, 0, m0, p.m, k_begin, p.m);
+        b.begin(p.b, 0, n0, p.n, k_begin, p.n);
     } else {
         TilesOfRows<kM, kBlock> tiles(p.groups, found);
         const uint32_t tiles_m = tiles.count();
@@ -259,8 +259,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
             k_end = min(k_begin + p.k_each, p.k);
         }
         const uint64_t which = p.b.group_stride ? group : 0;
-        a.begin(p.a, 0, m0, rows_m, k_begin);
-        b.begin(p.b, which, n0, kAcrossB ? p.n : min((uint32_t)kN, p.n - n0), k_begin);
+        a.begin(p.a, 0, m0, rows_m, k_begin, p.k);
+        b.begin(p.b, which, n0, kAcrossB ? p.n : min((uint32_t)kN, p.n - n0), k_begin, kAcrossB ? p.n : p.k);
     }
 
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -283,14 +283,14 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
             a.load(to, k, k_begin, k_end);
             b.load(to + kM * 128, k, k_begin, k_end);
         };
-        const auto brought = [&](char *to) {
-            a.store(to);
-            b.store(to + kM * 128);
+        const auto brought = [&](char *to, uint32_t k) {
+            a.store(to, k, k_end);
+            b.store(to + kM * 128, k, k_end);
             if (kDirect) landed();
             __syncthreads();
         };
         bring(lds, k_begin);
-        brought(lds);
+        brought(lds, k_begin);
         uint32_t now = 0;
         for (uint32_t k = k_begin; k < k_end; k += kK) {
             const bool more = k + kK < k_end;
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
                     for (int j = 0; j < kTn; ++j) mma32<T>(acc[i][j], fb[j], fa[i]);
             }
             now ^= kTile;
-            if (more) brought(lds + now);
+            if (more) brought(lds + now, k + kK);
         }
         __syncthreads();
     }
@@ -761,8 +761,13 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
         plan.splits = 1;
         return plan;
     }
-    plan.large = !skinny && k > 256 && take_large(tiles_of_rows(rows, groups, grouped, 256) * ((n + 255) / 256),
-                                       tiles_of_rows(rows, groups, grouped, 128) * ((n + 127) / 128));
+    // as many as there are on average: a group's last tile is half full
+    const auto tiles = [&](uint64_t tile) {
+        const uint64_t halves = grouped ? 2 * ((rows + tile - 1) / tile) + (rows < groups ? rows : groups) - 1
+                                        : 2 * ((rows + tile - 1) / tile);
+        return halves / 2 * ((n + tile - 1) / tile);
+    };
+    plan.large = !skinny && k > 256 && rows > 0 && take_large(tiles(256), tiles(128));
     const uint32_t km = plan.large ? 256 : 128, kn = skinny ? 32 : km;
     plan.tiles_n = (n + kn - 1) / kn;
     plan.tiles = tiles_of_rows(rows, groups, grouped, km) * plan.tiles_n;
@@ -790,8 +795,8 @@ Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool n
     plan.splits = 1;
     // narrow ones wait for memory more than they multiply: more blocks, shorter parts
     const bool narrow = narrow_m || narrow_n;
-    if (plan.tiles > 0 && !plan.large && plan.tiles < (narrow ? 768 : 256)) {
-        const uint64_t want = (narrow ? 1536 : 512) / plan.tiles, most = rows / groups / (narrow ? 96 : 256);
+    if (plan.tiles > 0 && !plan.large && plan.tiles < (narrow ? 768 : 400)) {
+        const uint64_t want = (narrow ? 1536 : 1024) / plan.tiles, most = rows / groups / (narrow ? 96 : 512);
         plan.splits = (uint32_t)(want < most ? want : most);
         if (plan.splits < 1) plan.splits = 1;
     }
