@@ -15,7 +15,7 @@ from typing import Iterable, Optional
 import torch
 
 from . import _lib
-from .labels import _TYPES, _call, _element_type, _no_tangent, _scratch
+from .labels import _TYPES, _call, _element_type, _no_gradient, _no_tangent, _scratch
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -39,6 +39,8 @@ def _gradients(call: str, gradients: Iterable[Optional[torch.Tensor]]):
         _element_type("gradients", g)
         if not g.is_contiguous() and g.numel() > 0 and not _dense(g):
             raise RuntimeError("gradients must fill their memory without gaps or overlaps")
+        if g.requires_grad:
+            _no_gradient(call, gradients=g)
         _no_tangent(call, gradients=g)
     device = some[0].get_device()
     for g in some:
@@ -117,7 +119,8 @@ def clip_gradients(gradients: Iterable[Optional[torch.Tensor]], max_norm: float,
             if o.get_device() != g.get_device():
                 raise RuntimeError("out must be on the device of the gradients")
             if o.requires_grad:
-                raise RuntimeError("out must not want a gradient")
+                _no_gradient("clip_gradients", out=o)
+            _no_tangent("clip_gradients", out=o)
     keep = [k for k, g in enumerate(tensors) if g is not None]
     norm = _run([tensors[k] for k in keep], [results[k] for k in keep], max_norm, scale, device)
     # autograd, and whoever looks at versions, sees the write

@@ -236,6 +236,9 @@ LINEARS = [  # rows, counts, width, out
     (16, [3, 13], 4097, 260), (3000, [2900, 60], 24, 40), (2048, [2000, 48], 8, 8),
     (20, [20], 0, 5), (20, [4, 15], 6, 0), (0, [0, 0], 4, 4), (64, [10, 6, 0, 33], 1024, 500),
     (17, [1, 2, 3, 4, 5], 2050, 70),
+    # large tiles, each way, whole pieces of 16 bytes and not
+    (8200, [5000, 3100], 264, 1288), (8200, [4000, 4100], 1288, 264), (8195, [8000], 301, 1289),
+    (300, [150, 149], 2056, 2064), (300, [150, 149], 2059, 2061),
 ]
 
 
@@ -277,6 +280,39 @@ def test_linear(dev, rows, counts, width, out, dtype):
     pad = torch.full((rows, width + 3), math.nan, dtype=dtype, device=dev)
     pad[:, 1:1 + width] = X
     assert torch.equal(sdfoam_amd.expert_linear(pad[:, 1:1 + width], W, o), got)
+
+
+def test_no_choices(dev):
+    order = sdfoam_amd.expert_order(torch.zeros((5, 0), dtype=torch.int64, device=dev), 3)
+    assert torch.equal(order.offsets.cpu(), torch.zeros(4, dtype=torch.int32))
+    assert sdfoam_amd.expert_rows(torch.ones((5, 6), device=dev), order).shape == (0, 6)
+    out = sdfoam_amd.expert_combine(torch.ones((0, 6), device=dev), order)
+    assert torch.equal(out, torch.zeros((5, 6), device=dev))
+
+
+def test_more_than_2_to_32_elements(dev):
+    """Rows whose elements pass 32 bits.  Small whole numbers: every sum is exact."""
+    rows, width = (1 << 21) + 133, 2056
+    at = torch.arange(rows, device=dev)
+    x = ((at % 5) - 2).to(torch.bfloat16)[:, None].expand(rows, width)
+    ids = (at % 3 == 0).long()[:, None]
+    order = sdfoam_amd.expert_order(ids, 2)
+    sorted_rows = sdfoam_amd.expert_rows(x, order)
+    p = order.places[:, 0].long()
+    assert torch.equal(sorted_rows[p[-1000:]], x[-1000:])
+    w = torch.ones((2, 16, width), dtype=torch.bfloat16, device=dev)
+    w[1] = -1.0
+    y = sdfoam_amd.expert_linear(sorted_rows, w, order.offsets)
+    want = (x[:, 0].float() * width * torch.where(ids[:, 0] == 1, -1.0, 1.0)).to(torch.bfloat16)
+    assert torch.equal(y[p], want[:, None].expand(rows, 16))
+    back = sdfoam_amd.expert_combine(sorted_rows, order)
+    assert torch.equal(back[-1000:], x[-1000:]) and torch.equal(back[:1000], x[:1000])
+    d = torch.ones((rows, 16), dtype=torch.bfloat16, device=dev)
+    dx, dw = sdfoam_amd.expert_linear_backward(d, sorted_rows, w, order.offsets)
+    sums = torch.stack([x[:, 0].float()[ids[:, 0] == e].sum() for e in (0, 1)]).to(torch.bfloat16)
+    assert torch.equal(dw, sums[:, None, None].expand(2, 16, width))
+    assert torch.equal(dx[p[-5:], 0].float().cpu(),
+                       torch.where(ids[-5:, 0] == 1, -16.0, 16.0).cpu())
 
 
 def test_linear_keeps_values_apart(dev):
@@ -369,6 +405,10 @@ ADAPTERS = [  # rows, adapters, rank, width, out, spread
     (50, 6, 0, 21, 22, "any"), (0, 3, 4, 5, 6, "any"), (40, 2, 3, 0, 7, "any"),
     (40, 2, 3, 7, 0, "any"), (4100, 12, 8, 17, 41, "few"), (150, 2048, 2, 24, 16, "any"),
     (60, 2, 32, 2100, 64, "any"), (33, 40, 256, 64, 72, "any"),
+    # rows whose adapters are added one by one: in the order they come, in order of adapters,
+    # in parts, along a short inner dimension
+    (60, 7, 5, 40, 100, "any"), (1500, 1500, 4, 70, 90, "any"), (1300, 700, 16, 1100, 130, "any"),
+    (1500, 1200, 9, 30, 70, "any"), (900, 300, 20, 600, 1100, "any"),
 ]
 
 

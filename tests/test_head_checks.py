@@ -150,6 +150,8 @@ def test_clip_gradients_refuses():
         for bad in (0.0, -1.0, float("nan"), float("inf")):
             with refused("scale must be positive and finite"):
                 call([t], scale=bad)
+        with refused("has no gradient for gradients: detach it"):
+            call([torch.zeros(4, requires_grad=True)])
         with refused("gradients must be on CUDA device"):
             call([t])
     for bad in (-1.0, float("nan")):
