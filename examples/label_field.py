@@ -111,7 +111,7 @@ class LabelField(torch.nn.Module):
 
 
 def main(points=20_000, labels=512, features=32, top=8, size=128, cameras=8, batch=16_384,
-         steps=60, seed=0, log=print):
+         steps=60, seed=0, max_norm=0.0, log=print):
     gen = torch.Generator(device="cuda").manual_seed(seed)
     torch.manual_seed(seed)
     field = LabelField(foam(points, gen), labels, features)
@@ -125,6 +125,8 @@ def main(points=20_000, labels=512, features=32, top=8, size=128, cameras=8, bat
         loss = sdfoam_amd.distill_loss(field(some), *teacher(some))
         optimizer.zero_grad(set_to_none=True)
         loss.backward()
+        if max_norm:
+            sdfoam_amd.clip_gradients([p.grad for p in field.parameters()], max_norm)
         optimizer.step()
         losses.append(loss.detach())
         if log and (step % 10 == 0 or step + 1 == steps):
@@ -156,4 +158,5 @@ if __name__ == "__main__":
                         ("size", 128), ("cameras", 8), ("batch", 16_384), ("steps", 60),
                         ("seed", 0)):
         ap.add_argument(f"--{name}", type=int, default=value)
+    ap.add_argument("--max-norm", type=float, default=0.0, help="clip gradients; 0: do not")
     main(**vars(ap.parse_args()))

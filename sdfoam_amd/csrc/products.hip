@@ -209,7 +209,11 @@ __device__ __forceinline__ void tile_of_block(uint32_t block, uint32_t tiles_m, 
 }
 
 // One tile of kM x kN, kWavesM x kWavesN waves: two tiles of the inner dimension in LDS,
-// one multiplied while the other is brought.
+// one multiplied while the other is brought.  Bound by the matrix units: 8,192^3 bf16 in
+// tiles of 256 x 256 at 1,145 TFLOP/s with both operands along k, 1,164 with b across, 1,125
+// with both (a large library product: 1,390, 1,310, 1,150), in tiles of 128 x 128 at 854;
+// 4,096^3 floats at 140 (131).  At rows that do not line up a third to a half of that.  Read
+// in pairs of words for want of alignment, LDS alone took as long: 550.
 template <typename T, bool kWeights, bool kAcrossB, int kM, int kN, int kWavesM, int kWavesN, bool kDirect>
 __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(ProductArgs p) {
     constexpr int kWaves = kWavesM * kWavesN, kBlock = 64 * kWaves;
@@ -352,8 +356,12 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
 
 constexpr int kThreads = 256;
 
-// One tile of kM x kN of the result, kWavesM x kWavesN waves.  Two tiles of the inner
-// dimension in LDS: while one is multiplied, the next is on its way to registers.
+// ---- narrow tiles: the adapters' ranks ---------------------------------------------------
+//
+// One tile of kM x kN of the result, kWavesM x kWavesN waves; operands of other types than T
+// are converted on their way.  Two tiles of the inner dimension in LDS: while one is
+// multiplied, the next is on its way to registers.  Bound by the waits for the long operand:
+// h of 160,000 rows of 64 fp16 13 us, b of 8,192 rows of 5,003 36, up's gradient 77.
 //
 // kWeights: the weights form (both operands across, k the rows of a group); else the rows
 // form, b across for gradients.
@@ -449,10 +457,6 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs p) {
 #pragma unroll
     for (int i = 0; i < kTm; ++i) {
         const uint32_t mi = wm + i * 32 + l32;
-        if constexpr (!kWeights)
-            if (p.beside.inner && split == 0)
-                add_beside<SB, kAcrossB, kTn>(p, m0, rows_m, mi, mi < rows_m ? p.beside.group_of[m0 + mi] : -1,
-                                              n0 + wn, acc[i]);
         if (mi >= rows_m) continue;
         const uint64_t row = kWeights ? (uint64_t)group * p.m + m0 + mi : m0 + mi;
 #pragma unroll
@@ -531,8 +535,9 @@ template <typename O, bool kAcross> __global__ __launch_bounds__(256) void join_
 //
 // At most 128 bytes of it: a wave keeps 32 rows in registers and goes over the columns, 64 at
 // a time, their fragments from the caches while the 64 before are written, without LDS but to
-// turn what it writes and without waiting for another wave.  Bound by what it reads and
-// writes; tiles wait in turn for rows, columns and each other.
+// turn what it writes and without waiting for another wave.  Bound by the waits for columns
+// and the VALU's share of conversions and addresses (160,000 rows of 64 -> 512 fp16: 63 us, with
+// adapters 79; tiles, which wait in turn for rows, columns and each other, 76 and 88).
 constexpr uint32_t kShortWaves = 4, kShortRows = 32 * kShortWaves;
 
 template <typename T> __global__ __launch_bounds__(64 * kShortWaves, 3) void short_kernel(ProductArgs p, uint32_t columns) {
@@ -591,13 +596,15 @@ template <typename T> __global__ __launch_bounds__(64 * kShortWaves, 3) void sho
 // 16 kMt rows by 16 kNt columns a block; each of four waves has a quarter of the inner
 // dimension and reads its operands straight into registers, 128 bytes of a row at a time,
 // since no other wave of the block needs them.  Bound by the bytes of the matrices; the
-// rows come from L2, as often as there are tiles of columns.
+// rows come from L2, as often as there are tiles of columns (64 rows of 2,048 -> 32,768: 60 us,
+// tiles 44; 32 rows: 44 both; 16: 37; the 64 entries of 16 rows over 64 experts of 1,024 ->
+// 2,048 bf16, 171 MB: 30 us, 5.6 TB/s).
 constexpr int kThinWaves = 4;
 
 template <typename T, int kMt, int kNt>
 __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ProductArgs p) {
     constexpr uint32_t kC = TileOf<T>::kC, kStep = TileOf<T>::kK; // a lane has two pieces a step
-    constexpr int kAhead = kMt * kNt <= 2 ? 4 : kMt * kNt <= 8 ? 2 : 1; // steps in flight
+    constexpr int kAhead = kMt * kNt <= 2 ? 4 : 2; // steps in flight
     __shared__ F4x sums[kThinWaves][kMt * kNt][64];
     __shared__ uint32_t found[20];
     const uint32_t tile_n = blockIdx.x % p.tiles_n, tile_m = blockIdx.x / p.tiles_n;
@@ -719,10 +726,7 @@ template <typename T> void launch_thin(const ProductArgs &p, const Plan &plan, h
     case 9: thin_kernel<T, 1, 1><<<grid, block, 0, s>>>(p); break;
     case 10: thin_kernel<T, 1, 2><<<grid, block, 0, s>>>(p); break;
     case 17: thin_kernel<T, 2, 1><<<grid, block, 0, s>>>(p); break;
-    case 18: thin_kernel<T, 2, 2><<<grid, block, 0, s>>>(p); break;
-    case 33: thin_kernel<T, 4, 1><<<grid, block, 0, s>>>(p); break;
-    case 34: thin_kernel<T, 4, 2><<<grid, block, 0, s>>>(p); break;
-    default: thin_kernel<T, 4, 4><<<grid, block, 0, s>>>(p); break;
+    default: thin_kernel<T, 2, 2><<<grid, block, 0, s>>>(p); break;
     }
 }
 
@@ -752,7 +756,7 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
         plan.thin_m = each <= 16 ? 1 : 2;
         const uint64_t tiles_m = tiles_of_rows(rows, groups, grouped, 16 * plan.thin_m);
         // wider where there are columns enough for every CU: the rows are read less often
-        plan.thin_n = plan.thin_m < 2 ? plan.thin_m : 2;
+        plan.thin_n = plan.thin_m;
         if (plan.thin_n < 2 && tiles_m * (n / 32) >= 1024) plan.thin_n = 2;
         while (plan.thin_n > 1 && tiles_m * ((n + 16 * plan.thin_n - 1) / (16 * plan.thin_n)) < 256)
             plan.thin_n /= 2;

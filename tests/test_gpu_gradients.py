@@ -174,6 +174,21 @@ def test_refusals_of_memory(dev):
     assert torch.equal(t, torch.ones(100, device=dev))
 
 
+def test_label_field_clips(dev):
+    """The example trains with clipped gradients."""
+    import importlib.util
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location(
+        "label_field", os.path.join(root, "examples", "label_field.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    r = example.main(points=3000, labels=32, features=8, size=32, cameras=3, batch=1024, steps=3,
+                     max_norm=0.01, log=None)
+    assert all(math.isfinite(x) for x in r["loss"])
+
+
 def test_in_a_graph(dev):
     g = torch.Generator().manual_seed(4)
     ref = [torch.randn(n, generator=g) for n in (5000, 33, 1)] * 40
