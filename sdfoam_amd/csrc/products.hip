@@ -937,7 +937,7 @@ int sdf_expert_linear(int type, const void *rows, uint64_t rows_stride, uint64_t
 
 size_t sdf_expert_linear_backward_scratch_bytes(uint64_t count, uint32_t num_experts,
                                                 uint32_t width, uint32_t out_width) {
-    if (count >= 1ull << 31 || num_experts > SDF_MAX_EXPERTS || num_experts == 0) return 0;
+    if (count >= 1ull << 31 || num_experts > SDF_MAX_EXPERTS) return 0;
     const size_t a = plan_rows(count, num_experts, true, width, out_width, true, false).bytes;
     const size_t b = plan_weights(count, num_experts, out_width, width, false, false).bytes;
     return a > b ? a : b; // one after the other

@@ -655,3 +655,20 @@ def test_on_another_stream(dev):
     for k in range(2):
         for g in got[k]:
             assert torch.equal(g, want[k])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,out", [(300, 6, 1024), (300, 1024, 6), (300, 2056, 1030),
+                                            (7, 1024, 1024)])
+def test_no_experts(dev, rows, width, out, dtype):
+    """No experts: zeros, also where the inner dimension is cut in parts."""
+    say("no experts", rows, width, out, dtype)
+    x = torch.ones((rows, width), dtype=dtype, device=dev).requires_grad_()
+    w = torch.empty((0, out, width), dtype=dtype, device=dev).requires_grad_()
+    o = torch.zeros(1, dtype=torch.int32, device=dev)
+    d = torch.ones((rows, out), dtype=dtype, device=dev)
+    y = sdfoam_amd.expert_linear(x, w, o)
+    assert y.shape == (rows, out) and not y.any()
+    for dx, dw in (sdfoam_amd.expert_linear_backward(d, x.detach(), w.detach(), o),
+                   torch.autograd.grad(y, (x, w), d)):
+        assert dx.shape == x.shape and not dx.any() and dw.shape == w.shape

@@ -238,3 +238,16 @@ def test_c_interface_refuses():
     halves = (C.c_int * 2)(1, 1)
     says(clip(2, types, at, counts, halves, at, 1.0, 1.0, p, p, need, None), "float32 or of")
     says(clip(2, halves, at, counts, types, at, 1.0, 1.0, p, p, need, None), "another type")
+
+
+def test_scratch_of_no_experts():
+    """Without experts the products of rows are zeros, and their plan may cut the inner
+    dimension all the same: the size that a caller asks for is the one that the call needs."""
+    L = _lib.lib()
+    p = 256
+    need = L.sdf_expert_linear_backward_scratch_bytes(300, 0, 6, 1024)
+    assert need > 0 and need == L.sdf_expert_linear_scratch_bytes(300, 0, 1024, 6)
+    for scratch, size in ((None, 0), (p, 0), (p, need - 1)):
+        rc = L.sdf_expert_linear_backward(0, p, 1024, p, 6, 300, 0, 6, 1024, None, p, p, None,
+                                          scratch, size, None)
+        assert rc == _lib.SDF_E_INVALID and "scratch must hold" in L.sdf_last_error().decode()
