@@ -39,7 +39,7 @@ __device__ __forceinline__ bool few_adapters(int32_t mine) {
 
 // Column n of kRows rows from `place` on (the last of `rows` again where there are fewer),
 // their values on their way together; the rows are the same in every lane, `groups` has
-// theirs from lane `from` on.
+// theirs from lane `from` on.  Every lane of the wave calls it.
 template <typename S, bool kAcross, int kRows>
 __device__ __forceinline__ void beside_of_rows(const ProductArgs &p, uint32_t place, uint32_t rows,
                                                int32_t groups, uint32_t from, uint32_t n, float *sum) {
@@ -160,7 +160,8 @@ __device__ __forceinline__ void write_rows(const ProductArgs &p, char *turn, con
 }
 
 // The same with the rows' adapters added one by one; a lane has a column.  The first row is
-// at `place`, lane l32 has the l32-th row's adapter.
+// at `place`, lane l32 has the l32-th row's adapter.  Lanes past the last column stay to the
+// end, with that column's values: the rows that the others write to are read from them.
 template <typename S, bool kAcross, typename O, int kTn, typename RowAt>
 __device__ __forceinline__ void write_by_row(const ProductArgs &p, char *turn, const F16x *sums, uint32_t place,
                                              uint32_t rows, uint32_t n0, int32_t to_row, int32_t adapters,
@@ -180,17 +181,18 @@ __device__ __forceinline__ void write_by_row(const ProductArgs &p, char *turn, c
             *reinterpret_cast<Few<float, 4> *>(turned + l32 * kFloats + j * 32 + q * 8 + half * 4) = o;
         }
     wave_sync();
+    if (n0 >= p.n) return; // all lanes of the wave
     const uint32_t n = n0 + lane;
-    if (n >= p.n) return;
     constexpr uint32_t kBatch = 4;
     for (uint32_t r = 0; r < rows; r += kBatch) {
         float extra[kBatch];
-        beside_of_rows<S, kAcross, kBatch>(p, place + r, rows - r, adapters, r, n, extra);
+        beside_of_rows<S, kAcross, kBatch>(p, place + r, rows - r, adapters, r, min(n, p.n - 1), extra);
 #pragma unroll
-        for (uint32_t i = 0; i < kBatch; ++i)
-            if (r + i < rows)
-                row_at(__builtin_amdgcn_readlane(to_row, r + i))[n] =
-                    (O)(turned[(r + i) * kFloats + lane] + extra[i]);
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            if (r + i >= rows) break;
+            const int32_t row = __builtin_amdgcn_readlane(to_row, r + i);
+            if (n < p.n) row_at(row)[n] = (O)(turned[(r + i) * kFloats + lane] + extra[i]);
+        }
     }
 }
 

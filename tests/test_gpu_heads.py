@@ -672,3 +672,26 @@ def test_no_experts(dev, rows, width, out, dtype):
     for dx, dw in (sdfoam_amd.expert_linear_backward(d, x.detach(), w.detach(), o),
                    torch.autograd.grad(y, (x, w), d)):
         assert dx.shape == x.shape and not dx.any() and dw.shape == w.shape
+
+
+LAST_COLUMNS = [  # rows, adapters, rank, width, out: many adapters in every 32 rows
+    (1100, 400, 4, 70, 65), (1100, 400, 4, 65, 129),  # tiles of 128 x 128, both ways
+    (1100, 400, 5, 30, 95), (1100, 400, 16, 8, 1),    # a short inner dimension
+    (1100, 400, 16, 1100, 70), (1100, 400, 8, 70, 1100),  # in parts, forward and back
+    (4100, 1500, 4, 264, 2180), (4100, 1500, 4, 2180, 264),  # tiles of 256 x 256
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,adapters,rank,width,out", LAST_COLUMNS)
+def test_adapters_last_columns(dev, rows, adapters, rank, width, out, dtype):
+    """Rows whose adapters are added one by one, where fewer than 32 columns are left for a
+    wavefront: where each row goes, and its adapter, lie in lanes past the last column."""
+    test_adapters(dev, rows, adapters, rank, width, out, "any", dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width,out", [(264, 2180), (2180, 264)])
+def test_adapters_in_large_tiles(dev, width, out, dtype):
+    """Few adapters in every 32 rows, added by the matrix units in tiles of 256 x 256."""
+    test_adapters(dev, 4100, 3, 16, width, out, "any", dtype)
