@@ -127,8 +127,8 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const double *sums, uint
 
 // 16 bytes of the result a thread, so that a wavefront writes whole lines; large results past
 // the caches.
-template <typename T, typename O>
-__device__ __forceinline__ void scaled(const void *in, void *out, uint64_t first, uint32_t n, float f, bool past) {
+template <typename T, typename O, typename Times>
+__device__ __forceinline__ void scaled(const void *in, void *out, uint64_t first, uint32_t n, Times times, bool past) {
     constexpr uint32_t kN = 16 / sizeof(O);
     struct In {
         T v[kN];
@@ -140,7 +140,7 @@ __device__ __forceinline__ void scaled(const void *in, void *out, uint64_t first
     O *o = static_cast<O *>(out) + first;
     // whole pieces begin where the result's 128 bytes do
     const uint32_t head = min(n, (uint32_t)(-reinterpret_cast<uintptr_t>(o) & 127u) / (uint32_t)sizeof(O));
-    if (threadIdx.x < head) o[threadIdx.x] = (O)(f * (float)p[threadIdx.x]);
+    if (threadIdx.x < head) o[threadIdx.x] = (O)times((float)p[threadIdx.x]);
     p += head, o += head, n -= head;
     const uint32_t whole = n / kN;
     const auto go = [&](auto store) {
@@ -150,13 +150,13 @@ __device__ __forceinline__ void scaled(const void *in, void *out, uint64_t first
             __builtin_memcpy(&v, p + (uint64_t)c * kN, sizeof(v));
             Out r;
 #pragma unroll
-            for (uint32_t e = 0; e < kN; ++e) r.v[e] = (O)(f * (float)v.v[e]);
+            for (uint32_t e = 0; e < kN; ++e) r.v[e] = (O)times((float)v.v[e]);
             store(o + (uint64_t)c * kN, r);
         }
     };
     if (past) go([](O *to, const Out &r) { store_past<sizeof(O)>(to, r); });
     else go([](O *to, const Out &r) { __builtin_memcpy(to, &r, sizeof(r)); });
-    for (uint32_t i = whole * kN + threadIdx.x; i < n; i += kThreads) o[i] = (O)(f * (float)p[i]);
+    for (uint32_t i = whole * kN + threadIdx.x; i < n; i += kThreads) o[i] = (O)times((float)p[i]);
 }
 
 // Every block adds the other pass's sums itself, in the same order (8 KB from L2).  Memory
@@ -169,18 +169,25 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Source t, const double 
     const double size = (double)scale * sqrt(total_of(sums, n, lds));
     double c = (double)max_norm / (size + 1e-6);
     c = c > 1.0 ? 1.0 : c; // NaN stays
-    const float f = (float)(scale * c);
+    const double wide = (double)scale * c;
+    const float f = (float)wide;
     const bool past = t.chunks >= kPastChunks;
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)size;
-    each_chunk<true>(t, [&](const Entry &k, uint64_t first, uint32_t n) {
-        if (k.in == k.out && f == 1.0f) return;
-        if (k.type == SDF_TYPE_F32) scaled<float, float>(k.in, k.out, first, n, f, past);
-        else if (k.type == SDF_TYPE_F16) {
-            if (k.out_type == SDF_TYPE_F32) scaled<half_t, float>(k.in, k.out, first, n, f, past);
-            else scaled<half_t, half_t>(k.in, k.out, first, n, f, past);
-        } else if (k.out_type == SDF_TYPE_F32) scaled<bf16_t, float>(k.in, k.out, first, n, f, past);
-        else scaled<bf16_t, bf16_t>(k.in, k.out, first, n, f, past);
-    });
+    const auto go = [&](auto times) {
+        each_chunk<true>(t, [&](const Entry &k, uint64_t first, uint32_t n) {
+            if (k.in == k.out && f == 1.0f) return;
+            if (k.type == SDF_TYPE_F32) scaled<float, float>(k.in, k.out, first, n, times, past);
+            else if (k.type == SDF_TYPE_F16) {
+                if (k.out_type == SDF_TYPE_F32) scaled<half_t, float>(k.in, k.out, first, n, times, past);
+                else scaled<half_t, half_t>(k.in, k.out, first, n, times, past);
+            } else if (k.out_type == SDF_TYPE_F32) scaled<bf16_t, float>(k.in, k.out, first, n, times, past);
+            else scaled<bf16_t, bf16_t>(k.in, k.out, first, n, times, past);
+        });
+    };
+    // A factor below fp32's normal range keeps few of its bits there, or none, and gradients
+    // of up to 3e38 lift its products back into the range: those in fp64.
+    if (wide > 0.0 && wide < 0x1p-126) go([wide](float g) { return (float)(wide * (double)g); });
+    else go([f](float g) { return f * g; });
 }
 
 constexpr uint64_t kMaxElements = 1ull << 40; // of all tensors: 32 bits count the chunks

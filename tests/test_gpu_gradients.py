@@ -213,3 +213,26 @@ def test_in_a_graph(dev):
         assert torch.equal(norm, want)
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("size,max_norm,scale", [
+    (1e37, 1e-6, 1.0), (1e37, 1e-3, 1.0), (3e36, 1.0, 2.0 ** -20), (1e37, 1e-38, 1.0),
+    (1e30, 1e-20, 1e-10), (1.0, 1e9, 1e-41)])
+def test_factors_below_the_range(dev, size, max_norm, scale):
+    """Factors that float32 holds with few bits or none, whose products it holds."""
+    say("small factors", size, max_norm, scale)
+    g = torch.Generator().manual_seed(7)
+    scale = float(torch.tensor(scale))  # as the call takes them
+    max_norm = float(torch.tensor(max_norm))
+    for own_type, out_type in ((torch.float32, None), (torch.bfloat16, None),
+                               (torch.bfloat16, torch.float32)):
+        t = (size * (1.0 + torch.rand(777, generator=g))).to(own_type)
+        norm, factor = expected([t], max_norm, scale)
+        own = t.to(dev)
+        out = None if out_type is None else [torch.empty_like(own, dtype=out_type)]
+        got = sdfoam_amd.clip_gradients([own], max_norm, scale, out=out)
+        if norm < 2.0 ** 128:
+            assert abs(float(got) - norm) <= 2 * U * norm + 2.0 ** -149
+        else:  # past float32's largest, 2^128 (1 - 2^-24), by more than half a step
+            assert float(got) == math.inf
+        check(own if out is None else out[0], t, factor)
