@@ -810,8 +810,10 @@ int sdf_adapter_linear_backward(
  * gradients[t].  The arrays are the host's, read before the call returns:
  * num_tensors types, device addresses and numbers of elements (fewer than 2^40
  * in all); out[t] of the gradient's type or float32, the gradient itself or
- * memory that no gradient and no other result lies on.  A norm that is not
- * finite leaves results that are not (infinite: 0 times each element; NaN: NaN). */
+ * memory that no gradient and no other result lies on.  The factor is that of the
+ * norm in fp64: finite gradients whose norm passes fp32's range are clipped, and
+ * *norm is infinite.  An infinite gradient makes each result 0 times its gradient
+ * (NaN where max_norm is infinite too), one of NaN makes each NaN. */
 size_t sdf_clip_gradients_scratch_bytes(uint32_t num_tensors);
 int sdf_clip_gradients(uint32_t num_tensors, const int *types,
                        const void *const *gradients, const uint64_t *counts,

@@ -95,8 +95,13 @@ def clip_gradients(gradients: Iterable[Optional[torch.Tensor]], max_norm: float,
     is rounded.  out (optional): tensors of the gradients' shapes, float32 or of their
     gradient's type, that the results are written to -- an optimizer's float32 copies --;
     default: the gradients themselves.  No result may lie on another, or on another
-    gradient.  A norm that is not finite is not mended: an infinite one leaves 0 times each
-    gradient, NaN leaves NaN."""
+    gradient.
+
+    The factor is that of the norm before it is rounded to float32: finite gradients whose
+    norm passes float32's range are clipped all the same, and the norm returned for them is
+    infinite.  Gradients that are not finite are not mended: with an infinite one among them
+    each result is 0 times its gradient (NaN where max_norm is infinite too), with NaN each
+    is NaN."""
     scale = _check_scale(scale)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

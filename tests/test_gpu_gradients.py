@@ -236,3 +236,26 @@ def test_factors_below_the_range(dev, size, max_norm, scale):
         else:  # past float32's largest, 2^128 (1 - 2^-24), by more than half a step
             assert float(got) == math.inf
         check(own if out is None else out[0], t, factor)
+
+
+def test_norms_past_the_range(dev):
+    """Finite gradients whose norm float32 does not hold: it is returned as infinite, and the
+    gradients are clipped by what it is."""
+    for kind in (torch.float32, torch.bfloat16):
+        t, u = torch.full((1000,), 3e38).to(kind), torch.full((33,), -2e38).to(kind)
+        norm, factor = expected([t, u], 2.0, 1.0)
+        a, b = t.to(dev), u.to(dev)
+        assert float(sdfoam_amd.gradient_norm([a, b])) == math.inf
+        assert float(sdfoam_amd.clip_gradients([a, b], 2.0)) == math.inf
+        check(a, t, factor)
+        check(b, u, factor)
+        assert abs(float(sdfoam_amd.gradient_norm([a, b])) - 2.0) <= 2.0 * (3 * U + ROUND[kind][0])
+        # an infinite gradient is another matter
+        a[5] = math.inf
+        assert float(sdfoam_amd.clip_gradients([a, b], 2.0)) == math.inf
+        assert torch.isnan(a[5]) and not a[:5].any() and not b.any()
+    a = torch.tensor([1.0, -2.0], device=dev)
+    sdfoam_amd.clip_gradients([a], math.inf, 0.5)
+    assert torch.equal(a.cpu(), torch.tensor([0.5, -1.0]))
+    a[0] = math.inf
+    assert float(sdfoam_amd.clip_gradients([a], math.inf)) == math.inf and torch.isnan(a).all()
