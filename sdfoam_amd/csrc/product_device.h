@@ -197,6 +197,7 @@ struct ProductArgs {
     float scale;              // narrow tiles and their joining; 1 for all others
     Beside beside;
     uint32_t tiles_n;
+    uint32_t first; // tile of the launch
 };
 
 // ---- large tiles: LDS as memory has it ----------------------------------------------------

@@ -228,13 +228,13 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
     Feed<T, kWeights || kAcrossB, kN, kWaves, kDirect> b;
 
     uint32_t tile_m, tile_n;
-    const uint32_t split = blockIdx.y;
+    const uint32_t split = blockIdx.y, block = p.first + blockIdx.x;
     uint32_t k_begin = 0, k_end = p.k, group, m0, rows_m, n0;
     if constexpr (kWeights) {
         const uint32_t tiles_m = (p.m + kM - 1) / kM;
         // every XCD has a share of each group, whose rows differ in number
-        group = blockIdx.x / (tiles_m * p.tiles_n);
-        tile_of_block(blockIdx.x - group * tiles_m * p.tiles_n, tiles_m, p.tiles_n, tile_m, tile_n);
+        group = block / (tiles_m * p.tiles_n);
+        tile_of_block(block - group * tiles_m * p.tiles_n, tiles_m, p.tiles_n, tile_m, tile_n);
         n0 = tile_n * kN;
         m0 = tile_m * kM;
         rows_m = min((uint32_t)kM, p.m - m0);
@@ -250,8 +250,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void tile_kernel(Product
     } else {
         TilesOfRows<kM, kBlock> tiles(p.groups, found);
         const uint32_t tiles_m = tiles.count();
-        if (blockIdx.x >= tiles_m * p.tiles_n) return; // left over
-        tile_of_block(blockIdx.x, tiles_m, p.tiles_n, tile_m, tile_n);
+        if (block >= tiles_m * p.tiles_n) return; // left over
+        tile_of_block(block, tiles_m, p.tiles_n, tile_m, tile_n);
         const TileOfRows t = tiles.find(tile_m);
         n0 = tile_n * kN;
         group = t.group;
@@ -376,8 +376,8 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs p) {
     typename LoaderOf<kWeights, T, SA, kM, kThreads>::type a;
     typename LoaderOf<kWeights || kAcrossB, T, SB, kN, kThreads>::type b;
 
-    const uint32_t tile_n = blockIdx.x % p.tiles_n, tile_m = blockIdx.x / p.tiles_n;
-    const uint32_t split = blockIdx.y;
+    const uint32_t block = p.first + blockIdx.x, split = blockIdx.y;
+    const uint32_t tile_n = block % p.tiles_n, tile_m = block / p.tiles_n;
     const uint32_t n0 = tile_n * kN;
     uint32_t k_begin = 0, k_end = p.k, group, m0, rows_m;
     if constexpr (kWeights) {
@@ -547,8 +547,9 @@ template <typename T> __global__ __launch_bounds__(64 * kShortWaves, 3) void sho
     __shared__ __attribute__((aligned(16))) char turns[kShortWaves * turn_bytes<2>()];
     __shared__ uint32_t found[20];
     TilesOfRows<kShortRows, 64 * kShortWaves> tiles(p.groups, found);
-    if (blockIdx.x >= tiles.count()) return;
-    const TileOfRows t = tiles.find(blockIdx.x);
+    const uint32_t block = p.first + blockIdx.x;
+    if (block >= tiles.count()) return;
+    const TileOfRows t = tiles.find(block);
     const bool none = p.groups.offsets && t.group == p.groups.groups; // rows of no group: zeros
     const uint32_t lane = threadIdx.x & 63u, l32 = lane & 31u, half = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ProductArgs p) {
     constexpr int kAhead = kMt * kNt <= 2 ? 4 : 2; // steps in flight
     __shared__ F4x sums[kThinWaves][kMt * kNt][64];
     __shared__ uint32_t found[20];
-    const uint32_t tile_n = blockIdx.x % p.tiles_n, tile_m = blockIdx.x / p.tiles_n;
+    const uint32_t block = p.first + blockIdx.x, tile_n = block % p.tiles_n, tile_m = block / p.tiles_n;
     TilesOfRows<16 * kMt, 64 * kThinWaves> tiles(p.groups, found);
     if (tile_m >= tiles.count()) return;
     const TileOfRows t = tiles.find(tile_m);
@@ -701,7 +702,16 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ProductArgs p) {
     }
 }
 
-constexpr uint64_t kMaxBlocks = 1ull << 23;
+constexpr uint64_t kMaxTiles = 1ull << 31; // 32 bits count them
+
+// f(p, tiles) for windows of the tiles: a launch holds fewer than 2^32 threads
+template <typename F> void each_window(ProductArgs p, uint64_t tiles, F f) {
+    constexpr uint64_t kWindow = 1ull << 22;
+    for (uint64_t t = 0; t < tiles; t += kWindow) {
+        p.first = (uint32_t)t;
+        f(p, (uint32_t)(tiles - t < kWindow ? tiles - t : kWindow));
+    }
+}
 
 // whether rows of n elements are whole pieces of 16 bytes wherever one begins
 bool lines_up(const Operand &o, int type, uint32_t n) {
@@ -711,10 +721,12 @@ bool lines_up(const Operand &o, int type, uint32_t n) {
 }
 
 template <typename T, bool kWeights, bool kAcross, bool kDirect>
-void launch_tiles_as(const ProductArgs &p, const Plan &plan, hipStream_t s) {
-    const dim3 grid((uint32_t)plan.tiles, plan.splits);
-    if (plan.large) tile_kernel<T, kWeights, kAcross, 256, 256, 2, 4, kDirect><<<grid, 512, 0, s>>>(p);
-    else tile_kernel<T, kWeights, kAcross, 128, 128, 2, 2, kDirect><<<grid, 256, 0, s>>>(p);
+void launch_tiles_as(const ProductArgs &args, const Plan &plan, hipStream_t s) {
+    each_window(args, plan.tiles, [&](const ProductArgs &p, uint32_t tiles) {
+        const dim3 grid(tiles, plan.splits);
+        if (plan.large) tile_kernel<T, kWeights, kAcross, 256, 256, 2, 4, kDirect><<<grid, 512, 0, s>>>(p);
+        else tile_kernel<T, kWeights, kAcross, 128, 128, 2, 2, kDirect><<<grid, 256, 0, s>>>(p);
+    });
 }
 template <typename T, bool kWeights, bool kAcross>
 void launch_tiles(const ProductArgs &p, const Plan &plan, bool direct, hipStream_t s) {
@@ -722,14 +734,38 @@ void launch_tiles(const ProductArgs &p, const Plan &plan, bool direct, hipStream
     else launch_tiles_as<T, kWeights, kAcross, false>(p, plan, s);
 }
 
-template <typename T> void launch_thin(const ProductArgs &p, const Plan &plan, hipStream_t s) {
-    const uint32_t grid = (uint32_t)plan.tiles, block = 64 * kThinWaves;
-    switch (plan.thin_m * 8 + plan.thin_n) {
-    case 9: thin_kernel<T, 1, 1><<<grid, block, 0, s>>>(p); break;
-    case 10: thin_kernel<T, 1, 2><<<grid, block, 0, s>>>(p); break;
-    case 17: thin_kernel<T, 2, 1><<<grid, block, 0, s>>>(p); break;
-    default: thin_kernel<T, 2, 2><<<grid, block, 0, s>>>(p); break;
-    }
+template <typename T> void launch_thin(const ProductArgs &args, const Plan &plan, hipStream_t s) {
+    const uint32_t block = 64 * kThinWaves;
+    each_window(args, plan.tiles, [&](const ProductArgs &p, uint32_t tiles) {
+        switch (plan.thin_m * 8 + plan.thin_n) {
+        case 9: thin_kernel<T, 1, 1><<<tiles, block, 0, s>>>(p); break;
+        case 10: thin_kernel<T, 1, 2><<<tiles, block, 0, s>>>(p); break;
+        case 17: thin_kernel<T, 2, 1><<<tiles, block, 0, s>>>(p); break;
+        default: thin_kernel<T, 2, 2><<<tiles, block, 0, s>>>(p); break;
+        }
+    });
+}
+
+// a wave keeps its rows; a share of the columns each, so many that the chip has waves enough
+template <typename T> void launch_short(const ProductArgs &args, hipStream_t s) {
+    const uint64_t all =
+        tiles_of_rows(args.groups.total, args.groups.groups, args.groups.offsets != nullptr, kShortRows);
+    const uint64_t shares = 2048 / all + 1, steps = (args.n + 63) / 64;
+    const uint32_t columns = 64 * (uint32_t)((steps + shares - 1) / shares);
+    each_window(args, all, [&](const ProductArgs &p, uint32_t tiles) {
+        const dim3 grid(tiles, (p.n + columns - 1) / columns);
+        short_kernel<T><<<grid, 64 * kShortWaves, 0, s>>>(p, columns);
+    });
+}
+
+// tiles of the adapters' ranks: kM x kN
+template <typename T, typename SA, typename SB, bool kWeights, bool kAcross, int kM, int kN, int kWavesM,
+          int kWavesN, typename O>
+void launch_narrow(const ProductArgs &args, const Plan &plan, hipStream_t s) {
+    each_window(args, plan.tiles, [&](const ProductArgs &p, uint32_t tiles) {
+        product_kernel<T, SA, SB, kWeights, kAcross, kM, kN, kWavesM, kWavesN, O>
+            <<<dim3(tiles, plan.splits), kThreads, 0, s>>>(p);
+    });
 }
 
 template <typename O> hipError_t join(const ProductArgs &p, uint64_t rows, hipStream_t s) {
@@ -828,21 +864,15 @@ hipError_t product_rows(int type, const ProductArgs &args, const Plan &plan, boo
     p.splits = plan.splits;
     p.k_each = plan.k_each;
     if (plan.late) p.beside.inner = nullptr;
-    const dim3 grid((uint32_t)plan.tiles, plan.splits);
     return with_type(type, [&](auto t) {
         typedef decltype(t) T;
         if (plan.thin_m) {
             launch_thin<T>(p, plan, s);
         } else if (!skinny && !across && !p.parts && p.k <= TileOf<T>::kK) {
-            // a share of the columns each, so many that the chip has waves enough
-            const uint64_t tiles = tiles_of_rows(p.groups.total, p.groups.groups, p.groups.offsets != nullptr, kShortRows);
-            const uint64_t shares = 2048 / tiles + 1, steps = (p.n + 63) / 64;
-            const uint32_t columns = 64 * (uint32_t)((steps + shares - 1) / shares);
-            const dim3 blocks((uint32_t)tiles, (p.n + columns - 1) / columns);
-            short_kernel<T><<<blocks, 64 * kShortWaves, 0, s>>>(p, columns);
+            launch_short<T>(p, s);
         } else if (skinny) {
-            if (across) product_kernel<T, T, T, false, true, 128, 32, 4, 1, float><<<grid, kThreads, 0, s>>>(p);
-            else product_kernel<T, T, T, false, false, 128, 32, 4, 1, float><<<grid, kThreads, 0, s>>>(p);
+            if (across) launch_narrow<T, T, T, false, true, 128, 32, 4, 1, float>(p, plan, s);
+            else launch_narrow<T, T, T, false, false, 128, 32, 4, 1, float>(p, plan, s);
         } else {
             const bool direct = lines_up(p.a, type, p.k) && lines_up(p.b, type, across ? p.n : p.k);
             if (across) launch_tiles<T, false, true>(p, plan, direct, s);
@@ -869,11 +899,10 @@ hipError_t product_weights(int type, ProductArgs p, const Plan &plan, bool narro
     p.tiles_n = plan.tiles_n;
     if (p.n_out == 0) p.n_out = p.n;
     p.splits = plan.splits;
-    const dim3 grid((uint32_t)plan.tiles, plan.splits);
     return with_type(type, [&](auto t) {
         typedef decltype(t) T;
-        if (narrow_m) product_kernel<float, float, T, true, true, 32, 128, 1, 4, T><<<grid, kThreads, 0, s>>>(p);
-        else if (narrow_n) product_kernel<float, T, float, true, true, 128, 32, 4, 1, T><<<grid, kThreads, 0, s>>>(p);
+        if (narrow_m) launch_narrow<float, float, T, true, true, 32, 128, 1, 4, T>(p, plan, s);
+        else if (narrow_n) launch_narrow<float, T, float, true, true, 128, 32, 4, 1, T>(p, plan, s);
         else launch_tiles<T, true, true>(p, plan, lines_up(p.a, type, p.m) && lines_up(p.b, type, p.n), s);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess || plan.splits == 1) return e;
@@ -882,7 +911,7 @@ hipError_t product_weights(int type, ProductArgs p, const Plan &plan, bool narro
 }
 
 int check_blocks(const char *call, const Plan &plan) {
-    if (plan.tiles > kMaxBlocks) return fail(SDF_E_INVALID, "%s: too many tiles of the result", call);
+    if (plan.tiles >= kMaxTiles) return fail(SDF_E_INVALID, "%s: too many tiles of the result", call);
     return SDF_OK;
 }
 
@@ -963,32 +992,33 @@ int sdf_expert_linear_backward(int type, const void *out_grad, uint64_t out_grad
     rc = check_scratch(scratch, scratch_bytes,
                        sdf_expert_linear_backward_scratch_bytes(count, num_experts, width, out_width));
     if (rc != SDF_OK) return rc;
+    const Plan rows_plan = plan_rows(count, num_experts, true, width, out_width, true, false);
+    const Plan weight_plan = plan_weights(count, num_experts, out_width, width, false, false);
+    if ((want_rows && (rc = check_blocks("sdf_expert_linear_backward", rows_plan)) != SDF_OK) ||
+        (want_weight && (rc = check_blocks("sdf_expert_linear_backward", weight_plan)) != SDF_OK))
+        return rc;
     ProductArgs p = {};
     p.groups = {offsets, num_experts, (uint32_t)count};
     p.partial = static_cast<float *>(scratch);
     p.scale = 1.0f;
     if (want_rows) {
-        const Plan plan = plan_rows(count, num_experts, true, width, out_width, true, false);
-        if ((rc = check_blocks("sdf_expert_linear_backward", plan)) != SDF_OK) return rc;
         p.a = {out_grad, out_grad_stride, 0, nullptr};
         p.b = {weight, width, (uint64_t)out_width * width, nullptr};
         p.n = width;
         p.k = out_width;
         p.out = rows_grad;
         p.out_stride = width;
-        const hipError_t e = product_rows(type, p, plan, true, false, false, s);
+        const hipError_t e = product_rows(type, p, rows_plan, true, false, false, s);
         if (e != hipSuccess) return hip_fail(e, "expert_linear_backward");
     }
     if (want_weight) {
-        const Plan plan = plan_weights(count, num_experts, out_width, width, false, false);
-        if ((rc = check_blocks("sdf_expert_linear_backward", plan)) != SDF_OK) return rc;
         p.a = {out_grad, out_grad_stride, 0, nullptr};
         p.b = {rows, rows_stride, 0, nullptr};
         p.m = out_width;
         p.n = width;
         p.out = weight_grad;
         p.out_stride = width;
-        const hipError_t e = product_weights(type, p, plan, false, false, s);
+        const hipError_t e = product_weights(type, p, weight_plan, false, false, s);
         if (e != hipSuccess) return hip_fail(e, "expert_linear_backward");
     }
     return SDF_OK;

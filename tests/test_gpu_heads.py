@@ -695,3 +695,135 @@ def test_adapters_last_columns(dev, rows, adapters, rank, width, out, dtype):
 def test_adapters_in_large_tiles(dev, width, out, dtype):
     """Few adapters in every 32 rows, added by the matrix units in tiles of 256 x 256."""
     test_adapters(dev, 4100, 3, 16, width, out, "any", dtype)
+
+
+# ---- results of more tiles, and of more rows, than one launch takes ------------------------------
+# Small whole numbers: every sum is exact.
+
+
+@pytest.fixture
+def much_memory(dev):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip("not enough free memory")
+    yield dev
+    torch.cuda.empty_cache()
+
+
+def soil(dev, *shape, dtype=torch.bfloat16):
+    """Memory that the next tensor of this size takes holds NaN."""
+    torch.full(shape, math.nan, dtype=dtype, device=dev)
+
+
+def test_many_experts_of_many_columns(much_memory):
+    dev, experts, each, width, out = much_memory, 2048, 16, 8, 65_600
+    say("many tiles of few rows")
+    rows = experts * each
+    x = (torch.arange(rows * width, device=dev) % 5 - 2).to(torch.bfloat16).reshape(rows, width)
+    c = ((torch.arange(experts, device=dev)[:, None] * 7 + torch.arange(out, device=dev) * 3) % 5 -
+         2).to(torch.bfloat16)
+    w = c[..., None].expand(experts, out, width).contiguous()
+    o = torch.arange(experts + 1, device=dev, dtype=torch.int32) * each
+    soil(dev, rows, out)
+    y = sdfoam_amd.expert_linear(x, w, o).view(experts, each, out)
+    sums = x.float().sum(1).to(torch.bfloat16).view(experts, each, 1)
+    for e in range(0, experts, 256):
+        assert torch.equal(y[e:e + 256], sums[e:e + 256] * c[e:e + 256, None])
+
+
+def test_narrow_rows_past_2_to_30(much_memory):
+    dev, rows = much_memory, (1 << 30) + 300
+    say("many narrow rows")
+    x = torch.empty(rows, dtype=torch.bfloat16, device=dev)
+    parts = [slice(k, min(k + (1 << 27), rows)) for k in range(0, rows, 1 << 27)]
+    for p in parts:
+        x[p] = (torch.arange(p.start, p.stop, device=dev) % 5 - 2).to(torch.bfloat16)
+    o = torch.tensor([0, (1 << 29) + 7, rows - 50], dtype=torch.int32, device=dev)
+    w = torch.tensor([3.0, -5.0], dtype=torch.bfloat16, device=dev).reshape(2, 1, 1)
+
+    def check(got, times):
+        for p in parts:
+            at = torch.arange(p.start, p.stop, device=dev)
+            f = torch.where(at < (1 << 29) + 7, times[0], times[1]) * (at < rows - 50)
+            assert torch.equal(got[p, 0], x[p] * f.to(torch.bfloat16))
+
+    soil(dev, rows, 1)
+    check(sdfoam_amd.expert_linear(x[:, None], w, o), (3.0, -5.0))
+    # 65 elements, the same row again and again
+    one = torch.ones((1, 65), dtype=torch.bfloat16, device=dev)
+    long = w.expand(2, 1, 65).contiguous()
+    soil(dev, rows, 1)
+    y = sdfoam_amd.expert_linear(one.expand(rows, 65), long, o)
+    x.fill_(1.0)
+    # -325 lies halfway between 162 and 163 steps of 2: the even one, -324, as `to` rounds it
+    check(y, (195.0, -325.0))
+    del y
+    soil(dev, rows, 1)
+    dx, none = sdfoam_amd.expert_linear_backward(one[:, :1].expand(rows, 1), x[:, None], w, o,
+                                                 need_weight=False)
+    assert none is None
+    check(dx, (3.0, -5.0))
+    del dx
+    # the same rows with an adapter each
+    ids = torch.zeros(rows, dtype=torch.int32, device=dev)
+    ids[(1 << 29) + 7:] = 1
+    ids[rows - 50:] = -1
+    up = torch.tensor([1.0, -7.0], dtype=torch.bfloat16, device=dev).reshape(2, 1, 1)
+    shared = torch.zeros((1, 1), dtype=torch.bfloat16, device=dev)
+    soil(dev, rows, 1)
+    y = sdfoam_amd.adapter_linear(x[:, None], shared, ids, torch.ones_like(up), up, 2.0)
+    check(y, (2.0, -14.0))
+
+
+def test_many_adapters_of_many_columns(much_memory):
+    """The gradient of `up`: a tile of 128 x 32 for each adapter and part of its matrix."""
+    dev, adapters, out, rank = much_memory, 2048, 1 << 18, 33
+    say("many adapters")
+    up = torch.zeros((adapters, out, rank), dtype=torch.bfloat16, device=dev)
+    down = torch.ones((adapters, rank, 4), dtype=torch.bfloat16, device=dev)
+    down[:, 32] = -2.0
+    ids = torch.tensor([2047, 0, 2047, 700, -1], device=dev)
+    x = torch.ones((5, 4), dtype=torch.bfloat16, device=dev)
+    x[2] = 2.0
+    d = (torch.arange(5 * out, device=dev) % 7 - 3).to(torch.bfloat16).reshape(5, out)
+    w = torch.zeros((out, 4), dtype=torch.bfloat16, device=dev)
+    soil(dev, adapters, out, rank)
+    _, _, _, up_grad = sdfoam_amd.adapter_linear_backward(d, x, w, ids, down, up,
+                                                          need_rows=False, need_weight=False)
+    h = down[0].float().sum(1)
+    for a, column in ((0, d[1].float()), (700, d[3].float()), (2047, d[0].float() + 2 * d[2].float())):
+        assert torch.equal(up_grad[a].float(), column[:, None] * h)
+        up_grad[a] = 0
+    for a in range(0, adapters, 64):
+        assert not up_grad[a:a + 64].any()
+
+
+def test_rows_past_2_to_25(much_memory):
+    """Rows of 64 lanes each, four a block."""
+    dev, rows, width = much_memory, (1 << 25) + 77, 132
+    say("many rows")
+    at = torch.arange(rows, device=dev)
+    x = torch.arange(width, device=dev, dtype=torch.float32).repeat(rows, 1)
+    x += (at % 65_521)[:, None]
+    ids = (at % 3).int()
+    ids[at % 1000 == 5] = -1
+    order = sdfoam_amd.expert_order(ids[:, None], 3)
+    soil(dev, rows, width, dtype=torch.float32)
+    y = sdfoam_amd.expert_rows(x, order)
+    p = order.places[:, 0].long()
+    named = p >= 0
+    parts = [slice(k, min(k + (1 << 22), rows)) for k in range(0, rows, 1 << 22)]
+    for s in parts:
+        assert torch.equal(y[torch.where(named[s], p[s], -1 - p[s])], x[s] * named[s, None])
+    gate = torch.where(at % 2 == 0, 2.0, -1.0)[:, None]
+    back = sdfoam_amd.expert_combine(y, order, gate)
+    for s in parts:
+        assert torch.equal(back[s], x[s] * (gate[s] * named[s, None]))
+    del back
+    soil(dev, rows, width, dtype=torch.float32)
+    rows_grad, gate_grad = sdfoam_amd.expert_combine_backward(
+        torch.ones((1, width), device=dev).expand(rows, width), y, order, gate)
+    for s in parts:
+        assert torch.equal(gate_grad[s, 0], x[s].sum(1) * named[s])
+        want = (gate[s] * named[s, None]).expand(-1, width)
+        assert torch.equal(rows_grad[torch.where(named[s], p[s], -1 - p[s])], want)
