@@ -53,7 +53,8 @@ template <typename T> __global__ __launch_bounds__(256) void few_rows_kernel(Few
         }
     }
     sum = group_sum<64>(sum);
-    if (lane == 0 && r < f.pitch) f.inner[row * f.pitch + r] = f.scale * sum;
+    // 0 past the rank, at any scale
+    if (lane == 0 && r < f.pitch) f.inner[row * f.pitch + r] = r < f.rank ? f.scale * sum : 0.0f;
 }
 
 struct Layout {

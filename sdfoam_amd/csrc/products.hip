@@ -467,16 +467,16 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs p) {
             for (int q = 0; q < 4; ++q) {
                 const uint32_t n = n0 + wn + j * 32 + q * 8 + half * 4;
                 if (n >= p.n_out) continue;
-                Few<float, 4> sum;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum.v[e] = n + e < p.n ? acc[i][j][q * 4 + e] : 0.0f;
                 if (p.parts) {
+                    Few<float, 4> sum;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum.v[e] = acc[i][j][q * 4 + e];
                     const uint64_t rows = kWeights ? (uint64_t)p.groups.groups * p.m : p.groups.total;
                     store_some<float, 4>(p.partial + (split * rows + row) * p.n_out + n, sum, p.n_out - n);
                 } else {
-                    Few<O, 4> o;
+                    Few<O, 4> o; // 0 past n, at any scale
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o.v[e] = (O)(p.scale * sum.v[e]);
+                    for (int e = 0; e < 4; ++e) o.v[e] = (O)(n + e < p.n ? p.scale * acc[i][j][q * 4 + e] : 0.0f);
                     store_some<O, 4>(static_cast<O *>(p.out) + (p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride + n,
                                      o, p.n_out - n);
                 }
@@ -500,7 +500,7 @@ template <typename O> __global__ __launch_bounds__(256) void join_kernel(Product
     O *to = static_cast<O *>(p.out) + (p.out_index ? (uint32_t)p.out_index[row] : row) * p.out_stride + n;
     Few<O, 4> o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o.v[e] = (O)(p.scale * sum[e]);
+    for (int e = 0; e < 4; ++e) o.v[e] = (O)(n + e < p.n ? p.scale * sum[e] : 0.0f);
     store_some<O, 4>(to, o, have);
 }
 

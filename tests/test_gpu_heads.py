@@ -827,3 +827,130 @@ def test_rows_past_2_to_25(much_memory):
         assert torch.equal(gate_grad[s, 0], x[s].sum(1) * named[s])
         want = (gate[s] * named[s, None]).expand(-1, width)
         assert torch.equal(rows_grad[torch.where(named[s], p[s], -1 - p[s])], want)
+
+
+# ---- values that are not finite, and values below the normal range --------------------------------
+
+
+def same(got, ref, tol, dtype):
+    """near(), and infinite where the reference is, with its sign."""
+    near(got, ref, tol, dtype)
+    got = got.detach().cpu().double()
+    infinite = torch.isinf(ref)
+    assert torch.equal(got[infinite], ref[infinite])
+
+
+INFINITE_ADAPTERS = [  # rows, adapters, rank, width, out
+    (7, 2, 1, 40, 50), (7, 2, 5, 40, 50), (64, 3, 1, 600, 130), (40, 3, 9, 70, 70),
+    (300, 4, 1, 40, 30), (300, 4, 3, 30, 90), (1100, 400, 1, 1100, 70), (1100, 400, 2, 20, 70),
+    (900, 300, 1, 600, 1100),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,adapters,rank,width,out", INFINITE_ADAPTERS)
+def test_adapters_infinite(dev, rows, adapters, rank, width, out, dtype):
+    """An infinite scale, and infinite elements: infinite results have their sign, sums of
+    both signs are NaN, and what only fills up a rank adds nothing."""
+    say("infinite", rows, adapters, rank, width, out, dtype)
+    x, w, ids, down, up, d = adapter_case(rows, adapters, rank, width, out, "any", dtype)
+    ids[0], ids[1] = 0, -1
+    c = ids.to(dev)
+    for scale in (math.inf, -math.inf, 1.5):
+        if scale == 1.5:
+            x[0, width // 2], d[0, out // 2] = math.inf, -math.inf
+            x[1, 0] = -math.inf
+        refs, tols = adapter_reference(x, w, ids, down, up, scale, d)
+        tols = [torch.nan_to_num(t, nan=0.0, posinf=0.0) if scale != 1.5 else t for t in tols]
+        X, W, A, B, D = (t.to(dev) for t in (x, w, down, up, d))
+        got = [sdfoam_amd.adapter_linear(X, W, c, A, B, scale),
+               *sdfoam_amd.adapter_linear_backward(D, X, W, c, A, B, scale)]
+        if scale != 1.5:  # rows without an adapter, and the projection's gradient: finite
+            n = ids < 0
+            same(got[0].cpu()[n], refs[0][n], bound(width) * (x.double().abs() @ w.double().abs().T)[n], dtype)
+            same(got[2], refs[2], bound(rows) * (d.double().abs().T @ x.double().abs()), dtype)
+        for k, (a, ref) in enumerate(zip(got, refs)):
+            if k == 2 and scale != 1.5:
+                continue
+            fine = torch.isfinite(ref)
+            a = a.cpu().double()
+            assert torch.equal(torch.isnan(a), torch.isnan(ref)), (scale, k)
+            assert torch.equal(a[torch.isinf(ref)], ref[torch.isinf(ref)]), (scale, k)
+            assert torch.isfinite(a[fine]).all(), (scale, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_and_combine_infinite(dev, dtype):
+    g = torch.Generator().manual_seed(4)
+    for rows, counts, width, out in ((6, [2, 4], 40, 20), (300, [100, 150], 30, 70),
+                                     (300, [100, 150], 600, 70), (130, [130], 1031, 90)):
+        say("infinite", rows, counts, width, out, dtype)
+        x, d = (torch.randn((rows, k), generator=g).to(dtype) for k in (width, out))
+        w = torch.randn((len(counts), out, width), generator=g).to(dtype)
+        x[1, 0], x[3, width - 1], d[0, out - 1], w[0, 5, 7] = math.inf, -math.inf, math.inf, math.inf
+        o = offsets_of(counts, rows)
+        refs = [torch.zeros((rows, out), dtype=torch.float64), torch.zeros((rows, width), dtype=torch.float64),
+                torch.zeros(w.shape, dtype=torch.float64)]
+        sizes = [torch.zeros_like(t) for t in refs]
+        for e in range(len(counts)):
+            p = slice(int(o[e]), int(o[e + 1]))
+            xe, we, de = x[p].double(), w[e].double(), d[p].double()
+            refs[0][p], sizes[0][p] = xe @ we.T, xe.abs() @ we.abs().T
+            refs[1][p], sizes[1][p] = de @ we, de.abs() @ we.abs()
+            refs[2][e], sizes[2][e] = de.T @ xe, de.abs().T @ xe.abs()
+        off = o.to(torch.int32).to(dev)
+        X, W, D = x.to(dev), w.to(dev), d.to(dev)
+        got = [sdfoam_amd.expert_linear(X, W, off), *sdfoam_amd.expert_linear_backward(D, X, W, off)]
+        for a, ref, size, n in zip(got, refs, sizes, (width, out, max(counts))):
+            same(a, ref, bound(n) * size, dtype)
+
+    y = torch.randn((6, 37), generator=g).to(dtype)
+    y[0, 3], y[4, 36], y[5, 0] = math.inf, -math.inf, math.nan
+    gate = torch.tensor([[1.0, -2.0], [0.5, 0.25], [math.inf, 3.0]])
+    places = torch.tensor([[0, 1], [-6, 4], [2, 3]], dtype=torch.int32)
+    order = sdfoam_amd.ExpertOrder(places.to(dev), torch.tensor([0, 5], dtype=torch.int32).to(dev))
+    live = (places >= 0).double()[..., None]
+    terms = torch.where(live > 0, gate.double()[..., None] * y.double()[places.clamp(min=0).long()], 0.0)
+    same(sdfoam_amd.expert_combine(y.to(dev), order, gate.to(dev)), terms.sum(1),
+         bound(2) * terms.abs().sum(1), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,out", [(3, 64, 32), (40, 64, 64), (300, 200, 136), (300, 201, 137),
+                                            (200, 16, 70), (8200, 264, 2056)])
+def test_below_the_normal_range(dev, rows, width, out, dtype):
+    """Operands below their type's normal range are not taken for 0.  Whole multiples of the
+    type's smallest step times powers of two: every sum is exact."""
+    say("below the normal range", rows, width, out, dtype)
+    step = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[dtype]
+    lift = {torch.float32: 2.0 ** 100, torch.float16: 2.0 ** 10, torch.bfloat16: 2.0 ** 100}[dtype]
+    g = torch.Generator().manual_seed(rows)
+    k = torch.randint(-2, 3, (rows, width), generator=g).double()
+    sign = torch.randint(0, 2, (out, width), generator=g).double() * 2 - 1
+    sign *= torch.rand((out, width), generator=g) < 8.0 / width  # sums below 2^8
+    x, w = (k * step).to(dtype), (sign * lift).to(dtype)
+    assert torch.equal(x.double(), k * step)
+    y = (k @ sign.T) * (step * lift)
+    assert torch.equal(y.to(dtype).double(), y)
+    o = torch.tensor([0, rows], dtype=torch.int32, device=dev)
+    assert torch.equal(sdfoam_amd.expert_linear(x.to(dev), w.to(dev)[None], o).cpu().double(), y)
+    # the same products as the gradient of the rows, and the other operand small
+    dx, _ = sdfoam_amd.expert_linear_backward(x.to(dev), torch.empty((rows, out), dtype=dtype, device=dev),
+                                              w.t().contiguous().to(dev)[None], o, need_weight=False)
+    assert torch.equal(dx.cpu().double(), y)
+    small, large = (sign * step).to(dtype), (k * lift).to(dtype)
+    assert torch.equal(sdfoam_amd.expert_linear(large.to(dev), small.to(dev)[None], o).cpu().double(), y)
+    # as an adapter beside a projection of zeros
+    none = torch.zeros((out, width), dtype=dtype, device=dev)
+    c = torch.zeros(rows, dtype=torch.int64, device=dev)
+    n = min(out, 32)
+    z = sdfoam_amd.adapter_linear(x.to(dev), none, c, w[:n].to(dev)[None],
+                                  torch.eye(out, n, dtype=dtype, device=dev)[None])
+    assert torch.equal(z.cpu().double()[:, :n], y[:, :n]) and not z[:, n:].any()
+    # as the gradient of the matrix: sums over few of the rows
+    few = torch.zeros((rows, 8), dtype=torch.float64)
+    few[:min(rows, 50)] = torch.randint(-1, 2, (min(rows, 50), 8), generator=g).double()
+    _, dw = sdfoam_amd.expert_linear_backward((few * lift).to(dtype).to(dev), x.to(dev),
+                                              torch.empty((1, 8, width), dtype=dtype, device=dev), o,
+                                              need_rows=False)
+    assert torch.equal(dw.cpu().double()[0], (few.T @ k) * (step * lift))
