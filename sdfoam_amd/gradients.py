@@ -77,8 +77,8 @@ def _check_scale(scale) -> float:
 
 def gradient_norm(gradients: Iterable[Optional[torch.Tensor]], scale: float = 1.0) -> torch.Tensor:
     """``scale`` times the Euclidean norm of all gradients together (float32, on their
-    device).  gradients: tensors of any shapes, empty ones and None (a parameter without a
-    gradient) among them; one that is there twice counts twice."""
+    device).  gradients: one tensor, or tensors of any shapes, empty ones and None (a
+    parameter without a gradient) among them; one that is there twice counts twice."""
     scale = _check_scale(scale)
     tensors, device = _gradients("gradient_norm", gradients)
     return _run([g for g in tensors if g is not None], None, 0.0, scale, device)
@@ -90,9 +90,9 @@ def clip_gradients(gradients: Iterable[Optional[torch.Tensor]], max_norm: float,
     """Scales all gradients by ``scale * min(1, max_norm / (norm + 1e-6))`` and returns
     ``norm``, ``scale`` times their Euclidean norm before (float32, on their device).
 
-    gradients: tensors of any shapes, for instance ``[p.grad for p in parameters]``; None
-    among them is passed over.  scale undoes a loss scale or averages sums, before anything
-    is rounded.  out (optional): tensors of the gradients' shapes, float32 or of their
+    gradients: one tensor, or tensors of any shapes, for instance ``[p.grad for p in
+    parameters]``; None among them is passed over.  scale undoes a loss scale or averages sums, before anything
+    is rounded.  out (optional): as many tensors of the gradients' shapes, float32 or of their
     gradient's type, that the results are written to -- an optimizer's float32 copies --;
     default: the gradients themselves.  No result may lie on another, or on another
     gradient.
@@ -107,6 +107,8 @@ def clip_gradients(gradients: Iterable[Optional[torch.Tensor]], max_norm: float,
     if not max_norm >= 0.0:
         raise RuntimeError("max_norm must not be negative")
     tensors, device = _gradients("clip_gradients", gradients)
+    if isinstance(gradients, torch.Tensor) and isinstance(out, torch.Tensor):
+        out = [out]
     results = tensors if out is None else list(out)
     if out is not None:
         if len(results) != len(tensors):

@@ -259,3 +259,21 @@ def test_norms_past_the_range(dev):
     assert torch.equal(a.cpu(), torch.tensor([0.5, -1.0]))
     a[0] = math.inf
     assert float(sdfoam_amd.clip_gradients([a], math.inf)) == math.inf and torch.isnan(a).all()
+
+
+def test_one_tensor_into_another(dev):
+    """One gradient and one result, neither in a list."""
+    g = torch.Generator().manual_seed(6)
+    for shape in ((40,), (5, 8), (1, 40), ()):
+        t = torch.randn(shape, generator=g).to(torch.bfloat16)
+        own, out = t.to(dev), torch.full(shape, math.nan, device=dev)
+        got = sdfoam_amd.clip_gradients(own, 0.25, out=out)
+        want = torch.empty_like(out)
+        assert torch.equal(got, sdfoam_amd.clip_gradients([own], 0.25, out=[want]))
+        assert torch.equal(out, want) and torch.equal(own.cpu(), t)
+    # the rows of a matrix are results too
+    rows = [torch.randn(8, generator=g).to(dev) for _ in range(3)]
+    matrix = torch.empty((3, 8), device=dev)
+    sdfoam_amd.clip_gradients(rows, 0.25, out=matrix)
+    sdfoam_amd.clip_gradients(rows, 0.25)
+    assert torch.equal(matrix, torch.stack(rows))
