@@ -5,8 +5,10 @@
 //
 // Squares are added in fp64: those of floats below 1e-19 or above 1e19 leave fp32's range,
 // and memory is the bound all the same.  The tensors' addresses travel in the launches'
-// arguments: nothing is copied to the device beforehand, a captured graph keeps them.  Every block's share is decided by the sizes alone, and the blocks'
-// sums are added in order: every run gives the same.
+// arguments, which a captured graph keeps: those of the two passes themselves, past 96 tensors
+// those of small launches that write them to a table on the device first.  Every block's share
+// is decided by the sizes alone, and the blocks' sums are added in order: every run gives the
+// same.
 #include <algorithm>
 #include <new>
 #include <vector>

@@ -6,11 +6,9 @@
 //   rows:     out[m, n] = sum_k a[m, k] b_g[n, k]   for the rows m of group g
 //   weights:  out_g[m, n] = sum over rows k of group g of a[k, m] b[k, n]
 //
-// Either operand may lie with k along its rows or across them; the tile in LDS always has
-// k along its rows (an operand that lies across is turned in registers on its way there),
-// so that every wave reads its fragments as 16 bytes a lane.  Chunks of 16 bytes are
-// swizzled: chunk c of row r lies at c ^ ((r ^ r >> 3) & 7), which keeps reads (32 rows,
-// the same chunk) and turned writes (every 4th or 8th row) off each other's banks.
+// Either operand may lie with k along its rows or across them.  Large tiles keep it in LDS
+// as memory has it and turn it when they read (Feed, Fragments); the narrow tiles of the
+// adapters' ranks turn it on its way there (Along, Across).
 #pragma once
 
 #include "head_device.h"
@@ -372,6 +370,10 @@ template <typename T, bool kAcross, int kRows, int kFragments> struct Fragments 
 };
 
 // ---- narrow tiles: turned on their way to LDS ---------------------------------------------
+//
+// The tile in LDS always has k along its rows, so that every wave reads its fragments as 16
+// bytes a lane.  Chunk c of row r lies at c ^ ((r ^ r >> 3) & 7), which keeps reads (32 rows,
+// the same chunk) and turned writes (every 4th or 8th row) off each other's banks.
 __device__ __forceinline__ uint32_t place_in_lds(uint32_t row, uint32_t chunk) {
     return row * 128u + ((chunk ^ ((row ^ row >> 3) & 7u)) << 4);
 }

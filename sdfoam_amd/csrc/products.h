@@ -24,7 +24,7 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
 Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool narrow_m, bool narrow_n);
 
 // the same plan with the adapters added late: where rows have an adapter each, more or less,
-// every row's is read by threads of its own (64 rows of 2,048 -> 32,768 bf16 and rank 16)
+// every row's is read by threads of its own
 Plan late(Plan plan, uint64_t rows, uint32_t n);
 
 hipError_t product_rows(int type, const ProductArgs &p, const Plan &plan, bool across, bool skinny,

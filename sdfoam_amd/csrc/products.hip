@@ -28,6 +28,10 @@ struct LoaderOf<true, T, S, kRows, kThreads> {
 // (add_beside; a lane has row m0 + mi, as the accumulators do), and for each row by itself
 // where they have many (beside_of_rows).  One after the other, each waits for its values: 200
 // rows, an adapter each, of 2,048 -> 32,768 bf16 and rank 16 took 247 us, 48 without them.
+// Microseconds by the matrix units and row by row, 4,096 rows of 512 -> 2,048 bf16 in order,
+// with 1, 3, 4 and 8 adapters in 32 rows: rank 8 37 and 70, 45 and 71, 52 and 77, 66 and 83;
+// rank 64 49 and 637, 81 and 639, 106 and 649, 213 and 690.  At these sizes the two meet at
+// more adapters than the limit.
 constexpr uint32_t kFewAdapters = 3;
 __device__ __forceinline__ bool few_adapters(int32_t mine) {
     uint64_t left = __ballot(mine >= 0);
@@ -538,8 +542,12 @@ template <typename O, bool kAcross> __global__ __launch_bounds__(256) void join_
 // At most 128 bytes of it: a wave keeps 32 rows in registers and goes over the columns, 64 at
 // a time, their fragments from the caches while the 64 before are written, without LDS but to
 // turn what it writes and without waiting for another wave.  Bound by the waits for columns
-// and the VALU's share of conversions and addresses (160,000 rows of 64 -> 512 fp16: 63 us, with
-// adapters 79; tiles, which wait in turn for rows, columns and each other, 76 and 88).
+// and the VALU's share of conversions and addresses (160,000 rows of 64 -> 512 fp16, other
+// rows each time: 63 us, with adapters 79; tiles, which wait in turn for rows, columns and
+// each other, 76 and 88).  Microseconds on the same rows again and again, tiles after: 10^6
+// rows of 64 -> 512 fp16 323 and 391, of 32 -> 64 floats 113 and 162; 160,000 of 16 -> 64 fp16
+// 14 and 17; but where the caches hold the result and it is wider, 64 -> 512 67 and 57, 64 ->
+// 256 39 and 30, of 32 -> 201 floats 65 and 57.
 constexpr uint32_t kShortWaves = 4, kShortRows = 32 * kShortWaves;
 
 template <typename T> __global__ __launch_bounds__(64 * kShortWaves, 3) void short_kernel(ProductArgs p, uint32_t columns) {
@@ -607,7 +615,9 @@ constexpr int kThinWaves = 4;
 template <typename T, int kMt, int kNt>
 __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ProductArgs p) {
     constexpr uint32_t kC = TileOf<T>::kC, kStep = TileOf<T>::kK; // a lane has two pieces a step
-    constexpr int kAhead = kMt * kNt <= 2 ? 4 : 2; // steps in flight
+    // steps asked for together; of their loads the compiler keeps some in flight: 16 bits,
+    // tiles of 16 x 16 eight, of 16 x 32 three, of 32 x 32 four; floats two to four
+    constexpr int kAhead = kMt * kNt <= 2 ? 4 : 2;
     __shared__ F4x sums[kThinWaves][kMt * kNt][64];
     __shared__ uint32_t found[20];
     const uint32_t block = p.first + blockIdx.x, tile_n = block % p.tiles_n, tile_m = block / p.tiles_n;
@@ -790,10 +800,18 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
                bool skinny) {
     Plan plan = {};
     const uint64_t each = grouped && groups > 0 ? (rows + groups - 1) / groups : rows;
+    // Microseconds of thin and of large tiles, 4,096 -> 4,096: 16 rows bf16 12 and 19, floats 24
+    // and 64; 32 rows 20 and 20, 38 and 66.  8 rows each of 16 experts, 1,024 -> 2,048 bf16 16 and
+    // 17, 32 rows each 21 and 18 (floats 37 and 73); 32 rows of 2,048 -> 32,768 bf16 35 and 29, 48
+    // rows 57 and 29.
     if (!skinny && !across && each <= 32) {
         plan.thin_m = each <= 16 ? 1 : 2;
         const uint64_t tiles_m = tiles_of_rows(rows, groups, grouped, 16 * plan.thin_m);
-        // wider where there are columns enough for every CU: the rows are read less often
+        // Wider where there are columns enough for every CU: the rows are read less often.
+        // Microseconds at 32 columns and at 16, bf16: 16 rows of 4,096 -> 32,768 54 and 63, 64
+        // entries over 64 experts of 1,024 -> 2,048 43 and 45, one row of 4,096 -> 4,096 13 and 9;
+        // 32 rows of 4,096 -> 4,096 20 and 16 (128 tiles of 32), -> 6,144 20 and 26, -> 8,192 20
+        // and 26 (256 tiles).
         plan.thin_n = plan.thin_m;
         if (plan.thin_n < 2 && tiles_m * (n / 32) >= 1024) plan.thin_n = 2;
         while (plan.thin_n > 1 && tiles_m * ((n + 16 * plan.thin_n - 1) / (16 * plan.thin_n)) < 256)
@@ -809,12 +827,20 @@ Plan plan_rows(uint64_t rows, uint32_t groups, bool grouped, uint32_t n, uint32_
                                         : 2 * ((rows + tile - 1) / tile);
         return halves / 2 * ((n + tile - 1) / tile);
     };
+    // not at a short inner dimension, where they gain little: 4,096 rows of 320 -> 4,096 bf16
+    // take 21 us by large tiles and 24 by small ones, of 256 20 and 22, of 128 16 and 18
     plan.large = !skinny && k > 256 && rows > 0 && take_large(tiles(256), tiles(128));
     const uint32_t km = plan.large ? 256 : 128, kn = skinny ? 32 : km;
     plan.tiles_n = (n + kn - 1) / kn;
     plan.tiles = tiles_of_rows(rows, groups, grouped, km) * plan.tiles_n;
-    // few tiles: the inner dimension in several parts, of 512 elements at least, until the
-    // chip has a block for each of its places
+    // Few tiles: the inner dimension in several parts, of 512 elements at least, until the
+    // chip has a block for each of its places.  Microseconds in parts and whole, 128 rows of
+    // 4,096 -> 4,096: bf16 22 and 46, floats 67 and 265; with 256 and 1,024 blocks bf16 31 and 24,
+    // floats 141 and 82.  512 rows bf16 41 and 47; 1,024 rows (256 tiles) whole 50, in parts 63.
+    // Parts of 256, 512 and 1,024 elements, 64 rows of 2,048 -> 2,048: bf16 15, 15 and 18, floats
+    // 29, 43 and 74.  Skinny ones wait for memory, in shorter parts: the gradients of 64 adapters
+    // of rank 16, 1,024 rows of 2,048 -> 2,048 bf16, take 53, with b and h whole 96, in parts of
+    // 128 62, of 512 57.
     plan.splits = 1;
     if (plan.tiles > 0 && !plan.large && plan.tiles < (skinny ? 768 : 256)) {
         const uint64_t want = (skinny ? 1536 : 512) / plan.tiles, most = k / (skinny ? 256 : 512);
@@ -835,7 +861,13 @@ Plan plan_weights(uint64_t rows, uint32_t groups, uint32_t m, uint32_t n, bool n
     plan.tiles_n = (n + kn - 1) / kn;
     plan.tiles = (uint64_t)groups * ((m + km - 1) / km) * plan.tiles_n;
     plan.splits = 1;
-    // narrow ones wait for memory more than they multiply: more blocks, shorter parts
+    // Parts of 512 rows at least, and blocks for two rounds of places.  Microseconds in parts
+    // and whole, 65,536 rows of 512 x 512: bf16 93 and 657 (512 blocks 83, 2,048 132), floats 293
+    // and 4,171; 8 experts of 1,024 rows, 1,024 x 1,024 bf16 (512 tiles) in parts 48, whole 25.
+    // Narrow ones wait for memory more than they multiply: more blocks, shorter parts.  The
+    // gradients of 12 adapters of rank 8, 8,192 rows of 1,000 -> 5,003 bf16, take 175 us; with
+    // the narrow products whole 256, in parts of 192 rows at least 190, of 48 178, in half as
+    // many blocks 189; 8 of rank 16, 4,096 -> 4,096, 217, whole 324, 192 rows 187.
     const bool narrow = narrow_m || narrow_n;
     if (plan.tiles > 0 && !plan.large && plan.tiles < (narrow ? 768 : 400)) {
         const uint64_t want = (narrow ? 1536 : 1024) / plan.tiles, most = rows / groups / (narrow ? 96 : 512);

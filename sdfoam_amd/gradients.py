@@ -91,11 +91,11 @@ def clip_gradients(gradients: Iterable[Optional[torch.Tensor]], max_norm: float,
     ``norm``, ``scale`` times their Euclidean norm before (float32, on their device).
 
     gradients: one tensor, or tensors of any shapes, for instance ``[p.grad for p in
-    parameters]``; None among them is passed over.  scale undoes a loss scale or averages sums, before anything
-    is rounded.  out (optional): as many tensors of the gradients' shapes, float32 or of their
-    gradient's type, that the results are written to -- an optimizer's float32 copies --;
-    default: the gradients themselves.  No result may lie on another, or on another
-    gradient.
+    parameters]``; None among them is passed over.  scale undoes a loss scale or averages
+    sums, before anything is rounded.  out (optional): as many tensors of the gradients'
+    shapes, float32 or of their gradient's type, that the results are written to -- an
+    optimizer's float32 copies --; default: the gradients themselves.  No result may lie on
+    another, or on another gradient.
 
     The factor is that of the norm before it is rounded to float32: finite gradients whose
     norm passes float32's range are clipped all the same, and the norm returned for them is
