@@ -162,7 +162,7 @@ __device__ __forceinline__ void scaled(const void *in, void *out, uint64_t first
 }
 
 // Every block adds the other pass's sums itself, in the same order (8 KB from L2).  Memory
-// bounds both passes: 500M bf16 elements into floats 163 us (6.1 TB/s) and 605 (5.0); with the
+// bounds both passes: 500M bf16 elements into floats 165 us (6.1 TB/s) and 604 (5.0); with the
 // results written through the caches 210 and 615, unaligned besides 214 and 622.
 template <typename Source>
 __global__ __launch_bounds__(kThreads) void scale_kernel(Source t, const double *sums, uint32_t n, float scale,
